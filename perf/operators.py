@@ -95,7 +95,7 @@ def draw(rng):
         heads, kv, dim = rng.choice(((32, 8, 128), (32, 8, 128), (32, 4, 128), (32, 32, 64), (24, 8, 128), (8, 1, 256)))
         if rng.random() < 0.7:
             seqs = _log(rng, 1, 48)
-            ctx = _log(rng, 1, min(131072, 2 * 16 * 32000 // (seqs * max(1, kv * dim // 1024))))
+            ctx = _log(rng, 1, min(131072, 410000 * 1024 // (seqs * kv * dim)))
             tokens = 1
         else:
             seqs = _log(rng, 1, 4)
