@@ -325,6 +325,164 @@ int iam_embed_gather(iam_ctx* ctx, const uint16_t* table_dev, int cols, int voca
 /* greedy pick (test_generation.cpp:235, :276): first index of the maximum */
 int iam_argmax(iam_ctx* ctx, const float* v_dev, int n, int* out_dev);
 
+/* ---------------------------------------------------- long-context operators
+ * No counterpart in the reference, which rotates one token with unscaled
+ * angles, keeps its cache in fp32 and answers with the first maximum. */
+
+/* number types of activations */
+#define IAM_F32 0
+#define IAM_F16 1
+#define IAM_BF16 2
+
+/* which values of a head form a pair: (i, i + rot_dim/2), or (2i, 2i + 1) */
+#define IAM_ROPE_HALF 0
+#define IAM_ROPE_INTERLEAVED 1
+
+/* Scaling of the rotary angles for contexts past the trained one.  With
+ * f_i = theta^(-2i/rot_dim), pair i turns by pos * f_i' and is multiplied by
+ * `magnitude` (0: 1, or RAMP's own):
+ *   NONE    f_i' = f_i
+ *   LINEAR  f_i / factor (position interpolation)
+ *   BASE    f_i of the base theta * factor^(rot_dim / (rot_dim - 2))
+ *   BANDS   with t_i = original_ctx * f_i / 2 pi turns over the trained
+ *           context: f_i where t_i >= high, f_i / factor where t_i <= low, in
+ *           between the mix of both that is linear in t_i
+ *   RAMP    f_i for pairs below the one that turns `high` times over the
+ *           trained context, f_i / factor past the one that turns `low`
+ *           times, linear in i between them (YaRN; their places
+ *           rot_dim * ln(original_ctx / (2 pi turns)) / (2 ln theta) rounded
+ *           down and up, kept in [0, rot_dim - 1]); magnitude 0.1 ln(factor) + 1
+ * factor is at least 1; original_ctx, low and high (0 < low < high) are read
+ * by BANDS and RAMP only. */
+#define IAM_ROPE_SCALE_NONE 0
+#define IAM_ROPE_SCALE_LINEAR 1
+#define IAM_ROPE_SCALE_BASE 2
+#define IAM_ROPE_SCALE_BANDS 3
+#define IAM_ROPE_SCALE_RAMP 4
+typedef struct {
+    int kind;
+    double factor;
+    double original_ctx;
+    double low;
+    double high;
+    double magnitude;
+} iam_rope_scaling;
+
+/* The table of iam_rope_tokens, fp32 [max_pos][rot_dim/2][2] of (cos, sin) on
+ * the device: angles, cosines and sines in fp64, each value rounded once
+ * (iam_rope_table rounds the angle to fp32 first, as the reference does,
+ * up to 0.004 radians off at position 100000; its tables have the same form
+ * and serve iam_rope_tokens too).  rot_dim is even, 2 .. 1024; scaling may be
+ * null (NONE).  table_dev is 8-byte aligned. */
+int iam_rope_scaled_table(iam_ctx* ctx, double theta, int rot_dim, int max_pos,
+                          const iam_rope_scaling* scaling, float* table_dev);
+/* Rotary positions of n_tokens rows of n_heads heads: the first rot_dim of a
+ * head's head_dim values are rotated in pairs (layout) by the table's row
+ * pos_dev[token], the others pass through.  Arithmetic in fp32 (iam_rope's
+ * operations), one rounding to the type.  Rows are x_stride / out_stride
+ * values apart (0: n_heads * head_dim), each row's heads contiguous; q and k
+ * that lie side by side are one call over their heads together.  out_dev may
+ * be x_dev with the same stride; else the two may not overlap.  A token whose
+ * position lies outside [0, max_pos) leaves its out row as it was. */
+int iam_rope_tokens(iam_ctx* ctx, const void* x_dev, int type, int n_tokens, int n_heads, int head_dim,
+                    int rot_dim, int layout, size_t x_stride, const float* table_dev, int max_pos,
+                    const int* pos_dev, void* out_dev, size_t out_stride);
+
+/* A KV cache in 8 bits for n_seq sequences of up to max_ctx tokens.  The
+ * tokens of a sequence are taken in blocks of IAM_KV8_BLOCK.  A full block
+ * holds, for each KV head, 8-bit numbers and one fp32 scale for K and one for
+ * V: scale = largest magnitude * fp32(1/127) and round(x / scale) for INT8,
+ * largest magnitude * fp32(1/448) and the nearest e4m3 number (3 bits behind
+ * the leading one, exponents down to 2^-6, then steps of 2^-9) for E4M3.  The
+ * scale is rounded to fp32, the numbers to nearest even of the exact
+ * quotient; a number stands for number * scale.  The block
+ * that is not full yet is held in fp16, so a token's place in the cache does
+ * not depend on how many came with it.  K and V are rounded to fp16 first, as
+ * in the fp16 cache.  A block that holds an infinity or a NaN in a head has
+ * the scale NaN there once it is full.
+ *
+ * Device memory, the caller's (iam_kv8_size says how much; every part 16-byte
+ * aligned).  b counts blocks (ceil(max_ctx / 64) of them), t tokens in a block,
+ * d values in a head:
+ *   k, v              bytes [n_seq][b][n_kv][64 * head_dim], INT8 as number + 128
+ *   k_scale, v_scale  fp32 [n_seq][b][n_kv]; negative: not full (iam_kv8_reset)
+ *   k_open, v_open    fp16 [n_seq][n_kv][64 * head_dim], the open block
+ * A block's 64 * head_dim values are in the order in which the matrix
+ * instructions of the attention take them (iam_kv8_read gives plain rows):
+ *   K: ((t/16 * head_dim/64 + d/64) * 64 + d%64/16 * 16 + t%16) * 16 + d%16
+ *   V: (d/16 * 64 + t/4%4 * 16 + d%16) * 16 + t/32 * 8 + t/16%2 * 4 + t%4
+ * head_dim is 64, 128 or 256. */
+#define IAM_KV8_BLOCK 64
+#define IAM_KV8_INT8 0
+#define IAM_KV8_E4M3 1
+typedef struct {
+    uint8_t* k;
+    uint8_t* v;
+    float* k_scale;
+    float* v_scale;
+    uint16_t* k_open;
+    uint16_t* v_open;
+    int n_seq;
+    int max_ctx;
+    int n_kv;
+    int head_dim;
+    int format;
+} iam_kv8_cache;
+
+/* Bytes of each part: k (and v), k_scale (and v_scale), k_open (and v_open). */
+int iam_kv8_size(int n_seq, int max_ctx, int n_kv, int head_dim, size_t* numbers, size_t* scales,
+                 size_t* open);
+/* Marks every block as not full.  Once, before the first append; a slot whose
+ * sequence is over is used again by appending from position 0. */
+int iam_kv8_reset(iam_ctx* ctx, const iam_kv8_cache* cache);
+/* Writes n_tokens tokens of each sequence, k and v [n_seq][n_tokens] rows of
+ * n_kv * head_dim values (of the type), kv_stride values apart (0: n_kv *
+ * head_dim), at positions pos_dev[s] and on.  count_dev, if not null, says
+ * how many of sequence s's tokens are there (the rest of a padded batch is
+ * not read).  Tokens at or past max_ctx are dropped; a negative position
+ * skips its sequence.  A sequence is appended to in order; going back (as
+ * after rejected draft tokens) is allowed: where the position lies inside a
+ * full block, the block's earlier tokens become open again as the values
+ * that it stands for, rounded to fp16. */
+int iam_kv8_append(iam_ctx* ctx, const iam_kv8_cache* cache, const void* k_dev, const void* v_dev, int type,
+                   int n_tokens, size_t kv_stride, const int* pos_dev, const int* count_dev);
+/* The values that positions pos_dev[s] .. pos_dev[s] + n_tokens - 1 stand for,
+ * as fp32 rows [n_seq][n_tokens][n_kv][head_dim].  Rows of positions outside
+ * [0, max_ctx) are left as they were; what a position holds that was never
+ * written is undefined. */
+int iam_kv8_read(iam_ctx* ctx, const iam_kv8_cache* cache, const int* pos_dev, int n_tokens, float* k_out_dev,
+                 float* v_out_dev);
+/* Attention of n_tokens consecutive tokens of each sequence over its cache
+ * (which holds them already): q and out [n_seq][n_tokens] rows of n_heads *
+ * head_dim values (of the type), q_stride / out_stride values apart (0: n_heads
+ * * head_dim).  Token t of sequence s is at position p = pos_dev[s] + t (past
+ * max_ctx: taken as max_ctx - 1) and sees positions 0 .. p, or the last
+ * `window` of them if window > 0.  Query head h reads KV head h * n_kv /
+ * n_heads.  The softmax takes scale * q.k (scale 0: 1 / sqrt(head_dim)).
+ * Sums and the softmax in fp32 (the products of an fp32 q and of the
+ * probabilities to 22 bits), one rounding to the type.  Sequences with a negative position give rows of zeros;
+ * rows of tokens from count_dev[s] on (if not null) are left as they were.  An
+ * infinity or a NaN makes the rows that see it NaN or infinite; in a full
+ * block, all rows that see any token of the block's head.  out may be q
+ * with the same stride. */
+int iam_attention_kv8(iam_ctx* ctx, const iam_kv8_cache* cache, const void* q_dev, int type, int n_heads,
+                      int n_tokens, size_t q_stride, const int* pos_dev, const int* count_dev, int window,
+                      float scale, void* out_dev, size_t out_stride);
+
+/* Log probabilities under softmax(row) of n_rows rows of `vocab` logits, `stride`
+ * values apart (0: vocab): logprob_dev[r] of token targets_dev[r] (0 for a
+ * target outside [0, vocab), the padding of a batch), entropy_dev[r] (may be
+ * null) and, for top_k > 0, the top_k most likely tokens, likeliest first,
+ * equal logits by the lower token: top_ids_dev and top_logprobs_dev
+ * [n_rows][top_k] (top_k at most min(vocab, 64); either may be null).
+ * Sums in fp64, one rounding to fp32.  A row of nothing but -inf gives -inf
+ * and the entropy 0; a row with a NaN or +inf gives NaN for both and for the
+ * alternatives' log probabilities (their tokens are ordered with NaN last). */
+#define IAM_LOGPROBS_MAX_TOP 64
+int iam_token_logprobs(iam_ctx* ctx, const void* logits_dev, int type, int n_rows, int vocab, size_t stride,
+                       const int* targets_dev, float* logprob_dev, float* entropy_dev, int top_k,
+                       int* top_ids_dev, float* top_logprobs_dev);
+
 /* -------------------------------------------------------- synthetic data */
 
 /* Counter-based generator shared with the CPU oracle: element n of tensor

@@ -119,6 +119,18 @@ struct Ctx {
     // and position, the splits' sums and partial outputs
     float* attn32 = nullptr;
     size_t attn32_cap = 0;
+    // attention over the 8-bit cache: partial results of its workgroups and
+    // the arrival counters (zero between calls)
+    float* kv8_part = nullptr;
+    size_t kv8_part_cap = 0;
+    uint32_t* kv8_ctr = nullptr;
+    size_t kv8_ctr_cap = 0;
+    // token log probabilities: the segments' results and arrival counters
+    // (zero between calls)
+    double* lp_part = nullptr;
+    size_t lp_part_cap = 0;
+    uint32_t* lp_ctr = nullptr;
+    size_t lp_ctr_cap = 0;
     // bumped whenever a context-owned scratch buffer is reallocated:
     // captured graphs hold those addresses and must be re-captured
     uint64_t scratch_gen = 0;
@@ -311,6 +323,10 @@ int bucketmul_fused(Ctx* c, int n, const MatOp* ops, int expert_no, float effort
                     const uint16_t* gain, float eps);
 int ensure_attn_scratch(Ctx* c, size_t acc_words, int n_heads);
 int ensure_attn32_scratch(Ctx* c, size_t floats);
+// attention over the 8-bit cache: floats of partial results, arrival counters
+int ensure_kv8_scratch(Ctx* c, size_t floats, size_t counters);
+// token log probabilities: doubles of partial results, arrival counters
+int ensure_lp_scratch(Ctx* c, size_t doubles, size_t counters);
 
 int quantile_of(float effort);
 double est_rows(int rows, float effort);

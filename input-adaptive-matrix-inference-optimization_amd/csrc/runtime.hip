@@ -148,6 +148,18 @@ int ensure_attn_scratch(Ctx* c, size_t acc_words, int n_heads)
     return grow_zeroed(c, (void**)&c->attn_ctr, &cap, kCounters, sizeof(uint32_t), "attention counter");
 }
 
+int ensure_kv8_scratch(Ctx* c, size_t floats, size_t counters)
+{
+    IAM_TRY(grow_zeroed(c, (void**)&c->kv8_part, &c->kv8_part_cap, floats, sizeof(float), "kv8 attention partials"));
+    return grow_zeroed(c, (void**)&c->kv8_ctr, &c->kv8_ctr_cap, counters, sizeof(uint32_t), "kv8 attention counter");
+}
+
+int ensure_lp_scratch(Ctx* c, size_t doubles, size_t counters)
+{
+    IAM_TRY(grow_zeroed(c, (void**)&c->lp_part, &c->lp_part_cap, doubles, sizeof(double), "logprobs partials"));
+    return grow_zeroed(c, (void**)&c->lp_ctr, &c->lp_ctr_cap, counters, sizeof(uint32_t), "logprobs counter");
+}
+
 int begin_launch(Ctx* c, const char* name, PendingEvent* ev)
 {
     for (int i = 0; i < 2; i++) {

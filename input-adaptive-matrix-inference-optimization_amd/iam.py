@@ -44,6 +44,35 @@ class ModelConfig(C.Structure):
                 ("norm_eps", C.c_float)]
 
 
+class RopeScaling(C.Structure):
+    _fields_ = [("kind", C.c_int), ("factor", C.c_double), ("original_ctx", C.c_double), ("low", C.c_double),
+                ("high", C.c_double), ("magnitude", C.c_double)]
+
+
+class Kv8Desc(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("k_open", C.c_void_p), ("v_open", C.c_void_p), ("n_seq", C.c_int), ("max_ctx", C.c_int),
+                ("n_kv", C.c_int), ("head_dim", C.c_int), ("format", C.c_int)]
+
+
+# number types of activations, rotary layouts and scalings, cache formats
+TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "base": 2, "bands": 3, "ramp": 4}
+KV8_FORMATS = {"int8": 0, "e4m3": 1}
+KV8_BLOCK = 64
+
+# the argument types of the calls that a serving loop makes for each token
+_P, _I, _Z, _F = C.c_void_p, C.c_int, C.c_size_t, C.c_float
+_ARGTYPES = {
+    "iam_rope_tokens": [_P, _P, _I, _I, _I, _I, _I, _I, _Z, _P, _I, _P, _P, _Z],
+    "iam_kv8_append": [_P, _P, _P, _P, _I, _I, _Z, _P, _P],
+    "iam_kv8_read": [_P, _P, _P, _I, _P, _P],
+    "iam_attention_kv8": [_P, _P, _P, _I, _I, _I, _Z, _P, _P, _I, _F, _P, _Z],
+    "iam_token_logprobs": [_P, _P, _I, _I, _I, _Z, _P, _P, _P, _I, _P, _P],
+}
+
+
 def lib():
     global _lib
     if _lib is None:
@@ -53,6 +82,8 @@ def lib():
         L.iam_last_error.restype = C.c_char_p
         L.iam_effort_quantile.restype = C.c_int
         L.iam_effort_quantile.argtypes = [C.c_float]
+        for name, types in _ARGTYPES.items():
+            getattr(L, name).argtypes = types
         _lib = L
     return _lib
 
@@ -76,6 +107,11 @@ def header_symbols(path=HEADER):
 
 def _vp(x):
     return C.c_void_p(x if isinstance(x, int) else x.ptr)
+
+
+def _ptr(x):
+    """The device address of a buffer, of an address, or of nothing."""
+    return x if x is None or isinstance(x, int) else x.ptr
 
 
 class DevBuf:
@@ -359,6 +395,33 @@ class Ctx:
     def argmax(self, v, n, out_dev):
         check(lib().iam_argmax(self.h, _vp(v), n, _vp(out_dev)))
 
+    # ---- long contexts, scored tokens
+    def rope_scaled_table(self, theta, rot_dim, max_pos, table, scaling=None):
+        """The (cos, sin) table of rope_tokens, angles in fp64.  scaling: None or
+        {"kind": "linear" | "base" | "bands" | "ramp", "factor": ...,
+        "original_ctx", "low", "high", "magnitude": ...}."""
+        s = None
+        if scaling is not None:
+            d = dict(scaling)
+            s = RopeScaling(ROPE_SCALINGS[d.pop("kind")], **d)
+        check(lib().iam_rope_scaled_table(self.h, C.c_double(theta), rot_dim, max_pos,
+                                          C.byref(s) if s is not None else None, _vp(table)))
+
+    def rope_tokens(self, x, type, n_tokens, n_heads, head_dim, rot_dim, layout, table, max_pos, pos, out,
+                    x_stride=0, out_stride=0):
+        """Rotary positions of n_tokens rows of heads (type "f32", "f16" or
+        "bf16"; layout "half" or "interleaved")."""
+        check(lib().iam_rope_tokens(self.h, _ptr(x), TYPES[type], n_tokens, n_heads, head_dim, rot_dim,
+                                    ROPE_LAYOUTS[layout], x_stride, _ptr(table), max_pos, _ptr(pos), _ptr(out),
+                                    out_stride))
+
+    def token_logprobs(self, logits, type, n_rows, vocab, targets, logprob, entropy=None, top_k=0, top_ids=None,
+                       top_logprobs=None, stride=0):
+        """Log probabilities of given tokens, the entropy and the top_k
+        alternatives of each row of logits."""
+        check(lib().iam_token_logprobs(self.h, _ptr(logits), TYPES[type], n_rows, vocab, stride, _ptr(targets),
+                                       _ptr(logprob), _ptr(entropy), top_k, _ptr(top_ids), _ptr(top_logprobs)))
+
     # ---- synthetic data
     def gen_f16(self, seed, tid, count, mean, sigma, out):
         check(lib().iam_gen_f16(self.h, C.c_uint64(seed), C.c_uint64(tid), C.c_size_t(count),
@@ -380,6 +443,51 @@ def rope_table(theta, head_dim, max_pos):
 
 def effort_quantile(effort):
     return lib().iam_effort_quantile(C.c_float(effort))
+
+
+class Kv8Cache:
+    """A KV cache in 8 bits (format "int8" or "e4m3"; a scale for each 64 tokens
+    and KV head, the open block in fp16) and the attention over it."""
+
+    def __init__(self, ctx, n_seq, max_ctx, n_kv, head_dim, format="int8"):
+        self.ctx = ctx
+        numbers, scales, opened = C.c_size_t(), C.c_size_t(), C.c_size_t()
+        check(lib().iam_kv8_size(n_seq, max_ctx, n_kv, head_dim, C.byref(numbers), C.byref(scales), C.byref(opened)))
+        self.parts = []
+        try:
+            for n, dt in ((numbers, np.uint8), (scales, np.float32), (opened, np.uint16)):
+                for _ in range(2):
+                    self.parts.append(DevBuf(ctx, n.value, dt))
+        except IamError:
+            self.free()
+            raise
+        self.desc = Kv8Desc(*[b.ptr for b in self.parts], n_seq, max_ctx, n_kv, head_dim, KV8_FORMATS[format])
+        self._at = C.addressof(self.desc)
+        self.reset()
+
+    def free(self):
+        for b in self.parts:
+            b.free()
+
+    def reset(self):
+        check(lib().iam_kv8_reset(self.ctx.h, C.byref(self.desc)))
+
+    def append(self, k, v, type, n_tokens, pos, count=None, stride=0):
+        """n_tokens tokens of each sequence at pos[s] and on (device int32s);
+        count[s] of them where given."""
+        check(lib().iam_kv8_append(self.ctx.h, self._at, _ptr(k), _ptr(v), TYPES[type], n_tokens, stride, _ptr(pos),
+                                   _ptr(count)))
+
+    def read(self, pos, n_tokens, k_out, v_out):
+        """What positions pos[s] .. pos[s] + n_tokens - 1 stand for, in fp32 rows."""
+        check(lib().iam_kv8_read(self.ctx.h, self._at, _ptr(pos), n_tokens, _ptr(k_out), _ptr(v_out)))
+
+    def attention(self, q, type, n_heads, n_tokens, pos, out, count=None, window=0, scale=0.0, q_stride=0,
+                  out_stride=0):
+        """Attention of the n_tokens tokens at pos[s] and on over what each
+        sequence's cache holds up to them."""
+        check(lib().iam_attention_kv8(self.ctx.h, self._at, _ptr(q), TYPES[type], n_heads, n_tokens, q_stride,
+                                      _ptr(pos), _ptr(count), window, scale, _ptr(out), out_stride))
 
 
 class Model:
