@@ -7,6 +7,7 @@
 // in one pass with the running maximum m[r] of the rows, o / l at the end.
 #include <cmath>
 
+#include "accum.h"
 #include "kv8.h"
 #include "wave.h"
 
@@ -168,6 +169,23 @@ __device__ __forceinline__ void store_row4(void* o, size_t at, floatx4 v)
 #pragma unroll
     for (int e = 0; e < 4; e++) r.v[e] = from_f32<T>(v[e]);
     *reinterpret_cast<Pack<T, 4, (int)sizeof(T)>*>(reinterpret_cast<T*>(o) + at) = r;
+}
+
+// four floats handed to another workgroup (two 8-byte words)
+__device__ __forceinline__ void put4(float* p, floatx4 v)
+{
+    typedef unsigned long long ull2 __attribute__((ext_vector_type(2)));
+    const ull2 u = __builtin_bit_cast(ull2, v);
+    acc_put(reinterpret_cast<unsigned long long*>(p), u[0]);
+    acc_put(reinterpret_cast<unsigned long long*>(p) + 1, u[1]);
+}
+__device__ __forceinline__ floatx4 peek4(float* p)
+{
+    typedef unsigned long long ull2 __attribute__((ext_vector_type(2)));
+    ull2 u;
+    u[0] = acc_peek(reinterpret_cast<unsigned long long*>(p));
+    u[1] = acc_peek(reinterpret_cast<unsigned long long*>(p) + 1);
+    return __builtin_bit_cast(floatx4, u);
 }
 
 // SPLIT: q is fp32, in two parts.  NT: tiles of 16 query rows an item has.
@@ -475,38 +493,33 @@ __global__ __launch_bounds__(kAttn8Threads) void k_kv8_attn(Attn8Args a)
 #pragma unroll
             for (int q = 1; q < NT; q++) tot = n == q ? sum[q] : tot;
             if (whole) put(n, d, x, tot);
-            else reinterpret_cast<floatx4*>(part)[(n * DT + d) * 64 + lane] = x;
+            else put4(part + ((n * DT + d) * 64 + lane) * 4, x);
         }
     }
     if (whole) return;
     if (w == 0 && g == 0)
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            part[R * HD + n * 16 + r16] = big[n];
-            part[R * HD + R + n * 16 + r16] = sum[n];
+            acc_put(part + R * HD + n * 16 + r16, big[n]);
+            acc_put(part + R * HD + R + n * 16 + r16, sum[n]);
         }
     // the last of the item's workgroups to arrive joins their results
-    __threadfence();
-    __syncthreads();
     uint32_t* ctr = a.ctr + (size_t)sh.item * a.g.n_kv + kvh;
-    if (tid == 0) s_last = atomicAdd(ctr, 1u) == (uint32_t)(sh.splits - 1);
-    __syncthreads();
-    if (!s_last) return;
-    __threadfence();
-    const float* parts = a.part + ((size_t)sh.slot0 * a.g.n_kv + kvh) * kPartWords;
+    if (!acc_arrive(ctr, (uint32_t)sh.splits, &s_last)) return;
+    float* parts = a.part + ((size_t)sh.slot0 * a.g.n_kv + kvh) * kPartWords;
     const size_t step = (size_t)a.g.n_kv * kPartWords;
 #pragma unroll 1
     for (int nd = w; nd < NT * DT; nd += kAttn8Waves) {
         const int n = nd / DT, row = n * 16 + r16;
         float t = -INFINITY;
-        for (int k = 0; k < sh.splits; k++) t = fmaxf(t, parts[k * step + R * HD + row]);
+        for (int k = 0; k < sh.splits; k++) t = fmaxf(t, acc_peek(parts + k * step + R * HD + row));
         const float safe = t == -INFINITY ? 0.0f : t;
         float tot = 0.0f;
         floatx4 x = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
         for (int k = 0; k < sh.splits; k++) {
-            const float f = __builtin_amdgcn_exp2f(parts[k * step + R * HD + row] - safe);
-            tot += parts[k * step + R * HD + R + row] * f;
-            x += reinterpret_cast<const floatx4*>(parts + k * step)[nd * 64 + lane] * f;
+            const float f = __builtin_amdgcn_exp2f(acc_peek(parts + k * step + R * HD + row) - safe);
+            tot += acc_peek(parts + k * step + R * HD + R + row) * f;
+            x += peek4(parts + k * step + (nd * 64 + lane) * 4) * f;
         }
         put(n, nd - n * DT, x, tot);
     }

@@ -3,6 +3,7 @@
 //
 // With m the row's maximum, z = sum e^(x - m) and s = sum e^(x - m) (x - m):
 //   log p(t) = x_t - m - log z,   entropy = log z - s / z.
+#include "accum.h"
 #include "numbers.h"
 #include "wave.h"
 
@@ -250,26 +251,21 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
         const int words = 3 + a.k;
         double* mine = a.part + ((size_t)row * a.segs + seg) * words;
         if (tid == 0) {
-            mine[0] = (double)m;
-            mine[1] = z;
-            mine[2] = s;
+            acc_put(mine, (double)m);
+            acc_put(mine + 1, z);
+            acc_put(mine + 2, s);
         }
         if constexpr (TOP)
             for (int i = tid; i < a.k; i += kLpThreads)
-                reinterpret_cast<uint64_t*>(mine)[3 + i] = i < best.have ? best.keys[i] : 0;
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) s_last = atomicAdd(a.ctr + row, 1u) == (uint32_t)(a.segs - 1);
-        __syncthreads();
-        if (!s_last) return;
-        __threadfence();
-        const double* parts = a.part + (size_t)row * a.segs * words;
+                acc_put(reinterpret_cast<unsigned long long*>(mine) + 3 + i, i < best.have ? best.keys[i] : 0);
+        if (!acc_arrive(a.ctr + row, (uint32_t)a.segs, &s_last)) return;
+        double* parts = a.part + (size_t)row * a.segs * words;
         m = -INFINITY;
         z = s = 0.0;
         if (tid < a.segs) {
-            m = (float)parts[tid * words];
-            z = parts[tid * words + 1];
-            s = parts[tid * words + 2];
+            m = (float)acc_peek(parts + tid * words);
+            z = acc_peek(parts + tid * words + 1);
+            s = acc_peek(parts + tid * words + 2);
         }
         lp_join(m, z, s, redf, redd);
         if constexpr (TOP) {
@@ -283,7 +279,7 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
                 for (int e = 0; e < N; e++) {
                     const int i = i0 + e * kLpThreads + tid;
                     y[e] = i < a.segs * a.k
-                               ? reinterpret_cast<const uint64_t*>(parts)[(size_t)(i / a.k) * words + 3 + i % a.k]
+                               ? acc_peek(reinterpret_cast<unsigned long long*>(parts) + (size_t)(i / a.k) * words + 3 + i % a.k)
                                : 0;
                 }
                 best.template offer<N>([&](int e) __attribute__((always_inline)) { return y[e]; }, true);
