@@ -26,8 +26,9 @@ namespace iam {
 // low (22 bits), after a power of two that brings them near the top of fp16's
 // range, and both are multiplied (an fp16 or bf16 q needs one part).
 constexpr int kAttn8Threads = 256, kAttn8Waves = 4;
-constexpr int kAlone = 24;            // blocks that one workgroup takes by itself: joining costs more
-constexpr int kMinBlocks = 8;         // blocks of a workgroup where an item is split
+constexpr int kAlone = 2 * kAttn8Waves;   // blocks that one workgroup takes by itself: joining costs 4 us
+constexpr int kMinBlocks = 8;         // blocks of a workgroup where an item is split,
+constexpr int kFewParts = 16;         // or 4 while that makes no more parts than these (read in one go when joined)
 constexpr int kMaxItems = 2048;       // items up to which they are dealt out by length
 constexpr float kProbShift = 12.0f;   // p is held as 2^12 p: its low part stays a normal number
 
@@ -63,11 +64,14 @@ struct Span {
     int p0;
 };
 
+// the token of row `row` of a sequence (no division for single tokens)
+__device__ __forceinline__ int token_of(const Attn8Args& a, int row) { return a.tokens == 1 ? 0 : row / a.rep; }
+
 // what item `it` has to read
 __device__ __forceinline__ Span span_of(const Attn8Args& a, int it, int rows_per_item)
 {
     Span s;
-    s.seq = it / a.groups;
+    s.seq = a.groups == 1 ? it : it / a.groups;
     s.first_row = (it - s.seq * a.groups) * rows_per_item;
     s.p0 = a.pos[s.seq];
     const int n = a.count ? min(a.tokens, a.count[s.seq]) : a.tokens;
@@ -75,7 +79,7 @@ __device__ __forceinline__ Span span_of(const Attn8Args& a, int it, int rows_per
     s.b0 = s.nb = 0;
     if (s.n_rows > 0 && s.p0 >= 0) {
         const int top = a.g.max_ctx - 1;
-        const int t0 = s.first_row / a.rep, t1 = (s.first_row + s.n_rows - 1) / a.rep;
+        const int t0 = token_of(a, s.first_row), t1 = token_of(a, s.first_row + s.n_rows - 1);
         const int hi = s.p0 > top - t1 ? top : s.p0 + t1, lo_p = s.p0 > top - t0 ? top : s.p0 + t0;
         const int lo = a.window > 0 ? max(0, lo_p - a.window + 1) : 0;
         s.b0 = lo / kBlk;
@@ -125,7 +129,12 @@ struct Deal {
 };
 
 __device__ __forceinline__ int up_div(int x, int y) { return (int)((unsigned)(x + y - 1) / (unsigned)y); }
-__device__ __forceinline__ int parts_of(int nb, int G) { return nb <= kAlone ? 1 : up_div(nb, G); }
+// G: kAttn8Waves where the card has workgroups to spare, else kMinBlocks or more
+__device__ __forceinline__ int parts_of(int nb, int G)
+{
+    if (nb <= kAlone) return 1;
+    return G > kAttn8Waves ? up_div(nb, G) : min(up_div(nb, kAttn8Waves), max(kFewParts, up_div(nb, kMinBlocks)));
+}
 
 // pre: LDS [items + 1], the items' blocks before each; false: no work
 __device__ __forceinline__ bool find_deal(const Attn8Args& a, int j, int rows_per_item, int* pre, Deal& d)
@@ -150,7 +159,8 @@ __device__ __forceinline__ bool find_deal(const Attn8Args& a, int j, int rows_pe
         __syncthreads();
     }
     const int spare = a.target - a.items;
-    const int G = spare > 0 ? max(kMinBlocks, up_div(total, spare)) : 0;
+    const int need = spare > 0 ? up_div(total, spare) : 0;   // with parts of this many blocks all fit
+    const int G = need <= kAttn8Waves ? kAttn8Waves : max(kMinBlocks, need);
     d.mode = spare > 0 && (G <= 2 * kMinBlocks || a.items <= a.target / 8) ? 0 : 1;
     if (d.mode == 0 && a.items == 1) {
         const int n = parts_of(total, G);
@@ -381,7 +391,7 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
         if (sp.n_rows > 0) {
             // positions that every row there sees: below lo_all and past hi_all a mask is needed
             const int top_ctx = a.g.max_ctx - 1;
-            const int t_first = sp.first_row / a.rep, t_last = (sp.first_row + sp.n_rows - 1) / a.rep;
+            const int t_first = token_of(a, sp.first_row), t_last = token_of(a, sp.first_row + sp.n_rows - 1);
             const int hi_all = sp.p0 > top_ctx - t_first ? top_ctx : sp.p0 + t_first;
             const int hi_max = sp.p0 > top_ctx - t_last ? top_ctx : sp.p0 + t_last;
             const int lo_all = a.window > 0 ? max(0, hi_max - a.window + 1) : 0;
@@ -403,7 +413,7 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
             for (int n = 0; n < NT; n++) {
                 const int row = sp.first_row + n * 16 + r16;
                 const bool there = n * 16 + r16 < sp.n_rows;
-                const int t = there ? row / a.rep : 0, head = kvh * a.rep + (there ? row - t * a.rep : 0);
+                const int t = there ? token_of(a, row) : 0, head = kvh * a.rep + (there ? row - t * a.rep : 0);
                 hi[n] = there && sp.p0 >= 0 ? (sp.p0 > top_ctx - t ? top_ctx : sp.p0 + t) : -1;
                 lo[n] = a.window > 0 ? max(0, hi[n] - a.window + 1) : 0;
                 const size_t at = (qrow0 + t) * a.q_stride + (size_t)head * HD;
@@ -424,9 +434,12 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
                 }
             }
             int b = bs + w;
+            float ksc = 0.0f, vsc = 0.0f;   // the scales of block b
             if (b < be) {   // (an open block's bytes are not looked at)
                 fetch_tile<RUNS, NT == 1>(a.kt + cell_of(b) * (size_t)TILE, place_k);
                 fetch_tile<RUNS, NT == 1>(a.vt + cell_of(b) * (size_t)TILE, place_v);
+                ksc = a.ks[cell_of(b)];
+                vsc = a.vs[cell_of(b)];
             }
 #pragma unroll
             for (int n = 0; n < NT; n++) {
@@ -531,7 +544,11 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
             while (b < bend) {
                 const int next = b + sh.stride;
                 const bool more = next < bend;
-                const float kscale = a.ks[cell_of(b)], vscale = a.vs[cell_of(b)];
+                const float kscale = ksc, vscale = vsc;
+                if (more) {
+                    ksc = a.ks[cell_of(next)];
+                    vsc = a.vs[cell_of(next)];
+                }
                 u32x4 run[RUNS];
                 read_tile<RUNS>(at_k, true, run);      // the V tile is younger
                 if (more) fetch_tile<RUNS, NT == 1>(a.kt + cell_of(next) * (size_t)TILE, place_k);
@@ -666,7 +683,7 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
 
             // four values of row `row` of the item, from dimension d on, to out
             auto put = [&](int row, int d, floatx4 x, float total) __attribute__((always_inline)) {
-                const int rr = sp.first_row + row, t = rr / a.rep, head = kvh * a.rep + rr - t * a.rep;
+                const int rr = sp.first_row + row, t = token_of(a, rr), head = kvh * a.rep + rr - t * a.rep;
                 const size_t at = (qrow0 + t) * a.out_stride + (size_t)head * HD + d;
                 // nothing seen: zeros
 #pragma unroll
@@ -802,7 +819,7 @@ static int attn8_launch(Ctx* c, Attn8Args a)
     int64_t per_head = items;
     if (a.planned) {
         per_head = a.target;
-        const int most = (kv8_blocks(a.g.max_ctx) + kMinBlocks - 1) / kMinBlocks;   // parts that an item can have
+        const int most = (kv8_blocks(a.g.max_ctx) + kAttn8Waves - 1) / kAttn8Waves;   // parts that an item can have
         if (items <= a.target / 8) per_head = std::min<int64_t>(per_head, items * most);
         IAM_TRY(ensure_kv8_scratch(c, 2 * (size_t)per_head * a.g.n_kv * (R * HD + 2 * R), (size_t)items * a.g.n_kv));
         a.part = c->kv8_part;
