@@ -42,97 +42,72 @@ __device__ __forceinline__ float key_value(uint64_t k)
     return o == 0u ? NAN : __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o);
 }
 
-// The best k keys offered so far by the workgroup's threads.  `keys` holds at
-// most cap = 33 k of them; `floor` is a key that k others are known to reach:
-// lower ones are not taken.  A thread offers N keys at a time.  Too many at
-// once (as in a row's first chunk): the k-th best of the threads' own best
-// keys becomes the floor, which leaves at most k threads with N <= 32 keys each.
-struct Best {
-    uint64_t* keys;       // LDS [cap]
-    uint64_t* own;        // LDS [kLpThreads]
-    uint64_t* floor_p;    // LDS
-    int* count;           // LDS
-    int k, cap;
-    int have = 0;         // uniform
-    uint64_t floor = 0;   // uniform: keys above it are taken
+// ---- the best k of a row's (or segment's) values
+// The k-th largest of the threads' own maxima bounds the k-th largest value
+// from below, and at most k threads (and ties) reach it: only their values are
+// looked at again, so that the pass over the logits itself needs no exchange.
+constexpr int kLpCap = 1024;    // keys held at a time
 
-    __device__ __forceinline__ void start()
-    {
-        if (threadIdx.x == 0) *count = 0;
-        __syncthreads();
-    }
-    // keeps the best k, in order
-    __device__ void prune()
-    {
-        uint64_t mine[9];
-        int rank[9];
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < 9; u++) {
-            const int i = (int)threadIdx.x + u * kLpThreads;
-            mine[u] = i < have ? keys[i] : 0;
-            rank[u] = 0;
-        }
-        for (int j = 0; j < have; j++) {
-            const uint64_t y = keys[j];
-#pragma unroll
-            for (int u = 0; u < 9; u++) rank[u] += y > mine[u];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < 9; u++)
-            if (mine[u] != 0 && rank[u] < k) keys[rank[u]] = mine[u];
-        have = min(have, k);
-        if (threadIdx.x == 0) *count = have;
-        __syncthreads();
-        if (have == k && keys[k - 1] > floor) floor = keys[k - 1];
-    }
-    template <int N, typename Key>
-    __device__ void offer(Key key, bool hot)
-    {
-        if (!__syncthreads_or(hot)) return;
-        int c = 0;
-#pragma unroll
-        for (int e = 0; e < N; e++) c += hot && key(e) > floor;
-        int at = c ? atomicAdd(count, c) : 0;
-        __syncthreads();
-        int total = *count;
-        if (total > cap) {
-            __syncthreads();
-            prune();      // also takes back the count
-            uint64_t b = 0;
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const uint64_t y = hot ? key(e) : 0;
-                b = y > b ? y : b;
-            }
-            own[threadIdx.x] = b;
-            if (threadIdx.x == 0) *floor_p = 0;
-            __syncthreads();
-            int rank = 0;
-            for (int j = 0; j < kLpThreads; j++) rank += own[j] > b;
-            if (b != 0 && rank == k - 1) *floor_p = b - 1;
-            __syncthreads();
-            if (*floor_p > floor) floor = *floor_p;
-            c = 0;
-#pragma unroll
-            for (int e = 0; e < N; e++) c += hot && key(e) > floor;
-            at = c ? atomicAdd(count, c) : 0;
-            __syncthreads();
-            total = *count;
-        }
-        if (c) {
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const uint64_t y = key(e);
-                if (y > floor && at < cap) keys[at++] = y;
-            }
-        }
-        have = min(total, cap);
-        __syncthreads();
-        if (have > 3 * k + 32) prune();
-    }
+struct Top {
+    uint64_t* keys;     // LDS [kLpCap]
+    uint64_t* own;      // LDS [kLpThreads]: the threads' maxima; places of the list's keys
+    int* n;             // LDS: keys there (may pass kLpCap: then only the first are)
 };
+
+// how many of the 256 keys of own[] are larger than y
+__device__ __forceinline__ int larger(const uint64_t* own, uint64_t y)
+{
+    int r = 0;
+#pragma unroll 8
+    for (int i = 0; i < kLpThreads; i++) r += own[i] > y;
+    return r;
+}
+
+// Orders the n <= kLpCap distinct keys of t.keys; the best min(k, n) end up in
+// order in front.  Where there are many, the k-th best of the threads' best
+// keys first thins them out.
+__device__ void lp_order(const Top& t, int n, int k)
+{
+    const int tid = threadIdx.x;
+    constexpr int U = kLpCap / kLpThreads;
+    uint64_t mine[U];
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; u++) mine[u] = tid + u * kLpThreads < n ? t.keys[tid + u * kLpThreads] : 0;
+    if (n > 128) {
+        uint64_t b = 0;
+#pragma unroll
+        for (int u = 0; u < U; u++) b = mine[u] > b ? mine[u] : b;
+        t.own[tid] = b;
+        __syncthreads();
+        const int r = larger(t.own, b);
+        __syncthreads();
+        // the keys of the k threads with the largest ones go on, a place each
+        // (0: none)
+        if (r < k) {
+#pragma unroll
+            for (int u = 0; u < U; u++) t.keys[r * U + u] = mine[u];
+        }
+        n = min(k, kLpThreads) * U;
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; u++) mine[u] = tid + u * kLpThreads < n ? t.keys[tid + u * kLpThreads] : 0;
+        __syncthreads();
+    }
+    int rank[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) rank[u] = 0;
+    for (int i = 0; i < n; i++) {
+        const uint64_t y = t.keys[i];
+#pragma unroll
+        for (int u = 0; u < U; u++) rank[u] += y > mine[u];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if (mine[u] != 0 && rank[u] < k) t.keys[rank[u]] = mine[u];
+    __syncthreads();
+}
 
 __device__ __forceinline__ double lp_sum(double v, double* red)
 {
@@ -170,35 +145,170 @@ __device__ __forceinline__ void lp_join(float& m, double& z, double& s, float* r
     m = M;
 }
 
+// VEC values from place i on; past v1, -inf
+template <typename T, int VEC>
+__device__ __forceinline__ void lp_load(const T* x, int i, int v1, float* v)
+{
+    if (i + VEC <= v1) {
+        const Pack<T, VEC, (int)sizeof(T)> r = *reinterpret_cast<const Pack<T, VEC, (int)sizeof(T)>*>(x + i);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) v[e] = to_f32(r.v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) v[e] = i + e < v1 ? to_f32(x[i + e]) : -INFINITY;
+    }
+}
+
+// The values of [v0, v1) that take(value) says, as keys behind the n there,
+// from the threads that `hot` lists (nh of them); t.n counts them all.
+template <typename T, int VEC, typename Take>
+__device__ __forceinline__ void lp_gather(const Top& t, const T* x, int v0, int v1, const int* hot, int nh, Take take)
+{
+    const int rounds = (v1 - v0 + kLpThreads * VEC - 1) / (kLpThreads * VEC);
+    for (int i0 = 0; i0 < rounds * nh; i0 += kLpThreads) {
+        const int q = i0 + (int)threadIdx.x;
+        if (q >= rounds * nh || *(volatile int*)t.n > kLpCap) continue;
+        const int r = q / nh, i = v0 + (r * kLpThreads + hot[q - r * nh]) * VEC;
+        float v[VEC];
+        lp_load<T, VEC>(x, i, v1, v);
+        int c = 0;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) c += i + e < v1 && take(v[e]);
+        if (!c) continue;
+        int at = atomicAdd(t.n, c);
+#pragma unroll
+        for (int e = 0; e < VEC; e++)
+            if (i + e < v1 && take(v[e])) {
+                if (at < kLpCap) t.keys[at] = key_of(v[e], i + e);
+                at++;
+            }
+    }
+    __syncthreads();
+}
+
+// The first `want` values of [v0, v1), by place, that take(value) says, as keys
+// behind the n there; how many there were
+template <typename T, int VEC, typename Take>
+__device__ int lp_first(const Top& t, const T* x, int v0, int v1, int n, int want, Take take)
+{
+    __shared__ int wsum[kLpWaves];
+    int got = 0;
+    for (int c0 = v0; c0 < v1 && got < want; c0 += kLpThreads * VEC) {
+        const int i = c0 + (int)threadIdx.x * VEC;
+        float v[VEC];
+        lp_load<T, VEC>(x, i, v1, v);
+        int c = 0;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) c += i + e < v1 && take(v[e]);
+        const int incl = wave_incl_sum(c), w = threadIdx.x >> 6;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 63) wsum[w] = incl;
+        __syncthreads();
+        int at = got + incl - c, all = 0;
+#pragma unroll
+        for (int u = 0; u < kLpWaves; u++) {
+            at += u < w ? wsum[u] : 0;
+            all += wsum[u];
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; e++)
+            if (i + e < v1 && take(v[e])) {
+                if (at < want) t.keys[n + at] = key_of(v[e], i + e);
+                at++;
+            }
+        got += all;
+    }
+    __syncthreads();
+    return min(got, want);
+}
+
+// The best min(k, v1 - v0) keys of [v0, v1) in order in front of t.keys; m: the
+// largest value of the thread's own loads (its place in every 256 * VEC).
+template <typename T, int VEC>
+__device__ int lp_top(const Top& t, int* hot, float* bound, const T* x, int v0, int v1, float m, int k)
+{
+    const int tid = threadIdx.x, have = min(k, v1 - v0);
+    // distinct: equal maxima by thread
+    const uint64_t mine = key_of(m, tid);
+    __syncthreads();
+    t.own[tid] = mine;
+    if (tid == 0) t.n[0] = t.n[1] = 0;
+    __syncthreads();
+    if (larger(t.own, mine) == k - 1) *bound = m;
+    __syncthreads();
+    const float b = *bound;
+    if (m >= b) hot[atomicAdd(t.n + 1, 1)] = tid;
+    __syncthreads();
+    const int nh = t.n[1];
+    lp_gather<T, VEC>(t, x, v0, v1, hot, nh, [&](float v) { return v >= b; });
+    int n = t.n[0];
+    if (n > kLpCap) {
+        // many equal values (a masked row's -inf): the larger ones, then the
+        // first of the equal ones
+        __syncthreads();
+        if (tid == 0) t.n[0] = 0;
+        __syncthreads();
+        lp_gather<T, VEC>(t, x, v0, v1, hot, nh, [&](float v) { return v > b; });
+        n = t.n[0];
+        __syncthreads();
+        if (n > kLpCap) {
+            // few threads hold very many of the largest (no order of a
+            // vocabulary does that by itself): one at a time
+            uint64_t last = ~0ull;
+            for (n = 0; n < have; n++) {
+                uint64_t best = 0;
+                for (int i = v0 + tid; i < v1; i += kLpThreads) {
+                    const uint64_t y = key_of(to_f32(x[i]), i);
+                    best = y < last && y > best ? y : best;
+                }
+                __syncthreads();
+                t.own[tid] = best;
+                __syncthreads();
+                for (int i = 0; i < kLpThreads; i++) best = t.own[i] > best ? t.own[i] : best;
+                last = best;
+                if (tid == 0) t.keys[n] = best;
+            }
+            __syncthreads();
+            return have;
+        }
+        if (n < have) n += lp_first<T, VEC>(t, x, v0, v1, n, have - n, [&](float v) { return v == b; });
+    }
+    // fewer numbers than k: the first NaN
+    if (n < have) n += lp_first<T, VEC>(t, x, v0, v1, n, have - n, [](float v) { return v != v; });
+    lp_order(t, n, k);
+    return have;
+}
+
 // A workgroup takes one segment of a row, in chunks of 256 * E values that
 // stay in registers: E of them a thread, by 16-byte loads issued together.
-// Each thread keeps its own running maximum (the factors of its sums change
-// at most once a chunk), terms of z are added in fp64 (so that log z keeps
-// its digits where one token has nearly all the probability), those of s in
-// fp32 within a chunk; the threads' sums meet at the row's end.  Bound by the
-// reads where rows are many.
+// Each wave has its own running maximum M (the factors of its sums change
+// where a chunk raises it, seldom).  z's terms are added in fp32 within a
+// chunk, without their whole part, which only values next to M have (it is
+// counted apart), then in fp64: log z keeps its digits where one token has
+// nearly all the probability, and no term costs fp64 instructions.  Bound by
+// the reads in fp32; in 16 bits the arithmetic of a value (13 issue slots, 4
+// of them its exponential) is about as long as its read.
 template <typename T, int E, bool TOP>
 __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
 {
     constexpr int VEC = 16 / (int)sizeof(T), J = E / VEC, CHUNK = kLpThreads * E;
-    extern __shared__ uint64_t cand[];
-    __shared__ uint64_t own[TOP ? kLpThreads : 1];
-    __shared__ uint64_t floor_s;
-    __shared__ int count_s, s_last;
+    __shared__ uint64_t keys[TOP ? kLpCap : 1], own[TOP ? kLpThreads : 1];
+    __shared__ int hot[TOP ? kLpThreads : 1], counts[2];
+    __shared__ float bound;
+    __shared__ int s_last;
     __shared__ double redd[kLpWaves];
     __shared__ float redf[kLpWaves];
     const int tid = threadIdx.x;
-    const int row = blockIdx.x / a.segs, seg = blockIdx.x - row * a.segs;
+    const int row = a.segs == 1 ? blockIdx.x : blockIdx.x / a.segs, seg = blockIdx.x - row * a.segs;
     const T* x = reinterpret_cast<const T*>(a.x) + (size_t)row * a.stride;
     const int v0 = seg * a.per, v1 = a.vocab - v0 > a.per ? v0 + a.per : a.vocab;
-    float m = -INFINITY;
-    double z = 0.0, s = 0.0;
-    Best best{cand, own, &floor_s, &count_s, a.k, 33 * a.k};
-    if constexpr (TOP) best.start();
+    float M = -INFINITY;            // the wave's
+    float most = -INFINITY;         // the thread's
+    double z = 0.0, s = 0.0;        // the thread's, without the `ones` terms that are 1
+    int ones = 0;
     for (int c0 = v0; c0 < v1; c0 += CHUNK) {
         float v[E];
-        const bool inside = c0 + CHUNK <= v1;
-        if (inside) {
+        if (c0 + CHUNK <= v1) {
             typedef Pack<T, VEC, (int)sizeof(T)> Run;
             Run r[J];
 #pragma unroll
@@ -209,43 +319,43 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
                 for (int e = 0; e < VEC; e++) v[j * VEC + e] = to_f32(r[j].v[e]);
         } else {
 #pragma unroll
-            for (int j = 0; j < J; j++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    const int i = (j * kLpThreads + tid) * VEC + e;
-                    v[j * VEC + e] = i < v1 - c0 ? to_f32(x[c0 + i]) : -INFINITY;
-                }
+            for (int j = 0; j < J; j++) lp_load<T, VEC>(x, c0 + (j * kLpThreads + tid) * VEC, v1, v + j * VEC);
         }
         float g = -INFINITY;
 #pragma unroll
         for (int e = 0; e < E; e++) g = fmaxf(g, v[e]);
-        if (g > m) {
-            const float d = m == -INFINITY ? 0.0f : m - g;
+        most = fmaxf(most, g);
+        const float gw = wave_max(g);
+        if (gw > M) {
+            const float d = M == -INFINITY ? 0.0f : M - gw;
             const double f = (double)__builtin_amdgcn_exp2f(d * kLog2e);
+            z += (double)ones;
             s = f * (s + (double)d * z);
             z = f * z;
-            m = g;
+            ones = 0;
+            M = gw;
         }
-        const float base = m == -INFINITY ? 0.0f : m;
-        float sc = 0.0f;
+        const float base = M == -INFINITY ? 0.0f : M;
+        float zc = 0.0f, sc = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const float d = v[e] - base;
             const float p = __builtin_amdgcn_exp2f(d * kLog2e);
-            z += (double)p;
+            zc += __builtin_amdgcn_fractf(p);
             sc = __builtin_fmaf(p, fmaxf(d, -200.0f), sc);   // p is 0 below
         }
-        s += (double)sc;
-        if constexpr (TOP) {
-            auto key = [&](int e) __attribute__((always_inline)) {
-                const int i = ((e / VEC) * kLpThreads + tid) * VEC + e % VEC;
-                return inside || i < v1 - c0 ? key_of(v[e], c0 + i) : 0ull;
-            };
-            // below the floor's value none of the thread's keys is taken
-            best.template offer<E>(key, best.floor < (1ull << 32) || g >= key_value(best.floor));
+        if (__builtin_amdgcn_exp2f((gw - base) * kLog2e) == 1.0f) {
+#pragma unroll
+            for (int e = 0; e < E; e++) ones += __builtin_amdgcn_exp2f((v[e] - base) * kLog2e) == 1.0f;
         }
+        z += (double)zc;
+        s += (double)sc;
     }
-    if constexpr (TOP) best.prune();
+    float m = M;
+    z += (double)ones;
+    int have = 0;
+    const Top top{keys, own, counts};
+    if constexpr (TOP) have = lp_top<T, VEC>(top, hot, &bound, x, v0, v1, most, a.k);
     lp_join(m, z, s, redf, redd);
     if (a.segs > 1) {
         const int words = 3 + a.k;
@@ -257,7 +367,7 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
         }
         if constexpr (TOP)
             for (int i = tid; i < a.k; i += kLpThreads)
-                acc_put(reinterpret_cast<unsigned long long*>(mine) + 3 + i, i < best.have ? best.keys[i] : 0);
+                acc_put(reinterpret_cast<unsigned long long*>(mine) + 3 + i, i < have ? keys[i] : 0);
         if (!acc_arrive(a.ctr + row, (uint32_t)a.segs, &s_last)) return;
         double* parts = a.part + (size_t)row * a.segs * words;
         m = -INFINITY;
@@ -267,25 +377,28 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
             z = acc_peek(parts + tid * words + 1);
             s = acc_peek(parts + tid * words + 2);
         }
-        lp_join(m, z, s, redf, redd);
         if constexpr (TOP) {
-            best.have = 0;
-            best.floor = 0;
-            best.start();
-            constexpr int N = 8;
-            for (int i0 = 0; i0 < a.segs * a.k; i0 += N * kLpThreads) {
-                uint64_t y[N];
+            // segs * k <= kLpCap; missing keys (of short segments) are left out
+            uint64_t y[kLpCap / kLpThreads];
+            int c = 0;
 #pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const int i = i0 + e * kLpThreads + tid;
-                    y[e] = i < a.segs * a.k
-                               ? acc_peek(reinterpret_cast<unsigned long long*>(parts) + (size_t)(i / a.k) * words + 3 + i % a.k)
-                               : 0;
-                }
-                best.template offer<N>([&](int e) __attribute__((always_inline)) { return y[e]; }, true);
+            for (int u = 0; u < kLpCap / kLpThreads; u++) {
+                const int i = u * kLpThreads + tid;
+                y[u] = i < a.segs * a.k
+                           ? acc_peek(reinterpret_cast<unsigned long long*>(parts) + (size_t)(i / a.k) * words + 3 + i % a.k)
+                           : 0;
+                c += y[u] != 0;
             }
-            best.prune();
+            if (tid == 0) counts[0] = 0;
+            __syncthreads();
+            int at = c ? atomicAdd(counts, c) : 0;
+#pragma unroll
+            for (int u = 0; u < kLpCap / kLpThreads; u++)
+                if (y[u] != 0) keys[at++] = y[u];
+            __syncthreads();
+            lp_order(top, counts[0], a.k);
         }
+        lp_join(m, z, s, redf, redd);
         if (tid == 0) a.ctr[row] = 0u;
     }
     const bool none = m == -INFINITY && z == 0.0;   // nothing but -inf
@@ -305,7 +418,7 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
     }
     if constexpr (TOP)
         for (int i = tid; i < a.k; i += kLpThreads) {
-            const uint64_t y = best.keys[i];
+            const uint64_t y = keys[i];
             const float v = key_value(y);
             if (a.ids) a.ids[(size_t)row * a.k + i] = key_id(y);
             if (a.top) a.top[(size_t)row * a.k + i] = none ? -INFINITY : (float)((double)v - (double)m - lz);
@@ -321,7 +434,8 @@ static int logprobs_launch(Ctx* c, LogprobArgs a)
 {
     constexpr int CHUNK = kLpThreads * E;
     const int chunks = (int)(((int64_t)a.vocab + CHUNK - 1) / CHUNK);
-    const int want = std::max(1, std::min({chunks, kLpMaxSegs, kLpTarget / std::max(a.rows, 1)}));
+    const int most = a.k ? std::min(kLpMaxSegs, kLpCap / a.k) : kLpMaxSegs;   // their keys are ordered together
+    const int want = std::max(1, std::min({chunks, most, kLpTarget / std::max(a.rows, 1)}));
     const int each = (chunks + want - 1) / want;
     a.segs = (chunks + each - 1) / each;
     a.per = (int)std::min<int64_t>((int64_t)each * CHUNK, 0x7fffffff);
@@ -332,7 +446,7 @@ static int logprobs_launch(Ctx* c, LogprobArgs a)
     }
     IAM_REQUIRE((int64_t)a.rows * a.segs < ((int64_t)1 << 31), "token_logprobs: too many rows");
     const dim3 grid((unsigned)(a.rows * a.segs));
-    return a.k ? launch(c, "token_logprobs", k_token_logprobs<T, E, true>, grid, dim3(kLpThreads), (size_t)33 * a.k * 8, a)
+    return a.k ? launch(c, "token_logprobs", k_token_logprobs<T, E, true>, grid, dim3(kLpThreads), 0, a)
                : launch(c, "token_logprobs", k_token_logprobs<T, E, false>, grid, dim3(kLpThreads), 0, a);
 }
 
