@@ -43,22 +43,22 @@ __device__ __forceinline__ float key_value(uint64_t k)
 }
 
 // ---- the best k of a row's (or segment's) values
-// The k-th largest of the threads' own maxima bounds the k-th largest value
-// from below, and at most k threads (and ties) reach it: only their values are
-// looked at again, so that the pass over the logits itself needs no exchange.
+// The k-th largest of 64 maxima (of four threads each) bounds the k-th largest
+// value from below, and few threads reach it: only their values are looked
+// at again, so that the pass over the logits itself needs no exchange.
 constexpr int kLpCap = 1024;    // keys held at a time
 
 struct Top {
     uint64_t* keys;     // LDS [kLpCap]
-    uint64_t* own;      // LDS [kLpThreads]: the threads' maxima; places of the list's keys
-    int* n;             // LDS: keys there (may pass kLpCap: then only the first are)
+    uint64_t* own;      // LDS [kLpThreads]: the threads' maxima
+    int* n;             // LDS [2]: keys there (may pass kLpCap: then only the first are); threads looked at
 };
 
 // how many of the 256 keys of own[] are larger than y
 __device__ __forceinline__ int larger(const uint64_t* own, uint64_t y)
 {
     int r = 0;
-#pragma unroll 8
+#pragma unroll 32
     for (int i = 0; i < kLpThreads; i++) r += own[i] > y;
     return r;
 }
@@ -66,7 +66,7 @@ __device__ __forceinline__ int larger(const uint64_t* own, uint64_t y)
 // Orders the n <= kLpCap distinct keys of t.keys; the best min(k, n) end up in
 // order in front.  Where there are many, the k-th best of the threads' best
 // keys first thins them out.
-__device__ void lp_order(const Top& t, int n, int k)
+__device__ __forceinline__ void lp_order(const Top& t, int n, int k)
 {
     const int tid = threadIdx.x;
     constexpr int U = kLpCap / kLpThreads;
@@ -74,7 +74,7 @@ __device__ void lp_order(const Top& t, int n, int k)
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < U; u++) mine[u] = tid + u * kLpThreads < n ? t.keys[tid + u * kLpThreads] : 0;
-    if (n > 128) {
+    if (n > kLpThreads) {
         uint64_t b = 0;
 #pragma unroll
         for (int u = 0; u < U; u++) b = mine[u] > b ? mine[u] : b;
@@ -97,10 +97,16 @@ __device__ void lp_order(const Top& t, int n, int k)
     int rank[U];
 #pragma unroll
     for (int u = 0; u < U; u++) rank[u] = 0;
-    for (int i = 0; i < n; i++) {
-        const uint64_t y = t.keys[i];
+    if (n <= kLpThreads) {
+#pragma unroll 8
+        for (int i = 0; i < n; i++) rank[0] += t.keys[i] > mine[0];
+    } else {
+#pragma unroll 4
+        for (int i = 0; i < n; i++) {
+            const uint64_t y = t.keys[i];
 #pragma unroll
-        for (int u = 0; u < U; u++) rank[u] += y > mine[u];
+            for (int u = 0; u < U; u++) rank[u] += y > mine[u];
+        }
     }
     __syncthreads();
 #pragma unroll
@@ -145,43 +151,52 @@ __device__ __forceinline__ void lp_join(float& m, double& z, double& s, float* r
     m = M;
 }
 
-// VEC values from place i on; past v1, -inf
+// VEC values from place i on; outside [v0, v1), -inf
 template <typename T, int VEC>
-__device__ __forceinline__ void lp_load(const T* x, int i, int v1, float* v)
+__device__ __forceinline__ void lp_load(const T* x, int i, int v0, int v1, float* v)
 {
-    if (i + VEC <= v1) {
-        const Pack<T, VEC, (int)sizeof(T)> r = *reinterpret_cast<const Pack<T, VEC, (int)sizeof(T)>*>(x + i);
+    if (i >= v0 && i + VEC <= v1) {
+        const Pack<T, VEC> r = *reinterpret_cast<const Pack<T, VEC>*>(x + i);
 #pragma unroll
         for (int e = 0; e < VEC; e++) v[e] = to_f32(r.v[e]);
     } else {
 #pragma unroll
-        for (int e = 0; e < VEC; e++) v[e] = i + e < v1 ? to_f32(x[i + e]) : -INFINITY;
+        for (int e = 0; e < VEC; e++) v[e] = i + e >= v0 && i + e < v1 ? to_f32(x[i + e]) : -INFINITY;
     }
 }
 
 // The values of [v0, v1) that take(value) says, as keys behind the n there,
-// from the threads that `hot` lists (nh of them); t.n counts them all.
+// from the threads that `hot` lists (nh of them), whose first load is at place
+// o; t.n counts them all.
 template <typename T, int VEC, typename Take>
-__device__ __forceinline__ void lp_gather(const Top& t, const T* x, int v0, int v1, const int* hot, int nh, Take take)
+__device__ __forceinline__ void lp_gather(const Top& t, const T* x, int o, int v0, int v1, const int* hot, int nh, Take take)
 {
-    const int rounds = (v1 - v0 + kLpThreads * VEC - 1) / (kLpThreads * VEC);
-    for (int i0 = 0; i0 < rounds * nh; i0 += kLpThreads) {
-        const int q = i0 + (int)threadIdx.x;
-        if (q >= rounds * nh || *(volatile int*)t.n > kLpCap) continue;
-        const int r = q / nh, i = v0 + (r * kLpThreads + hot[q - r * nh]) * VEC;
-        float v[VEC];
-        lp_load<T, VEC>(x, i, v1, v);
-        int c = 0;
+    constexpr int B = 4;   // loads in flight
+    const int rounds = (v1 - o + kLpThreads * VEC - 1) / (kLpThreads * VEC), all = rounds * nh;
+    for (int i0 = 0; i0 < all; i0 += B * kLpThreads) {
+        float v[B][VEC];
+        int at[B];
 #pragma unroll
-        for (int e = 0; e < VEC; e++) c += i + e < v1 && take(v[e]);
-        if (!c) continue;
-        int at = atomicAdd(t.n, c);
+        for (int u = 0; u < B; u++) {
+            const int q = i0 + u * kLpThreads + (int)threadIdx.x, r = q / nh;
+            at[u] = q < all ? o + (r * kLpThreads + hot[q - r * nh]) * VEC : v1;
+            lp_load<T, VEC>(x, at[u], v0, v1, v[u]);
+        }
+        if (*(volatile int*)t.n > kLpCap) continue;   // too many already
 #pragma unroll
-        for (int e = 0; e < VEC; e++)
-            if (i + e < v1 && take(v[e])) {
-                if (at < kLpCap) t.keys[at] = key_of(v[e], i + e);
-                at++;
-            }
+        for (int u = 0; u < B; u++) {
+            int c = 0;
+#pragma unroll
+            for (int e = 0; e < VEC; e++) c += at[u] + e >= v0 && at[u] + e < v1 && take(v[u][e]);
+            if (!c) continue;
+            int p = atomicAdd(t.n, c);
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                if (at[u] + e >= v0 && at[u] + e < v1 && take(v[u][e])) {
+                    if (p < kLpCap) t.keys[p] = key_of(v[u][e], at[u] + e);
+                    p++;
+                }
+        }
     }
     __syncthreads();
 }
@@ -189,17 +204,17 @@ __device__ __forceinline__ void lp_gather(const Top& t, const T* x, int v0, int 
 // The first `want` values of [v0, v1), by place, that take(value) says, as keys
 // behind the n there; how many there were
 template <typename T, int VEC, typename Take>
-__device__ int lp_first(const Top& t, const T* x, int v0, int v1, int n, int want, Take take)
+__device__ __forceinline__ int lp_first(const Top& t, const T* x, int o, int v0, int v1, int n, int want, Take take)
 {
     __shared__ int wsum[kLpWaves];
     int got = 0;
-    for (int c0 = v0; c0 < v1 && got < want; c0 += kLpThreads * VEC) {
+    for (int c0 = o; c0 < v1 && got < want; c0 += kLpThreads * VEC) {
         const int i = c0 + (int)threadIdx.x * VEC;
         float v[VEC];
-        lp_load<T, VEC>(x, i, v1, v);
+        lp_load<T, VEC>(x, i, v0, v1, v);
         int c = 0;
 #pragma unroll
-        for (int e = 0; e < VEC; e++) c += i + e < v1 && take(v[e]);
+        for (int e = 0; e < VEC; e++) c += i + e >= v0 && i + e < v1 && take(v[e]);
         const int incl = wave_incl_sum(c), w = threadIdx.x >> 6;
         __syncthreads();
         if ((threadIdx.x & 63) == 63) wsum[w] = incl;
@@ -212,7 +227,7 @@ __device__ int lp_first(const Top& t, const T* x, int v0, int v1, int n, int wan
         }
 #pragma unroll
         for (int e = 0; e < VEC; e++)
-            if (i + e < v1 && take(v[e])) {
+            if (i + e >= v0 && i + e < v1 && take(v[e])) {
                 if (at < want) t.keys[n + at] = key_of(v[e], i + e);
                 at++;
             }
@@ -223,24 +238,49 @@ __device__ int lp_first(const Top& t, const T* x, int v0, int v1, int n, int wan
 }
 
 // The best min(k, v1 - v0) keys of [v0, v1) in order in front of t.keys; m: the
-// largest value of the thread's own loads (its place in every 256 * VEC).
-template <typename T, int VEC>
-__device__ int lp_top(const Top& t, int* hot, float* bound, const T* x, int v0, int v1, float m, int k)
+// largest value of the thread's own loads (from place o on, its part of every
+// 256 * VEC).  kept: the thread's E values, where the segment is one chunk
+// (`whole`): nothing is read again.
+template <typename T, int VEC, int E>
+__device__ __forceinline__ int lp_top(const Top& t, int* hot, const T* x, int o, int v0, int v1, float m, int k, bool whole,
+                                      const float* kept)
 {
     const int tid = threadIdx.x, have = min(k, v1 - v0);
-    // distinct: equal maxima by thread
-    const uint64_t mine = key_of(m, tid);
+    float* lane_max = reinterpret_cast<float*>(t.own);   // [kLpWaves][64]
     __syncthreads();
-    t.own[tid] = mine;
+    lane_max[tid] = m;
     if (tid == 0) t.n[0] = t.n[1] = 0;
     __syncthreads();
-    if (larger(t.own, mine) == k - 1) *bound = m;
-    __syncthreads();
-    const float b = *bound;
+    float g = lane_max[tid & 63];
+#pragma unroll
+    for (int w = 1; w < kLpWaves; w++) g = fmaxf(g, lane_max[w * 64 + (tid & 63)]);
+    // bit by bit, the largest number that k of the wave's 64 reach
+    const uint32_t mine = (uint32_t)(key_of(g, 0) >> 32);
+    uint32_t kth = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 0; bit--) {
+        const uint32_t y = kth | 1u << bit;
+        if (__popcll(__ballot(mine >= y)) >= k) kth = y;
+    }
+    const float b = key_value((uint64_t)kth << 32);
     if (m >= b) hot[atomicAdd(t.n + 1, 1)] = tid;
     __syncthreads();
     const int nh = t.n[1];
-    lp_gather<T, VEC>(t, x, v0, v1, hot, nh, [&](float v) { return v >= b; });
+    if (whole) {
+        if (m >= b) {
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int i = o + (e / VEC * kLpThreads + tid) * VEC + e % VEC;
+                if (kept[e] >= b && i >= v0 && i < v1) {
+                    const int p = atomicAdd(t.n, 1);
+                    if (p < kLpCap) t.keys[p] = key_of(kept[e], i);
+                }
+            }
+        }
+        __syncthreads();
+    } else {
+        lp_gather<T, VEC>(t, x, o, v0, v1, hot, nh, [&](float v) { return v >= b; });
+    }
     int n = t.n[0];
     if (n > kLpCap) {
         // many equal values (a masked row's -inf): the larger ones, then the
@@ -248,7 +288,7 @@ __device__ int lp_top(const Top& t, int* hot, float* bound, const T* x, int v0, 
         __syncthreads();
         if (tid == 0) t.n[0] = 0;
         __syncthreads();
-        lp_gather<T, VEC>(t, x, v0, v1, hot, nh, [&](float v) { return v > b; });
+        lp_gather<T, VEC>(t, x, o, v0, v1, hot, nh, [&](float v) { return v > b; });
         n = t.n[0];
         __syncthreads();
         if (n > kLpCap) {
@@ -271,10 +311,10 @@ __device__ int lp_top(const Top& t, int* hot, float* bound, const T* x, int v0, 
             __syncthreads();
             return have;
         }
-        if (n < have) n += lp_first<T, VEC>(t, x, v0, v1, n, have - n, [&](float v) { return v == b; });
+        if (n < have) n += lp_first<T, VEC>(t, x, o, v0, v1, n, have - n, [&](float v) { return v == b; });
     }
     // fewer numbers than k: the first NaN
-    if (n < have) n += lp_first<T, VEC>(t, x, v0, v1, n, have - n, [](float v) { return v != v; });
+    if (n < have) n += lp_first<T, VEC>(t, x, o, v0, v1, n, have - n, [](float v) { return v != v; });
     lp_order(t, n, k);
     return have;
 }
@@ -294,22 +334,25 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
     constexpr int VEC = 16 / (int)sizeof(T), J = E / VEC, CHUNK = kLpThreads * E;
     __shared__ uint64_t keys[TOP ? kLpCap : 1], own[TOP ? kLpThreads : 1];
     __shared__ int hot[TOP ? kLpThreads : 1], counts[2];
-    __shared__ float bound;
     __shared__ int s_last;
     __shared__ double redd[kLpWaves];
     __shared__ float redf[kLpWaves];
     const int tid = threadIdx.x;
     const int row = a.segs == 1 ? blockIdx.x : blockIdx.x / a.segs, seg = blockIdx.x - row * a.segs;
     const T* x = reinterpret_cast<const T*>(a.x) + (size_t)row * a.stride;
-    const int v0 = seg * a.per, v1 = a.vocab - v0 > a.per ? v0 + a.per : a.vocab;
+    // Chunks start at multiples of 16 bytes in memory, before the row's (or
+    // segment's) first value if need be: rows at 2-byte boundaries, read as
+    // they lie, took 69 us instead of 60 (1024 x 128000 bf16).
+    const int off = (int)((uintptr_t)x / sizeof(T) % VEC);
+    const int o = seg * a.per - off, v0 = max(o, 0), v1 = a.vocab - o > a.per ? o + a.per : a.vocab;
     float M = -INFINITY;            // the wave's
     float most = -INFINITY;         // the thread's
     double z = 0.0, s = 0.0;        // the thread's, without the `ones` terms that are 1
     int ones = 0;
-    for (int c0 = v0; c0 < v1; c0 += CHUNK) {
-        float v[E];
-        if (c0 + CHUNK <= v1) {
-            typedef Pack<T, VEC, (int)sizeof(T)> Run;
+    float v[E];
+    for (int c0 = o; c0 < v1; c0 += CHUNK) {
+        if (c0 >= v0 && c0 + CHUNK <= v1) {
+            typedef Pack<T, VEC> Run;
             Run r[J];
 #pragma unroll
             for (int j = 0; j < J; j++) r[j] = *reinterpret_cast<const Run*>(x + c0 + (j * kLpThreads + tid) * VEC);
@@ -319,7 +362,7 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
                 for (int e = 0; e < VEC; e++) v[j * VEC + e] = to_f32(r[j].v[e]);
         } else {
 #pragma unroll
-            for (int j = 0; j < J; j++) lp_load<T, VEC>(x, c0 + (j * kLpThreads + tid) * VEC, v1, v + j * VEC);
+            for (int j = 0; j < J; j++) lp_load<T, VEC>(x, c0 + (j * kLpThreads + tid) * VEC, v0, v1, v + j * VEC);
         }
         float g = -INFINITY;
 #pragma unroll
@@ -342,7 +385,7 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
             const float d = v[e] - base;
             const float p = __builtin_amdgcn_exp2f(d * kLog2e);
             zc += __builtin_amdgcn_fractf(p);
-            sc = __builtin_fmaf(p, fmaxf(d, -200.0f), sc);   // p is 0 below
+            sc = __builtin_fmaf(p, __builtin_amdgcn_fmed3f(d, -200.0f, 0.0f), sc);   // p is 0 below
         }
         if (__builtin_amdgcn_exp2f((gw - base) * kLog2e) == 1.0f) {
 #pragma unroll
@@ -355,7 +398,7 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
     z += (double)ones;
     int have = 0;
     const Top top{keys, own, counts};
-    if constexpr (TOP) have = lp_top<T, VEC>(top, hot, &bound, x, v0, v1, most, a.k);
+    if constexpr (TOP) have = lp_top<T, VEC, E>(top, hot, x, o, v0, v1, most, a.k, v1 - o <= CHUNK, v);
     lp_join(m, z, s, redf, redd);
     if (a.segs > 1) {
         const int words = 3 + a.k;
@@ -433,7 +476,10 @@ template <typename T, int E>
 static int logprobs_launch(Ctx* c, LogprobArgs a)
 {
     constexpr int CHUNK = kLpThreads * E;
-    const int chunks = (int)(((int64_t)a.vocab + CHUNK - 1) / CHUNK);
+    // values before a row's first that its first chunk holds, at most
+    constexpr int VEC = 16 / (int)sizeof(T);
+    const int off = a.rows == 1 || a.stride % VEC == 0 ? (int)((uintptr_t)a.x / sizeof(T) % VEC) : VEC - 1;
+    const int chunks = (int)(((int64_t)a.vocab + off + CHUNK - 1) / CHUNK);
     const int most = a.k ? std::min(kLpMaxSegs, kLpCap / a.k) : kLpMaxSegs;   // their keys are ordered together
     const int want = std::max(1, std::min({chunks, most, kLpTarget / std::max(a.rows, 1)}));
     const int each = (chunks + want - 1) / want;
