@@ -51,25 +51,30 @@ __device__ __forceinline__ void widen4(uint32_t w, half2v& lo, half2v& hi)
 }
 
 // The exact quotient x / s rounded to odd: one more rounding, to nearest even
-// at 22 bits or fewer, then gives the correctly rounded result.  The
-// remainder x - q s is exact (q is the correctly rounded quotient).
-__device__ __forceinline__ float quotient_odd(float x, float s)
+// at 22 bits or fewer, then gives the correctly rounded result.  r: 1 / s,
+// correctly rounded.  q is x r with its error taken out, within a step of
+// the quotient; the sign of x - q s says on which side.
+__device__ __forceinline__ float quotient_odd(float x, float s, float r)
 {
-    const float q = __fdiv_rn(x, s);
-    const float r = __builtin_fmaf(-q, s, x);
+    const float q0 = __fmul_rn(x, r);
+    const float q = __builtin_fmaf(__builtin_fmaf(-q0, s, x), r, q0);
+    const float e = __builtin_fmaf(-q, s, x);
     int b = __float_as_int(q);
-    if (r != 0.0f && !(b & 1)) b += ((r > 0.0f) == (x > 0.0f)) ? 1 : -1;
+    if (e != 0.0f && !(b & 1)) b += ((e > 0.0f) == (x > 0.0f)) ? 1 : -1;
     return __int_as_float(b);
 }
 
-// x / s as an 8-bit number (0 where the scale is 0 or NaN), in the low byte
+// x / s as an 8-bit number, in the low byte; s > 0
 template <int FMT>
-__device__ __forceinline__ uint32_t narrow(float x, float s)
+__device__ __forceinline__ uint32_t narrow(float x, float s, float r)
 {
-    const float q = s > 0.0f && x != 0.0f ? quotient_odd(x, s) : 0.0f;
+    const float q = x != 0.0f ? quotient_odd(x, s, r) : 0.0f;
     if constexpr (FMT == IAM_KV8_INT8) return (uint32_t)((int)rintf(q) + 128);
     else return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q, q, 0, false) & 0xffu;
 }
+// the number 0
+template <int FMT>
+constexpr uint32_t kv8_zero() { return FMT == IAM_KV8_INT8 ? 128u : 0u; }
 
 // the scale of a block whose largest magnitude is 1
 template <int FMT>

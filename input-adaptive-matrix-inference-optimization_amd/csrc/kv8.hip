@@ -1,5 +1,6 @@
 // The 8-bit KV cache: writing tokens, reading back what they stand for.
 #include "kv8.h"
+#include "wave.h"
 
 namespace iam {
 
@@ -17,7 +18,6 @@ struct AppendArgs {
     size_t stride;           // values between tokens
 };
 
-__device__ __forceinline__ uint16_t half_bits(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
 __device__ __forceinline__ float half_value(uint16_t b) { return (float)__builtin_bit_cast(_Float16, b); }
 
 // what a byte of a tile stands for, before its scale
@@ -29,20 +29,57 @@ __device__ __forceinline__ float number(uint8_t b)
     return (float)lo[0];
 }
 
+// the 16 values (t, d) of run r of a tile: r = 64 * group + 16 * g + m
+template <int HD, bool IS_V>
+__device__ __forceinline__ int run_token(int r, int e)
+{
+    const int g = (r >> 4) & 3, m = r & 15, grp = r >> 6;
+    return IS_V ? (e >> 3) * 32 + ((e >> 2) & 1) * 16 + g * 4 + (e & 3) : grp / (HD / 64) * 16 + m;
+}
+template <int HD, bool IS_V>
+__device__ __forceinline__ int run_dim(int r, int e)
+{
+    const int g = (r >> 4) & 3, m = r & 15, grp = r >> 6;
+    return IS_V ? grp * 16 + m : grp % (HD / 64) * 64 + g * 16 + e;
+}
+
+// n_new rows from token t0 of the open block on, 8 values at a time
+template <typename T, int HD, bool IS_V>
+__device__ __forceinline__ void open_rows(uint16_t* open, const T* src, size_t stride, int t0, int n_new)
+{
+    constexpr int Q = HD / 8;
+    typedef Pack<T, 8, (int)sizeof(T)> Eight;
+    for (int i = threadIdx.x; i < n_new * Q; i += kAppendThreads) {
+        const int t = i / Q, d = i % Q * 8;
+        const Eight x = *reinterpret_cast<const Eight*>(src + (size_t)t * stride + d);
+        half8 h;
+#pragma unroll
+        for (int e = 0; e < 8; e++) h[e] = (_Float16)to_f32(x.v[e]);
+        if constexpr (IS_V) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) open[v_place(t0 + t, d + e)] = __builtin_bit_cast(uint16_t, (_Float16)h[e]);
+        } else {
+            *reinterpret_cast<half8*>(open + k_place<HD>(t0 + t, d)) = h;
+        }
+    }
+}
+
 // Workgroup (unit, KV head, K or V; sequence) takes the unit-th block that the
-// call's tokens of the sequence touch.  A block that they fill is brought into
-// LDS as fp16 rows (its earlier tokens from the open block, or from the block
-// itself where the sequence went back into it), its largest magnitude gives the
-// scale, and each thread writes 16-byte runs of the tile.  A block that stays
-// open gets its new tokens in fp16.  Only the first block reads the open block
-// and only the last may write it, so unit 0 takes both, one after the other.
-// Bound by the values read (and, for one token, by the launch).
+// call's tokens of the sequence touch.  Its new tokens' rows come in 8 values
+// at a time.  A block that they fill: the rows go to LDS as fp16, and each
+// thread takes HD / 64 runs of 16 values in the tile's order, the earlier
+// tokens' from the open block (which is in that order), or from the tile
+// where the sequence went back into it; the largest magnitude of all gives the
+// scale, and each run becomes 16 bytes.  A block that stays open gets its new
+// tokens in fp16.  Only the first block reads the open block and only the last
+// may write it, so unit 0 takes both, one after the other.  Bound by the
+// values read (and, for one token, by the launch).
 template <typename T, int HD, int FMT, bool IS_V>
 __device__ __forceinline__ void append_block(const AppendArgs& a, uint16_t* rows, float* red, int seq, int head, int block,
                                              int p0, int p1)
 {
     constexpr int RS = HD + 8;                       // LDS row stride: 16 bytes of padding
-    constexpr int NT = kAppendThreads;
+    constexpr int NT = kAppendThreads, Q = HD / 8, LOADS = kBlk * Q / NT, RUNS = kBlk * HD / 16 / NT;
     const int tid = threadIdx.x;
     const int t0 = max(p0 - block * kBlk, 0);        // new tokens t0 .. t1 of the block
     const int t1 = min(p1 - block * kBlk, kBlk - 1);
@@ -53,59 +90,104 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, uint16_t* rows
     float* scale_p = a.scales[IS_V] + cell;
     const float was = t0 > 0 ? *scale_p : -1.0f;
     const bool reopened = !(was < 0.0f);             // the earlier tokens are in the tile
-    const T* src = reinterpret_cast<const T*>(a.src[IS_V]) + (size_t)head * HD;
-    // the call's token at position p is row p - p0
-    auto fresh = [&](int t, int d) {
-        return half_bits(to_f32(src[((size_t)seq * a.tokens + (size_t)(block * kBlk + t - p0)) * a.stride + d]));
-    };
-    auto earlier = [&](int t, int d) {
-        const int i = place<HD, IS_V>(t, d);
-        return reopened ? half_bits(number<FMT>(tile[i]) * was) : open[i];
+    // the call's token at position p is row p - p0; the new rows, 8 values a load
+    const T* src = reinterpret_cast<const T*>(a.src[IS_V]) + (size_t)head * HD +
+                   ((size_t)seq * a.tokens + (size_t)(block * kBlk + t0 - p0)) * a.stride;
+    const int n_new = t1 - t0 + 1;
+    auto run_of_tile = [&](int r, _Float16* v) __attribute__((always_inline)) {
+        const uint4 w = *reinterpret_cast<const uint4*>(tile + (size_t)r * 16);
+        const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            half2v lo, hi;
+            widen4<FMT>(wd[i], lo, hi);
+            v[4 * i] = (_Float16)((float)lo[0] * was);
+            v[4 * i + 1] = (_Float16)((float)lo[1] * was);
+            v[4 * i + 2] = (_Float16)((float)hi[0] * was);
+            v[4 * i + 3] = (_Float16)((float)hi[1] * was);
+        }
     };
     if (!full) {
-        if (reopened)
-            for (int i = tid; i < t0 * HD; i += NT) {
-                const int t = i / HD, d = i - t * HD;
-                open[place<HD, IS_V>(t, d)] = earlier(t, d);
+        if (reopened) {
+            // all of the tile's values (those from t0 on are written over, or
+            // lie past the sequence's end)
+#pragma unroll 1
+            for (int r = tid; r < kBlk * HD / 16; r += NT) {
+                _Float16 v[16];
+                run_of_tile(r, v);
+#pragma unroll
+                for (int e = 0; e < 16; e++) open[r * 16 + e] = __builtin_bit_cast(uint16_t, v[e]);
             }
-        for (int i = tid; i < (t1 - t0 + 1) * HD; i += NT) {
-            const int t = i / HD, d = i - t * HD;
-            open[place<HD, IS_V>(t0 + t, d)] = fresh(t0 + t, d);
         }
-        __syncthreads();                             // every thread has read the scale
+        __syncthreads();                             // (every thread has read the scale, too)
+        open_rows<T, HD, IS_V>(open, src, a.stride, t0, n_new);
         if (tid == 0) *scale_p = -1.0f;
         return;
     }
+    typedef Pack<T, 8, (int)sizeof(T)> Eight;
+    half8 got[LOADS];
+#pragma unroll
+    for (int u = 0; u < LOADS; u++) {
+        const int i = tid + u * NT, t = i / Q, d = i % Q * 8;
+        if (t < n_new) {
+            const Eight x = *reinterpret_cast<const Eight*>(src + (size_t)t * a.stride + d);
+#pragma unroll
+            for (int e = 0; e < 8; e++) got[u][e] = (_Float16)to_f32(x.v[e]);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < LOADS; u++) {
+        const int i = tid + u * NT, t = i / Q, d = i % Q * 8;
+        if (t < n_new) *reinterpret_cast<half8*>(rows + (t0 + t) * RS + d) = got[u];
+    }
+    _Float16 v[RUNS][16];
+    if (t0 > 0) {
+#pragma unroll
+        for (int u = 0; u < RUNS; u++) {
+            const int r = tid + u * NT;
+            if (reopened) {
+                run_of_tile(r, v[u]);
+            } else {
+                const half8 x = *reinterpret_cast<const half8*>(open + r * 16), y = *reinterpret_cast<const half8*>(open + r * 16 + 8);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    v[u][e] = x[e];
+                    v[u][8 + e] = y[e];
+                }
+            }
+        }
+    }
+    __syncthreads();
     float top = 0.0f;
     bool bad = false;
-    for (int i = tid; i < kBlk * HD; i += NT) {
-        const int t = i / HD, d = i - t * HD;
-        const uint16_t h = t < t0 ? earlier(t, d) : fresh(t, d);
-        rows[t * RS + d] = h;
-        top = fmaxf(top, fabsf(half_value(h)));
-        bad |= (h & 0x7c00) == 0x7c00;
+#pragma unroll
+    for (int u = 0; u < RUNS; u++) {
+        const int r = tid + u * NT;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const int t = run_token<HD, IS_V>(r, e);
+            if (t >= t0) v[u][e] = __builtin_bit_cast(_Float16, rows[t * RS + run_dim<HD, IS_V>(r, e)]);
+            top = fmaxf(top, fabsf((float)v[u][e]));
+            bad |= (__builtin_bit_cast(uint16_t, v[u][e]) & 0x7c00) == 0x7c00;
+        }
     }
     if (bad) top = INFINITY;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    top = wave_max(top);
     if ((tid & 63) == 0) red[tid >> 6] = top;
     __syncthreads();
     top = red[0];
 #pragma unroll
     for (int w = 1; w < NT / 64; w++) top = fmaxf(top, red[w]);
     const float scale = top < INFINITY ? __fmul_rn(top, kv8_unit<FMT>()) : NAN;
-    for (int r = tid; r < kBlk * HD / 16; r += NT) {
-        // the run's 16 values: lane l = r % 64 of group r / 64
-        const int grp = r >> 6, g = (r >> 4) & 3, m = r & 15;
-        uint32_t w[4];
+    const bool some = scale > 0.0f;                  // else the numbers are zeros
+    const float r1 = some ? __fdiv_rn(1.0f, scale) : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int t = IS_V ? (e >> 3) * 32 + ((e >> 2) & 1) * 16 + g * 4 + (e & 3) : grp / (HD / 64) * 16 + m;
-            const int d = IS_V ? grp * 16 + m : grp % (HD / 64) * 64 + g * 16 + e;
-            const uint32_t b = narrow<FMT>(half_value(rows[t * RS + d]), scale);
-            w[e >> 2] = (e & 3) == 0 ? b : w[e >> 2] | b << ((e & 3) * 8);
-        }
-        *reinterpret_cast<uint4*>(tile + (size_t)r * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int u = 0; u < RUNS; u++) {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            w[e >> 2] |= (some ? narrow<FMT>((float)v[u][e], scale, r1) : kv8_zero<FMT>()) << ((e & 3) * 8);
+        *reinterpret_cast<uint4*>(tile + (size_t)(tid + u * NT) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     if (tid == 0) *scale_p = scale;
 }
@@ -113,7 +195,7 @@ __device__ __forceinline__ void append_block(const AppendArgs& a, uint16_t* rows
 template <typename T, int HD, int FMT>
 __global__ __launch_bounds__(kAppendThreads) void k_kv8_append(AppendArgs a)
 {
-    __shared__ uint16_t rows[kBlk * (HD + 8)];
+    __shared__ __align__(16) uint16_t rows[kBlk * (HD + 8)];
     __shared__ float red[kAppendThreads / 64];
     const int seq = blockIdx.y;
     const bool is_v = blockIdx.x & 1;
@@ -127,14 +209,17 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv8_append(AppendArgs a)
     const bool stays_open = p1 % kBlk != kBlk - 1;   // the last block
     const int block = first + unit;
     if (block > last || (unit > 0 && block == last && stays_open)) return;
-    auto run = [&](int b) __attribute__((always_inline)) {
-        if (is_v) append_block<T, HD, FMT, true>(a, rows, red, seq, head, b, p0, p1);
-        else append_block<T, HD, FMT, false>(a, rows, red, seq, head, b, p0, p1);
-    };
-    run(block);
+    if (is_v) append_block<T, HD, FMT, true>(a, rows, red, seq, head, block, p0, p1);
+    else append_block<T, HD, FMT, false>(a, rows, red, seq, head, block, p0, p1);
     if (unit == 0 && last > first && stays_open) {
         __syncthreads();                             // the first block's reads of the open one are done
-        run(last);
+        const T* src = reinterpret_cast<const T*>(a.src[is_v]) + (size_t)head * HD +
+                       ((size_t)seq * a.tokens + (size_t)(last * kBlk - p0)) * a.stride;
+        uint16_t* open = a.open[is_v] + ((size_t)seq * a.g.n_kv + head) * (size_t)(kBlk * HD);
+        const int n = p1 - last * kBlk + 1;
+        if (is_v) open_rows<T, HD, true>(open, src, a.stride, 0, n);
+        else open_rows<T, HD, false>(open, src, a.stride, 0, n);
+        if (threadIdx.x == 0) a.scales[is_v][kv8_cell(a.g, seq, last, head)] = -1.0f;
     }
 }
 
@@ -148,7 +233,82 @@ struct ReadArgs {
     int tokens;
 };
 
-// One thread per value.
+// Many tokens: workgroup (unit, KV head, K or V; sequence) takes the unit-th
+// block that the rows touch: its runs into LDS (as fp16, numbers before their
+// scale: exact), then out by rows, 8 values a thread.  Bound by the writes.
+template <int HD, int FMT>
+__global__ __launch_bounds__(256) void k_kv8_read_blocks(ReadArgs a)
+{
+    constexpr int RS = HD + 8, NT = 256, RUNS = kBlk * HD / 16 / NT, Q = HD / 8;
+    __shared__ __align__(16) uint16_t rows[kBlk * RS];
+    const int tid = threadIdx.x, seq = blockIdx.y, is_v = blockIdx.x & 1;
+    const int head = (blockIdx.x >> 1) % a.g.n_kv, unit = (blockIdx.x >> 1) / a.g.n_kv;
+    const long long q0 = a.pos[seq], q1 = q0 + a.tokens;                 // the positions asked for
+    const int p0 = (int)max(q0, 0ll), p1 = (int)min(q1, (long long)a.g.max_ctx);   // of them, those there are
+    const int block = p0 / kBlk + unit;
+    if (p0 >= p1 || block > (p1 - 1) / kBlk) return;
+    const size_t cell = kv8_cell(a.g, seq, block, head);
+    const float scale = a.scales[is_v][cell];
+    const bool is_open = scale < 0.0f;
+    auto spread = [&](int r, const _Float16* v) __attribute__((always_inline)) {
+        if (is_v) {
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                rows[run_token<HD, true>(r, e) * RS + run_dim<HD, true>(r, e)] = __builtin_bit_cast(uint16_t, v[e]);
+        } else {
+            half8 x, y;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                x[e] = v[e];
+                y[e] = v[8 + e];
+            }
+            uint16_t* to = rows + run_token<HD, false>(r, 0) * RS + run_dim<HD, false>(r, 0);
+            *reinterpret_cast<half8*>(to) = x;
+            *reinterpret_cast<half8*>(to + 8) = y;
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < RUNS; u++) {
+        const int r = tid + u * NT;
+        _Float16 v[16];
+        if (is_open) {
+            const half8* o = reinterpret_cast<const half8*>(a.open[is_v] + ((size_t)seq * a.g.n_kv + head) * (size_t)(kBlk * HD) + r * 16);
+            const half8 x = o[0], y = o[1];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                v[e] = x[e];
+                v[8 + e] = y[e];
+            }
+        } else {
+            const uint4 w = *reinterpret_cast<const uint4*>(a.tiles[is_v] + cell * (size_t)(kBlk * HD) + r * 16);
+            const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                half2v lo, hi;
+                widen4<FMT>(wd[i], lo, hi);
+                v[4 * i] = lo[0];
+                v[4 * i + 1] = lo[1];
+                v[4 * i + 2] = hi[0];
+                v[4 * i + 3] = hi[1];
+            }
+        }
+        spread(r, v);
+    }
+    __syncthreads();
+    const float f = is_open ? 1.0f : scale;
+    const int t0 = max(p0 - block * kBlk, 0), n = min(p1 - block * kBlk, kBlk) - t0;
+    float* out = a.out[is_v] + ((size_t)seq * a.tokens + (size_t)(block * kBlk + t0 - q0)) * ((size_t)a.g.n_kv * HD) + (size_t)head * HD;
+    for (int i = tid; i < n * Q; i += NT) {
+        const int t = i / Q, d = i % Q * 8;
+        const half8 x = *reinterpret_cast<const half8*>(rows + (t0 + t) * RS + d);
+        Pack<float, 8, 4> y;
+#pragma unroll
+        for (int e = 0; e < 8; e++) y.v[e] = (float)x[e] * f;
+        *reinterpret_cast<Pack<float, 8, 4>*>(out + (size_t)t * a.g.n_kv * HD + d) = y;
+    }
+}
+
+// A few tokens: one thread per value.
 template <int HD, int FMT>
 __global__ __launch_bounds__(256) void k_kv8_read(ReadArgs a)
 {
@@ -216,9 +376,22 @@ static int append_dim(Ctx* c, const AppendArgs& a, const iam_kv8_cache* k, dim3 
     return append_typed<T, 256>(c, a, k->format, grid);
 }
 
+// Tokens from which blocks are read as a whole (8 KV heads of 128, one
+// sequence, a launch: by value 4.0 us for 1 and 2 tokens, 4.7 to 5.1 for 4;
+// by blocks 4.1 for 8 to 64, and 11 for 4000 where by value took 23)
+constexpr int kReadBlocks = 4;
+
 template <int HD>
-static int read_dim(Ctx* c, const ReadArgs& a, int format, dim3 grid)
+static int read_dim(Ctx* c, const ReadArgs& a, int format)
 {
+    if (a.tokens >= kReadBlocks) {
+        const int units = std::min((a.tokens - 1 + kBlk - 1) / kBlk + 1, a.g.blocks);
+        const dim3 grid((unsigned)units * a.g.n_kv * 2, (unsigned)a.g.n_seq);
+        return format == IAM_KV8_INT8 ? launch(c, "kv8_read", k_kv8_read_blocks<HD, IAM_KV8_INT8>, grid, dim3(256), 0, a)
+                                      : launch(c, "kv8_read", k_kv8_read_blocks<HD, IAM_KV8_E4M3>, grid, dim3(256), 0, a);
+    }
+    const size_t per = (size_t)a.tokens * a.g.n_kv * HD;
+    const dim3 grid((unsigned)((per + 255) / 256), (unsigned)a.g.n_seq, 2);
     return format == IAM_KV8_INT8 ? launch(c, "kv8_read", k_kv8_read<HD, IAM_KV8_INT8>, grid, dim3(256), 0, a)
                                   : launch(c, "kv8_read", k_kv8_read<HD, IAM_KV8_E4M3>, grid, dim3(256), 0, a);
 }
@@ -322,10 +495,9 @@ int iam_kv8_read(iam_ctx* c, const iam_kv8_cache* k, const int* pos, int n_token
     a.pos = pos;
     a.g = geometry(k);
     a.tokens = n_tokens;
-    const dim3 grid((unsigned)((per + 255) / 256), (unsigned)k->n_seq, 2);
-    if (k->head_dim == 64) return read_dim<64>(c, a, k->format, grid);
-    if (k->head_dim == 128) return read_dim<128>(c, a, k->format, grid);
-    return read_dim<256>(c, a, k->format, grid);
+    if (k->head_dim == 64) return read_dim<64>(c, a, k->format);
+    if (k->head_dim == 128) return read_dim<128>(c, a, k->format);
+    return read_dim<256>(c, a, k->format);
 }
 
 }  // extern "C"
