@@ -90,6 +90,7 @@ __device__ __forceinline__ Span span_of(const Attn8Args& a, int it, int rows_per
     return s;
 }
 
+template <int WAVES>
 __device__ __forceinline__ int block_sum_scan(int v, int* wsum, int& total)
 {
     const int w = threadIdx.x >> 6;
@@ -100,7 +101,7 @@ __device__ __forceinline__ int block_sum_scan(int v, int* wsum, int& total)
     int before = 0;
     total = 0;
 #pragma unroll
-    for (int i = 0; i < kAttn8Waves; i++) {
+    for (int i = 0; i < WAVES; i++) {
         before += i < w ? wsum[i] : 0;
         total += wsum[i];
     }
@@ -140,12 +141,13 @@ __device__ __forceinline__ int parts_of(int nb, int G)
 
 // pre: LDS [items + 1], the items' blocks before each; least: 0, or mode 1 with
 // pieces of at least so many blocks; false: no work
+template <int WAVES = kAttn8Waves>
 __device__ __forceinline__ bool find_deal(const Attn8Args& a, int j, int rows_per_item, int* pre, Deal& d, int least = 0)
 {
-    __shared__ int wsum[kAttn8Waves];
+    __shared__ int wsum[WAVES];
     __shared__ Share found;
     const int tid = threadIdx.x;
-    const int per = (a.items + kAttn8Threads - 1) / kAttn8Threads;
+    const int per = (a.items + 64 * WAVES - 1) / (64 * WAVES);
     const int i0 = tid * per, i1 = min(a.items, i0 + per);
     int total;
     if (a.items == 1) {
@@ -153,7 +155,7 @@ __device__ __forceinline__ bool find_deal(const Attn8Args& a, int j, int rows_pe
     } else {
         int mine = 0;
         for (int i = i0; i < i1; i++) mine += span_of(a, i, rows_per_item).nb;
-        int at = block_sum_scan(mine, wsum, total);
+        int at = block_sum_scan<WAVES>(mine, wsum, total);
         for (int i = i0; i < i1; i++) {
             pre[i] = at;
             at += span_of(a, i, rows_per_item).nb;
@@ -178,7 +180,7 @@ __device__ __forceinline__ bool find_deal(const Attn8Args& a, int j, int rows_pe
             ws += n;
             slots += n > 1 ? n : 0;
         }
-        int w0 = block_sum_scan(ws, wsum, all), s0 = block_sum_scan(slots, wsum, all_slots);
+        int w0 = block_sum_scan<WAVES>(ws, wsum, all), s0 = block_sum_scan<WAVES>(slots, wsum, all_slots);
         if (j >= all) return false;
         if (j >= w0 && j < w0 + ws)
             for (int i = i0; i < i1; i++) {
@@ -402,12 +404,12 @@ __device__ __forceinline__ void put_row(const Attn8Args& a, const Span& sp, int 
 }
 
 // ------------------------------------------------------------------ host ---
-// workgroups of 256 threads that the card holds at once
+// workgroups that the card holds at once
 template <typename Kernel>
-int attn8_resident(Kernel k)
+int attn8_resident(Kernel k, int threads)
 {
     int per_cu = 0, dev = 0, cus = 0;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, k, kAttn8Threads, 0) != hipSuccess ||
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, k, threads, 0) != hipSuccess ||
         hipGetDevice(&dev) != hipSuccess ||
         hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
         return 256;

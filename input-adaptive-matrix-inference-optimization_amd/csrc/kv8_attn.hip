@@ -457,7 +457,7 @@ static int attn8_launch(Ctx* c, Attn8Args a)
     const int64_t items = (int64_t)a.groups * a.g.n_seq;
     IAM_REQUIRE(items * a.g.n_kv < ((int64_t)1 << 31), "attention_kv8: too many rows");
     a.items = (int)items;
-    static const int resident = attn8_resident(k_kv8_attn<HD, FMT, SPLIT, NT>);
+    static const int resident = attn8_resident(k_kv8_attn<HD, FMT, SPLIT, NT>, kAttn8Threads);
     a.target = (resident + a.g.n_kv - 1) / a.g.n_kv;
     a.planned = items <= kMaxItems;
     int64_t per_head = items;

@@ -4,26 +4,37 @@
 
 namespace iam {
 
-// An item is 128 rows, 32 of a wave.  The workgroup brings one block of K and V
-// at a time into LDS as fp16 operands, each wave a quarter (so that the widening
+// An item is 128 rows.  The workgroup brings one block of K and V at a time
+// into LDS as fp16 operands, each wave its share (so that the widening
 // of a number is paid once for 128 rows); the next block's bytes are on their
 // way meanwhile.  Bound by the matrix instructions (48 to 64 a block and 16
 // rows) and the softmax beside them, which two workgroups of a CU overlap: so
 // the low parts of an fp32 q are in LDS, or they would not both fit the
 // registers.  v_scale is taken into the probabilities' shift: o is kept in
 // units of one block's v_scale (v_unit), so that the products add onto o itself.
-constexpr int kRowsTiles = 2;                                  // of 16 rows, a wave
-constexpr int kRowsItem = 16 * kRowsTiles * kAttn8Waves;
-constexpr int kRowsLeast = 2;                                  // blocks of a workgroup where an item is split
+// Waves and tiles of 16 rows of each: two tiles share every operand read from
+// LDS, where the registers of two workgroups a CU hold them (500 tokens
+// behind 3.6k, heads of 128: 98 us, with 8 waves of one tile 110; heads of
+// 256, one KV head: 94 and 66).
+template <int HD>
+struct RowsShape {
+    static constexpr int TILES = HD <= 128 ? 2 : 1, WAVES = HD <= 128 ? 4 : 8;
+};
+constexpr int kRowsItem = 128;
+#ifndef LEAST
+#define LEAST 2
+#endif
+constexpr int kRowsLeast = LEAST;                              // blocks of a workgroup where an item is split
 
 template <int HD, int FMT, bool SPLIT>
-__global__ __launch_bounds__(kAttn8Threads, HD <= 128 ? 2 : 1) void k_kv8_attn_rows(Attn8Args a)
+__global__ __launch_bounds__(64 * RowsShape<HD>::WAVES, 2) void k_kv8_attn_rows(Attn8Args a)
 {
-    constexpr int NT = kRowsTiles, KS = HD / 32, DT = HD / 16, R = kRowsItem;
-    constexpr int RUNS = HD / 16, TILE = kBlk * HD, MINE = 2 * RUNS / kAttn8Waves;
+    constexpr int NT = RowsShape<HD>::TILES, W = RowsShape<HD>::WAVES, KS = HD / 32, DT = HD / 16, R = kRowsItem;
+    static_assert(16 * NT * W == R, "the waves' rows");
+    constexpr int RUNS = HD / 16, TILE = kBlk * HD, MINE = 2 * RUNS / W;
     constexpr int kPartWords = R * HD + 2 * R;
     __shared__ half8 tiles[4 * RUNS][64];        // K: operand (t, k) at KS t + k; V: (d, h) at 2 RUNS + 2 d + h
-    __shared__ half8 low[SPLIT ? kAttn8Waves : 1][SPLIT ? NT : 1][SPLIT ? KS : 1][64];
+    __shared__ half8 low[SPLIT ? W : 1][SPLIT ? NT : 1][SPLIT ? KS : 1][64];
     __shared__ int pre[kMaxItems + 1];
     __shared__ unsigned long long bad_s;         // open block: positions whose V is not finite
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, r16 = lane & 15;
@@ -32,7 +43,7 @@ __global__ __launch_bounds__(kAttn8Threads, HD <= 128 ? 2 : 1) void k_kv8_attn_r
     Deal deal{};
     Share sh{};
     if (a.planned) {
-        if (!find_deal(a, j, R, pre, deal, kRowsLeast)) return;
+        if (!find_deal<W>(a, j, R, pre, deal, kRowsLeast)) return;
         if (!next_share(a, pre, j, deal, sh)) return;
     } else {
         sh.item = a.items - 1 - j;   // the row groups with the longest contexts first
@@ -51,13 +62,14 @@ __global__ __launch_bounds__(kAttn8Threads, HD <= 128 ? 2 : 1) void k_kv8_attn_r
             if (tid == 0) bad_s = 0;
             __syncthreads();
 
-            u32x4 raw[MINE];   // runs 4 i + w of K, then of V
+            u32x4 raw[MINE];   // runs w, w + W, ... of K's and then V's
             auto fetch = [&](int b) __attribute__((always_inline)) {
                 const size_t at = cell_of(b) * (size_t)TILE + lane * 16;
 #pragma unroll
                 for (int i = 0; i < MINE; i++) {
-                    const uint8_t* t = i < MINE / 2 ? a.kt : a.vt;
-                    raw[i] = *reinterpret_cast<const u32x4*>(t + at + (size_t)((i % (MINE / 2)) * kAttn8Waves + w) * 1024);
+                    const int run = i * W + w;
+                    const uint8_t* t = run < RUNS ? a.kt : a.vt;
+                    raw[i] = *reinterpret_cast<const u32x4*>(t + at + (size_t)(run % RUNS) * 1024);
                 }
             };
             auto store = [&](int b) __attribute__((always_inline)) {
@@ -68,12 +80,12 @@ __global__ __launch_bounds__(kAttn8Threads, HD <= 128 ? 2 : 1) void k_kv8_attn_r
                     uint32_t bad = 0;
 #pragma unroll
                     for (int i = 0; i < MINE; i++) {
-                        const int run = (i % (MINE / 2)) * kAttn8Waves + w;
-                        const half8* o = reinterpret_cast<const half8*>((i < MINE / 2 ? a.ko : a.vo) + ob) + run * 128 + lane * 2;
+                        const int run = i * W + w;
+                        const half8* o = reinterpret_cast<const half8*>((run < RUNS ? a.ko : a.vo) + ob) + run % RUNS * 128 + lane * 2;
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
                             half8 x = o[h];
-                            if (i >= MINE / 2) {
+                            if (run >= RUNS) {
 #pragma unroll
                                 for (int e = 0; e < 8; e++)
                                     if ((__builtin_bit_cast(uint16_t, (_Float16)x[e]) & 0x7c00) == 0x7c00) {
@@ -81,22 +93,22 @@ __global__ __launch_bounds__(kAttn8Threads, HD <= 128 ? 2 : 1) void k_kv8_attn_r
                                         x[e] = (_Float16)0.0f;
                                     }
                             }
-                            tiles[(i < MINE / 2 ? 0 : 2 * RUNS) + 2 * run + h][lane] = x;
+                            tiles[2 * run + h][lane] = x;
                         }
                     }
                     if (bad) {
-                        unsigned long long m = 0;
-                        for (int e = 0; e < 16; e++)
-                            if (bad >> e & 1) m |= 1ull << ((e >> 3) * 32 + ((e >> 2) & 1) * 16 + g * 4 + (e & 3));
-                        atomicOr(&bad_s, m);
+                        // (the lane's run holds positions 4 g .. of each 16)
+                        const unsigned long long m = (unsigned long long)(bad & 15) | (unsigned long long)(bad >> 4 & 15) << 16 |
+                                                     (unsigned long long)(bad >> 8 & 15) << 32 | (unsigned long long)(bad >> 12) << 48;
+                        atomicOr(&bad_s, m << (g * 4));
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < MINE; i++) {
-                        const int run = (i % (MINE / 2)) * kAttn8Waves + w;
+                        const int run = i * W + w;
 #pragma unroll
                         for (int h = 0; h < 2; h++)
-                            tiles[(i < MINE / 2 ? 0 : 2 * RUNS) + 2 * run + h][lane] = operand<FMT>(raw[i], h);
+                            tiles[2 * run + h][lane] = operand<FMT>(raw[i], h);
                     }
                 }
             };
@@ -135,10 +147,11 @@ __global__ __launch_bounds__(kAttn8Threads, HD <= 128 ? 2 : 1) void k_kv8_attn_r
                 if (b + 1 < be) fetch(b + 1);
                 __syncthreads();
                 if (mine_there) {
-                    uint64_t bad = 0;
+                    uint32_t bad = 0;   // a bit for each of the lane's 16 positions
                     if (b == open_at) {
                         ksc = vsc = 1.0f;
-                        bad = bad_s;
+                        const unsigned long long m = bad_s >> (g * 4);
+                        bad = (uint32_t)(m & 15) | (uint32_t)(m >> 12 & 0xf0) | (uint32_t)(m >> 24 & 0xf00) | (uint32_t)(m >> 36 & 0xf000);
                     }
                     const half8(*tv)[64] = tiles + 2 * RUNS;
                     floatx4 s[NT][4];
@@ -191,15 +204,15 @@ __global__ __launch_bounds__(kAttn8Threads, HD <= 128 ? 2 : 1) void k_kv8_attn_r
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
                         const float f = mult[n] * ksc;
-                        uint32_t hidden = 0;   // a bit for each of the lane's 16 positions
+                        uint32_t hidden = 0;   // bits as in bad
                         if (edge) {
+                            const int from = lo[n] - (b * kBlk + g * 4), to = hi[n] - (b * kBlk + g * 4);
 #pragma unroll
                             for (int t = 0; t < 4; t++)
 #pragma unroll
                                 for (int i = 0; i < 4; i++) {
-                                    const int p = t * 16 + g * 4 + i;
-                                    if (bad >> p & 1) s[n][t][i] = NAN;
-                                    if (b * kBlk + p < lo[n] || b * kBlk + p > hi[n]) {
+                                    if (bad & 1u << (t * 4 + i)) s[n][t][i] = NAN;
+                                    if (t * 16 + i < from || t * 16 + i > to) {
                                         hidden |= 1u << (t * 4 + i);
                                         s[n][t][i] = -INFINITY;
                                     }
@@ -226,7 +239,7 @@ __global__ __launch_bounds__(kAttn8Threads, HD <= 128 ? 2 : 1) void k_kv8_attn_r
                             for (int t = 0; t < 4; t++)
 #pragma unroll
                                 for (int i = 0; i < 4; i++)
-                                    if (hidden >> (t * 4 + i) & 1) s[n][t][i] = 0.0f;   // also where f is 0 or NaN
+                                    if (hidden & 1u << (t * 4 + i)) s[n][t][i] = 0.0f;   // also where f is 0 or NaN
                         }
                         float sum = 0.0f;
 #pragma unroll
@@ -355,7 +368,7 @@ static int rows_launch(Ctx* c, Attn8Args a)
     const int64_t items = (int64_t)a.groups * a.g.n_seq;
     IAM_REQUIRE(items * a.g.n_kv < ((int64_t)1 << 31), "attention_kv8: too many rows");
     a.items = (int)items;
-    static const int resident = attn8_resident(k_kv8_attn_rows<HD, FMT, SPLIT>);
+    static const int resident = attn8_resident(k_kv8_attn_rows<HD, FMT, SPLIT>, 64 * RowsShape<HD>::WAVES);
     a.target = (resident + a.g.n_kv - 1) / a.g.n_kv;
     a.planned = items <= kMaxItems;
     int64_t per_head = items;
@@ -368,7 +381,7 @@ static int rows_launch(Ctx* c, Attn8Args a)
         a.joins = reinterpret_cast<int4*>(a.part + words);
     }
     const dim3 grid((unsigned)(per_head * a.g.n_kv));
-    IAM_TRY(launch(c, "kv8_attention", k_kv8_attn_rows<HD, FMT, SPLIT>, grid, dim3(kAttn8Threads), 0, a));
+    IAM_TRY(launch(c, "kv8_attention", k_kv8_attn_rows<HD, FMT, SPLIT>, grid, dim3(64 * RowsShape<HD>::WAVES), 0, a));
     if (!a.planned || per_head == 1) return IAM_OK;
     const dim3 join((unsigned)(items * a.g.n_kv * (R * (HD / 4) / kAttn8Threads)));
     return launch(c, "kv8_attention.join", k_kv8_join<HD, SPLIT>, join, dim3(kAttn8Threads), 0, a);
