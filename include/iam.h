@@ -373,7 +373,7 @@ typedef struct {
  * (iam_rope_table rounds the angle to fp32 first, as the reference does,
  * up to 0.004 radians off at position 100000; its tables have the same form
  * and serve iam_rope_tokens too).  rot_dim is even, 2 .. 1024; scaling may be
- * null (NONE).  table_dev is 8-byte aligned. */
+ * null (NONE).  table_dev is 8-byte aligned.  Blocking. */
 int iam_rope_scaled_table(iam_ctx* ctx, double theta, int rot_dim, int max_pos,
                           const iam_rope_scaling* scaling, float* table_dev);
 /* Rotary positions of n_tokens rows of n_heads heads: the first rot_dim of a
@@ -459,12 +459,12 @@ int iam_kv8_read(iam_ctx* ctx, const iam_kv8_cache* cache, const int* pos_dev, i
  * max_ctx: taken as max_ctx - 1) and sees positions 0 .. p, or the last
  * `window` of them if window > 0.  Query head h reads KV head h * n_kv /
  * n_heads.  The softmax takes scale * q.k (scale 0: 1 / sqrt(head_dim)).
- * Sums and the softmax in fp32 (the products of an fp32 q and of the
- * probabilities to 22 bits), one rounding to the type.  Sequences with a negative position give rows of zeros;
- * rows of tokens from count_dev[s] on (if not null) are left as they were.  An
- * infinity or a NaN makes the rows that see it NaN or infinite; in a full
- * block, all rows that see any token of the block's head.  out may be q
- * with the same stride. */
+ * Sums and the softmax in fp32 (an fp32 q enters the products to 22 bits, the
+ * probabilities to 21), one rounding to the type.  Sequences with a negative
+ * position give rows of zeros; rows of tokens from count_dev[s] on (if not
+ * null) are left as they were.  An infinity or a NaN makes the rows that see
+ * it NaN or infinite; in a full block, all rows that see any token of the
+ * block's head.  out may be q with the same stride. */
 int iam_attention_kv8(iam_ctx* ctx, const iam_kv8_cache* cache, const void* q_dev, int type, int n_heads,
                       int n_tokens, size_t q_stride, const int* pos_dev, const int* count_dev, int window,
                       float scale, void* out_dev, size_t out_stride);

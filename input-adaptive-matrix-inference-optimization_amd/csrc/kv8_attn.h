@@ -24,8 +24,9 @@ namespace iam {
 //                softmax's registers into the product without moving lanes.
 // Rows are in lanes (r), so the rescaling by 2^(m - m') is one factor a lane.
 // Precision: q and p are fp32; each is split into two fp16 parts, high and
-// low (22 bits), after a power of two that brings them near the top of fp16's
-// range, and both are multiplied (an fp16 or bf16 q needs one part).
+// low (22 bits of q, 21 of p), after a power of two that brings them near the
+// top of fp16's range, and both are multiplied (an fp16 or bf16 q needs one
+// part).
 constexpr int kAttn8Threads = 256, kAttn8Waves = 4;
 constexpr int kAlone = 2 * kAttn8Waves;   // blocks that one workgroup takes by itself: joining costs 4 us
 constexpr int kMinBlocks = 8;         // blocks of a workgroup where an item is split,
@@ -46,7 +47,7 @@ struct Attn8Args {
     const int* count;
     Kv8Geometry g;
     int type;
-    int heads, rep;          // query heads; of them per KV head
+    int rep;                 // query heads of a KV head
     int tokens, rows;        // of a sequence; rows = tokens * rep
     int groups;              // row groups of a sequence
     int items;               // n_seq * groups

@@ -482,9 +482,17 @@ static int attn8_few(Ctx* c, const Attn8Args& a)
     return attn8_launch<HD, FMT, SPLIT, 1>(c, a);
 }
 
-// Up to this many rows (tokens * query heads of a KV head) every wave takes
-// blocks of its own (this file); with more, rows of its own.
-static int few_rows(int head_dim) { return head_dim <= 128 ? 32 : 16; }
+// Up to this many rows of a sequence (tokens * query heads of a KV head) every
+// wave takes blocks of its own (this file), with more it takes rows of its own:
+// 16, one tile, or 64 where sequences and KV heads alone give the card enough
+// to do, so that the widening is not what counts (heads of 128, 8 KV heads,
+// 2000 tokens, 32 rows, us here and by rows: 1 to 2 sequences 25 and 19, 8
+// sequences 31 and 30, 16 36 and 41, 32 46 and 70; 64 rows of 16 sequences 43
+// and 53; 96 rows 83 and 61).
+static int few_rows(int head_dim, int64_t pairs)
+{
+    return head_dim <= 128 && pairs * 128 >= (int64_t)64 * head_dim ? 64 : 16;
+}
 
 template <int HD>
 static int attn8_dim(Ctx* c, const Attn8Args& a, int format)
@@ -544,7 +552,6 @@ extern "C" int iam_attention_kv8(iam_ctx* c, const iam_kv8_cache* k, const void*
     a.count = count;
     a.g = {k->n_seq, k->max_ctx, k->n_kv, kv8_blocks(k->max_ctx)};
     a.type = type;
-    a.heads = n_heads;
     a.rep = n_heads / k->n_kv;
     a.tokens = n_tokens;
     a.rows = n_tokens * a.rep;
@@ -552,7 +559,7 @@ extern "C" int iam_attention_kv8(iam_ctx* c, const iam_kv8_cache* k, const void*
     a.out_stride = out_stride;
     a.window = window;
     a.scale_log2 = (float)((scale > 0.0f ? (double)scale : 1.0 / std::sqrt((double)k->head_dim)) * 1.4426950408889634);
-    if (a.rows > few_rows(k->head_dim)) return attn8_rows(c, a, k->head_dim, k->format);
+    if (a.rows > few_rows(k->head_dim, (int64_t)k->n_seq * k->n_kv)) return attn8_rows(c, a, k->head_dim, k->format);
     if (k->head_dim == 64) return attn8_dim<64>(c, a, k->format);
     if (k->head_dim == 128) return attn8_dim<128>(c, a, k->format);
     return attn8_dim<256>(c, a, k->format);

@@ -21,10 +21,7 @@ struct RowsShape {
     static constexpr int TILES = HD <= 128 ? 2 : 1, WAVES = HD <= 128 ? 4 : 8;
 };
 constexpr int kRowsItem = 128;
-#ifndef LEAST
-#define LEAST 2
-#endif
-constexpr int kRowsLeast = LEAST;                              // blocks of a workgroup where an item is split
+constexpr int kRowsLeast = 2;                              // blocks of a workgroup where an item is split
 
 template <int HD, int FMT, bool SPLIT>
 __global__ __launch_bounds__(64 * RowsShape<HD>::WAVES, 2) void k_kv8_attn_rows(Attn8Args a)
@@ -184,19 +181,14 @@ __global__ __launch_bounds__(64 * RowsShape<HD>::WAVES, 2) void k_kv8_attn_rows(
                     const bool edge = b * kBlk + kBlk - 1 > see.hi_all || b * kBlk < see.lo_all;
                     // The probabilities carry vsc / v_unit, kept within [2^-6,
                     // 2^3] (a block of zeros: any): o's unit changes seldom.
-                    float ratio = vsc > 0.0f ? vsc / v_unit : 1.0f, turn = 1.0f;
-                    if (!(ratio <= 8.0f && ratio >= 0.015625f)) {
+                    float turn = 1.0f;
+                    if (vsc != vsc) {
+                        ksc = vsc;                 // NaN, for the rows that see the block
+                    } else if (vsc > 0.0f && !(vsc <= 8.0f * v_unit && vsc >= 0.015625f * v_unit)) {
                         turn = v_unit / vsc;       // o into the new unit
                         v_unit = vsc;
-                        ratio = 1.0f;
-                        if (!(vsc > 0.0f)) {       // NaN: through s, for the rows that see it
-                            turn = v_unit = 1.0f;
-                        }
                     }
-                    if (vsc != vsc) {
-                        ksc = vsc;
-                        v_unit = v_unit == v_unit ? v_unit : 1.0f;
-                    }
+                    const float ratio = vsc > 0.0f ? vsc / v_unit : 1.0f;
                     const float bias = kProbShift + log2f(ratio), back = 1.0f / ratio;
                     half8 ph[NT][2], pl[NT][2];
                     float alpha[NT];

@@ -94,7 +94,7 @@ def attention(q, k, v, pos, window=0, scale=0.0):
       factors: its error is at most (2 dim + 8) 2^-24 sum |q k| scale + 2^-22 of
       the same sum;
     - p = 2^x by an instruction good to 2^-22, x's own subtractions to 4 |s|
-      2^-24, and p held to 22 bits;
+      2^-24, and p held to 21 bits;
     - the sums over T positions, block by block: (64 + T / 64 + 8) 2^-24, twice
       (over p v and over p), and the rescalings of the running maximum, one
       rounding each (T / 64 + 8 at most)."""

@@ -291,6 +291,71 @@ def test_decode_step_as_it_is_used(iam, ctx):
     c.free()
 
 
+# sequences, tokens, heads, KV heads, width, longest: more items than the card
+# holds workgroups (taken as one row of blocks), more than are dealt out by
+# length, and the same by rows of a chunk
+@pytest.mark.parametrize("S,n,heads,kv,dim,longest", [(300, 1, 4, 2, 64, 400), (70, 1, 16, 8, 128, 900), (2100, 1, 2, 1, 64, 70),
+                                                      (30, 2, 32, 8, 64, 700), (2100, 20, 1, 1, 64, 70), (3, 150, 4, 1, 256, 500),
+                                                      (5, 70, 8, 4, 128, 333), (260, 20, 4, 2, 64, 130)])
+def test_many_sequences(iam, ctx, S, n, heads, kv, dim, longest):
+    rng = np.random.default_rng(S + n)
+    lengths = rng.integers(n, longest + 1, S)
+    lengths[:3] = [longest, n, min(max(n, 64), longest)]
+    c = fill(iam, ctx, rng, S, longest, kv, dim, "int8", lengths.tolist())
+    pos = (lengths - n).tolist()
+    pos[S // 2] = -1
+    got, _, val = attend(ctx, c, rng.normal(0, 1, (S, n, heads, dim)), "f32", pos)
+    assert (got[S // 2] == 0).all()
+    for s in set(range(0, S, max(1, S // 60))) | {0, 1, 2, S - 1}:
+        if pos[s] < 0:
+            continue
+        k, v = values(c, s)
+        rows = sorted({0, n - 1, n // 2})
+        for i in rows:
+            want, bound = P.attention(val[s, i:i + 1], k, v, pos[s] + i)
+            P.close(got[s, i:i + 1], want, bound, "f32")
+    c.free()
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_drawn(iam, ctx, seed):
+    """Shapes, windows, counts and types drawn over the whole range."""
+    rng = np.random.default_rng(1000 + seed)
+    kv, rep, dim = int(rng.choice([1, 2, 4, 8])), int(rng.choice([1, 2, 3, 4, 7, 8])), int(rng.choice([64, 128, 256]))
+    S = int(rng.integers(1, 6))
+    n = int(np.exp(rng.uniform(0, np.log(90))))
+    T = n + int(np.exp(rng.uniform(0, np.log(900))))
+    format, type = str(rng.choice(["int8", "e4m3"])), str(rng.choice(P.TYPES))
+    lengths = rng.integers(n, T + 1, S).tolist()
+    c = fill(iam, ctx, rng, S, T + int(rng.integers(0, 70)), kv, dim, format, lengths)
+    back = int(rng.integers(0, 40)) if rng.random() < 0.3 else 0       # tokens in the cache behind the queries
+    pos = [max(0, x - n - back) for x in lengths]
+    count = rng.integers(-1, n + 2, S).tolist() if rng.random() < 0.4 else None
+    window = int(rng.integers(1, T + 1)) if rng.random() < 0.4 else 0
+    q = rng.normal(0, 1, (S, n, kv * rep, dim)) * np.exp2(rng.integers(-6, 3))
+    check(ctx, c, q, type, pos, window=window, count=count, qpad=int(rng.choice([0, 0, 1, 8])), opad=int(rng.choice([0, 0, 3])))
+    c.free()
+
+
+def test_blocks_of_unlike_scales(iam, ctx):
+    """V from block to block 2^-20 to 2^12 of another, blocks of zeros among
+    them, for single tokens and by rows."""
+    rng = np.random.default_rng(20)
+    c = Cache(iam, ctx, 1, 64 * 12 + 10, 1, 128, "int8")
+    k, v = rng.normal(0, 1, (1, 64 * 12 + 5, 1, 128)), rng.normal(0, 1, (1, 64 * 12 + 5, 1, 128))
+    for b, e in enumerate([0, 8, -6, -20, 12, 0, -8, 3, -3, 1, 10, -10]):
+        v[:, 64 * b:64 * b + 64] *= 2.0 ** e
+    v[:, 64 * 5:64 * 6] = 0
+    k[:, 64 * 7:64 * 8] = 0
+    c.append(k, v, pos=[0])
+    for n in (1, 30, 200):
+        check(ctx, c, rng.normal(0, 1, (1, n, 4, 128)), "f32", [64 * 12 + 5 - n])
+    # windows that end in each of them alone
+    for b in range(12):
+        check(ctx, c, rng.normal(0, 1, (1, 20, 4, 128)), "f32", [64 * b + 44], window=21)
+    c.free()
+
+
 def test_refusals(iam, ctx):
     c = iam.Kv8Cache(ctx, 2, 64, 2, 64, "int8")
     n = 2 * 3 * 4 * 64
