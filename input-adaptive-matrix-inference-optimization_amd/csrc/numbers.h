@@ -50,10 +50,16 @@ inline bool overlaps(const void* a, size_t an, const void* b, size_t bn)
     return x < y + bn && y < x + an;
 }
 
-// bytes of `rows` rows of `width` values, `stride` values apart
+// bytes of `rows` rows of `width` values, `stride` values apart (2^62, which no
+// allocation holds, where they would not fit 64 bits)
 inline size_t rows_bytes(size_t rows, size_t width, size_t stride, size_t value)
 {
-    return rows ? ((rows - 1) * stride + width) * value : 0;
+    size_t n;
+    if (!rows) return 0;
+    if (__builtin_mul_overflow(rows - 1, stride, &n) || __builtin_add_overflow(n, width, &n) ||
+        __builtin_mul_overflow(n, value, &n))
+        return (size_t)1 << 62;
+    return std::min(n, (size_t)1 << 62);
 }
 
 }  // namespace iam

@@ -281,3 +281,19 @@ def test_refusals(iam, ctx):
     for b in (x, p, o1, o2):
         b.free()
     c.free()
+
+
+def test_rows_past_64_bits_are_refused(iam, ctx):
+    """641 * 6700417 - 1 is 2^32: rows 2^30 values apart end at 2^64 bytes, as
+    if they were one."""
+    c = iam.Kv8Cache(ctx, 641, 64, 1, 64, "int8")
+    x, pos = ctx.empty(64, np.float32), ctx.upload(np.full(641, -1, np.int32))
+    with pytest.raises(iam.IamError) as e:
+        c.append(x, x, "f32", 6700417, pos, stride=1 << 30)
+    assert e.value.code == iam.IAM_E_INVALID and "kv8_append k" in str(e.value)
+    with pytest.raises(iam.IamError) as e:
+        c.attention(x, "f32", 1, 6700417, pos, x, q_stride=1 << 30, out_stride=1 << 30)
+    assert e.value.code == iam.IAM_E_INVALID and "attention_kv8 q" in str(e.value)
+    for d in (x, pos):
+        d.free()
+    c.free()

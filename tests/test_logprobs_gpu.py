@@ -201,3 +201,14 @@ def test_refusals(iam, ctx):
         assert err.value.code == iam.IAM_E_INVALID, bad
     for b in (x, t, l, e, i, p):
         b.free()
+
+
+def test_rows_past_64_bits_are_refused(iam, ctx):
+    """2^27 rows 2^39 values apart end at 2^64 bytes, as if they were one."""
+    n = (1 << 27) + 1
+    x, t, l = ctx.empty(16, np.float32), ctx.empty(n, np.int32), ctx.empty(n, np.float32)
+    with pytest.raises(iam.IamError) as e:
+        ctx.token_logprobs(x, "f32", n, 16, t, l, stride=1 << 39)
+    assert e.value.code == iam.IAM_E_INVALID and "token_logprobs logits" in str(e.value)
+    for b in (x, t, l):
+        b.free()

@@ -160,3 +160,13 @@ def test_refusals(iam, ctx):
         assert e.value.code == iam.IAM_E_INVALID, (rot, n, theta, s)
     for d in (x, t, p, o):
         d.free()
+
+
+def test_rows_past_64_bits_are_refused(iam, ctx):
+    """(n_tokens - 1) * stride is a multiple of 2^64: the range would seem to be one row."""
+    x, t, p = ctx.empty(256, np.float32), ctx.empty(64 * 64, np.float32), ctx.upload(np.full(8, -1, np.int32))
+    with pytest.raises(iam.IamError) as e:
+        ctx.rope_tokens(x, "f32", (1 << 27) + 1, 2, 128, 64, "half", t, 64, p, x, x_stride=1 << 39, out_stride=1 << 39)
+    assert e.value.code == iam.IAM_E_INVALID and "rope_tokens x" in str(e.value)
+    for d in (x, t, p):
+        d.free()
