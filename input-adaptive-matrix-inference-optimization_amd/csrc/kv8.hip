@@ -386,6 +386,7 @@ static int read_dim(Ctx* c, const ReadArgs& a, int format)
 {
     if (a.tokens >= kReadBlocks) {
         const int units = std::min((a.tokens - 1 + kBlk - 1) / kBlk + 1, a.g.blocks);
+        IAM_REQUIRE((int64_t)units * a.g.n_kv < (1 << 23), "kv8_read: too many tokens at a time");
         const dim3 grid((unsigned)units * a.g.n_kv * 2, (unsigned)a.g.n_seq);
         return format == IAM_KV8_INT8 ? launch(c, "kv8_read", k_kv8_read_blocks<HD, IAM_KV8_INT8>, grid, dim3(256), 0, a)
                                       : launch(c, "kv8_read", k_kv8_read_blocks<HD, IAM_KV8_E4M3>, grid, dim3(256), 0, a);
@@ -462,6 +463,7 @@ int iam_kv8_append(iam_ctx* c, const iam_kv8_cache* k, const void* key, const vo
     a.stride = stride;
     // n tokens touch at most ceil((n - 1) / 64) + 1 blocks
     const int units = std::min((n_tokens - 1 + kBlk - 1) / kBlk + 1, kv8_blocks(k->max_ctx));
+    IAM_REQUIRE((int64_t)units * k->n_kv < (1 << 23), "kv8_append: too many tokens at a time");
     const dim3 grid((unsigned)units * k->n_kv * 2, (unsigned)k->n_seq);
     if (type == IAM_F32) return append_dim<float>(c, a, k, grid);
     if (type == IAM_F16) return append_dim<_Float16>(c, a, k, grid);

@@ -455,7 +455,7 @@ static int attn8_launch(Ctx* c, Attn8Args a)
     constexpr int R = 16 * NT;
     a.groups = (int)(((int64_t)a.rows + R - 1) / R);
     const int64_t items = (int64_t)a.groups * a.g.n_seq;
-    IAM_REQUIRE(items * a.g.n_kv < ((int64_t)1 << 31), "attention_kv8: too many rows");
+    IAM_REQUIRE(items * a.g.n_kv < ((int64_t)1 << 24), "attention_kv8: too many rows");
     a.items = (int)items;
     static const int resident = attn8_resident(k_kv8_attn<HD, FMT, SPLIT, NT>, kAttn8Threads);
     a.target = (resident + a.g.n_kv - 1) / a.g.n_kv;

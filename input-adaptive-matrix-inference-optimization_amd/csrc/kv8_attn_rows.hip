@@ -310,13 +310,13 @@ __global__ __launch_bounds__(64 * RowsShape<HD>::WAVES, 2) void k_kv8_attn_rows(
 template <int HD, bool SPLIT>
 __global__ __launch_bounds__(kAttn8Threads) void k_kv8_join(Attn8Args a)
 {
-    constexpr int R = kRowsItem, Q = HD / 4, ROWS = kAttn8Threads / Q, CH = R / ROWS, U = 8;
+    constexpr int R = kRowsItem, Q = HD / 4, ROWS = kAttn8Threads / Q, U = 8;
     constexpr int kPartWords = R * HD + 2 * R;
-    const int kvh = blockIdx.x % a.g.n_kv, u = blockIdx.x / a.g.n_kv, it = u / CH;
+    const int kvh = blockIdx.x % a.g.n_kv, u = blockIdx.x / a.g.n_kv, it = blockIdx.y;
     const int4 jn = a.joins[it];    // splits, first, base, step
     if (jn.x <= 1) return;
     const Span sp = span_of(a, it, R);
-    const int row = (u - it * CH) * ROWS + (int)threadIdx.x / Q, d = (int)threadIdx.x % Q * 4;
+    const int row = u * ROWS + (int)threadIdx.x / Q, d = (int)threadIdx.x % Q * 4;
     if (row >= sp.n_rows) return;
     const size_t step = (size_t)a.g.n_kv * kPartWords;
     const float* parts = a.part + (size_t)kvh * kPartWords;
@@ -358,7 +358,7 @@ static int rows_launch(Ctx* c, Attn8Args a)
     constexpr int R = kRowsItem;
     a.groups = (int)(((int64_t)a.rows + R - 1) / R);
     const int64_t items = (int64_t)a.groups * a.g.n_seq;
-    IAM_REQUIRE(items * a.g.n_kv < ((int64_t)1 << 31), "attention_kv8: too many rows");
+    IAM_REQUIRE(items * a.g.n_kv < ((int64_t)1 << 23), "attention_kv8: too many rows");
     a.items = (int)items;
     static const int resident = attn8_resident(k_kv8_attn_rows<HD, FMT, SPLIT>, 64 * RowsShape<HD>::WAVES);
     a.target = (resident + a.g.n_kv - 1) / a.g.n_kv;
@@ -375,7 +375,7 @@ static int rows_launch(Ctx* c, Attn8Args a)
     const dim3 grid((unsigned)(per_head * a.g.n_kv));
     IAM_TRY(launch(c, "kv8_attention", k_kv8_attn_rows<HD, FMT, SPLIT>, grid, dim3(64 * RowsShape<HD>::WAVES), 0, a));
     if (!a.planned || per_head == 1) return IAM_OK;
-    const dim3 join((unsigned)(items * a.g.n_kv * (R * (HD / 4) / kAttn8Threads)));
+    const dim3 join((unsigned)a.g.n_kv * (R * (HD / 4) / kAttn8Threads), (unsigned)items);
     return launch(c, "kv8_attention.join", k_kv8_join<HD, SPLIT>, join, dim3(kAttn8Threads), 0, a);
 }
 

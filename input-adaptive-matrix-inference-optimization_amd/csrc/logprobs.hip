@@ -471,6 +471,7 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
 // ------------------------------------------------------------------ host ---
 constexpr int kLpTarget = 2048;    // workgroups that fill the card: 8 on each of 256 CUs
 constexpr int kLpMaxSegs = 64;
+constexpr int kLpSlice = 1 << 22;  // rows of a launch (of 2^32 threads at most)
 
 template <typename T, int E>
 static int logprobs_launch(Ctx* c, LogprobArgs a)
@@ -490,18 +491,27 @@ static int logprobs_launch(Ctx* c, LogprobArgs a)
         a.part = c->lp_part;
         a.ctr = c->lp_ctr;
     }
-    IAM_REQUIRE((int64_t)a.rows * a.segs < ((int64_t)1 << 31), "token_logprobs: too many rows");
     const dim3 grid((unsigned)(a.rows * a.segs));
     return a.k ? launch(c, "token_logprobs", k_token_logprobs<T, E, true>, grid, dim3(kLpThreads), 0, a)
                : launch(c, "token_logprobs", k_token_logprobs<T, E, false>, grid, dim3(kLpThreads), 0, a);
 }
 
 template <typename T>
-static int logprobs_typed(Ctx* c, const LogprobArgs& a)
+static int logprobs_typed(Ctx* c, LogprobArgs a)
 {
-    // few values in all: smaller chunks, so that more workgroups share them
-    if ((int64_t)a.rows * a.vocab <= (int64_t)256 * kLpThreads * 32) return logprobs_launch<T, 8>(c, a);
-    return logprobs_launch<T, 32>(c, a);
+    for (int left = a.rows; left > 0; left -= kLpSlice) {
+        a.rows = std::min(left, kLpSlice);
+        // few values in all: smaller chunks, so that more workgroups share them
+        if ((int64_t)a.rows * a.vocab <= (int64_t)256 * kLpThreads * 32) IAM_TRY((logprobs_launch<T, 8>(c, a)));
+        else IAM_TRY((logprobs_launch<T, 32>(c, a)));
+        a.x = reinterpret_cast<const T*>(a.x) + a.rows * a.stride;
+        a.targets += a.rows;
+        a.lp += a.rows;
+        if (a.entropy) a.entropy += a.rows;
+        if (a.ids) a.ids += (size_t)a.rows * a.k;
+        if (a.top) a.top += (size_t)a.rows * a.k;
+    }
+    return IAM_OK;
 }
 
 }  // namespace iam

@@ -20,14 +20,14 @@ struct RopeFreqs {
 __global__ __launch_bounds__(256) void k_rope_table(const double* __restrict__ freqs, int pairs, int max_pos,
                                                     double magnitude, float2* __restrict__ table)
 {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
     const size_t n = (size_t)pairs * max_pos;
-    if (i >= n) return;
-    const size_t pos = i / (unsigned)pairs;
-    const double angle = (double)pos * freqs[i - pos * pairs];
-    double s, c;
-    sincos(angle, &s, &c);
-    table[i] = make_float2((float)(c * magnitude), (float)(s * magnitude));
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const size_t pos = i / (unsigned)pairs;
+        const double angle = (double)pos * freqs[i - pos * pairs];
+        double s, c;
+        sincos(angle, &s, &c);
+        table[i] = make_float2((float)(c * magnitude), (float)(s * magnitude));
+    }
 }
 
 // the angle of each pair for one position, and the rotation's factor
@@ -201,7 +201,7 @@ int iam_rope_scaled_table(iam_ctx* c, double theta, int rot, int max_pos, const 
     if (hipMemcpyAsync(dev, f.f, sizeof(double) * (rot / 2), hipMemcpyHostToDevice, c->stream) != hipSuccess)
         rc = fail(IAM_E_HIP, "rope_scaled_table: copy failed");
     if (rc == IAM_OK)
-        rc = launch(c, "rope_table", k_rope_table, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (const double*)dev,
+        rc = launch(c, "rope_table", k_rope_table, dim3((unsigned)std::min<size_t>((n + 255) / 256, 1 << 20)), dim3(256), 0, (const double*)dev,
                     rot / 2, max_pos, magnitude, reinterpret_cast<float2*>(table));
     if (hipStreamSynchronize(c->stream) != hipSuccess && rc == IAM_OK) rc = fail(IAM_E_HIP, "rope_scaled_table: sync failed");
     (void)ctx_free(c, dev);

@@ -157,6 +157,42 @@ def test_masked_and_not_finite(ctx, vocab):
     check(ctx, x[6:], "f32", [2], 6)
 
 
+@pytest.mark.parametrize("k,low,vocab", [(5, 4, 2 ** 21), (64, 63, 2 ** 17), (64, 63, 12000), (20, 3, 300000), (2, 1, 2 ** 21)])
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_largest_values_in_few_places(ctx, type, k, low, vocab):
+    """The largest values lie at every 64th run of 16 bytes, so that few
+    threads see them all; with ties in 16 bits."""
+    rng = np.random.default_rng(k)
+    x = rng.normal(0, 1, (2, vocab))
+    x += np.where(np.arange(vocab) // (4 if type == "f32" else 8) % 64 < low, 20.0, 0.0)
+    check(ctx, x, type, [1, vocab - 1], k)
+
+
+@pytest.mark.parametrize("k,vocab,numbers", [(64, 100000, 3), (5, 2 ** 20, 4), (8, 70, 0), (64, 2000, 63), (1, 9000, 0)])
+def test_fewer_numbers_than_alternatives(ctx, k, vocab, numbers):
+    """NaN but for a few values: those in order, then the first NaN."""
+    rng = np.random.default_rng(vocab)
+    x = np.full((3, vocab), np.nan)
+    for r in range(3):
+        at = np.sort(rng.choice(vocab, numbers, replace=False))
+        x[r, at] = rng.integers(0, 2, numbers)
+        if r == 2:
+            x[r, at] = -np.inf
+    val, l, e, ids, top = run(ctx, x, "f32", [0, 1, 2], k)
+    for r in range(3):
+        want = np.lexsort((np.arange(vocab), np.where(np.isnan(x[r]), 0, -np.nan_to_num(x[r], neginf=-9)), np.isnan(x[r])))
+        assert np.array_equal(ids[r], want[:k])
+    assert np.isnan(l).all() and np.isnan(top).all()
+
+
+def test_very_many_rows(ctx):
+    """More rows than one launch takes, without and with alternatives."""
+    rng = np.random.default_rng(11)
+    x = rng.normal(0, 2, (2 ** 22 + 77, 3)).astype(np.float32)
+    check(ctx, x, "f32", rng.integers(0, 3, len(x)), 0)
+    check(ctx, x, "f16", rng.integers(0, 3, len(x)), 2)
+
+
 def test_calls_repeat(ctx):
     rng = np.random.default_rng(6)
     a, b = logits(rng, 2, 100000), logits(rng, 300, 9000)
