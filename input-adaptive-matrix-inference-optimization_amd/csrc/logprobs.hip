@@ -43,28 +43,29 @@ __device__ __forceinline__ float key_value(uint64_t k)
 }
 
 // ---- the best k of a row's (or segment's) values
-// The k-th largest of 64 maxima (of four threads each) bounds the k-th largest
-// value from below, and few threads reach it: only their values are looked
-// at again, so that the pass over the logits itself needs no exchange.
+// The k-th largest of the threads' maxima bounds the k-th largest value from
+// below, and few threads reach it, most of them in one chunk alone: only those
+// values are looked at again, so that the pass over the logits itself needs no
+// exchange.
 constexpr int kLpCap = 1024;    // keys held at a time
 
 struct Top {
     uint64_t* keys;     // LDS [kLpCap]
     uint64_t* own;      // LDS [kLpThreads]: the threads' maxima
-    int* n;             // LDS [2]: keys there (may pass kLpCap: then only the first are); threads looked at
+    int* n;             // LDS [3]: keys there (may pass kLpCap: then only the first are); threads looked at
 };
 
 // how many of the 256 keys of own[] are larger than y
 __device__ __forceinline__ int larger(const uint64_t* own, uint64_t y)
 {
     int r = 0;
-#pragma unroll 32
+#pragma unroll 16
     for (int i = 0; i < kLpThreads; i++) r += own[i] > y;
     return r;
 }
 
-// Orders the n <= kLpCap distinct keys of t.keys; the best min(k, n) end up in
-// order in front.  Where there are many, the k-th best of the threads' best
+// Orders the n <= kLpCap keys of t.keys (distinct, but for places that hold 0:
+// nothing); the best min(k, n) end up in order in front.  Where there are many, the k-th best of the threads' best
 // keys first thins them out.
 __device__ __forceinline__ void lp_order(const Top& t, int n, int k)
 {
@@ -115,40 +116,42 @@ __device__ __forceinline__ void lp_order(const Top& t, int n, int k)
     __syncthreads();
 }
 
-__device__ __forceinline__ double lp_sum(double v, double* red)
-{
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double t = red[0];
-#pragma unroll
-    for (int w = 1; w < kLpWaves; w++) t += red[w];
-    return t;
-}
+// (m, z, s) of all threads from each one's, in every thread: a wave's first,
+// then those of the four (sums to m0 become sums to M: e^(m0 - M) times z, and
+// times s + (m0 - M) z)
+struct Sums {
+    float m;
+    double z, s;
 
-__device__ __forceinline__ float lp_max(float v, float* red)
+    __device__ __forceinline__ void raise(float M)
+    {
+        const float d = m == -INFINITY ? 0.0f : m - M;
+        const double f = m == -INFINITY ? (z != z ? NAN : 0.0) : (double)__builtin_amdgcn_exp2f(d * kLog2e);
+        s = f * (s + (double)d * z);
+        z = f * z;
+        m = M;
+    }
+};
+__device__ __forceinline__ void lp_join(float& m, double& z, double& s, Sums* red)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    Sums x{m, z, s};
+    x.raise(wave_max(m));
+    x.z = wave_sum(x.z);
+    x.s = wave_sum(x.s);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
     __syncthreads();
-    float t = red[0];
+    m = red[0].m;
 #pragma unroll
-    for (int w = 1; w < kLpWaves; w++) t = fmaxf(t, red[w]);
-    return t;
-}
-
-// (m, z, s) of all threads from each one's, in every thread
-__device__ __forceinline__ void lp_join(float& m, double& z, double& s, float* redf, double* redd)
-{
-    const float M = lp_max(m, redf);
-    const float d = m == -INFINITY ? 0.0f : m - M;
-    const double f = m == -INFINITY ? (z != z ? NAN : 0.0) : (double)__builtin_amdgcn_exp2f(d * kLog2e);
-    s = lp_sum(f * (s + (double)d * z), redd);
-    z = lp_sum(f * z, redd);
-    m = M;
+    for (int w = 1; w < kLpWaves; w++) m = fmaxf(m, red[w].m);
+    z = s = 0.0;
+#pragma unroll
+    for (int w = 0; w < kLpWaves; w++) {
+        Sums y = red[w];
+        y.raise(m);
+        z += y.z;
+        s += y.s;
+    }
 }
 
 // VEC values from place i on; outside [v0, v1), -inf
@@ -165,21 +168,32 @@ __device__ __forceinline__ void lp_load(const T* x, int i, int v0, int v1, float
     }
 }
 
-// The values of [v0, v1) that take(value) says, as keys behind the n there,
-// from the threads that `hot` lists (nh of them), whose first load is at place
-// o; t.n counts them all.
-template <typename T, int VEC, typename Take>
-__device__ __forceinline__ void lp_gather(const Top& t, const T* x, int o, int v0, int v1, const int* hot, int nh, Take take)
+// The values of [v0, v1) that take(value) says, as keys behind the n there, of
+// n1 threads in one chunk (from the front of `hot`: thread and chunk) and of n2
+// threads in all of them (from its back); t.n counts them all.  The first load
+// is at place o, a chunk has J for a thread.
+template <typename T, int VEC, int J, typename Take>
+__device__ __forceinline__ void lp_gather(const Top& t, const T* x, int o, int v0, int v1, const int* hot, int n1, int n2, Take take)
 {
     constexpr int B = 4;   // loads in flight
-    const int rounds = (v1 - o + kLpThreads * VEC - 1) / (kLpThreads * VEC), all = rounds * nh;
+    const int rounds = (v1 - o + kLpThreads * VEC - 1) / (kLpThreads * VEC), one = n1 * J, all = one + rounds * n2;
+#pragma unroll 1
     for (int i0 = 0; i0 < all; i0 += B * kLpThreads) {
         float v[B][VEC];
         int at[B];
 #pragma unroll
         for (int u = 0; u < B; u++) {
-            const int q = i0 + u * kLpThreads + (int)threadIdx.x, r = q / nh;
-            at[u] = q < all ? o + (r * kLpThreads + hot[q - r * nh]) * VEC : v1;
+            const int q = i0 + u * kLpThreads + (int)threadIdx.x;
+            int r, h;
+            if (q < one) {
+                h = hot[q / J];
+                r = (h >> 8) * J + q % J;
+                h &= 255;
+            } else {
+                r = (q - one) / max(n2, 1);
+                h = q < all ? hot[kLpThreads - 1 - (q - one - r * n2)] : 0;
+            }
+            at[u] = q < all ? o + (r * kLpThreads + h) * VEC : v1;
             lp_load<T, VEC>(x, at[u], v0, v1, v[u]);
         }
         if (*(volatile int*)t.n > kLpCap) continue;   // too many already
@@ -237,36 +251,67 @@ __device__ __forceinline__ int lp_first(const Top& t, const T* x, int o, int v0,
     return min(got, want);
 }
 
-// The best min(k, v1 - v0) keys of [v0, v1) in order in front of t.keys; m: the
-// largest value of the thread's own loads (from place o on, its part of every
-// 256 * VEC).  kept: the thread's E values, where the segment is one chunk
-// (`whole`): nothing is read again.
-template <typename T, int VEC, int E>
-__device__ __forceinline__ int lp_top(const Top& t, int* hot, const T* x, int o, int v0, int v1, float m, int k, bool whole,
-                                      const float* kept)
+// The thread's largest value of the segment, in which chunk that is, and the
+// largest one of its other chunks.
+struct Most {
+    float m = -INFINITY, other = -INFINITY;
+    int chunk = 0;
+
+    __device__ __forceinline__ void add(float g, int c)
+    {
+        other = fmaxf(other, fminf(m, g));
+        chunk = g > m ? c : chunk;
+        m = fmaxf(m, g);
+    }
+};
+
+// The best min(k, v1 - v0) keys of [v0, v1) in order in front of t.keys; most:
+// of the thread's own loads (from place o on, its part of every 256 * VEC).
+// kept: the thread's E values, where the segment is one chunk (`whole`):
+// nothing is read again.
+template <typename T, int VEC, int E, bool KEEP>
+__device__ __forceinline__ int lp_top(const Top& t, int* hot, const T* x, int o, int v0, int v1, const Most& most, int k,
+                                      bool whole, const float* kept)
 {
     const int tid = threadIdx.x, have = min(k, v1 - v0);
     float* lane_max = reinterpret_cast<float*>(t.own);   // [kLpWaves][64]
+    const float m = most.m;
     __syncthreads();
     lane_max[tid] = m;
-    if (tid == 0) t.n[0] = t.n[1] = 0;
+    if (tid < 3) t.n[tid] = 0;
     __syncthreads();
-    float g = lane_max[tid & 63];
+    // In each wave bit by bit, the largest number that k of the maxima reach: of
+    // 64 (each of four threads), or of all 256 where 64 would bound little (1024
+    // x 128001 bf16 with 64 alternatives 70 us, else 126; with 20 64 and 63).
+    uint32_t mine[kLpWaves];
 #pragma unroll
-    for (int w = 1; w < kLpWaves; w++) g = fmaxf(g, lane_max[w * 64 + (tid & 63)]);
-    // bit by bit, the largest number that k of the wave's 64 reach
-    const uint32_t mine = (uint32_t)(key_of(g, 0) >> 32);
+    for (int w = 0; w < kLpWaves; w++) mine[w] = (uint32_t)(key_of(lane_max[w * 64 + (tid & 63)], 0) >> 32);
     uint32_t kth = 0;
+    if (k <= 32) {
+        uint32_t g = mine[0];
 #pragma unroll
-    for (int bit = 31; bit >= 0; bit--) {
-        const uint32_t y = kth | 1u << bit;
-        if (__popcll(__ballot(mine >= y)) >= k) kth = y;
+        for (int w = 1; w < kLpWaves; w++) g = max(g, mine[w]);
+#pragma unroll
+        for (int bit = 31; bit >= 0; bit--) {
+            const uint32_t y = kth | 1u << bit;
+            if (__popcll(__ballot(g >= y)) >= k) kth = y;
+        }
+    } else {
+#pragma unroll 1
+        for (int bit = 31; bit >= 0; bit--) {
+            const uint32_t y = kth | 1u << bit;
+            int c = 0;
+#pragma unroll
+            for (int w = 0; w < kLpWaves; w++) c += __popcll(__ballot(mine[w] >= y));
+            if (c >= k) kth = y;
+        }
     }
     const float b = key_value((uint64_t)kth << 32);
-    if (m >= b) hot[atomicAdd(t.n + 1, 1)] = tid;
+    if (most.other >= b) hot[kLpThreads - 1 - atomicAdd(t.n + 2, 1)] = tid;
+    else if (m >= b) hot[atomicAdd(t.n + 1, 1)] = tid | most.chunk << 8;
     __syncthreads();
-    const int nh = t.n[1];
-    if (whole) {
+    const int n1 = t.n[1], n2 = t.n[2];
+    if (KEEP && whole) {
         if (m >= b) {
 #pragma unroll
             for (int e = 0; e < E; e++) {
@@ -279,16 +324,17 @@ __device__ __forceinline__ int lp_top(const Top& t, int* hot, const T* x, int o,
         }
         __syncthreads();
     } else {
-        lp_gather<T, VEC>(t, x, o, v0, v1, hot, nh, [&](float v) { return v >= b; });
+        lp_gather<T, VEC, E / VEC>(t, x, o, v0, v1, hot, n1, n2, [&](float v) { return v >= b; });
     }
     int n = t.n[0];
-    if (n > kLpCap) {
+    const bool many = n > kLpCap;
+    if (many) {
         // many equal values (a masked row's -inf): the larger ones, then the
         // first of the equal ones
         __syncthreads();
         if (tid == 0) t.n[0] = 0;
         __syncthreads();
-        lp_gather<T, VEC>(t, x, o, v0, v1, hot, nh, [&](float v) { return v > b; });
+        lp_gather<T, VEC, E / VEC>(t, x, o, v0, v1, hot, n1, n2, [&](float v) { return v > b; });
         n = t.n[0];
         __syncthreads();
         if (n > kLpCap) {
@@ -297,6 +343,7 @@ __device__ __forceinline__ int lp_top(const Top& t, int* hot, const T* x, int o,
             uint64_t last = ~0ull;
             for (n = 0; n < have; n++) {
                 uint64_t best = 0;
+#pragma unroll 1
                 for (int i = v0 + tid; i < v1; i += kLpThreads) {
                     const uint64_t y = key_of(to_f32(x[i]), i);
                     best = y < last && y > best ? y : best;
@@ -304,6 +351,7 @@ __device__ __forceinline__ int lp_top(const Top& t, int* hot, const T* x, int o,
                 __syncthreads();
                 t.own[tid] = best;
                 __syncthreads();
+#pragma unroll 4
                 for (int i = 0; i < kLpThreads; i++) best = t.own[i] > best ? t.own[i] : best;
                 last = best;
                 if (tid == 0) t.keys[n] = best;
@@ -311,10 +359,11 @@ __device__ __forceinline__ int lp_top(const Top& t, int* hot, const T* x, int o,
             __syncthreads();
             return have;
         }
-        if (n < have) n += lp_first<T, VEC>(t, x, o, v0, v1, n, have - n, [&](float v) { return v == b; });
     }
-    // fewer numbers than k: the first NaN
-    if (n < have) n += lp_first<T, VEC>(t, x, o, v0, v1, n, have - n, [](float v) { return v != v; });
+    // what is missing: the first that equal b, then the first NaN
+#pragma unroll 1
+    for (int nan = 0; nan < 2 && n < have; nan++)
+        if (nan || many) n += lp_first<T, VEC>(t, x, o, v0, v1, n, have - n, [&](float v) { return nan ? v != v : v == b; });
     lp_order(t, n, k);
     return have;
 }
@@ -333,20 +382,19 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
 {
     constexpr int VEC = 16 / (int)sizeof(T), J = E / VEC, CHUNK = kLpThreads * E;
     __shared__ uint64_t keys[TOP ? kLpCap : 1], own[TOP ? kLpThreads : 1];
-    __shared__ int hot[TOP ? kLpThreads : 1], counts[2];
+    __shared__ int hot[TOP ? kLpThreads : 1], counts[3];
     __shared__ int s_last;
-    __shared__ double redd[kLpWaves];
-    __shared__ float redf[kLpWaves];
+    __shared__ Sums red[kLpWaves];
     const int tid = threadIdx.x;
     const int row = a.segs == 1 ? blockIdx.x : blockIdx.x / a.segs, seg = blockIdx.x - row * a.segs;
     const T* x = reinterpret_cast<const T*>(a.x) + (size_t)row * a.stride;
     // Chunks start at multiples of 16 bytes in memory, before the row's (or
     // segment's) first value if need be: rows at 2-byte boundaries, read as
-    // they lie, took 69 us instead of 60 (1024 x 128000 bf16).
+    // they lie, took 9 us more (1024 x 128001 bf16, 54 us this way).
     const int off = (int)((uintptr_t)x / sizeof(T) % VEC);
     const int o = seg * a.per - off, v0 = max(o, 0), v1 = a.vocab - o > a.per ? o + a.per : a.vocab;
     float M = -INFINITY;            // the wave's
-    float most = -INFINITY;         // the thread's
+    Most most;                      // the thread's
     double z = 0.0, s = 0.0;        // the thread's, without the `ones` terms that are 1
     int ones = 0;
     float v[E];
@@ -367,7 +415,7 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
         float g = -INFINITY;
 #pragma unroll
         for (int e = 0; e < E; e++) g = fmaxf(g, v[e]);
-        most = fmaxf(most, g);
+        if constexpr (TOP) most.add(g, (c0 - o) / CHUNK);
         const float gw = wave_max(g);
         if (gw > M) {
             const float d = M == -INFINITY ? 0.0f : M - gw;
@@ -398,8 +446,8 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
     z += (double)ones;
     int have = 0;
     const Top top{keys, own, counts};
-    if constexpr (TOP) have = lp_top<T, VEC, E>(top, hot, x, o, v0, v1, most, a.k, v1 - o <= CHUNK, v);
-    lp_join(m, z, s, redf, redd);
+    if constexpr (TOP) have = lp_top<T, VEC, E, E == 8>(top, hot, x, o, v0, v1, most, a.k, v1 - o <= CHUNK, v);
+    lp_join(m, z, s, red);
     if (a.segs > 1) {
         const int words = 3 + a.k;
         double* mine = a.part + ((size_t)row * a.segs + seg) * words;
@@ -421,27 +469,21 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
             s = acc_peek(parts + tid * words + 2);
         }
         if constexpr (TOP) {
-            // segs * k <= kLpCap; missing keys (of short segments) are left out
+            // segs * k <= kLpCap; missing keys (of short segments) are 0
             uint64_t y[kLpCap / kLpThreads];
-            int c = 0;
 #pragma unroll
             for (int u = 0; u < kLpCap / kLpThreads; u++) {
                 const int i = u * kLpThreads + tid;
                 y[u] = i < a.segs * a.k
                            ? acc_peek(reinterpret_cast<unsigned long long*>(parts) + (size_t)(i / a.k) * words + 3 + i % a.k)
                            : 0;
-                c += y[u] != 0;
             }
-            if (tid == 0) counts[0] = 0;
-            __syncthreads();
-            int at = c ? atomicAdd(counts, c) : 0;
 #pragma unroll
             for (int u = 0; u < kLpCap / kLpThreads; u++)
-                if (y[u] != 0) keys[at++] = y[u];
-            __syncthreads();
-            lp_order(top, counts[0], a.k);
+                if (u * kLpThreads + tid < a.segs * a.k) keys[u * kLpThreads + tid] = y[u];
+            lp_order(top, a.segs * a.k, a.k);
         }
-        lp_join(m, z, s, redf, redd);
+        lp_join(m, z, s, red);
         if (tid == 0) a.ctr[row] = 0u;
     }
     const bool none = m == -INFINITY && z == 0.0;   // nothing but -inf
@@ -469,7 +511,10 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
 }
 
 // ------------------------------------------------------------------ host ---
-constexpr int kLpTarget = 2048;    // workgroups that fill the card: 8 on each of 256 CUs
+// workgroups that the rows are cut into segments for: 4 on each of 256 CUs (389
+// x 32000 fp32 15 us, 1024 x 128001 bf16 54; with 8 on each 16 and 62: a row's
+// join costs about as much as a segment)
+constexpr int kLpTarget = 1024;
 constexpr int kLpMaxSegs = 64;
 constexpr int kLpSlice = 1 << 22;  // rows of a launch (of 2^32 threads at most)
 
@@ -481,7 +526,11 @@ static int logprobs_launch(Ctx* c, LogprobArgs a)
     constexpr int VEC = 16 / (int)sizeof(T);
     const int off = a.rows == 1 || a.stride % VEC == 0 ? (int)((uintptr_t)a.x / sizeof(T) % VEC) : VEC - 1;
     const int chunks = (int)(((int64_t)a.vocab + off + CHUNK - 1) / CHUNK);
-    const int most = a.k ? std::min(kLpMaxSegs, kLpCap / a.k) : kLpMaxSegs;   // their keys are ordered together
+    // A row's segments' keys are ordered together, quickest up to 256 of them
+    // (64 x 32000 with 20 alternatives 15.7 us, with 320 keys 20.4), unless
+    // segments would be long (1 x 1000000 with 20: 31 us, with 1020 keys 19).
+    const int keys = (int64_t)chunks * a.k <= 8 * kLpThreads ? kLpThreads : kLpCap;
+    const int most = a.k ? std::min(kLpMaxSegs, keys / a.k) : kLpMaxSegs;
     const int want = std::max(1, std::min({chunks, most, kLpTarget / std::max(a.rows, 1)}));
     const int each = (chunks + want - 1) / want;
     a.segs = (chunks + each - 1) / each;
