@@ -61,6 +61,7 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
     constexpr int DC = NT * DT <= 8 ? DT : 8 / NT;   // dimension tiles the waves' sums meet in at a time
     constexpr int kPartWords = R * HD + 2 * R;       // a partial result: o of the rows there, m, l
     constexpr int PARTS = SPLIT ? 2 : 1;             // fp16 parts of q
+    constexpr int DD = 4 / NT;                       // dimension tiles whose products run side by side
     constexpr int MEET = kAttn8Waves * NT * DC * 64 * 16, RING = kAttn8Waves * 2 * TILE;
     static_assert(MEET >= kAttn8Threads * 24, "the joining sums fit");
     __shared__ __align__(1024) char lds[MEET > RING ? MEET : RING];
@@ -100,6 +101,18 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
                                     (unsigned)(be - 1 - bs) % (unsigned)sh.stride < kAttn8Waves;
             const float end_scale = end_inside ? a.ks[cell_of(be - 1)] : 0.0f;
 
+            // its loads go out before its scale is known, with all others
+            half8 kk[KS], vv[DT];
+            if (end_inside) {
+                const size_t ob = ((size_t)sp.seq * a.g.n_kv + kvh) * (size_t)TILE;
+                const half8* ko = reinterpret_cast<const half8*>(a.ko + ob) + lane * 2 + w * (HD / 64) * 128;
+                const half8* vo = reinterpret_cast<const half8*>(a.vo + ob) + lane * 2 + (w >> 1);
+#pragma unroll
+                for (int k = 0; k < KS; k++) kk[k] = ko[(k >> 1) * 128 + (k & 1)];
+#pragma unroll
+                for (int d = 0; d < DT; d++) vv[d] = vo[d * 128];
+            }
+
             Query<HD, SPLIT> query[NT];        // this lane's rows
 #pragma unroll
             for (int n = 0; n < NT; n++) query[n].load(a, sp, kvh, n * 16 + r16, g);
@@ -137,36 +150,39 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
             // go by their positions' s.
             const bool open_end = end_scale < 0.0f;
             if (open_end) {
-                const size_t ob = ((size_t)sp.seq * a.g.n_kv + kvh) * (size_t)TILE;
-                const half8* ko = reinterpret_cast<const half8*>(a.ko + ob) + lane * 2 + w * (HD / 64) * 128;
-                const half8* vo = reinterpret_cast<const half8*>(a.vo + ob) + lane * 2 + (w >> 1);
-                half8 kk[KS], vv[DT];
-#pragma unroll
-                for (int k = 0; k < KS; k++) kk[k] = ko[(k >> 1) * 128 + (k & 1)];
-#pragma unroll
-                for (int d = 0; d < DT; d++) vv[d] = vo[d * 128];
                 const int at = (be - 1) * kBlk + w * 16 + g * 4;   // the lane's 4 positions:
                 const bool upper = w & 1;                          // the second 4 of an operand's 8, or the first
+                // an exponent of all ones carries into its half's top bit
+                uint32_t ones = 0;
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const u32x4 x = __builtin_bit_cast(u32x4, vv[d]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) ones |= (x[e] & 0x7c007c00u) + 0x04000400u;
+                }
                 uint32_t bad = 0;
+                if (__any((ones & 0x80008000u) != 0)) {
 #pragma unroll
-                for (int d = 0; d < DT; d++)
+                    for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if ((__builtin_bit_cast(uint16_t, (_Float16)vv[d][e]) & 0x7c00) == 0x7c00) {
-                            bad |= 1u << e;
-                            vv[d][e] = (_Float16)0.0f;
-                        }
+                        for (int e = 0; e < 8; e++)
+                            if ((__builtin_bit_cast(uint16_t, (_Float16)vv[d][e]) & 0x7c00) == 0x7c00) {
+                                bad |= 1u << e;
+                                vv[d][e] = (_Float16)0.0f;
+                            }
 #pragma unroll
-                for (int x = 1; x < 16; x <<= 1) bad |= (uint32_t)__shfl_xor((int)bad, x, 64);
-                bad = upper ? bad >> 4 : bad;
+                    for (int x = 1; x < 16; x <<= 1) bad |= (uint32_t)__shfl_xor((int)bad, x, 64);
+                    bad = upper ? bad >> 4 : bad;
+                }
                 half8 ph[NT], pl[NT];
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    floatx4 s = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                    floatx4 sk[2] = {floatx4{0.0f, 0.0f, 0.0f, 0.0f}, floatx4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
                     for (int k = 0; k < KS; k++)
 #pragma unroll
-                        for (int x = 0; x < PARTS; x++) s = mfma(kk[k], qh[x][n][k], s);
+                        for (int x = 0; x < PARTS; x++) sk[k & 1] = mfma(kk[k], qh[x][n][k], sk[k & 1]);
+                    floatx4 s = sk[0] + sk[1];
                     float top = -INFINITY;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
@@ -214,16 +230,19 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int t = 0; t < 4; t++) s[n][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                // (sums of other tiles between two that add onto one)
 #pragma unroll
-                for (int t = 0; t < 4; t++)
+                for (int k = 0; k < KS; k++) {
+                    half8 ka[4];
 #pragma unroll
-                    for (int k = 0; k < KS; k++) {
-                        const half8 ka = operand<FMT>(run[t * (HD / 64) + (k >> 1)], k & 1);
+                    for (int t = 0; t < 4; t++) ka[t] = operand<FMT>(run[t * (HD / 64) + (k >> 1)], k & 1);
 #pragma unroll
-                        for (int n = 0; n < NT; n++)
+                    for (int x = 0; x < PARTS; x++)
 #pragma unroll
-                            for (int x = 0; x < PARTS; x++) s[n][t] = mfma(ka, qh[x][n][k], s[n][t]);
-                    }
+                        for (int t = 0; t < 4; t++)
+#pragma unroll
+                            for (int n = 0; n < NT; n++) s[n][t] = mfma(ka[t], qh[x][n][k], s[n][t]);
+                }
                 const bool edge = b * kBlk + kBlk - 1 > see.hi_all || b * kBlk < see.lo_all;
                 half8 ph[NT][2], pl[NT][2];
                 float alpha[NT], vsr[NT];
@@ -296,18 +315,26 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
                 read_tile<RUNS>(at_v, more, run);
                 if (more) fetch_tile<RUNS, NT == 1>(a.vt + cell_of(next) * (size_t)TILE, place_v);
 #pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    const half8 v0 = operand<FMT>(run[d], 0), v1 = operand<FMT>(run[d], 1);
+                for (int d = 0; d < DT; d += DD) {
+                    half8 v[2][DD];
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        floatx4 x = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-                        x = mfma(v0, ph[n][0], x);
-                        x = mfma(v1, ph[n][1], x);
-                        x = mfma(v0, pl[n][0], x);
-                        x = mfma(v1, pl[n][1], x);
+                    for (int h = 0; h < 2; h++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) o[n][d][i] = __builtin_fmaf(x[i], vsr[n], o[n][d][i]);
-                    }
+                        for (int e = 0; e < DD; e++) v[h][e] = operand<FMT>(run[d + e], h);
+                    floatx4 x[NT][DD];
+#pragma unroll
+                    for (int y = 0; y < 4; y++)
+#pragma unroll
+                        for (int e = 0; e < DD; e++)
+#pragma unroll
+                            for (int n = 0; n < NT; n++)
+                                x[n][e] = mfma(v[y & 1][e], (y < 2 ? ph : pl)[n][y & 1], y ? x[n][e] : floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 0; e < DD; e++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) o[n][d + e][i] = __builtin_fmaf(x[n][e][i], vsr[n], o[n][d + e][i]);
                 }
                 b = next;
             }
@@ -350,7 +377,8 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int d = 0; d < DC; d++) meet[w][n * DC + d][lane] = o[n][d0 + d] * mine[n];
+                    for (int d = 0; d < DC; d++)
+                        if (n * 16 + r16 < sp.n_rows) meet[w][n * DC + d][lane] = o[n][d0 + d] * mine[n];
                 __syncthreads();
 #pragma unroll
                 for (int u = 0; u < NT * DC / kAttn8Waves; u++) {
@@ -380,7 +408,8 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
                 uint32_t* ctr = a.ctr + (size_t)sh.item * a.g.n_kv + kvh;
                 if (acc_arrive(ctr, (uint32_t)sh.splits, &s_last)) {
                     constexpr int U = 8, Q = HD / 4;
-                    float* parts = a.part + (size_t)kvh * kPartWords;
+                    // offsets in 32 bits: the results of a full card are far smaller
+                    const uint32_t step32 = (uint32_t)step;
                     const int E = sp.n_rows * Q, KP = max(1, min(kAttn8Threads / E, sh.splits));
                     floatx4* jo = reinterpret_cast<floatx4*>(lds);
                     float* jml = reinterpret_cast<float*>(jo + kAttn8Threads);
@@ -397,10 +426,10 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
 #pragma unroll
                                 for (int u = 0; u < U; u++) {
                                     const int k = min(k0 + u * KP, sh.splits - 1);
-                                    float* p = parts + (k ? sh.base + k * sh.step : sh.first) * step;
-                                    pm[u] = acc_peek(p + R * HD + row);
-                                    pl[u] = acc_peek(p + R * HD + R + row);
-                                    px[u] = peek4(p + e * 4);
+                                    const uint32_t at = (uint32_t)kvh * kPartWords + (uint32_t)(k ? sh.base + k * sh.step : sh.first) * step32;
+                                    pm[u] = acc_peek(a.part + (at + R * HD + row));
+                                    pl[u] = acc_peek(a.part + (at + R * HD + R + row));
+                                    px[u] = peek4(a.part + (at + e * 4));
                                 }
                                 float t = jm;
 #pragma unroll
@@ -410,12 +439,12 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
                                 jl *= f0;
                                 jx *= f0;
 #pragma unroll
-                                for (int u = 0; u < U; u++)
-                                    if (k0 + u * KP < sh.splits) {
-                                        const float f = exp2_fast(pm[u] - safe);
-                                        jl += pl[u] * f;
-                                        jx += px[u] * f;
-                                    }
+                                for (int u = 0; u < U; u++) {
+                                    const float f = k0 + u * KP < sh.splits ? exp2_fast(pm[u] - safe) : 0.0f;
+                                    jl = __builtin_fmaf(pl[u], f, jl);
+#pragma unroll
+                                    for (int i = 0; i < 4; i++) jx[i] = __builtin_fmaf(px[u][i], f, jx[i]);
+                                }
                             }
                         if (KP > 1) {
                             jo[tid] = jx;
