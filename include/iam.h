@@ -443,7 +443,8 @@ int iam_kv8_reset(iam_ctx* ctx, const iam_kv8_cache* cache);
  * skips its sequence.  A sequence is appended to in order; going back (as
  * after rejected draft tokens) is allowed: where the position lies inside a
  * full block, the block's earlier tokens become open again as the values
- * that it stands for, rounded to fp16. */
+ * that it stands for, rounded to fp16.  A call's blocks times n_kv stay below
+ * 2^23 (here and in iam_kv8_read). */
 int iam_kv8_append(iam_ctx* ctx, const iam_kv8_cache* cache, const void* k_dev, const void* v_dev, int type,
                    int n_tokens, size_t kv_stride, const int* pos_dev, const int* count_dev);
 /* The values that positions pos_dev[s] .. pos_dev[s] + n_tokens - 1 stand for,
@@ -464,7 +465,8 @@ int iam_kv8_read(iam_ctx* ctx, const iam_kv8_cache* cache, const int* pos_dev, i
  * position give rows of zeros; rows of tokens from count_dev[s] on (if not
  * null) are left as they were.  An infinity or a NaN makes the rows that see
  * it NaN or infinite; in a full block, all rows that see any token of the
- * block's head.  out may be q with the same stride. */
+ * block's head.  out may be q with the same stride.  The rows of a sequence
+ * and KV head are taken in groups of 16 to 128: below 2^23 of them a call. */
 int iam_attention_kv8(iam_ctx* ctx, const iam_kv8_cache* cache, const void* q_dev, int type, int n_heads,
                       int n_tokens, size_t q_stride, const int* pos_dev, const int* count_dev, int window,
                       float scale, void* out_dev, size_t out_stride);
@@ -475,7 +477,8 @@ int iam_attention_kv8(iam_ctx* ctx, const iam_kv8_cache* cache, const void* q_de
  * null) and, for top_k > 0, the top_k most likely tokens, likeliest first,
  * equal logits by the lower token: top_ids_dev and top_logprobs_dev
  * [n_rows][top_k] (top_k at most min(vocab, 64); either may be null).
- * Sums in fp64, one rounding to fp32.  A row of nothing but -inf gives -inf
+ * Sums in fp64 (of at most 32 terms at a time in fp32), one rounding to fp32.
+ * A row of nothing but -inf gives -inf
  * and the entropy 0; a row with a NaN or +inf gives NaN for both and for the
  * alternatives' log probabilities (their tokens are ordered with NaN last). */
 #define IAM_LOGPROBS_MAX_TOP 64

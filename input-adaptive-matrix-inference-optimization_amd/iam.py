@@ -450,7 +450,7 @@ class Kv8Cache:
     and KV head, the open block in fp16) and the attention over it."""
 
     def __init__(self, ctx, n_seq, max_ctx, n_kv, head_dim, format="int8"):
-        self.ctx = ctx
+        self.ctx, kind = ctx, KV8_FORMATS[format]
         numbers, scales, opened = C.c_size_t(), C.c_size_t(), C.c_size_t()
         check(lib().iam_kv8_size(n_seq, max_ctx, n_kv, head_dim, C.byref(numbers), C.byref(scales), C.byref(opened)))
         self.parts = []
@@ -461,7 +461,7 @@ class Kv8Cache:
         except IamError:
             self.free()
             raise
-        self.desc = Kv8Desc(*[b.ptr for b in self.parts], n_seq, max_ctx, n_kv, head_dim, KV8_FORMATS[format])
+        self.desc = Kv8Desc(*[b.ptr for b in self.parts], n_seq, max_ctx, n_kv, head_dim, kind)
         self._at = C.addressof(self.desc)
         self.reset()
 
