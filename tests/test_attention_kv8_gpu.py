@@ -173,6 +173,40 @@ def test_not_finite(iam, ctx, type):
     c.free()
 
 
+@pytest.mark.parametrize("n,heads,kv,dim", [(1, 8, 2, 64), (4, 8, 2, 128), (2, 3, 1, 256), (16, 64, 32, 64)])
+@pytest.mark.parametrize("format", ["int8", "e4m3"])
+def test_not_finite_few_rows(iam, ctx, format, n, heads, kv, dim):
+    """The same for few rows: a poisoned block of K, of V, and tokens of the
+    open block, seen or behind or before what is seen."""
+    rng = np.random.default_rng(8)
+    S, T = 2, 64 * 5 + 30
+    c = Cache(iam, ctx, S, T, kv, dim, format)
+    k, v = rng.normal(0, 1, (S, T, kv, dim)), rng.normal(0, 1, (S, T, kv, dim))
+    k[0, 70, kv - 1, 0] = np.inf       # block 1 of K
+    v[1, 140, 0, 3] = np.nan           # block 2 of V
+    v[:, T - 10, kv - 1, 5] = -np.inf  # open
+    k[1, T - 3, 0, 5] = np.nan
+    c.append(k, v, pos=[0, 0])
+    h = np.arange(heads) // (heads // kv)
+    q = rng.normal(0, 1, (S, n, heads, dim))
+    for pos in (10, 63, 64 * 2 + 7, 64 * 4, T - 30, T - 10, T - 4, T - n):
+        for window in (0, 40, 100):
+            got, _, val = attend(ctx, c, q, "f16", [pos] * S, window=window)
+            for s in range(S):
+                kk, vv = values(c, s)
+                poison = ~np.isfinite(kk).all(-1) | ~np.isfinite(vv).all(-1)        # [T][kv]
+                if n == 1 or pos + n <= T:
+                    for i in range(n):
+                        p = min(pos + i, T - 1)
+                        lo = max(0, p - window + 1) if window else 0
+                        bad = poison[lo:p + 1].any(0)[h]
+                        assert np.array_equal(np.isfinite(got[s, i]).all(-1), ~bad), (pos, window, s, i)
+                want, bound = P.attention(val[s], np.nan_to_num(kk, posinf=0, neginf=0), np.nan_to_num(vv, posinf=0, neginf=0), pos, window)
+                fine = np.isfinite(got[s]).all(-1)
+                P.close(got[s][fine], want[fine], bound[fine], "f16")
+    c.free()
+
+
 def test_what_the_open_block_held_before(iam, ctx):
     """A slot used again: NaN of the sequence before behind the new one's end."""
     rng = np.random.default_rng(9)

@@ -243,6 +243,27 @@ def test_ends_of_the_cache(iam, ctx):
     c.free()
 
 
+@pytest.mark.parametrize("format", ["int8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_reads_at_any_place(iam, ctx, format, dim):
+    rng = np.random.default_rng(dim)
+    T, held = 230, 211
+    c = Cache(iam, ctx, 2, T, 3, dim, format)
+    c.append(rows(rng, 2, held, 3, dim), rows(rng, 2, held, 3, dim), pos=[0, 0])
+    stand = [[P.stands_for(x[s, :held], format)[0] for s in range(2)] for x in (c.k, c.v)]
+    for n in (1, 3, 4, 5, 63, 64, 65, 130, 300):
+        for first in ((0, 1), (13, 63), (64, 70), (-3, 200), (127, -64)):
+            for got, want in zip(c.read(first, n), stand):
+                for s in range(2):
+                    for i in range(n):
+                        p = first[s] + i
+                        if p < 0 or p >= T:
+                            assert (got[s, i] == 7.25).all()
+                        elif p < held:
+                            assert np.array_equal(got[s, i], want[s][p]), (n, p)
+    c.free()
+
+
 def test_refusals(iam, ctx):
     import ctypes as C
     for bad in ((0, 64, 1, 64), (65536, 64, 1, 64), (1, 0, 1, 64), (1, (1 << 24) + 1, 1, 64), (1, 64, 0, 64), (1, 64, 513, 64), (1, 64, 1, 96)):
