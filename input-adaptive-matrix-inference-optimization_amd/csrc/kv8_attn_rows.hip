@@ -8,20 +8,22 @@ namespace iam {
 // into LDS as fp16 operands, each wave its share (so that the widening
 // of a number is paid once for 128 rows); the next block's bytes are on their
 // way meanwhile.  Bound by the matrix instructions (48 to 64 a block and 16
-// rows) and the softmax beside them, which two workgroups of a CU overlap: so
-// the low parts of an fp32 q are in LDS, or they would not both fit the
+// rows) and the softmax beside them, which two workgroups of a CU overlap (a
+// block takes the two 3.7 us, half of it matrix instructions: 1 PFLOP/s with
+// the low parts; beside the blocks a call takes 28 us, half of that partial
+// results): so the low parts of an fp32 q are in LDS, or they would not both fit the
 // registers.  v_scale is taken into the probabilities' shift: o is kept in
 // units of one block's v_scale (v_unit), so that the products add onto o itself.
 // Waves and tiles of 16 rows of each: two tiles share every operand read from
 // LDS, where the registers of two workgroups a CU hold them (500 tokens
-// behind 3.6k, heads of 128: 98 us, with 8 waves of one tile 110; heads of
-// 256, one KV head: 94 and 66).
+// behind 3.6k, heads of 128: 80 us now; 8 waves of one tile took 12 % more.
+// Heads of 256, one KV head: two tiles 94 us, 8 waves of one 66).
 template <int HD>
 struct RowsShape {
     static constexpr int TILES = HD <= 128 ? 2 : 1, WAVES = HD <= 128 ? 4 : 8;
 };
 constexpr int kRowsItem = 128;
-constexpr int kRowsLeast = 2;                              // blocks of a workgroup where an item is split
+constexpr int kRowsLeast = 2;   // blocks of a workgroup where an item is split (4 and 8 were no faster)
 
 template <int HD, int FMT, bool SPLIT>
 __global__ __launch_bounds__(64 * RowsShape<HD>::WAVES, 2) void k_kv8_attn_rows(Attn8Args a)
@@ -41,7 +43,8 @@ __global__ __launch_bounds__(64 * RowsShape<HD>::WAVES, 2) void k_kv8_attn_rows(
     Share sh{};
     if (a.planned) {
         if (!find_deal<W>(a, j, R, pre, deal, kRowsLeast)) return;
-        if (!next_share(a, pre, j, deal, sh)) return;
+        if (deal.mode == 0) sh = deal.one;
+        else if (!next_share(a, pre, j, deal, sh)) return;
     } else {
         sh.item = a.items - 1 - j;   // the row groups with the longest contexts first
         sh.splits = 1;
@@ -60,8 +63,11 @@ __global__ __launch_bounds__(64 * RowsShape<HD>::WAVES, 2) void k_kv8_attn_rows(
             __syncthreads();
 
             u32x4 raw[MINE];   // runs w, w + W, ... of K's and then V's
+            float ks_next = 0.0f, vs_next = 0.0f;
             auto fetch = [&](int b) __attribute__((always_inline)) {
                 const size_t at = cell_of(b) * (size_t)TILE + lane * 16;
+                ks_next = a.ks[cell_of(b)];
+                vs_next = a.vs[cell_of(b)];
 #pragma unroll
                 for (int i = 0; i < MINE; i++) {
                     const int run = i * W + w;
@@ -139,8 +145,10 @@ __global__ __launch_bounds__(64 * RowsShape<HD>::WAVES, 2) void k_kv8_attn_rows(
             float v_unit = 1.0f;
             const bool mine_there = w * 16 * NT < sp.n_rows;   // the wave has rows
             for (int b = bs; b < be; b++) {
-                float ksc = a.ks[cell_of(b)], vsc = a.vs[cell_of(b)];
                 store(b);
+                // (they came with the bytes: a wait for them here would wait for
+                // the next block's, too)
+                float ksc = ks_next, vsc = vs_next;
                 if (b + 1 < be) fetch(b + 1);
                 __syncthreads();
                 if (mine_there) {
@@ -297,7 +305,7 @@ __global__ __launch_bounds__(64 * RowsShape<HD>::WAVES, 2) void k_kv8_attn_rows(
             }
         }
         if (a.planned && kvh == 0 && sh.from == 0 && tid == 0) a.joins[sh.item] = make_int4(sh.splits, sh.first, sh.base, sh.step);
-        if (!a.planned || !next_share(a, pre, j, deal, sh)) return;
+        if (!a.planned || deal.mode == 0 || !next_share(a, pre, j, deal, sh)) return;
         __syncthreads();   // LDS is used again
     }
 }
