@@ -24,18 +24,19 @@ __device__ __forceinline__ void fetch_tile(const uint8_t* src, char* lds)
 // wave's last YOUNGER vector memory instructions are done.  In one piece of
 // assembly with its waits: the compiler, which cannot tell the tiles apart,
 // would wait for every fetch in flight before any read.
+constexpr int kRun = 64 * 16;   // bytes of a wave's load
 template <int YOUNGER>
 __device__ __forceinline__ void read_runs(uint32_t at, u32x4* r)
 {
     asm volatile(
         "s_waitcnt vmcnt(%5)\n\t"
         "ds_read_b128 %0, %4\n\t"
-        "ds_read_b128 %1, %4 offset:1024\n\t"
-        "ds_read_b128 %2, %4 offset:2048\n\t"
-        "ds_read_b128 %3, %4 offset:3072\n\t"
+        "ds_read_b128 %1, %4 offset:%6\n\t"
+        "ds_read_b128 %2, %4 offset:%7\n\t"
+        "ds_read_b128 %3, %4 offset:%8\n\t"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
-        : "v"(at), "n"(YOUNGER)
+        : "v"(at), "n"(YOUNGER), "n"(kRun), "n"(2 * kRun), "n"(3 * kRun)
         : "memory");
 }
 // the whole tile; `more`: a younger tile of RUNS instructions is in flight
