@@ -58,7 +58,8 @@ struct Attn8Args {
     int window;
     float scale_log2;
     float* part;             // partial results of the split items
-    uint32_t* ctr;           // [items * n_kv] arrivals, zero on entry (left zero)
+    uint32_t* ctr;           // [(items + upper) * n_kv] arrivals, zero on entry (left zero)
+    int upper;               // slots of partial results; the results of groups of them lie behind
     int4* joins;             // [items] many rows: parts of an item and where they are
 };
 

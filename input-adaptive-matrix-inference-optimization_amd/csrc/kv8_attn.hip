@@ -49,6 +49,8 @@ __device__ __forceinline__ void read_tile(uint32_t at, bool more, u32x4* r)
     for (int i = 4; i < RUNS; i += 4) read_runs<63>(at + i * 1024, r + i);
 }
 
+constexpr int kRounds = 6;   // rounds of loads that one workgroup joins results in (2 to 8 alike, but for few parts)
+
 // SPLIT: q is fp32, in two parts.  NT: tiles of 16 query rows an item has.
 // A wave's K and V tiles come through its own two places in LDS: a tile is
 // read into registers as soon as it is there and its place fetched again at
@@ -405,15 +407,36 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
                 // The last of the item's workgroups to arrive joins their
                 // results: thread (k0, four values e) takes every KP-th
                 // one, 8 of their loads in flight, joined as blocks are; then
-                // the KP sums meet.
-                uint32_t* ctr = a.ctr + (size_t)sh.item * a.g.n_kv + kvh;
-                if (acc_arrive(ctr, (uint32_t)sh.splits, &s_last)) {
-                    constexpr int U = 8, Q = HD / 4;
-                    // offsets in 32 bits: the results of a full card are far smaller
-                    const uint32_t step32 = (uint32_t)step;
-                    const int E = sp.n_rows * Q, KP = max(1, min(kAttn8Threads / E, sh.splits));
-                    floatx4* jo = reinterpret_cast<floatx4*>(lds);
-                    float* jml = reinterpret_cast<float*>(jo + kAttn8Threads);
+                // the KP sums meet.  Where that would take one workgroup many
+                // rounds of loads, groups of about the root of their number
+                // are joined first, each by its last one (1 KV head of 256, 8
+                // query heads, 73769 tokens: 50 us, in groups 28.5; 1 of 128, 16
+                // query heads, 131000 tokens: 68 and 23).
+                constexpr int U = 8, Q = HD / 4;
+                // offsets in 32 bits: the results of a full card are far smaller
+                const uint32_t step32 = (uint32_t)step;
+                auto slot_of = [&](int k) { return k ? sh.base + k * sh.step : sh.first; };
+                const int E = sp.n_rows * Q, passes = (E + kAttn8Threads - 1) / kAttn8Threads;
+                const int wide = max(1, kAttn8Threads / E) * U;   // results that a round takes
+                const bool tree = passes * sh.splits > kRounds * wide;
+                int group = 1, groups = 1, q = 0;   // results of a group, groups, this one's
+                if (tree) {
+                    group = (int)ceilf(sqrtf((float)sh.splits));
+                    groups = up_div(sh.splits, group);
+                    q = (sh.slot == sh.first ? 0 : (sh.slot - sh.base) / sh.step) / group;
+                }
+                floatx4* jo = reinterpret_cast<floatx4*>(lds);
+                float* jml = reinterpret_cast<float*>(jo + kAttn8Threads);
+#pragma unroll 1
+                for (int level = tree ? 0 : 1; level < 2; level++) {
+                    const int n = level == 0 ? min(group, sh.splits - q * group) : tree ? groups : sh.splits;
+                    uint32_t* ctr = level == 0 ? a.ctr + ((size_t)a.items + slot_of(q * group)) * a.g.n_kv + kvh
+                                               : a.ctr + (size_t)sh.item * a.g.n_kv + kvh;
+                    if (!acc_arrive(ctr, (uint32_t)n, &s_last)) break;
+                    // the k-th result to join
+                    const int stride = level == 1 && tree ? group : 1, from = level == 0 ? q * group : 0;
+                    const int off = level == 1 && tree ? a.upper : 0;
+                    const int KP = max(1, min(kAttn8Threads / E, n));
                     for (int e0 = 0; e0 < E; e0 += kAttn8Threads) {
                         const int kp = KP > 1 ? tid / E : 0, e = KP > 1 ? tid - kp * E : e0 + tid;
                         const bool on = kp < KP && e < E;
@@ -421,13 +444,13 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
                         float jm = -INFINITY, jl = 0.0f;
                         floatx4 jx = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
                         if (on)
-                            for (int k0 = kp; k0 < sh.splits; k0 += U * KP) {
+                            for (int k0 = kp; k0 < n; k0 += U * KP) {
                                 float pm[U], pl[U];
                                 floatx4 px[U];
 #pragma unroll
                                 for (int u = 0; u < U; u++) {
-                                    const int k = min(k0 + u * KP, sh.splits - 1);
-                                    const uint32_t at = (uint32_t)kvh * kPartWords + (uint32_t)(k ? sh.base + k * sh.step : sh.first) * step32;
+                                    const int k = from + min(k0 + u * KP, n - 1) * stride;
+                                    const uint32_t at = (uint32_t)kvh * kPartWords + (uint32_t)(off + slot_of(k)) * step32;
                                     pm[u] = acc_peek(a.part + (at + R * HD + row));
                                     pl[u] = acc_peek(a.part + (at + R * HD + R + row));
                                     px[u] = peek4(a.part + (at + e * 4));
@@ -441,7 +464,7 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
                                 jx *= f0;
 #pragma unroll
                                 for (int u = 0; u < U; u++) {
-                                    const float f = k0 + u * KP < sh.splits ? exp2_fast(pm[u] - safe) : 0.0f;
+                                    const float f = k0 + u * KP < n ? exp2_fast(pm[u] - safe) : 0.0f;
                                     jl = __builtin_fmaf(pl[u], f, jl);
 #pragma unroll
                                     for (int i = 0; i < 4; i++) jx[i] = __builtin_fmaf(px[u][i], f, jx[i]);
@@ -456,6 +479,7 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
                                 float t = jm;
                                 for (int k = 1; k < KP; k++) t = fmaxf(t, jml[2 * (tid + k * E)]);
                                 const float safe = t == -INFINITY ? 0.0f : t, f0 = exp2_fast(jm - safe);
+                                jm = t;
                                 jl *= f0;
                                 jx *= f0;
                                 for (int k = 1; k < KP; k++) {
@@ -465,7 +489,18 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
                                 }
                             }
                         }
-                        if (on && kp == 0) put(row, (e - row * Q) * 4, jx, jl);
+                        if (on && kp == 0) {
+                            if (level == 1) {
+                                put(row, (e - row * Q) * 4, jx, jl);
+                            } else {
+                                float* up = a.part + (uint32_t)kvh * kPartWords + (size_t)(a.upper + slot_of(q * group)) * step32;
+                                put4(up + e * 4, jx);
+                                if (e == row * Q) {
+                                    acc_put(up + R * HD + row, jm);
+                                    acc_put(up + R * HD + R + row, jl);
+                                }
+                            }
+                        }
                     }
                     if (tid == 0) *ctr = 0u;
                 }
@@ -495,7 +530,9 @@ static int attn8_launch(Ctx* c, Attn8Args a)
         per_head = a.target;
         const int most = (kv8_blocks(a.g.max_ctx) + kAttn8Waves - 1) / kAttn8Waves;   // parts that an item can have
         if (items <= a.target / 8) per_head = std::min<int64_t>(per_head, items * most);
-        IAM_TRY(ensure_kv8_scratch(c, 2 * (size_t)per_head * a.g.n_kv * (R * HD + 2 * R), (size_t)items * a.g.n_kv));
+        // two results a workgroup, and as many of groups
+        a.upper = (int)(2 * per_head);
+        IAM_TRY(ensure_kv8_scratch(c, 2 * (size_t)a.upper * a.g.n_kv * (R * HD + 2 * R), (size_t)(items + a.upper) * a.g.n_kv));
         a.part = c->kv8_part;
         a.ctr = c->kv8_ctr;
     }

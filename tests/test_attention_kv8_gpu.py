@@ -371,6 +371,24 @@ def test_drawn(iam, ctx, seed):
     c.free()
 
 
+@pytest.mark.parametrize("S,n,heads,kv,dim,length", [(1, 1, 8, 1, 256, 73769), (1, 2, 8, 1, 256, 9001), (2, 1, 16, 1, 128, 30000),
+                                                     (3, 4, 4, 1, 64, 20011), (1, 16, 1, 1, 128, 50000)])
+def test_many_parts_of_one_sequence(iam, ctx, S, n, heads, kv, dim, length):
+    """Few KV heads and a long context: more parts than one workgroup joins at
+    once; twice, since the second call finds the first one's counters."""
+    rng = np.random.default_rng(length)
+    lengths = [length - 1000 * s for s in range(S)]
+    c = fill(iam, ctx, rng, S, length, kv, dim, "int8", lengths)
+    q = rng.normal(0, 1, (S, n, heads, dim)) * 2
+    pos = [x - n for x in lengths]
+    first = attend(ctx, c, q, "f32", pos)[1]
+    for _ in range(3):
+        assert np.array_equal(attend(ctx, c, q, "f32", pos)[1].view(np.uint32), first.view(np.uint32))
+    check(ctx, c, q, "f32", pos)
+    check(ctx, c, q, "bf16", pos, window=length // 2)
+    c.free()
+
+
 def test_blocks_of_unlike_scales(iam, ctx):
     """V from block to block 2^-20 to 2^12 of another, blocks of zeros among
     them, for single tokens and by rows."""
