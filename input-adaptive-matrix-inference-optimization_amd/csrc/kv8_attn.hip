@@ -555,10 +555,12 @@ static int attn8_few(Ctx* c, const Attn8Args& a)
 // to do, so that the widening is not what counts (heads of 128, 8 KV heads,
 // 2000 tokens, 32 rows, us here and by rows: 1 to 2 sequences 25 and 19, 8
 // sequences 31 and 30, 16 36 and 41, 32 46 and 70; 64 rows of 16 sequences 43
-// and 53; 96 rows 83 and 61).
+// and 53; 96 rows 83 and 61), and for heads of 64, where it costs half (32
+// rows, 1 KV head, 2048 tokens 11.5 and 14, 32768 17 and 28; 64 rows, 8 KV
+// heads, 8192 tokens 20 and 20).
 static int few_rows(int head_dim, int64_t pairs)
 {
-    return head_dim <= 128 && pairs * 128 >= (int64_t)64 * head_dim ? 64 : 16;
+    return head_dim == 64 || (head_dim == 128 && pairs >= 64) ? 64 : 16;
 }
 
 template <int HD>

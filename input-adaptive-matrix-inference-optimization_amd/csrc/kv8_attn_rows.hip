@@ -310,32 +310,39 @@ __global__ __launch_bounds__(64 * RowsShape<HD>::WAVES, 2) void k_kv8_attn_rows(
     }
 }
 
-// The split items' results joined: a workgroup takes 1024 values of an item
-// and KV head, a thread four, 8 of the partial results' loads in flight.  A
-// launch of its own, since a chunk's partial results are many (an item's 64 KB
+// The split items' results joined: 256 threads take 1024 values of an item and
+// KV head, a thread four, 8 of the partial results' loads in flight; PARTS
+// such groups take every PARTS-th result (4 where an item has more than 8 in
+// the mean: 32 rows over 32768 tokens 52 us with 1, 28 with 4; 500 tokens
+// behind 3600 80 and 85).  A launch of its own, since a chunk's partial results are many (an item's 64 KB
 // a workgroup): joined by the last workgroup to arrive, as for single tokens,
 // they took 100 us for 64 tokens behind 4000.
-template <int HD, bool SPLIT>
-__global__ __launch_bounds__(kAttn8Threads) void k_kv8_join(Attn8Args a)
+constexpr int kJoinThreads = 256;
+template <int HD, bool SPLIT, int PARTS>
+__global__ __launch_bounds__(kJoinThreads * PARTS) void k_kv8_join(Attn8Args a)
 {
-    constexpr int R = kRowsItem, Q = HD / 4, ROWS = kAttn8Threads / Q, U = 8;
+    constexpr int R = kRowsItem, Q = HD / 4, ROWS = kJoinThreads / Q, U = 8;
     constexpr int kPartWords = R * HD + 2 * R;
+    __shared__ floatx4 sx[PARTS > 1 ? PARTS : 1][PARTS > 1 ? kJoinThreads : 1];
+    __shared__ float sm[PARTS > 1 ? PARTS : 1][PARTS > 1 ? kJoinThreads : 1], sl[PARTS > 1 ? PARTS : 1][PARTS > 1 ? kJoinThreads : 1];
     const int kvh = blockIdx.x % a.g.n_kv, u = blockIdx.x / a.g.n_kv, it = blockIdx.y;
     const int4 jn = a.joins[it];    // splits, first, base, step
+    const int tid = threadIdx.x % kJoinThreads, part = threadIdx.x / kJoinThreads;
     if (jn.x <= 1) return;
     const Span sp = span_of(a, it, R);
-    const int row = u * ROWS + (int)threadIdx.x / Q, d = (int)threadIdx.x % Q * 4;
-    if (row >= sp.n_rows) return;
+    if (u * ROWS >= sp.n_rows) return;
+    const int row = u * ROWS + tid / Q, d = tid % Q * 4;
+    const bool there = row < sp.n_rows;
     const size_t step = (size_t)a.g.n_kv * kPartWords;
     const float* parts = a.part + (size_t)kvh * kPartWords;
     float jm = -INFINITY, jl = 0.0f;
     floatx4 jx = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k0 = 0; k0 < jn.x; k0 += U) {
+    for (int k0 = part; there && k0 < jn.x; k0 += U * PARTS) {
         float pm[U], pl[U];
         floatx4 px[U];
 #pragma unroll
         for (int i = 0; i < U; i++) {
-            const int k = min(k0 + i, jn.x - 1);
+            const int k = min(k0 + i * PARTS, jn.x - 1);
             const float* p = parts + (k ? jn.z + k * jn.w : jn.y) * step;
             pm[i] = p[R * HD + row];
             pl[i] = p[R * HD + R + row];
@@ -350,13 +357,32 @@ __global__ __launch_bounds__(kAttn8Threads) void k_kv8_join(Attn8Args a)
         jx *= f0;
 #pragma unroll
         for (int i = 0; i < U; i++)
-            if (k0 + i < jn.x) {
+            if (k0 + i * PARTS < jn.x) {
                 const float f = exp2_fast(pm[i] - safe);
                 jl += pl[i] * f;
                 jx += px[i] * f;
             }
     }
-    put_row<HD, SPLIT>(a, sp, kvh, row, d, jx, jl);
+    if constexpr (PARTS > 1) {
+        sx[part][tid] = jx;
+        sm[part][tid] = jm;
+        sl[part][tid] = jl;
+        __syncthreads();
+        if (part > 0) return;
+        float t = jm;
+#pragma unroll
+        for (int k = 1; k < PARTS; k++) t = fmaxf(t, sm[k][tid]);
+        const float safe = t == -INFINITY ? 0.0f : t, f0 = exp2_fast(jm - safe);
+        jl *= f0;
+        jx *= f0;
+#pragma unroll
+        for (int k = 1; k < PARTS; k++) {
+            const float f = exp2_fast(sm[k][tid] - safe);
+            jl += sl[k][tid] * f;
+            jx += sx[k][tid] * f;
+        }
+    }
+    if (there) put_row<HD, SPLIT>(a, sp, kvh, row, d, jx, jl);
 }
 
 // ------------------------------------------------------------------ host ---
@@ -383,8 +409,9 @@ static int rows_launch(Ctx* c, Attn8Args a)
     const dim3 grid((unsigned)(per_head * a.g.n_kv));
     IAM_TRY(launch(c, "kv8_attention", k_kv8_attn_rows<HD, FMT, SPLIT>, grid, dim3(64 * RowsShape<HD>::WAVES), 0, a));
     if (!a.planned || per_head == 1) return IAM_OK;
-    const dim3 join((unsigned)a.g.n_kv * (R * (HD / 4) / kAttn8Threads), (unsigned)items);
-    return launch(c, "kv8_attention.join", k_kv8_join<HD, SPLIT>, join, dim3(kAttn8Threads), 0, a);
+    const dim3 join((unsigned)a.g.n_kv * (R * (HD / 4) / kJoinThreads), (unsigned)items);
+    return per_head > 8 * items ? launch(c, "kv8_attention.join", k_kv8_join<HD, SPLIT, 4>, join, dim3(kJoinThreads * 4), 0, a)
+                                : launch(c, "kv8_attention.join", k_kv8_join<HD, SPLIT, 1>, join, dim3(kJoinThreads), 0, a);
 }
 
 template <int HD>
