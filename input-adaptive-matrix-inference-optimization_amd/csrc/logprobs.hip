@@ -550,8 +550,12 @@ static int logprobs_typed(Ctx* c, LogprobArgs a)
 {
     for (int left = a.rows; left > 0; left -= kLpSlice) {
         a.rows = std::min(left, kLpSlice);
-        // few values in all: smaller chunks, so that more workgroups share them
-        if ((int64_t)a.rows * a.vocab <= (int64_t)256 * kLpThreads * 32) IAM_TRY((logprobs_launch<T, 8>(c, a)));
+        // Smaller chunks for few values in all, so that more workgroups share
+        // them, and where large ones would be empty by a quarter of a row or
+        // more (1500 rows of 2425 bf16 with 1 alternative 16 us, with large
+        // chunks 21; of 12000 21 and 24; of 24000 29 and 28).
+        const int64_t large = (int64_t)kLpThreads * 32, empty = (a.vocab + large - 1) / large * large - a.vocab;
+        if (a.rows * (int64_t)a.vocab <= 256 * large || 4 * empty > a.vocab) IAM_TRY((logprobs_launch<T, 8>(c, a)));
         else IAM_TRY((logprobs_launch<T, 32>(c, a)));
         a.x = reinterpret_cast<const T*>(a.x) + a.rows * a.stride;
         a.targets += a.rows;

@@ -86,6 +86,15 @@ def test_many_rows(ctx, type):
     check(ctx, logits(rng, 2500, 8300), type, rng.integers(0, 8300, 2500), 3)
 
 
+@pytest.mark.parametrize("type", P.TYPES)
+@pytest.mark.parametrize("k", [0, 1, 33, 64])
+@pytest.mark.parametrize("rows,vocab", [(300, 16000), (1100, 8192), (90, 32001)])
+def test_many_values(ctx, type, k, rows, vocab):
+    """Large chunks: one, two and several of them, segments of one and more."""
+    rng = np.random.default_rng(rows)
+    check(ctx, logits(rng, rows, vocab), type, rng.integers(0, vocab, rows), k)
+
+
 @pytest.mark.parametrize("vocab", [1, 2, 7])
 def test_tiny_vocabularies(ctx, vocab):
     rng = np.random.default_rng(vocab)
