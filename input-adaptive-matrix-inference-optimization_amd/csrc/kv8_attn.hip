@@ -558,8 +558,16 @@ static int attn8_few(Ctx* c, const Attn8Args& a)
 // and 53; 96 rows 83 and 61), and for heads of 64, where it costs half (32
 // rows, 1 KV head, 2048 tokens 11.5 and 14, 32768 17 and 28; 64 rows, 8 KV
 // heads, 8192 tokens 20 and 20).
-static int few_rows(int head_dim, int64_t pairs)
+// Where no row sees more than 4 blocks (a small cache or window), parts and
+// their joining cost more than the widening: up to 128 rows, as long as they are
+// a workgroup a CU (256 tokens, 8 KV heads of 128: 20 to 128 rows of 4
+// sequences 14 and 16 to 19; 64 rows of 32 sequences, two a CU, 28 and 28).
+static int few_rows(const Attn8Args& a, int head_dim)
 {
+    const int64_t pairs = (int64_t)a.g.n_seq * a.g.n_kv;
+    const int64_t span = a.window > 0 ? ((int64_t)a.window + a.tokens + 2 * kBlk - 2) / kBlk : a.g.blocks;
+    const int tile = head_dim == 256 ? 16 : 32;
+    if (std::min<int64_t>(span, a.g.blocks) <= 4 && pairs * ((a.rows + tile - 1) / tile) <= 256) return 128;
     return head_dim == 64 || (head_dim == 128 && pairs >= 64) ? 64 : 16;
 }
 
@@ -628,7 +636,7 @@ extern "C" int iam_attention_kv8(iam_ctx* c, const iam_kv8_cache* k, const void*
     a.out_stride = out_stride;
     a.window = window;
     a.scale_log2 = (float)((scale > 0.0f ? (double)scale : 1.0 / std::sqrt((double)k->head_dim)) * 1.4426950408889634);
-    if (a.rows > few_rows(k->head_dim, (int64_t)k->n_seq * k->n_kv)) return attn8_rows(c, a, k->head_dim, k->format);
+    if (a.rows > few_rows(a, k->head_dim)) return attn8_rows(c, a, k->head_dim, k->format);
     if (k->head_dim == 64) return attn8_dim<64>(c, a, k->format);
     if (k->head_dim == 128) return attn8_dim<128>(c, a, k->format);
     return attn8_dim<256>(c, a, k->format);

@@ -351,6 +351,19 @@ def test_many_sequences(iam, ctx, S, n, heads, kv, dim, longest):
     c.free()
 
 
+@pytest.mark.parametrize("S,n,heads,kv,dim,T,window", [(1, 32, 8, 2, 128, 256, 0), (3, 11, 16, 2, 256, 130, 0), (2, 90, 2, 2, 64, 250, 0),
+                                                       (2, 30, 8, 2, 128, 3000, 90), (40, 16, 8, 2, 128, 200, 0), (1, 129, 1, 1, 128, 256, 0)])
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_many_rows_of_little_context(iam, ctx, type, S, n, heads, kv, dim, T, window):
+    """Small caches and windows, up to 128 rows and past them."""
+    rng = np.random.default_rng(T + n)
+    lengths = rng.integers(n, T + 1, S).tolist()
+    lengths[0] = T
+    c = fill(iam, ctx, rng, S, T, kv, dim, "int8", lengths)
+    check(ctx, c, rng.normal(0, 1, (S, n, heads, dim)), type, [x - n for x in lengths], window=window)
+    c.free()
+
+
 @pytest.mark.parametrize("seed", range(30))
 def test_drawn(iam, ctx, seed):
     """Shapes, windows, counts and types drawn over the whole range."""
