@@ -478,9 +478,9 @@ int iam_attention_kv8(iam_ctx* ctx, const iam_kv8_cache* cache, const void* q_de
  * equal logits by the lower token: top_ids_dev and top_logprobs_dev
  * [n_rows][top_k] (top_k at most min(vocab, 64); either may be null).
  * Sums in fp64 (of at most 32 terms at a time in fp32), one rounding to fp32.
- * A row of nothing but -inf gives -inf
- * and the entropy 0; a row with a NaN or +inf gives NaN for both and for the
- * alternatives' log probabilities (their tokens are ordered with NaN last). */
+ * A row of nothing but -inf gives -inf and the entropy 0; a row with a NaN or
+ * +inf gives NaN for both and for the alternatives' log probabilities (their
+ * tokens are ordered with NaN last). */
 #define IAM_LOGPROBS_MAX_TOP 64
 int iam_token_logprobs(iam_ctx* ctx, const void* logits_dev, int type, int n_rows, int vocab, size_t stride,
                        const int* targets_dev, float* logprob_dev, float* entropy_dev, int top_k,
