@@ -116,6 +116,15 @@ __device__ __forceinline__ void lp_order(const Top& t, int n, int k)
     __syncthreads();
 }
 
+// How far the maximum m lies below M, at most 200 (e^-200 is 0 in fp32): two
+// finite ones can be farther apart than the largest number, and the factor 0
+// times that infinity would be NaN.
+__device__ __forceinline__ float lp_below(float m, float M)
+{
+    const float d = m - M;
+    return d < -200.0f ? -200.0f : d;
+}
+
 // (m, z, s) of all threads from each one's, in every thread: a wave's first,
 // then those of the four (sums to m0 become sums to M: e^(m0 - M) times z, and
 // times s + (m0 - M) z)
@@ -125,7 +134,7 @@ struct Sums {
 
     __device__ __forceinline__ void raise(float M)
     {
-        const float d = m == -INFINITY ? 0.0f : m - M;
+        const float d = m == -INFINITY ? 0.0f : lp_below(m, M);
         const double f = m == -INFINITY ? (z != z ? NAN : 0.0) : (double)__builtin_amdgcn_exp2f(d * kLog2e);
         s = f * (s + (double)d * z);
         z = f * z;
@@ -418,7 +427,7 @@ __global__ __launch_bounds__(kLpThreads) void k_token_logprobs(LogprobArgs a)
         if constexpr (TOP) most.add(g, (c0 - o) / CHUNK);
         const float gw = wave_max(g);
         if (gw > M) {
-            const float d = M == -INFINITY ? 0.0f : M - gw;
+            const float d = M == -INFINITY ? 0.0f : lp_below(M, gw);
             const double f = (double)__builtin_amdgcn_exp2f(d * kLog2e);
             z += (double)ones;
             s = f * (s + (double)d * z);

@@ -141,6 +141,23 @@ def test_nearly_certain_and_far_values(ctx):
     check(ctx, x, "f32", [7, 3999, 0, 12, 2], 4)
 
 
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("k", [0, 4])
+@pytest.mark.parametrize("rows,vocab", [(1, 4096), (1, 70000), (400, 16384), (300, 40003)])
+def test_maxima_farther_apart_than_the_largest_number(ctx, type, k, rows, vocab):
+    """-3e38 and 3e38 in one row: their difference is past fp32's range, and
+    the maxima that a wave, the waves, or a row's segments join lie so far
+    apart.  By halves of a wave's loads, of a chunk, of a row, the low ones first
+    or last, one high value alone, in turn."""
+    x = np.full((rows, vocab), -3e38)
+    i = np.arange(vocab)
+    for r in range(rows):
+        high = (i >= vocab // 2, i < vocab // 2, i // 2048 % 2 == 1, i // 1024 % 2 == 0, i // 256 % 2 == 1, i // 4096 % 2 == 1,
+                i // 8192 % 2 == 1, i % 2 == 1, i == vocab - 1, i == 0)[r % 10 if rows > 1 else 0]
+        x[r, high] = 3e38
+    check(ctx, x, type, i[:rows] if rows > 1 else [vocab - 1], k)
+
+
 @pytest.mark.parametrize("vocab", [50, 20000])
 def test_masked_and_not_finite(ctx, vocab):
     rng = np.random.default_rng(5)
