@@ -189,6 +189,8 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
                     float top = -INFINITY;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
+                        // an infinite K (its sum of -inf would drop the position): NaN, by 0 * inf
+                        s[i] = __builtin_fmaf(s[i], 0.0f, s[i]);
                         s[i] = bad >> i & 1 ? NAN : s[i] * mult[n];
                         s[i] = at + i >= lo[n] && at + i <= hi[n] ? s[i] : -INFINITY;
                         top = fmaxf(top, s[i]);

@@ -211,6 +211,8 @@ __global__ __launch_bounds__(64 * RowsShape<HD>::WAVES, 2) void k_kv8_attn_rows(
                             for (int t = 0; t < 4; t++)
 #pragma unroll
                                 for (int i = 0; i < 4; i++) {
+                                    // an infinite K (its sum of -inf would drop the position): NaN, by 0 * inf
+                                    s[n][t][i] = __builtin_fmaf(s[n][t][i], 0.0f, s[n][t][i]);
                                     if (bad & 1u << (t * 4 + i)) s[n][t][i] = NAN;
                                     if (t * 16 + i < from || t * 16 + i > to) {
                                         hidden |= 1u << (t * 4 + i);

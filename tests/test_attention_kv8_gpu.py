@@ -207,6 +207,44 @@ def test_not_finite_few_rows(iam, ctx, format, n, heads, kv, dim):
     c.free()
 
 
+@pytest.mark.parametrize("n,heads,kv,dim", [(1, 8, 2, 64), (1, 4, 2, 128), (2, 6, 2, 256), (20, 12, 2, 128), (40, 16, 2, 64), (30, 4, 2, 256)])
+@pytest.mark.parametrize("type", P.TYPES)
+def test_infinite_keys_of_the_open_block(iam, ctx, type, n, heads, kv, dim):
+    """Keys past fp16's range (infinities) of both signs: every row that sees one
+    is NaN or infinite, whatever the sign of its query there, as it is
+    once the block is full; the others are as without them."""
+    rng = np.random.default_rng(21)
+    S, T = 2, 64 * 3
+    c = Cache(iam, ctx, S, T, kv, dim, "int8")
+    k, v = rng.normal(0, 1, (S, 120, kv, dim)), rng.normal(0, 1, (S, 120, kv, dim))
+    k[0, 70, 1, 5], k[0, 90, 0, dim - 1] = 1e6, -1e6
+    k[1, 85, 0, 3], k[1, 100, 1, 0] = -1e6, 1e6
+    c.append(k, v, pos=[0] * S)
+    q = rng.normal(0, 1, (S, n, heads, dim))
+    h = np.arange(heads) // (heads // kv)
+
+    def see(pos, window):
+        got, _, val = attend(ctx, c, q, type, [pos] * S, window=window)
+        for s in range(S):
+            kk, vv = values(c, s)
+            poison = ~np.isfinite(kk).all(-1)
+            for i in range(n):
+                lo = max(0, pos + i - window + 1) if window else 0
+                bad = poison[lo:pos + i + 1].any(0)[h]
+                assert np.array_equal(np.isfinite(got[s, i]).all(-1), ~bad), (pos, window, s, i)
+            want, bound = P.attention(val[s], np.nan_to_num(kk, posinf=0, neginf=0), vv, pos, window)
+            fine = np.isfinite(got[s]).all(-1)
+            P.close(got[s][fine], want[fine], bound[fine], type)
+
+    for pos in (66, 75, 120 - n):
+        for window in (0, 12):
+            see(pos, window)
+    more = rng.normal(0, 1, (S, 8, kv, dim))
+    c.append(more, more, pos=[120] * S)          # the block is full
+    see(128 - n, 0)
+    c.free()
+
+
 def test_what_the_open_block_held_before(iam, ctx):
     """A slot used again: NaN of the sequence before behind the new one's end."""
     rng = np.random.default_rng(9)
