@@ -463,10 +463,11 @@ int iam_kv8_read(iam_ctx* ctx, const iam_kv8_cache* cache, const int* pos_dev, i
  * Sums and the softmax in fp32 (an fp32 q enters the products to 22 bits, the
  * probabilities to 21), one rounding to the type.  Sequences with a negative
  * position give rows of zeros; rows of tokens from count_dev[s] on (if not
- * null) are left as they were.  An infinity or a NaN makes the rows that see
- * it NaN or infinite; in a full block, all rows that see any token of the
- * block's head.  out may be q with the same stride.  The rows of a sequence
- * and KV head are taken in groups of 16 to 128: below 2^23 of them a call. */
+ * null) are left as they were.  An infinity or a NaN in the cache makes the
+ * rows that see it NaN or infinite; in a full block, all rows that see any
+ * token of the block's head.  In a row of q it makes that row NaN.  out may be
+ * q with the same stride.  The rows of a sequence and KV head are taken in
+ * groups of 16 to 128: below 2^23 of them a call. */
 int iam_attention_kv8(iam_ctx* ctx, const iam_kv8_cache* cache, const void* q_dev, int type, int n_heads,
                       int n_tokens, size_t q_stride, const int* pos_dev, const int* count_dev, int window,
                       float scale, void* out_dev, size_t out_stride);

@@ -400,7 +400,9 @@ struct Query {
             }
         }
     }
-    // the operands' parts; the factor that takes the products to log2 units
+    // the operands' parts; the factor that takes the products to log2 units: NaN
+    // where a value is infinite, as scores that are all -inf would else be a
+    // row that sees nothing
     __device__ __forceinline__ float split(const Attn8Args& a, half8* high, half8* low)
     {
         float top = 0.0f;
@@ -421,7 +423,7 @@ struct Query {
                 high[k][e] = h;
                 if constexpr (SPLIT) low[k][e] = (_Float16)(x - (float)h);
             }
-        return ldexpf(a.scale_log2, ex - 10);
+        return top < INFINITY ? ldexpf(a.scale_log2, ex - 10) : NAN;
     }
 };
 

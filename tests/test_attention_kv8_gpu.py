@@ -245,6 +245,31 @@ def test_infinite_keys_of_the_open_block(iam, ctx, type, n, heads, kv, dim):
     c.free()
 
 
+@pytest.mark.parametrize("n,heads,kv,dim,T", [(1, 8, 2, 64, 50), (1, 4, 2, 128, 700), (2, 6, 2, 256, 128), (20, 12, 2, 128, 300),
+                                              (40, 16, 2, 64, 64), (30, 4, 2, 256, 90)])
+@pytest.mark.parametrize("type", P.TYPES)
+def test_infinite_queries(iam, ctx, type, n, heads, kv, dim, T):
+    """A query with an infinity is a row of NaN, also where all its scores are
+    -inf; the others are as without it."""
+    rng = np.random.default_rng(22)
+    c = Cache(iam, ctx, 1, T, kv, dim, "e4m3")
+    k, v = rng.normal(0, 1, (1, T, kv, dim)), rng.normal(0, 1, (1, T, kv, dim))
+    k[..., 3] = np.abs(k[..., 3]) + 1
+    c.append(k, v, pos=[0])
+    q = rng.normal(0, 1, (1, n, heads, dim))
+    bad = np.zeros((n, heads), bool)
+    for x in (-np.inf, np.inf):
+        i, j = int(rng.integers(n)), int(rng.integers(heads))
+        q[0, i, j, 3] = x
+        bad[i, j] = True
+    got, _, val = attend(ctx, c, q, type, [T - n])
+    assert np.array_equal(np.isnan(got[0]).all(-1), bad)
+    kk, vv = values(c, 0)
+    want, bound = P.attention(np.where(np.isfinite(val[0]), val[0], 0), kk, vv, T - n)
+    P.close(got[0][~bad], want[~bad], bound[~bad], type)
+    c.free()
+
+
 def test_what_the_open_block_held_before(iam, ctx):
     """A slot used again: NaN of the sequence before behind the new one's end."""
     rng = np.random.default_rng(9)
