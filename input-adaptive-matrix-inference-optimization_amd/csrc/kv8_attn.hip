@@ -123,6 +123,7 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
             float ksc = 0.0f, vsc = 0.0f;   // the scales of block b
             if (b < be) {   // (an open block's bytes are not looked at)
                 fetch_tile<RUNS, NT == 1>(a.kt + cell_of(b) * (size_t)TILE, place_k);
+                asm volatile("" ::: "memory");   // K's first: its wait counts V's as the younger ones
                 fetch_tile<RUNS, NT == 1>(a.vt + cell_of(b) * (size_t)TILE, place_v);
                 ksc = a.ks[cell_of(b)];
                 vsc = a.vs[cell_of(b)];
