@@ -28,11 +28,6 @@ __host__ __device__ __forceinline__ int v_place(int t, int d)
 {
     return ((d >> 4) * 64 + ((t >> 2) & 3) * 16 + (d & 15)) * 16 + (t >> 5) * 8 + ((t >> 4) & 1) * 4 + (t & 3);
 }
-template <int HD, bool IS_V>
-__host__ __device__ __forceinline__ int place(int t, int d)
-{
-    return IS_V ? v_place(t, d) : k_place<HD>(t, d);
-}
 
 // Four 8-bit numbers as fp16 (exact): two pairs, low bytes first.
 // INT8: the byte (number + 128) under the exponent of 1024 is 1024 + byte,
