@@ -478,7 +478,9 @@ int iam_attention_kv8(iam_ctx* ctx, const iam_kv8_cache* cache, const void* q_de
  * null) and, for top_k > 0, the top_k most likely tokens, likeliest first,
  * equal logits by the lower token: top_ids_dev and top_logprobs_dev
  * [n_rows][top_k] (top_k at most min(vocab, 64); either may be null).
- * Sums in fp64 (of at most 32 terms at a time in fp32), one rounding to fp32.
+ * The terms e^(x - max) and their products with x - max are fp32 (exponentials
+ * good to 2^-22 of a rounded argument), added up in fp32 for at most 32 at a
+ * time and in fp64 from there; one rounding to fp32.
  * A row of nothing but -inf gives -inf and the entropy 0; a row with a NaN or
  * +inf gives NaN for both and for the alternatives' log probabilities (their
  * tokens are ordered with NaN last). */

@@ -72,8 +72,11 @@ __device__ __forceinline__ void open_rows(uint16_t* open, const T* src, size_t s
 // where the sequence went back into it; the largest magnitude of all gives the
 // scale, and each run becomes 16 bytes.  A block that stays open gets its new
 // tokens in fp16.  Only the first block reads the open block and only the last
-// may write it, so unit 0 takes both, one after the other.  Bound by the
-// values read (and, for one token, by the launch).
+// may write it, so unit 0 takes both, one after the other.  4000 tokens of 8 x
+// 128 fp16 as e4m3 take 12.5 us, 24.6 MB (5 us at a copy's rate): all
+// workgroups run at once, and their loads do not hide the arithmetic, 29
+// instructions a value, the exact quotients above all (6 us), nor the 2-byte
+// reads of V's rows from LDS.  One token is bound by the launch.
 template <typename T, int HD, int FMT, bool IS_V>
 __device__ __forceinline__ void append_block(const AppendArgs& a, uint16_t* rows, float* red, int seq, int head, int block,
                                              int p0, int p1)

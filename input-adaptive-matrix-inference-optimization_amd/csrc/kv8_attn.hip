@@ -104,7 +104,9 @@ __global__ __launch_bounds__(kAttn8Threads, HD * NT <= 128 ? 2 : 1) void k_kv8_a
                                     (unsigned)(be - 1 - bs) % (unsigned)sh.stride < kAttn8Waves;
             const float end_scale = end_inside ? a.ks[cell_of(be - 1)] : 0.0f;
 
-            // its loads go out before its scale is known, with all others
+            // Its loads do not depend on its scale (as compiled, they wait for
+            // the scale's comparison all the same: a link of 0.8 us in the
+            // chain before the first tile).
             half8 kk[KS], vv[DT];
             if (end_inside) {
                 const size_t ob = ((size_t)sp.seq * a.g.n_kv + kvh) * (size_t)TILE;

@@ -7,16 +7,18 @@ namespace iam {
 // An item is 128 rows.  The workgroup brings one block of K and V at a time
 // into LDS as fp16 operands, each wave its share (so that the widening of a
 // number is paid once for 128 rows); the next block's bytes are on their way
-// meanwhile.  Bound by the matrix instructions (48 to 64 a block and 16 rows)
-// and the softmax beside them, which two workgroups of a CU overlap: a block
-// takes the two 3.7 us, half of it matrix instructions, 1 PFLOP/s with the low
-// parts; beside its blocks a call takes 25 us, half of that partial results.
+// meanwhile.  Bound by the softmax and the matrix instructions (48 to 64 a block
+// and 16 rows): of 67 us (500 tokens behind 3.6k, fp32) a SIMD's vector
+// instructions are busy 36 and its matrix units 26, and two workgroups of a CU
+// overlap little of them.  Beside its blocks a call takes 25 us, half of that
+// partial results.
 // The low parts of an fp32 q are in LDS, or two workgroups would not fit the
 // registers.  v_scale is taken into the probabilities' shift: o is kept in units
 // of one block's v_scale (v_unit), so that the products add onto o itself.
 // Waves and tiles of 16 rows of each: two tiles share every operand read from
-// LDS, where the registers of two workgroups a CU hold them (500 tokens
-// behind 3.6k, heads of 128: 80 us now; 8 waves of one tile took 12 % more.
+// LDS, where the registers of two workgroups a CU hold them, nearly: with heads
+// of 128 and an fp32 q, 4 (int8) and 2 (e4m3) vector registers are spilled (500
+// tokens behind 3.6k, heads of 128: 81 us; 8 waves of one tile took 12 % more.
 // Heads of 256, one KV head: two tiles 94 us, 8 waves of one 66).
 template <int HD>
 struct RowsShape {
