@@ -489,6 +489,121 @@ int iam_token_logprobs(iam_ctx* ctx, const void* logits_dev, int type, int n_row
                        const int* targets_dev, float* logprob_dev, float* entropy_dev, int top_k,
                        int* top_ids_dev, float* top_logprobs_dev);
 
+/* --------------------------------------- 4-bit weights and drafted tokens
+ * No counterpart in the reference, whose weights are fp16 and whose steps
+ * give one token each. */
+
+/* 8-bit number types of rows: signed whole numbers -127 .. 127, and e4m3 (as in
+ * IAM_KV8_E4M3, up to 448).  A number stands for number * scale. */
+#define IAM_I8 3
+#define IAM_E4M3 4
+
+/* A matrix of 4-bit weights, out_dim rows of in_dim.  Each row's inputs are
+ * taken in groups of `group` (32, 64 or 128; the last one may be short); weight
+ * (o, k) is scale * (n - zero) with n in 0 .. 15 and the scale (fp16) and the
+ * zero point (a whole number 0 .. 15; 8 for a matrix without zero points, where
+ * `zeros` is null) of row o's group.
+ *
+ * Device memory, the caller's (iam_q4_size says how much; every part 16-byte
+ * aligned), in the order in which the matrix instructions take it.  Rows come
+ * in strips of 16, inputs in tiles of 128 and chunks of four tiles:
+ *   numbers  [strip][tile][lane 16 g + row][step j] 4-byte words: inputs 32 j +
+ *            8 g + e of the tile, e = 0, 2, 4, 6, 1, 3, 5, 7 from the lowest
+ *            four bits on, each n xor 8
+ *   scales   fp16 [strip][chunk][row / 4][group of the chunk][row % 4]
+ *   zeros    bytes [strip][chunk][row][group of the chunk]
+ * What lies past the matrix in its last strip or chunk is 0. */
+typedef struct {
+    uint8_t* numbers;
+    uint16_t* scales;
+    uint8_t* zeros;
+    int out_dim;
+    int in_dim;
+    int group;
+} iam_q4_matrix;
+
+/* Bytes of each part (zeros: if there are any).  out_dim is at most 2^24,
+ * in_dim 2^20. */
+int iam_q4_size(int out_dim, int in_dim, int group, size_t* numbers, size_t* scales, size_t* zeros);
+/* Lays out a matrix once, from n as rows of ceil(in_dim / 2) bytes (input 2 i in
+ * the low half of byte i), scales fp16 and zero points (bytes; null if
+ * matrix->zeros is) as rows of ceil(in_dim / group).  The sources are not
+ * needed afterwards. */
+int iam_q4_pack(iam_ctx* ctx, const iam_q4_matrix* matrix, const uint8_t* n_dev, const uint16_t* scale_dev,
+                const uint8_t* zero_dev);
+/* Rounds the rows of a matrix in a float type (w_stride values apart, 0: in_dim)
+ * to 4 bits.  Without zero points scale = fp16(largest magnitude / 7); with them,
+ * low and high being the group's smallest and largest weight and 0, scale =
+ * fp16((high - low) / 15) and zero = round(-low / scale), at most 15.  n =
+ * round(w / scale) + zero, kept in 0 .. 15; quotients in fp32, halves to even.
+ * A group whose scale is not finite has the scale NaN; one whose scale is 0
+ * stands for zeros. */
+int iam_q4_quantize(iam_ctx* ctx, const iam_q4_matrix* matrix, const void* w_dev, int type, size_t w_stride);
+/* What rows first_row .. first_row + n_rows - 1 stand for, as fp32 rows of
+ * in_dim (exact: 11 bits times 5). */
+int iam_q4_read(iam_ctx* ctx, const iam_q4_matrix* matrix, int first_row, int n_rows, float* out_dev);
+/* Products of n_rows rows of in_dim values with the matrix: y[r][o] = sum over k
+ * of x[r][k] * weight (o, k).  Rows are x_stride / y_stride values apart (0: no
+ * gaps).  x is of a float type (x_scale_dev null), or in 8 bits with fp32 scales
+ * x_scale_dev [n_rows][1] (x_group 0) or [n_rows][ceil(in_dim / 128)] (x_group
+ * 128).  y is of a float type, rounded once.  Products of whole numbers are
+ * exact and sums fp32; a float row enters to 22 bits of the largest value of
+ * its 128 inputs or better.  Matrices that share their input are one matrix of
+ * their rows.  A row of x that holds an infinity or a NaN (or a scale that is
+ * one) gives infinities and NaN in its own row of y only.  y may not overlap
+ * the inputs. */
+int iam_q4_mul(iam_ctx* ctx, const iam_q4_matrix* matrix, const void* x_dev, int x_type, size_t x_stride,
+               const float* x_scale_dev, int x_group, int n_rows, void* y_dev, int y_type, size_t y_stride);
+
+/* Root-mean-square norm of n_rows rows of dim values, with the residual's
+ * addition before it.  h = x + residual (fp32, rounded to residual_type, which
+ * is x's type or IAM_F32; h = x where residual_dev is null), kept in sum_dev if
+ * that is not null; y = h / sqrt(mean of h^2 + eps) * gain (fp16, null: 1) in
+ * fp64, rounded once to out_type: a float type, or IAM_I8 / IAM_E4M3 with
+ * scale = fp32(largest magnitude / 127 or 448) of the row (group 0) or of each
+ * 128 values (group 128) in scale_dev [n_rows][groups], and the number nearest
+ * to y / scale (halves to even; 0 where the scale is 0).  Where y is infinite
+ * or NaN the scale of its group is NaN and the group's numbers are 0.  Rows are
+ * x_stride, residual_stride (sum_dev too) and out_stride values apart (0: dim).
+ * sum_dev may be residual_dev; with a float out_type of x's type out_dev may be
+ * x_dev with the same stride.  No other overlaps.  dim is at most 2^20. */
+int iam_rmsnorm_rows(iam_ctx* ctx, const void* x_dev, int type, size_t x_stride, const void* residual_dev,
+                     int residual_type, size_t residual_stride, void* sum_dev, int n_rows, int dim,
+                     const uint16_t* gain_dev, float eps, void* out_dev, int out_type, size_t out_stride,
+                     float* scale_dev, int group);
+/* The values that 8-bit rows (stride values apart, 0: dim) stand for, as fp32
+ * rows of dim: number * scale. */
+int iam_rows8_read(iam_ctx* ctx, const void* x_dev, int type, size_t stride, const float* scale_dev, int group,
+                   int n_rows, int dim, float* out_dev);
+
+/* Judges drafted tokens.  Sequence s has drafted tokens tokens_dev[s][i], i <
+ * n_draft (the first count_dev[s] of them where count_dev is not null), and
+ * n_draft + 1 rows of the target's logits, target_stride values apart (0:
+ * vocab), row i of the place that token i was drafted for.  With p_i the softmax
+ * of row i / temperature and q_i that of the draft's logits for the same place
+ * / draft_temperature ([n_seq][n_draft] rows draft_stride apart; draft_dev null:
+ * q_i is 1 at token i), token i is accepted if uniform_dev[s][i] * q_i(token) <
+ * p_i(token).  Of the a tokens before the first rejected one (all, if none is)
+ * out_dev[s][0 .. a-1] are copies; out_dev[s][a] is drawn from max(p_a - q_a, 0)
+ * if token a was rejected, else from p_a: the lowest token whose weights up to
+ * it add up to more than uniform_dev[s][n_draft] times all of them (or the last
+ * one of any weight).  The rest of out_dev [n_seq][n_draft + 1] is -1;
+ * accepted_dev[s] = a.  All in fp64 from the logits on.
+ * temperature 0: token i is accepted if it is the first largest logit of row i,
+ * which also is the one that follows; no random numbers or drafts' logits are
+ * read (both pointers may be null).
+ * A drafted token outside the vocabulary is rejected (q_i is then taken as 0).
+ * A row of the target with a NaN, a +inf or nothing but -inf has no
+ * distribution: its token is rejected, and the one that follows is -1.  Where
+ * the draft's row has none the token is rejected and the next is drawn from p,
+ * as it is where p - q is nowhere positive.  temperatures are 2^-64 to 2^64
+ * (or 0, as above); n_draft 0 .. 64; random numbers lie in [0, 1). */
+#define IAM_VERIFY_MAX_DRAFT 64
+int iam_verify_drafts(iam_ctx* ctx, const void* target_dev, int target_type, size_t target_stride,
+                      const void* draft_dev, int draft_type, size_t draft_stride, int n_seq, int n_draft, int vocab,
+                      double temperature, double draft_temperature, const int* tokens_dev, const int* count_dev,
+                      const float* uniform_dev, int* out_dev, int* accepted_dev);
+
 /* -------------------------------------------------------- synthetic data */
 
 /* Counter-based generator shared with the CPU oracle: element n of tensor

@@ -131,6 +131,12 @@ struct Ctx {
     size_t lp_part_cap = 0;
     uint32_t* lp_ctr = nullptr;
     size_t lp_ctr_cap = 0;
+    // verification of drafted tokens: the rows' results and arrival counters
+    // (zero between calls)
+    double* ver_part = nullptr;
+    size_t ver_part_cap = 0;
+    uint32_t* ver_ctr = nullptr;
+    size_t ver_ctr_cap = 0;
     // bumped whenever a context-owned scratch buffer is reallocated:
     // captured graphs hold those addresses and must be re-captured
     uint64_t scratch_gen = 0;
@@ -327,6 +333,8 @@ int ensure_attn32_scratch(Ctx* c, size_t floats);
 int ensure_kv8_scratch(Ctx* c, size_t floats, size_t counters);
 // token log probabilities: doubles of partial results, arrival counters
 int ensure_lp_scratch(Ctx* c, size_t doubles, size_t counters);
+// verification of drafted tokens: the same
+int ensure_verify_scratch(Ctx* c, size_t doubles, size_t counters);
 
 int quantile_of(float effort);
 double est_rows(int rows, float effort);

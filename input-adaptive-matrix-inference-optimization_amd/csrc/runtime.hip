@@ -160,6 +160,12 @@ int ensure_lp_scratch(Ctx* c, size_t doubles, size_t counters)
     return grow_zeroed(c, (void**)&c->lp_ctr, &c->lp_ctr_cap, counters, sizeof(uint32_t), "logprobs counter");
 }
 
+int ensure_verify_scratch(Ctx* c, size_t doubles, size_t counters)
+{
+    IAM_TRY(grow_zeroed(c, (void**)&c->ver_part, &c->ver_part_cap, doubles, sizeof(double), "verification partials"));
+    return grow_zeroed(c, (void**)&c->ver_ctr, &c->ver_ctr_cap, counters, sizeof(uint32_t), "verification counter");
+}
+
 int begin_launch(Ctx* c, const char* name, PendingEvent* ev)
 {
     for (int i = 0; i < 2; i++) {

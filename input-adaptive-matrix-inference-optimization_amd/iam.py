@@ -44,6 +44,11 @@ class ModelConfig(C.Structure):
                 ("norm_eps", C.c_float)]
 
 
+class Q4Desc(C.Structure):
+    _fields_ = [("numbers", C.c_void_p), ("scales", C.c_void_p), ("zeros", C.c_void_p), ("out_dim", C.c_int),
+                ("in_dim", C.c_int), ("group", C.c_int)]
+
+
 class RopeScaling(C.Structure):
     _fields_ = [("kind", C.c_int), ("factor", C.c_double), ("original_ctx", C.c_double), ("low", C.c_double),
                 ("high", C.c_double), ("magnitude", C.c_double)]
@@ -60,6 +65,8 @@ TYPES = {"f32": 0, "f16": 1, "bf16": 2}
 ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
 ROPE_SCALINGS = {"none": 0, "linear": 1, "base": 2, "bands": 3, "ramp": 4}
 KV8_FORMATS = {"int8": 0, "e4m3": 1}
+# number types of rows in 8 bits, beside those above
+ROW_TYPES = dict(TYPES, int8=3, e4m3=4)
 KV8_BLOCK = 64
 
 # the argument types of the calls that a serving loop makes for each token
@@ -70,6 +77,13 @@ _ARGTYPES = {
     "iam_kv8_read": [_P, _P, _P, _I, _P, _P],
     "iam_attention_kv8": [_P, _P, _P, _I, _I, _I, _Z, _P, _P, _I, _F, _P, _Z],
     "iam_token_logprobs": [_P, _P, _I, _I, _I, _Z, _P, _P, _P, _I, _P, _P],
+    "iam_q4_pack": [_P, _P, _P, _P, _P],
+    "iam_q4_quantize": [_P, _P, _P, _I, _Z],
+    "iam_q4_read": [_P, _P, _I, _I, _P],
+    "iam_q4_mul": [_P, _P, _P, _I, _Z, _P, _I, _I, _P, _I, _Z],
+    "iam_rmsnorm_rows": [_P, _P, _I, _Z, _P, _I, _Z, _P, _I, _I, _P, _F, _P, _I, _Z, _P, _I],
+    "iam_rows8_read": [_P, _P, _I, _Z, _P, _I, _I, _I, _P],
+    "iam_verify_drafts": [_P, _P, _I, _Z, _P, _I, _Z, _I, _I, _I, C.c_double, C.c_double, _P, _P, _P, _P, _P],
 }
 
 
@@ -422,6 +436,30 @@ class Ctx:
         check(lib().iam_token_logprobs(self.h, _ptr(logits), TYPES[type], n_rows, vocab, stride, _ptr(targets),
                                        _ptr(logprob), _ptr(entropy), top_k, _ptr(top_ids), _ptr(top_logprobs)))
 
+    # ---- rows in 8 bits, drafted tokens
+    def rmsnorm_rows(self, x, type, n_rows, dim, gain, eps, out, out_type, residual=None, residual_type="f32",
+                     sum=None, scale=None, group=0, x_stride=0, residual_stride=0, out_stride=0):
+        """RMS norm of rows, with the residual's addition; out in a float type, or
+        in "int8" / "e4m3" with fp32 scales of each row (group 0) or 128 values."""
+        check(lib().iam_rmsnorm_rows(self.h, _ptr(x), TYPES[type], x_stride, _ptr(residual), TYPES[residual_type],
+                                     residual_stride, _ptr(sum), n_rows, dim, _ptr(gain), eps, _ptr(out),
+                                     ROW_TYPES[out_type], out_stride, _ptr(scale), group))
+
+    def rows8_read(self, x, type, n_rows, dim, scale, out, group=0, stride=0):
+        """What rows in 8 bits stand for, in fp32."""
+        check(lib().iam_rows8_read(self.h, _ptr(x), ROW_TYPES[type], stride, _ptr(scale), group, n_rows, dim, _ptr(out)))
+
+    def verify_drafts(self, target, type, n_seq, n_draft, vocab, tokens, uniform, out, accepted, temperature=1.0,
+                      draft=None, draft_type="f32", draft_temperature=None, count=None, target_stride=0,
+                      draft_stride=0):
+        """Accepts drafted tokens by the target's logits and given random numbers,
+        and draws the token after the accepted ones (draft_temperature: the
+        target's, if None)."""
+        check(lib().iam_verify_drafts(self.h, _ptr(target), TYPES[type], target_stride, _ptr(draft), TYPES[draft_type],
+                                      draft_stride, n_seq, n_draft, vocab, temperature,
+                                      temperature if draft_temperature is None else draft_temperature, _ptr(tokens),
+                                      _ptr(count), _ptr(uniform), _ptr(out), _ptr(accepted)))
+
     # ---- synthetic data
     def gen_f16(self, seed, tid, count, mean, sigma, out):
         check(lib().iam_gen_f16(self.h, C.c_uint64(seed), C.c_uint64(tid), C.c_size_t(count),
@@ -488,6 +526,47 @@ class Kv8Cache:
         sequence's cache holds up to them."""
         check(lib().iam_attention_kv8(self.ctx.h, self._at, _ptr(q), TYPES[type], n_heads, n_tokens, q_stride,
                                       _ptr(pos), _ptr(count), window, scale, _ptr(out), out_stride))
+
+
+class Q4Matrix:
+    """A matrix of 4-bit weights, with fp16 scales (and zero points) for groups
+    of 32, 64 or 128 inputs."""
+
+    def __init__(self, ctx, out_dim, in_dim, group=128, zeros=False):
+        self.ctx = ctx
+        sizes = [C.c_size_t() for _ in range(3)]
+        check(lib().iam_q4_size(out_dim, in_dim, group, *[C.byref(n) for n in sizes]))
+        self.parts = []
+        try:
+            for n in sizes if zeros else sizes[:2]:
+                self.parts.append(DevBuf(ctx, n.value))
+        except IamError:
+            self.free()
+            raise
+        self.desc = Q4Desc(*[b.ptr for b in self.parts], *([] if zeros else [None]), out_dim, in_dim, group)
+        self._at = C.addressof(self.desc)
+
+    def free(self):
+        for b in self.parts:
+            b.free()
+
+    def pack(self, n, scale, zero=None):
+        """From plain rows: two numbers 0 .. 15 a byte, fp16 scales, zero points."""
+        check(lib().iam_q4_pack(self.ctx.h, self._at, _ptr(n), _ptr(scale), _ptr(zero)))
+
+    def quantize(self, w, type="f16", stride=0):
+        """From rows of weights in a float type, rounded to 4 bits."""
+        check(lib().iam_q4_quantize(self.ctx.h, self._at, _ptr(w), TYPES[type], stride))
+
+    def read(self, first_row, n_rows, out):
+        """What rows stand for, in fp32."""
+        check(lib().iam_q4_read(self.ctx.h, self._at, first_row, n_rows, _ptr(out)))
+
+    def mul(self, x, type, n_rows, y, y_type, x_scale=None, x_group=0, x_stride=0, y_stride=0):
+        """y[r] = the matrix times x[r] for n_rows rows (type "f32", "f16", "bf16",
+        or "int8" / "e4m3" with x_scale)."""
+        check(lib().iam_q4_mul(self.ctx.h, self._at, _ptr(x), ROW_TYPES[type], x_stride, _ptr(x_scale), x_group,
+                               n_rows, _ptr(y), TYPES[y_type], y_stride))
 
 
 class Model:

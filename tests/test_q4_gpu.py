@@ -1,0 +1,262 @@
+"""Matrices of 4-bit weights and their products (through libiam.so) against
+float64."""
+import numpy as np
+import pytest
+
+import plain64 as P
+import plain_rows as R
+
+pytestmark = pytest.mark.gpu
+
+GUARD = 24
+
+
+def packed(iam, ctx, w):
+    m = iam.Q4Matrix(ctx, w.out, w.inp, w.group, zeros=w.zero is not None)
+    src = [ctx.upload(w.plain_bytes()), ctx.upload(w.scale)] + ([ctx.upload(w.zero)] if w.zero is not None else [])
+    m.pack(*src)
+    ctx.sync()
+    for b in src:
+        b.free()
+    return m
+
+
+def rows_of(rng, rows, inp, type, x_group=0):
+    """(stored words, scales or None, float64 values) of random rows."""
+    x = rng.normal(0, 1, (rows, inp)) * np.where(rng.random(inp) < 0.02, 20, 1)
+    if type in P.TYPES:
+        w, v = P.to_type(x, type)
+        return w, None, v
+    q = rng.integers(-127, 128, (rows, inp)) if type == "int8" else R.e4m3(rng.integers(0, 127, (rows, inp)) | rng.integers(0, 2, (rows, inp)) << 7)
+    s = rng.uniform(0.5, 2, (rows, -(-inp // x_group) if x_group else 1)).astype(np.float32)
+    return R.bytes_of(q, type), s, q * R.spread(s, x_group, inp)
+
+
+def product(ctx, m, words, scale, type, y_type, x_group=0, x_stride=0, y_stride=0, first=0):
+    """Rows laid out `x_stride` apart from element `first` on; y between guards.
+    What lies between the rows is NaN (or the largest number)."""
+    rows, inp = words.shape
+    xs, ys = x_stride or inp, y_stride or m.desc.out_dim
+    out = m.desc.out_dim
+    flat = np.full(first + rows * xs + GUARD, 0x7f if words.dtype == np.uint8 else 0x7fff if words.dtype == np.uint16 else np.nan, words.dtype)
+    flat[first:first + rows * xs].reshape(rows, xs)[:, :inp] = words
+    dt = P.storage(y_type)
+    guard = np.full(rows * ys + 2 * GUARD, 77, dt)
+    dx, dy = ctx.upload(flat), ctx.upload(guard)
+    ds = ctx.upload(scale) if scale is not None else None
+    m.mul(dx.ptr + first * words.itemsize, type, rows, dy.ptr + GUARD * dt().itemsize, y_type, x_scale=ds, x_group=x_group,
+          x_stride=x_stride, y_stride=y_stride)
+    got = dy.read()
+    for b in (dx, dy, ds):
+        if b is not None:
+            b.free()
+    body = got[GUARD:-GUARD].reshape(rows, ys)
+    assert (got[:GUARD] == 77).all() and (got[-GUARD:] == 77).all() and (body[:, out:] == 77).all()
+    return P.from_bits(body[:, :out], y_type)
+
+
+def check(iam, ctx, rng, rows, inp, out, group, zeros, type, y_type, x_group=0, **kw):
+    w = R.random_weights(rng, out, inp, group, zeros)
+    m = packed(iam, ctx, w)
+    words, scale, x = rows_of(rng, rows, inp, type, x_group)
+    got = product(ctx, m, words, scale, type, y_type, x_group, **kw)
+    m.free()
+    v = w.values()
+    P.close(got, x @ v.T, R.product_bound(x, v), y_type)
+
+
+# one token and few, odd widths, a row or a tile too many or too few of each kind
+SHAPES = [(1, 1, 1), (1, 4096, 1024), (1, 14336, 40), (1, 1000, 2001), (2, 31, 17), (3, 129, 16), (4, 700, 100), (5, 100, 33), (5, 2048, 4100),
+          (6, 512, 15), (8, 1024, 65), (11, 640, 48), (16, 1100, 70), (17, 1000, 250), (32, 2048, 130), (33, 384, 129), (48, 4096, 64),
+          (64, 2048, 96), (65, 257, 130), (100, 5000, 31), (129, 1024, 272), (300, 700, 520), (513, 130, 1030)]
+
+
+@pytest.mark.parametrize("type", R.ROW_TYPES)
+@pytest.mark.parametrize("rows,inp,out", SHAPES)
+def test_products(iam, ctx, rows, inp, out, type):
+    rng = np.random.default_rng(rows * 7 + inp + out)
+    k = rows + inp + R.ROW_TYPES.index(type)
+    check(iam, ctx, rng, rows, inp, out, (32, 64, 128)[k % 3], k % 2 == 0, type, P.TYPES[k // 2 % 3], 128 * (k // 3 % 2) if type not in P.TYPES else 0)
+
+
+@pytest.mark.parametrize("type", R.ROW_TYPES)
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows", [1, 7, 40, 200])
+def test_whole_numbers_are_exact(iam, ctx, rows, group, zeros, type):
+    """Small whole numbers: every product and sum is one that fp32 holds, so the
+    result is equal whatever the order (sums below 900 * 15 * 15)."""
+    rng = np.random.default_rng(group + rows)
+    inp, out = 900, 200
+    groups = -(-inp // group)
+    w = R.Weights(rng.integers(0, 16, (out, inp)), np.exp2(rng.integers(-1, 2, (out, groups))), rng.integers(0, 16, (out, groups)).astype(np.uint8) if zeros else None, group)
+    x = rng.integers(-15, 16, (rows, inp)).astype(np.float64)
+    words = P.to_type(x, type)[0] if type in P.TYPES else R.bytes_of(x, type)
+    scale = None if type in P.TYPES else np.full((rows, 1), 0.5, np.float32)
+    m = packed(iam, ctx, w)
+    got = product(ctx, m, words, scale, type, "f32")
+    m.free()
+    assert np.array_equal(got, (x * (1 if scale is None else 0.5)) @ w.values().T)
+
+
+@pytest.mark.parametrize("type,first,x_stride", [("f32", 1, 4097), ("f32", 3, 4100), ("f16", 1, 4097), ("bf16", 5, 4104), ("f16", 8, 4104), ("int8", 3, 4099), ("int8", 16, 4112), ("e4m3", 1, 0)])
+@pytest.mark.parametrize("rows", [1, 5, 30, 150])
+def test_strides_and_alignment(iam, ctx, rows, type, first, x_stride):
+    rng = np.random.default_rng(first)
+    check(iam, ctx, rng, rows, 4096, 100, 128, False, type, "f16" if type == "f16" else "f32", first=first, x_stride=x_stride, y_stride=103)
+
+
+@pytest.mark.parametrize("rows", [1, 20, 140])
+@pytest.mark.parametrize("type", P.TYPES)
+def test_values_far_apart(iam, ctx, rows, type):
+    """Tiles of unlike size, tiny and huge ones, all zeros."""
+    rng = np.random.default_rng(3)
+    w = R.random_weights(rng, 48, 1280, 64, True)
+    x = rng.normal(0, 1, (rows, 1280)) * np.repeat(10.0 ** np.array([0, 4, -7, 3, -3, 0, -9, 4, -2, 1]), 128)
+    x[:, 640:768] = 0
+    if rows > 1:
+        x[1] = 0
+    words, v = P.to_type(x, type)
+    m = packed(iam, ctx, w)
+    got = product(ctx, m, words, None, type, "f32")
+    m.free()
+    P.close(got, v @ w.values().T, R.product_bound(v, w.values()), "f32")
+
+
+@pytest.mark.parametrize("rows", [1, 9, 130])
+@pytest.mark.parametrize("type", P.TYPES)
+def test_not_finite_rows(iam, ctx, rows, type):
+    """An infinity or a NaN makes nothing of its own row's finite, and the others stay."""
+    rng = np.random.default_rng(4)
+    w = R.random_weights(rng, 70, 600, 128, False)
+    w.n[:, 5] = 9    # no zero weight meets it
+    x = rng.normal(0, 1, (rows, 600))
+    x[0, 5] = np.inf if type != "bf16" else np.nan
+    if rows > 3:
+        x[3, 599] = -np.inf
+        w.n[:, 599] = 3
+    words, v = P.to_type(x, type)
+    m = packed(iam, ctx, w)
+    got = product(ctx, m, words, None, type, "f32")
+    m.free()
+    assert not np.isfinite(got[0]).any()
+    if rows > 3:
+        assert not np.isfinite(got[3]).any()
+        keep = [r for r in range(rows) if r not in (0, 3)]
+        P.close(got[keep], v[keep] @ w.values().T, R.product_bound(v[keep], w.values()), "f32")
+
+
+def test_not_finite_scales(iam, ctx):
+    rng = np.random.default_rng(5)
+    w = R.random_weights(rng, 40, 300, 64, False)
+    m = packed(iam, ctx, w)
+    words, scale, x = rows_of(rng, 3, 300, "int8")
+    scale[1] = np.nan
+    got = product(ctx, m, words, scale, "int8", "f32")
+    m.free()
+    assert np.isnan(got[1]).all()
+    P.close(got[[0, 2]], x[[0, 2]] @ w.values().T, R.product_bound(x[[0, 2]], w.values()), "f32")
+
+
+@pytest.mark.parametrize("rows", [1, 6, 150])
+def test_calls_repeat(iam, ctx, rows):
+    rng = np.random.default_rng(6)
+    w = R.random_weights(rng, 500, 3000, 128, True)
+    m = packed(iam, ctx, w)
+    words = rows_of(rng, rows, 3000, "f32")[0]
+    first = product(ctx, m, words, None, "f32", "f32")
+    for _ in range(3):
+        assert np.array_equal(first, product(ctx, m, words, None, "f32", "f32"))
+    m.free()
+
+
+@pytest.mark.parametrize("out,inp,group,zeros", [(1, 1, 32, False), (17, 33, 32, True), (40, 513, 64, True), (33, 1100, 128, False), (16, 512, 128, True)])
+def test_layout_and_read(iam, ctx, out, inp, group, zeros):
+    rng = np.random.default_rng(out)
+    w = R.random_weights(rng, out, inp, group, zeros)
+    m = packed(iam, ctx, w)
+    for part, want in zip(m.parts, R.layout(w)):
+        assert np.array_equal(part.read(), want.reshape(-1).view(np.uint8))
+    d = ctx.empty(out * inp, np.float32)
+    m.read(0, out, d)
+    assert np.array_equal(d.read().reshape(out, inp), w.values())
+    if out > 20:
+        m.read(18, 2, d)
+        assert np.array_equal(d.read()[:2 * inp].reshape(2, inp), w.values()[18:20])
+    m.free()
+    d.free()
+
+
+@pytest.mark.parametrize("type", P.TYPES)
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("out,inp,group,stride", [(20, 300, 32, 0), (33, 1029, 128, 1031), (1, 5, 64, 0)])
+def test_quantize(iam, ctx, out, inp, group, stride, zeros, type):
+    rng = np.random.default_rng(inp)
+    x = rng.normal(0, 1, (out, inp))
+    x[0, :group] = 0
+    if out > 2:
+        x[2] = np.abs(x[2])
+        x[1] = -np.abs(x[1])
+        x[-1, 7] = 3e4
+    words, v = P.to_type(x, type)
+    flat = np.zeros((out, stride or inp), words.dtype)
+    flat[:, :inp] = words
+    d = ctx.upload(flat)
+    m = iam.Q4Matrix(ctx, out, inp, group, zeros=zeros)
+    m.quantize(d, type, stride)
+    want = R.quantize(v, group, zeros)
+    for part, p in zip(m.parts, R.layout(want)):
+        assert np.array_equal(part.read(), p.reshape(-1).view(np.uint8))
+    m.free()
+    d.free()
+
+
+def test_quantize_not_finite(iam, ctx):
+    x = np.ones((3, 128), np.float32)
+    x[0, 3], x[1, 40], x[2, 100] = np.inf, np.nan, 3e38
+    d, out = ctx.upload(x), ctx.empty(3 * 128, np.float32)
+    m = iam.Q4Matrix(ctx, 3, 128, 32, zeros=True)
+    m.quantize(d, "f32")
+    m.read(0, 3, out)
+    got = out.read().reshape(3, 4, 32)
+    bad = np.isnan(got).all(2)
+    assert bad.tolist() == [[True, False, False, False], [False, True, False, False], [False, False, False, True]]
+    # 15 times the scale, which is 1/15 rounded to fp16: off by half a step
+    assert (got[~bad] == np.float32(15) * np.float32(np.float16(1 / 15))).all() and abs(15 * np.float64(np.float16(1 / 15)) - 1) <= 2.0 ** -11
+    for b in (d, out, m):
+        b.free()
+
+
+def test_refusals(iam, ctx):
+    m = iam.Q4Matrix(ctx, 40, 300, 64)
+    z = iam.Q4Matrix(ctx, 40, 300, 64, zeros=True)
+    n, s, zero = ctx.empty(40 * 150, np.uint8), ctx.empty(40 * 5, np.uint16), ctx.empty(40 * 5, np.uint8)
+    x, y, xs = ctx.empty(4 * 300, np.float32), ctx.empty(4 * 40, np.float32), ctx.empty(4 * 3, np.float32)
+    m.pack(n, s)
+    z.pack(n, s, zero)
+    ok = dict(x=x, type="f32", n_rows=4, y=y, y_type="f32")
+    m.mul(**ok)
+    m.mul(**dict(ok, n_rows=0))
+    m.mul(**dict(ok, type="int8", x_scale=xs, x_group=128))
+    refused = [lambda: m.pack(n, s, zero), lambda: z.pack(n, s), lambda: m.pack(None, s), lambda: m.pack(n, s.ptr + 2), lambda: m.pack(n.ptr + 1, s),
+               lambda: m.pack(m.parts[0], s), lambda: m.quantize(x, "f32"), lambda: m.quantize(None), lambda: m.read(0, 41, x), lambda: m.read(-1, 2, x),
+               lambda: m.read(41, 0, x), lambda: m.read(0, 5, x), lambda: m.read(0, 1, m.parts[0])]
+    for bad in (dict(x=None), dict(y=None), dict(n_rows=-1), dict(n_rows=5), dict(x_scale=xs), dict(type="int8"), dict(x_group=128),
+                dict(type="int8", x_scale=xs, x_group=64), dict(type="int8", x_scale=xs.ptr + 4, x_group=128), dict(x_stride=299), dict(y_stride=39),
+                dict(x_stride=301), dict(y_stride=41), dict(x=x.ptr + 2, n_rows=1), dict(y=x), dict(y=m.parts[0]), dict(n_rows=(1 << 22) + 1),
+                dict(x_stride=1 << 40)):
+        refused.append(lambda bad=bad: m.mul(**dict(ok, **bad)))
+    for call in refused:
+        with pytest.raises(iam.IamError) as e:
+            call()
+        assert e.value.code == iam.IAM_E_INVALID
+    for field, v in (("numbers", 0), ("numbers", m.desc.numbers + 8), ("scales", m.desc.scales + 2), ("zeros", m.desc.scales), ("out_dim", 60), ("in_dim", 0), ("group", 48)):
+        was = getattr(m.desc, field)
+        setattr(m.desc, field, v)
+        with pytest.raises(iam.IamError) as e:
+            m.mul(**ok)
+        assert e.value.code == iam.IAM_E_INVALID, field
+        setattr(m.desc, field, was)
+    m.mul(**ok)
+    for b in (m, z, n, s, zero, x, y, xs):
+        b.free()
