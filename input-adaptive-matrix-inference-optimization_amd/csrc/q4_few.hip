@@ -1,0 +1,238 @@
+// Products of a few rows (single tokens, drafted ones) with 4-bit weights.
+//
+// With the rows of x as whole numbers n = sum over d of 256^d n_d, the digits n_d
+// signed bytes, and one power of two for each row and tile of 128 inputs:
+//   y[r][o] = sum over d of 256^d  sum over tiles, groups of
+//             (2^e[r][tile] scale[o][group]) * (sum over the group of n_d[r][k] (w[o][k] - zero))
+// The innermost sums are exact, on the 8-bit matrix instructions, whose 16
+// columns are the rows' digits: three of a float row (22 bits of the tile's
+// largest value and its sign), one of an int8 row.  4-bit weights become bytes
+// with three instructions for eight of them, and what one row costs, five cost too.
+#include "q4_mul.h"
+
+namespace iam {
+
+struct FewArgs {
+    MulArgs u;
+    int waves;      // of a workgroup
+};
+
+constexpr int kFewMaxWaves = 16;
+constexpr int kFewCols = 16;
+
+// A strip's words of a chunk, its scales and zero points, in a lane's registers.
+template <int GROUP, bool ZEROS>
+struct FewWeights {
+    static constexpr int PER = kChunk / GROUP;
+    uint4 w[4];
+    uint4 s[PER / 2];                 // [PER][4] halves
+    uint32_t z[ZEROS ? PER / 4 : 1];  // [PER] bytes of the lane's row
+
+    __device__ __forceinline__ void load(const Q4& m, int strip, int chunk, int lane)
+    {
+        const int tiles = m.tiles - chunk * 4;
+        const uint4* p = reinterpret_cast<const uint4*>(m.numbers) + ((size_t)strip * m.tiles + chunk * 4) * 64 + lane;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+            if (t < tiles) w[t] = p[t * 64];
+        const size_t cell = (size_t)strip * m.chunks + chunk;
+        const uint4* q = reinterpret_cast<const uint4*>(m.scales) + (cell * 4 + (lane >> 4)) * (PER / 2);
+#pragma unroll
+        for (int i = 0; i < PER / 2; i++) s[i] = q[i];
+        if constexpr (ZEROS) {
+            const uint32_t* r = reinterpret_cast<const uint32_t*>(m.zeros) + (cell * kStrip + (lane & 15)) * (PER / 4);
+#pragma unroll
+            for (int i = 0; i < PER / 4; i++) z[i] = r[i];
+        }
+    }
+};
+
+// Eight weights as signed bytes: without zero points 16 (n - 8) (the stored four
+// bits are n - 8 in two's complement, at the top of a byte 16 times that),
+// with them n - zero.
+template <bool ZEROS>
+__device__ __forceinline__ void widen8(uint32_t w, uint32_t zero4, uint32_t& lo, uint32_t& hi)
+{
+    if constexpr (ZEROS) {
+        lo = (((w & 0x0f0f0f0fu) ^ 0x88888888u) - zero4) ^ 0x80808080u;          // 128 + n - zero, no borrows
+        hi = (((w >> 4 & 0x0f0f0f0fu) ^ 0x88888888u) - zero4) ^ 0x80808080u;
+    } else {
+        lo = w << 4 & 0xf0f0f0f0u;
+        hi = w & 0xf0f0f0f0u;
+    }
+}
+
+// the largest of 16 neighbouring lanes', in each of them
+__device__ __forceinline__ uint32_t max16(uint32_t v)
+{
+    v = max(v, dpp_t<0x128>(v, v));
+    v = max(v, dpp_t<0x124>(v, v));
+    v = max(v, dpp_t<0x122>(v, v));
+    return max(v, dpp_t<0x121>(v, v));
+}
+
+// A wave's LDS operations take place in order: this keeps them in the order they are written in.
+__device__ __forceinline__ void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A workgroup takes a strip of 16 rows of the matrix; its waves deal the chunks
+// of 512 inputs among themselves.  A wave brings the rows' 512 values into its
+// own part of LDS as digits in the operands' order (16 lanes a tile, 8 values
+// each) while the weights are on their way, and needs no other wave until the
+// sums are joined.
+template <int D, int GROUP, bool ZEROS>
+__global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
+{
+    extern __shared__ uint4 lds[];
+    const MulArgs& u = a.u;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c = lane & 15;
+    const int strip = xcd_remap(blockIdx.x, gridDim.x), cols = u.rows * D;
+    uint4* digits = lds + wave * (32 * cols);                                       // [tile][step][g][col] 16 bytes
+    float* factor = reinterpret_cast<float*>(lds + a.waves * (32 * cols)) + wave * 4 * kFewCols;   // [tile][row]
+    const int col = min(c, cols - 1), mine = col / D;
+    floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    FewWeights<GROUP, ZEROS> now;
+    for (int chunk = wave; chunk < u.m.chunks; chunk += a.waves) {
+        const int t16 = lane >> 4, k8 = lane & 15, k = chunk * kChunk + t16 * kTile + k8 * 8;
+        Raw8 raw = load_raw8(u.x, u.x_type, 0, k, u.m.in);
+        float xs = D == 1 || u.x_scale ? u.x_scale[u.x_groups > 1 ? min(chunk * 4 + t16, u.x_groups - 1) : 0] : 1.0f;
+        now.load(u.m, strip, chunk, lane);
+        uint2* to = reinterpret_cast<uint2*>(digits + ((t16 * 2 + (k8 >> 3)) * 4 + (k8 & 3)) * cols) + (k8 >> 2 & 1);
+        for (int r = 0; r < u.rows; r++) {
+            const Raw8 mine8 = raw;
+            const float scale = xs;
+            if (r + 1 < u.rows) {
+                raw = load_raw8(u.x, u.x_type, (size_t)(r + 1) * u.x_stride, k, u.m.in);
+                if (D == 1 || u.x_scale)
+                    xs = u.x_scale[(size_t)(r + 1) * u.x_groups + (u.x_groups > 1 ? min(chunk * 4 + t16, u.x_groups - 1) : 0)];
+            }
+            if constexpr (D == 1) {
+                const uint32_t p = mine8.a.x, q = mine8.a.y;
+                to[r * 2] = {__builtin_amdgcn_perm(q, p, 0x05010400u), __builtin_amdgcn_perm(q, p, 0x07030602u)};
+                if (k8 == 0) factor[t16 * kFewCols + r] = scale;
+            } else {
+                float v[8];
+                values8(mine8, u.x_type, v);
+                uint32_t top = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+                top = max16(top);
+                // n = round(v 2^(148 - e)), below 2^22; 2^(e - 148) back (NaN
+                // where a value is not finite).  Tiles below 2^-102 count as if
+                // they were that large.
+                const uint32_t e8 = max(top >> 23, 24u);
+                const float up = __uint_as_float((275u - e8) << 23);
+                uint32_t n[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++)   // 1.5 2^23 + n has n in its low bits; 128 more in each digit makes them whole bytes
+                    n[e] = __float_as_uint(__builtin_fmaf(v[e], up, 12582912.0f)) + (0x00808080u - 0x4b400000u);
+                {
+                    const uint32_t a0 = __builtin_amdgcn_perm(n[4], n[0], 0x05010400u), a1 = __builtin_amdgcn_perm(n[5], n[1], 0x05010400u);
+                    const uint32_t b0 = __builtin_amdgcn_perm(n[6], n[2], 0x05010400u), b1 = __builtin_amdgcn_perm(n[7], n[3], 0x05010400u);
+                    const uint32_t a2 = __builtin_amdgcn_perm(n[4], n[0], 0x0c0c0602u), a3 = __builtin_amdgcn_perm(n[5], n[1], 0x0c0c0602u);
+                    const uint32_t b2 = __builtin_amdgcn_perm(n[6], n[2], 0x0c0c0602u), b3 = __builtin_amdgcn_perm(n[7], n[3], 0x0c0c0602u);
+                    uint2* at = to + r * 2 * D;
+                    at[0] = {__builtin_amdgcn_perm(a1, a0, 0x05040100u) ^ 0x80808080u, __builtin_amdgcn_perm(b1, b0, 0x05040100u) ^ 0x80808080u};
+                    at[2] = {__builtin_amdgcn_perm(a1, a0, 0x07060302u) ^ 0x80808080u, __builtin_amdgcn_perm(b1, b0, 0x07060302u) ^ 0x80808080u};
+                    at[4] = {__builtin_amdgcn_perm(a3, a2, 0x05040100u) ^ 0x80808080u, __builtin_amdgcn_perm(b3, b2, 0x05040100u) ^ 0x80808080u};
+                }
+                if (k8 == 0) factor[t16 * kFewCols + r] = top >= 0x7f800000u ? NAN : __uint_as_float((e8 - 21u) << 23) * scale;
+            }
+        }
+        wave_sync();
+        const int tiles = min(4, u.m.tiles - chunk * 4);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            if (t >= tiles) break;
+            const float f = factor[t * kFewCols + mine] * (ZEROS ? 1.0f : 0.0625f);
+            const uint32_t wd[4] = {now.w[t].x, now.w[t].y, now.w[t].z, now.w[t].w};
+            intx4 sum = {0, 0, 0, 0};
+#pragma unroll
+            for (int step = 0; step < 2; step++) {
+                const uint4 b = digits[((t * 2 + step) * 4 + g) * cols + col];
+                uint32_t lo[2], hi[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int grp = (t * kTile + (step * 2 + j) * 32) / GROUP;
+                    uint32_t z4 = 0;
+                    if constexpr (ZEROS) z4 = __builtin_amdgcn_perm(0u, now.z[grp / 4], 0x01010101u * (grp % 4));
+                    widen8<ZEROS>(wd[step * 2 + j], z4, lo[j], hi[j]);
+                }
+                auto join = [&](int grp) {
+                    const uint32_t s0 = grp % 2 ? now.s[grp / 2].z : now.s[grp / 2].x, s1 = grp % 2 ? now.s[grp / 2].w : now.s[grp / 2].y;
+                    const half4 s = __builtin_bit_cast(half4, (uint64_t)s1 << 32 | s0);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[i] = __builtin_fmaf((float)sum[i], (float)s[i] * f, acc[i]);
+                    sum = intx4{0, 0, 0, 0};
+                };
+                if constexpr (GROUP == 32) {
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const long x8 = (long)((uint64_t)(j ? b.w : b.y) << 32 | (j ? b.z : b.x));
+                        sum = __builtin_amdgcn_mfma_i32_16x16x32_i8((long)((uint64_t)hi[j] << 32 | lo[j]), x8, sum, 0, 0, 0);
+                        join(t * 4 + step * 2 + j);
+                    }
+                } else {
+                    const intx4 w8 = {(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
+                    sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(w8, __builtin_bit_cast(intx4, b), sum, 0, 0, 0);
+                    if constexpr (GROUP == 64) join(t * 2 + step);
+                    else if (step == 1) join(t);
+                }
+            }
+        }
+        wave_sync();
+    }
+    // the waves' sums: [wave][col][16]
+    float* part = reinterpret_cast<float*>(lds);
+    __syncthreads();
+    if (c < cols) *reinterpret_cast<floatx4*>(part + (wave * cols + c) * 16 + 4 * g) = acc;
+    __syncthreads();
+    for (int i = tid; i < u.rows * 16; i += a.waves * 64) {
+        const int r = i >> 4, o = strip * kStrip + (i & 15);
+        float y = 0.0f;
+#pragma unroll
+        for (int d = D - 1; d >= 0; d--) {
+            float s = 0.0f;
+            for (int w = 0; w < a.waves; w++) s += part[(w * cols + r * D + d) * 16 + (i & 15)];
+            y = __builtin_fmaf(y, 256.0f, s);
+        }
+        if (o < u.m.out) put_value(u.y, u.y_type, (size_t)r * u.y_stride + o, y);
+    }
+}
+
+// ------------------------------------------------------------------ host ---
+int q4_few_most(int x_type) { return x_type == IAM_I8 ? kFewCols : kFewCols / 3; }
+
+template <int D, int GROUP>
+static int few_launch(Ctx* c, const FewArgs& a)
+{
+    const int cols = a.u.rows * D;
+    const size_t stage = (size_t)a.waves * (32 * cols * 16 + 4 * kFewCols * 4), join = (size_t)a.waves * cols * 64;
+    const dim3 grid((unsigned)q4_strips(a.u.m.out)), block((unsigned)a.waves * 64);
+    return a.u.m.zeros ? launch(c, "q4_mul.few", k_q4_few<D, GROUP, true>, grid, block, std::max(stage, join), a)
+                       : launch(c, "q4_mul.few", k_q4_few<D, GROUP, false>, grid, block, std::max(stage, join), a);
+}
+
+template <int D>
+static int few_grouped(Ctx* c, const FewArgs& a)
+{
+    if (a.u.m.group == 32) return few_launch<D, 32>(c, a);
+    if (a.u.m.group == 64) return few_launch<D, 64>(c, a);
+    return few_launch<D, 128>(c, a);
+}
+
+int q4_mul_few(Ctx* c, const MulArgs& u)
+{
+    const int cols = u.x_type == IAM_I8 ? u.rows : u.rows * 3;
+    // A wave for each chunk, as many as 160 KB of LDS hold digits of (512 bytes
+    // a column and 256 of factors each).
+    const int most = std::min(kFewMaxWaves, (160 * 1024) / (512 * cols + 256));
+    const int rounds = (u.m.chunks + most - 1) / most;
+    const FewArgs a{u, (u.m.chunks + rounds - 1) / rounds};
+    return u.x_type == IAM_I8 ? few_grouped<1>(c, a) : few_grouped<3>(c, a);
+}
+
+}  // namespace iam

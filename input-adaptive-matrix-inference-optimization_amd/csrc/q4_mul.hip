@@ -1,22 +1,9 @@
 // Products of rows with a matrix of 4-bit weights.
-#include "q4.h"
-#include "wave.h"
+#include "q4_mul.h"
 
 namespace iam {
 
 constexpr int kMulThreads = 256;
-
-struct MulArgs {
-    Q4 m;
-    const void* x;
-    size_t x_stride;
-    const float* x_scale;   // 8-bit rows
-    int x_groups;           // scales of a row
-    int rows;
-    void* y;
-    int y_type;
-    size_t y_stride;
-};
 
 // a value of a row: a float type's, or an 8-bit number's
 template <typename T>
@@ -25,13 +12,6 @@ template <>
 __device__ __forceinline__ float value_of<int8_t>(int8_t v) { return (float)v; }
 template <>
 __device__ __forceinline__ float value_of<uint8_t>(uint8_t v) { return e4m3_value(v); }   // e4m3
-
-__device__ __forceinline__ void put_value(void* y, int type, size_t at, float v)
-{
-    if (type == IAM_F32) reinterpret_cast<float*>(y)[at] = v;
-    else if (type == IAM_F16) reinterpret_cast<_Float16*>(y)[at] = (_Float16)v;
-    else reinterpret_cast<__bf16*>(y)[at] = (__bf16)v;
-}
 
 // A wave takes a strip of 16 rows for one row of x: lane 16 g + r the words of
 // row r that lie in it.
@@ -106,6 +86,7 @@ extern "C" int iam_q4_mul(iam_ctx* c, const iam_q4_matrix* m, const void* x, int
     MulArgs a{};
     a.m = q4_of(m);
     a.x = x;
+    a.x_type = x_type;
     a.x_stride = x_stride;
     a.x_scale = x_scale;
     a.x_groups = (int)x_groups;
@@ -113,6 +94,7 @@ extern "C" int iam_q4_mul(iam_ctx* c, const iam_q4_matrix* m, const void* x, int
     a.y = y;
     a.y_type = y_type;
     a.y_stride = y_stride;
+    if (rows <= q4_few_most(x_type)) return q4_mul_few(c, a);
     switch (x_type) {
     case IAM_F32: return mul_typed<float>(c, a);
     case IAM_F16: return mul_typed<_Float16>(c, a);
