@@ -137,6 +137,9 @@ struct Ctx {
     size_t ver_part_cap = 0;
     uint32_t* ver_ctr = nullptr;
     size_t ver_ctr_cap = 0;
+    // products with 4-bit weights: the rows of x in the operands' order
+    uint8_t* q4_part = nullptr;
+    size_t q4_part_cap = 0;
     // bumped whenever a context-owned scratch buffer is reallocated:
     // captured graphs hold those addresses and must be re-captured
     uint64_t scratch_gen = 0;
@@ -333,6 +336,8 @@ int ensure_attn32_scratch(Ctx* c, size_t floats);
 int ensure_kv8_scratch(Ctx* c, size_t floats, size_t counters);
 // token log probabilities: doubles of partial results, arrival counters
 int ensure_lp_scratch(Ctx* c, size_t doubles, size_t counters);
+// products with 4-bit weights: bytes of operands
+int ensure_q4_scratch(Ctx* c, size_t bytes);
 // verification of drafted tokens: the same
 int ensure_verify_scratch(Ctx* c, size_t doubles, size_t counters);
 

@@ -103,5 +103,7 @@ __device__ __forceinline__ void values8(const Raw8& r, int type, float* v)
 // rows that fit the one-launch kernel for few of them
 int q4_few_most(int x_type);
 int q4_mul_few(Ctx* c, const MulArgs& a);
+// any number of them
+int q4_mul_rows(Ctx* c, const MulArgs& a);
 
 }  // namespace iam

@@ -1,59 +1,5 @@
-// Products of rows with a matrix of 4-bit weights.
+// The entry point of the products of rows with a matrix of 4-bit weights.
 #include "q4_mul.h"
-
-namespace iam {
-
-constexpr int kMulThreads = 256;
-
-// a value of a row: a float type's, or an 8-bit number's
-template <typename T>
-__device__ __forceinline__ float value_of(T v) { return to_f32(v); }
-template <>
-__device__ __forceinline__ float value_of<int8_t>(int8_t v) { return (float)v; }
-template <>
-__device__ __forceinline__ float value_of<uint8_t>(uint8_t v) { return e4m3_value(v); }   // e4m3
-
-// A wave takes a strip of 16 rows for one row of x: lane 16 g + r the words of
-// row r that lie in it.
-template <typename T>
-__global__ __launch_bounds__(kMulThreads) void k_q4_mul(MulArgs a)
-{
-    const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
-    const int strips = q4_strips(a.m.out);
-    const size_t w = (size_t)blockIdx.x * (kMulThreads / 64) + (threadIdx.x >> 6);
-    if (w >= (size_t)strips * a.rows) return;
-    const int strip = (int)(w % strips), row = (int)(w / strips), o = strip * kStrip + r;
-    const T* x = reinterpret_cast<const T*>(a.x) + (size_t)row * a.x_stride;
-    const uint4* words = reinterpret_cast<const uint4*>(a.m.numbers) + (size_t)strip * a.m.tiles * 64 + lane;
-    float sum = 0.0f;
-    for (int t = 0; t < a.m.tiles; t++) {
-        const uint4 q = words[(size_t)t * 64];
-        const uint32_t wd[4] = {q.x, q.y, q.z, q.w};
-        float tile = 0.0f;
-        for (int j = 0; j < 4; j++) {
-            const int k = t * kTile + 32 * j + 8 * g;
-            const float s = (float)__builtin_bit_cast(_Float16, a.m.scales[q4_scale(a.m, o, k)]);
-            const int z = a.m.zeros ? a.m.zeros[q4_zero(a.m, o, k)] : 8;
-            float part = 0.0f;
-            for (int e = 0; e < 8; e++)
-                if (k + e < a.m.in) part += value_of<T>(x[k + e]) * (float)((int)((wd[j] >> q4_shift(e) & 15u) ^ 8u) - z);
-            tile += part * s;
-        }
-        sum += a.x_scale ? tile * a.x_scale[(size_t)row * a.x_groups + (a.x_groups > 1 ? t : 0)] : tile;
-    }
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
-    if (g == 0 && o < a.m.out) put_value(a.y, a.y_type, (size_t)row * a.y_stride + o, sum);
-}
-
-template <typename T>
-static int mul_typed(Ctx* c, MulArgs a)
-{
-    const size_t waves = (size_t)q4_strips(a.m.out) * a.rows;
-    return launch(c, "q4_mul", k_q4_mul<T>, dim3((unsigned)((waves + 3) / 4)), dim3(kMulThreads), 0, a);
-}
-
-}  // namespace iam
 
 using namespace iam;
 
@@ -94,12 +40,5 @@ extern "C" int iam_q4_mul(iam_ctx* c, const iam_q4_matrix* m, const void* x, int
     a.y = y;
     a.y_type = y_type;
     a.y_stride = y_stride;
-    if (rows <= q4_few_most(x_type)) return q4_mul_few(c, a);
-    switch (x_type) {
-    case IAM_F32: return mul_typed<float>(c, a);
-    case IAM_F16: return mul_typed<_Float16>(c, a);
-    case IAM_BF16: return mul_typed<__bf16>(c, a);
-    case IAM_I8: return mul_typed<int8_t>(c, a);
-    default: return mul_typed<uint8_t>(c, a);
-    }
+    return rows <= q4_few_most(x_type) ? q4_mul_few(c, a) : q4_mul_rows(c, a);
 }

@@ -1,0 +1,315 @@
+// Products of many rows (batches, prompts) with 4-bit weights, on the fp16 matrix
+// instructions.
+//
+// A launch of its own brings x into the instructions' order as fp16: one part
+// of values that fp16 holds (fp16 and 8-bit numbers; bf16 of a tile of 128 after
+// a power of two where its largest value lies outside [2^-2, 2^15)), two, high
+// and low, of fp32 (22 bits).  4-bit weights become fp16 under the exponents of
+// 1024 and 64, n - zero exactly.  Products are then exact; a group's are added
+// in fp32 by the instructions and go to the row's sum with the group's scale.
+#include "q4_mul.h"
+
+namespace iam {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+// ---- x in the operands' order
+// parts  fp16 [part][block of 16 rows][tile][j][lane 16 g + row][8]: inputs
+//        32 j + 8 g and on of the tile
+// factor fp32 [block][tile][16]: what the tile's values were divided by
+struct PrepArgs {
+    const void* x;
+    int type;
+    size_t stride;
+    const float* x_scale;    // with a scale for each tile (else null)
+    int rows, in, tiles;
+    _Float16* parts;
+    size_t part_stride;      // values of a part
+    float* factor;
+    int parts_n;
+};
+
+constexpr int kPrepThreads = 256;
+
+// A wave takes a tile of a block of 16 rows: lane (g, c) 32 values of row c.
+__global__ __launch_bounds__(kPrepThreads) void k_q4_prep(PrepArgs a)
+{
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int tile = blockIdx.x * (kPrepThreads / 64) + (threadIdx.x >> 6), block = blockIdx.y;
+    if (tile >= a.tiles) return;
+    const int row = block * 16 + c;
+    const bool there = row < a.rows;
+    float v[4][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const Raw8 r = load_raw8(a.x, a.type, (size_t)(there ? row : 0) * a.stride, tile * kTile + 32 * j + 8 * g, there ? a.in : 0);
+        values8(r, a.type, v[j]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(v[j][e]) & 0x7fffffffu);
+    }
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    float up = 1.0f, f = 1.0f;
+    if (a.type == IAM_F32 || a.type == IAM_BF16) {
+        // exponents -2 .. 14 (and 0) stay; else the largest value goes to [2^14, 2^15)
+        const int e = (int)(top >> 23) - 127;
+        if (top != 0u && e < 128 && (e < -2 || e > 14)) {
+            const int sh = min(14 - e, 126);
+            up = ldexpf(1.0f, sh);
+            f = ldexpf(1.0f, -sh);
+        }
+    }
+    if (a.x_scale) f = there ? a.x_scale[(size_t)row * a.tiles + tile] : 1.0f;
+    const size_t at = ((size_t)block * a.tiles + tile) * 4 * 64 * 8;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        half8 h, l;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float y = v[j][e] * up;
+            h[e] = (_Float16)y;
+            l[e] = fabsf((float)h[e]) < INFINITY ? (_Float16)(y - (float)h[e]) : (_Float16)0.0f;
+        }
+        *reinterpret_cast<half8*>(a.parts + at + (j * 64 + lane) * 8) = h;
+        if (a.parts_n == 2) *reinterpret_cast<half8*>(a.parts + a.part_stride + at + (j * 64 + lane) * 8) = l;
+    }
+    if (g == 0) a.factor[((size_t)block * a.tiles + tile) * 16 + c] = f;
+}
+
+// ---- the products
+struct RowsArgs {
+    MulArgs u;
+    const _Float16* parts;
+    size_t part_stride;
+    const float* factor;
+    const float* row_scale;   // of a whole row, or null
+    int blocks;               // of 16 rows
+    int waves;
+};
+
+// Eight weights as fp16, n - zero: under the exponent of 1024 a number's step is
+// 1, under that of 64 it is 1/16.
+__device__ __forceinline__ half8 widen_half(uint32_t w, uint32_t minus1024, uint32_t minus64)
+{
+    const uint32_t v = w >> 8;
+    const half2v a = __builtin_bit_cast(half2v, (w & 0x000f000fu) ^ 0x64086408u) + __builtin_bit_cast(half2v, minus1024);
+    const half2v b = __builtin_bit_cast(half2v, (w & 0x00f000f0u) ^ 0x54805480u) + __builtin_bit_cast(half2v, minus64);
+    const half2v c = __builtin_bit_cast(half2v, (v & 0x000f000fu) ^ 0x64086408u) + __builtin_bit_cast(half2v, minus1024);
+    const half2v d = __builtin_bit_cast(half2v, (v & 0x00f000f0u) ^ 0x54805480u) + __builtin_bit_cast(half2v, minus64);
+    return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// what is subtracted for a zero point: -(1024 + zero) and -(64 + zero), twice
+struct Minus {
+    uint32_t k1024, k64;
+};
+__device__ __forceinline__ Minus minus_of(uint32_t zero)
+{
+    const uint32_t two = zero | zero << 16;
+    return {0xe400e400u | two, 0xd400d400u | two << 4};
+}
+
+__device__ __forceinline__ floatx4 mfma_f16(half8 a, half8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// four results of row r, outputs o and on
+__device__ __forceinline__ void put_four(const MulArgs& u, int r, int o, floatx4 v)
+{
+    const size_t at = (size_t)r * u.y_stride + o;
+    if (o + 4 <= u.m.out) {
+        if (u.y_type == IAM_F32) {
+            *reinterpret_cast<Pack<float, 4, 4>*>(reinterpret_cast<float*>(u.y) + at) = {v[0], v[1], v[2], v[3]};
+        } else if (u.y_type == IAM_F16) {
+            *reinterpret_cast<Pack<_Float16, 4, 2>*>(reinterpret_cast<_Float16*>(u.y) + at) = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+        } else {
+            *reinterpret_cast<Pack<__bf16, 4, 2>*>(reinterpret_cast<__bf16*>(u.y) + at) = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (o + i < u.m.out) put_value(u.y, u.y_type, at + i, v[i]);
+}
+
+// A workgroup takes S strips of the matrix and NB blocks of 16 rows; its waves
+// deal the tiles of 128 inputs among themselves and join their sums in LDS.
+// Every operand comes straight from memory in the order in which it is used.
+template <int PARTS, int GROUP, int S, int NB>
+__global__ __launch_bounds__(1024) void k_q4_batch(RowsArgs a)
+{
+    extern __shared__ floatx4 join[];
+    constexpr int GT = kTile / GROUP;      // groups of a tile
+    const MulArgs& u = a.u;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int strips = q4_strips(u.m.out), s0 = xcd_remap(blockIdx.x, gridDim.x) * S, b0 = blockIdx.y * NB;
+    floatx4 acc[S][NB];
+#pragma unroll
+    for (int s = 0; s < S; s++)
+#pragma unroll
+        for (int n = 0; n < NB; n++) acc[s][n] = floatx4{0, 0, 0, 0};
+    const uint4* words[S];
+    int strip[S];
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        strip[s] = min(s0 + s, strips - 1);
+        words[s] = reinterpret_cast<const uint4*>(u.m.numbers) + (size_t)strip[s] * u.m.tiles * 64 + lane;
+    }
+    uint4 next[S];
+    if (wave < u.m.tiles) {
+#pragma unroll
+        for (int s = 0; s < S; s++) next[s] = words[s][(size_t)wave * 64];
+    }
+    for (int t = wave; t < u.m.tiles; t += a.waves) {
+        half8 x[PARTS][NB][4];
+        float f[NB];
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+            const size_t cell = (size_t)min(b0 + n, a.blocks - 1) * u.m.tiles + t;
+#pragma unroll
+            for (int p = 0; p < PARTS; p++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[p][n][j] = *reinterpret_cast<const half8*>(a.parts + p * a.part_stride + (cell * 4 + j) * 512 + lane * 8);
+            f[n] = a.factor[cell * 16 + c];
+        }
+        uint4 w[S];
+        half4 sc[S][GT];
+        uint32_t zero[S];
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            w[s] = next[s];
+            const size_t cell = (size_t)strip[s] * u.m.chunks + (t >> 2);
+            const half4* q = reinterpret_cast<const half4*>(u.m.scales) + (cell * 4 + g) * (4 * GT) + (t & 3) * GT;
+#pragma unroll
+            for (int i = 0; i < GT; i++) sc[s][i] = q[i];
+            zero[s] = 0x08080808u;
+            if (u.m.zeros) {
+                const uint8_t* z = u.m.zeros + (cell * kStrip + c) * (4 * GT) + (t & 3) * GT;
+                if constexpr (GT == 1) zero[s] = *z;
+                else if constexpr (GT == 2) zero[s] = *reinterpret_cast<const uint16_t*>(z);
+                else zero[s] = *reinterpret_cast<const uint32_t*>(z);
+            }
+        }
+        if (t + a.waves < u.m.tiles) {
+#pragma unroll
+            for (int s = 0; s < S; s++) next[s] = words[s][(size_t)(t + a.waves) * 64];
+        }
+        bool scaled = false;
+#pragma unroll
+        for (int n = 0; n < NB; n++) scaled |= __any(f[n] != 1.0f);
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            const uint32_t wd[4] = {w[s].x, w[s].y, w[s].z, w[s].w};
+            half8 wide[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const Minus m = minus_of(zero[s] >> (8 * (j * 32 / GROUP)) & 255u);
+                wide[j] = widen_half(wd[j], m.k1024, m.k64);
+            }
+#pragma unroll
+            for (int i = 0; i < GT; i++) {
+#pragma unroll
+                for (int n = 0; n < NB; n++) {
+                    floatx4 d = {0, 0, 0, 0};
+#pragma unroll
+                    for (int j = i * 4 / GT; j < (i + 1) * 4 / GT; j++)
+#pragma unroll
+                        for (int p = 0; p < PARTS; p++) d = mfma_f16(wide[j], x[p][n][j], d);
+                    if (scaled) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) d[e] *= f[n];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[s][n][e] = __builtin_fmaf(d[e], (float)sc[s][i][e], acc[s][n][e]);
+                }
+            }
+        }
+    }
+    if (a.waves > 1) {
+#pragma unroll
+        for (int s = 0; s < S; s++)
+#pragma unroll
+            for (int n = 0; n < NB; n++) join[(wave * S * NB + s * NB + n) * 64 + lane] = acc[s][n];
+        __syncthreads();
+    }
+#pragma unroll
+    for (int s = 0; s < S; s++)
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+            const int i = s * NB + n;
+            if (i % a.waves != wave) continue;
+            floatx4 v = acc[s][n];
+            if (a.waves > 1) {
+                v = join[i * 64 + lane];
+                for (int q = 1; q < a.waves; q++) v += join[(q * S * NB + i) * 64 + lane];
+            }
+            const int r = (b0 + n) * 16 + c;
+            if (s0 + s >= strips || r >= u.rows) continue;
+            if (a.row_scale) v *= a.row_scale[r];
+            put_four(u, r, (s0 + s) * kStrip + 4 * g, v);
+        }
+}
+
+// ------------------------------------------------------------------ host ---
+template <int PARTS, int GROUP, int S, int NB>
+static int batch_launch(Ctx* c, RowsArgs a)
+{
+    // as many waves as there are tiles, up to 16 and what LDS holds of their sums
+    const int most = std::min(16, 160 / (S * NB));
+    const int rounds = (a.u.m.tiles + most - 1) / most;
+    a.waves = (a.u.m.tiles + rounds - 1) / rounds;
+    const dim3 grid((unsigned)((q4_strips(a.u.m.out) + S - 1) / S), (unsigned)((a.blocks + NB - 1) / NB));
+    return launch(c, "q4_mul.batch", k_q4_batch<PARTS, GROUP, S, NB>, grid, dim3((unsigned)a.waves * 64), (size_t)a.waves * S * NB * 1024, a);
+}
+
+template <int PARTS, int GROUP>
+static int batch_sized(Ctx* c, const RowsArgs& a)
+{
+    if (a.blocks == 1) return batch_launch<PARTS, GROUP, 2, 1>(c, a);
+    if (a.blocks == 2 || PARTS == 2) return batch_launch<PARTS, GROUP, 1, 2>(c, a);
+    return batch_launch<PARTS, GROUP, 2, PARTS == 2 ? 2 : 4>(c, a);
+}
+
+template <int PARTS>
+static int batch_grouped(Ctx* c, const RowsArgs& a)
+{
+    if (a.u.m.group == 32) return batch_sized<PARTS, 32>(c, a);
+    if (a.u.m.group == 64) return batch_sized<PARTS, 64>(c, a);
+    return batch_sized<PARTS, 128>(c, a);
+}
+
+// rows of a pass: what x takes as parts stays small beside the card's memory
+constexpr int kRowsSlice = 1 << 14;
+
+int q4_mul_rows(Ctx* c, const MulArgs& all)
+{
+    const int parts = all.x_type == IAM_F32 ? 2 : 1;
+    const int slice = std::min(all.rows, kRowsSlice);
+    const size_t blocks = (size_t)(slice + 15) / 16, values = blocks * all.m.tiles * 2048;
+    IAM_TRY(ensure_q4_scratch(c, values * 2 * parts + blocks * all.m.tiles * 64));
+    for (int r0 = 0; r0 < all.rows; r0 += slice) {
+        MulArgs u = all;
+        u.rows = std::min(slice, all.rows - r0);
+        u.x = reinterpret_cast<const uint8_t*>(all.x) + (size_t)r0 * all.x_stride * row_type_bytes(all.x_type);
+        u.y = reinterpret_cast<uint8_t*>(all.y) + (size_t)r0 * all.y_stride * type_bytes(all.y_type);
+        if (u.x_scale) u.x_scale += (size_t)r0 * u.x_groups;
+        RowsArgs a{};
+        a.u = u;
+        a.parts = reinterpret_cast<_Float16*>(c->q4_part);
+        a.part_stride = values;
+        a.blocks = (u.rows + 15) / 16;
+        float* factor = reinterpret_cast<float*>(c->q4_part + values * 2 * parts);
+        a.factor = factor;
+        // a scale for each tile goes with the tiles; one of the whole row at the end
+        const bool by_tile = u.x_groups > 1;
+        a.row_scale = by_tile ? nullptr : u.x_scale;
+        const PrepArgs p{u.x, u.x_type, u.x_stride, by_tile ? u.x_scale : nullptr, u.rows, u.m.in, u.m.tiles,
+                         reinterpret_cast<_Float16*>(c->q4_part), values, factor, parts};
+        const dim3 grid((unsigned)((u.m.tiles + 3) / 4), (unsigned)a.blocks);
+        IAM_TRY(launch(c, "q4_mul.prepare", k_q4_prep, grid, dim3(kPrepThreads), 0, p));
+        IAM_TRY(parts == 2 ? batch_grouped<2>(c, a) : batch_grouped<1>(c, a));
+    }
+    return IAM_OK;
+}
+
+}  // namespace iam

@@ -160,6 +160,11 @@ int ensure_lp_scratch(Ctx* c, size_t doubles, size_t counters)
     return grow_zeroed(c, (void**)&c->lp_ctr, &c->lp_ctr_cap, counters, sizeof(uint32_t), "logprobs counter");
 }
 
+int ensure_q4_scratch(Ctx* c, size_t bytes)
+{
+    return grow_zeroed(c, (void**)&c->q4_part, &c->q4_part_cap, bytes, 1, "q4 operands");
+}
+
 int ensure_verify_scratch(Ctx* c, size_t doubles, size_t counters)
 {
     IAM_TRY(grow_zeroed(c, (void**)&c->ver_part, &c->ver_part_cap, doubles, sizeof(double), "verification partials"));
