@@ -85,6 +85,7 @@ struct RowsArgs {
     size_t part_stride;
     const float* factor;
     const float* row_scale;   // of a whole row, or null
+    bool factors;             // whether factor may hold anything but 1
     int blocks;               // of 16 rows
     int waves;
 };
@@ -194,9 +195,6 @@ __global__ __launch_bounds__(1024) void k_q4_batch(RowsArgs a)
 #pragma unroll
             for (int s = 0; s < S; s++) next[s] = words[s][(size_t)(t + a.waves) * 64];
         }
-        bool scaled = false;
-#pragma unroll
-        for (int n = 0; n < NB; n++) scaled |= __any(f[n] != 1.0f);
 #pragma unroll
         for (int s = 0; s < S; s++) {
             const uint32_t wd[4] = {w[s].x, w[s].y, w[s].z, w[s].w};
@@ -215,12 +213,8 @@ __global__ __launch_bounds__(1024) void k_q4_batch(RowsArgs a)
                     for (int j = i * 4 / GT; j < (i + 1) * 4 / GT; j++)
 #pragma unroll
                         for (int p = 0; p < PARTS; p++) d = mfma_f16(wide[j], x[p][n][j], d);
-                    if (scaled) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) d[e] *= f[n];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[s][n][e] = __builtin_fmaf(d[e], (float)sc[s][i][e], acc[s][n][e]);
+                    for (int e = 0; e < 4; e++) acc[s][n][e] = __builtin_fmaf(d[e] * f[n], (float)sc[s][i][e], acc[s][n][e]);
                 }
             }
         }
@@ -250,6 +244,176 @@ __global__ __launch_bounds__(1024) void k_q4_batch(RowsArgs a)
         }
 }
 
+// Many rows: a workgroup takes 128 rows of the matrix and 32 NB of x, its four
+// waves two by two 64 x 16 NB of them.  The operands and weights of a tile of
+// 128 inputs go to LDS, past the registers, while the tile before is computed:
+// x's from registers, a strip's weights read and widened when it is their turn.
+constexpr int kGemmStrips = 4;     // of a wave
+constexpr int kGemmPanel = 8;      // workgroups side by side along x's rows that run together
+
+template <int PARTS, int NB>
+struct GemmStage {
+    static constexpr int RUNS = PARTS * 2 * NB * 4, ALL = RUNS + 2 * kGemmStrips;   // runs of 1 KB: x's operands, the strips' words
+    uint4 at[2][ALL * 64];
+};
+
+// Tiles of a workgroup's products, with x's factors or (they are all 1) without.
+// The two are loops of their own: no branch may lie between a matrix
+// instruction and its results' first use, where the compiler leaves out the
+// wait states of the edge that jumps.
+template <int PARTS, int GROUP, int NB, bool FACTORS>
+__device__ __forceinline__ void gemm_tiles(const RowsArgs& a, GemmStage<PARTS, NB>& stage, int s0, int b0, floatx4 (&acc)[kGemmStrips][NB])
+{
+    typedef GemmStage<PARTS, NB> Stage;
+    constexpr int GT = kTile / GROUP, S = kGemmStrips, RUNS = Stage::RUNS, ALL = Stage::ALL;
+    const MulArgs& u = a.u;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int wo = wave >> 1, wx = wave & 1, last = q4_strips(u.m.out) - 1;
+    // a wave brings every fourth run: (part, block, j) of x, then one a strip
+    auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < ALL / 4; q++) {
+            const int i = wave + 4 * q;
+            const uint8_t* src;
+            if (q < RUNS / 4) {
+                const int b = min(b0 + (i >> 2) % (2 * NB), a.blocks - 1), p = (i >> 2) / (2 * NB);
+                src = reinterpret_cast<const uint8_t*>(a.parts + p * a.part_stride + (((size_t)b * u.m.tiles + t) * 4 + (i & 3)) * 512);
+            } else {
+                src = u.m.numbers + ((size_t)min(s0 + i - RUNS, last) * u.m.tiles + t) * 1024;
+            }
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + lane * 16),
+                                             (__attribute__((address_space(3))) void*)(stage.at[buf] + i * 64), 16, 0, 0);
+        }
+    };
+    half4 sc[S][GT];
+    uint32_t zero[S];
+    float f[NB];
+    auto load = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            const size_t cell = (size_t)min(s0 + wo * S + s, last) * u.m.chunks + (t >> 2);
+            const half4* q = reinterpret_cast<const half4*>(u.m.scales) + cell * (16 * GT) + (t & 3) * GT;
+#pragma unroll
+            for (int i = 0; i < GT; i++) sc[s][i] = q[g * (4 * GT) + i];
+            zero[s] = 0x08080808u;
+            if (u.m.zeros) {
+                const uint8_t* z = u.m.zeros + cell * (kStrip * 4 * GT) + (t & 3) * GT + c * (4 * GT);
+                if constexpr (GT == 1) zero[s] = *z;
+                else if constexpr (GT == 2) zero[s] = *reinterpret_cast<const uint16_t*>(z);
+                else zero[s] = *reinterpret_cast<const uint32_t*>(z);
+            }
+        }
+        if constexpr (FACTORS) {
+#pragma unroll
+            for (int n = 0; n < NB; n++) f[n] = a.factor[((size_t)min(b0 + wx * NB + n, a.blocks - 1) * u.m.tiles + t) * 16 + c];
+        }
+    };
+    fetch(0, 0);
+    load(0);
+#pragma unroll 1
+    for (int t = 0; t < u.m.tiles; t++) {
+        // this tile's operands have arrived, every wave's
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        const uint4* at = stage.at[t & 1] + lane;
+        half8 x[PARTS][NB][4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int p = 0; p < PARTS; p++)
+#pragma unroll
+                for (int n = 0; n < NB; n++) x[p][n][j] = __builtin_bit_cast(half8, at[((p * 2 * NB + wx * NB + n) * 4 + j) * 64]);
+        uint4 w[S];
+#pragma unroll
+        for (int s = 0; s < S; s++) w[s] = at[(RUNS + wo * S + s) * 64];
+        const int next = min(t + 1, u.m.tiles - 1);
+        fetch(next, (t + 1) & 1);   // behind the last tile, the last one again
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            const uint32_t wd[4] = {w[s].x, w[s].y, w[s].z, w[s].w};
+            half8 wide[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const Minus m = minus_of(zero[s] >> (8 * (j * 32 / GROUP)) & 255u);
+                wide[j] = widen_half(wd[j], m.k1024, m.k64);
+            }
+#pragma unroll
+            for (int i = 0; i < GT; i++) {
+                floatx4 d[NB];
+#pragma unroll
+                for (int n = 0; n < NB; n++) d[n] = floatx4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = i * 4 / GT; j < (i + 1) * 4 / GT; j++)
+#pragma unroll
+                    for (int p = 0; p < PARTS; p++)
+#pragma unroll
+                        for (int n = 0; n < NB; n++) d[n] = mfma_f16(wide[j], x[p][n][j], d[n]);
+#pragma unroll
+                for (int n = 0; n < NB; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[s][n][e] = __builtin_fmaf(FACTORS ? d[n][e] * f[n] : d[n][e], (float)sc[s][i][e], acc[s][n][e]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        load(next);
+    }
+    // the last fetch is over before its buffer is another's
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
+template <int PARTS, int GROUP, int NB>
+__global__ __launch_bounds__(256, 2) void k_q4_gemm(RowsArgs a)
+{
+    constexpr int S = kGemmStrips;
+    __shared__ GemmStage<PARTS, NB> stage;
+    const MulArgs& u = a.u;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int strips = q4_strips(u.m.out);
+    // panels of kGemmPanel along x's rows, the matrix's rows outermost in a panel
+    const int along = (a.blocks + 2 * NB - 1) / (2 * NB), across = (strips + 2 * S - 1) / (2 * S);
+    const int id = xcd_remap(blockIdx.x, gridDim.x), panel = id / (kGemmPanel * across), p0 = panel * kGemmPanel;
+    const int width = min(kGemmPanel, along - p0), in_panel = id - panel * kGemmPanel * across;
+    const int xt = p0 + in_panel % width, ot = in_panel / width;
+    const int s0 = ot * 2 * S, b0 = xt * 2 * NB;
+    bool factors = false;
+    if (a.factors) {
+        // whether any is not 1
+        const int blocks = min(2 * NB, a.blocks - b0);
+        const float4* q = reinterpret_cast<const float4*>(a.factor + (size_t)b0 * u.m.tiles * 16);
+        bool mine = false;
+        for (int i = threadIdx.x; i < blocks * u.m.tiles * 4; i += 256) {
+            const float4 v = q[i];
+            mine |= v.x != 1.0f || v.y != 1.0f || v.z != 1.0f || v.w != 1.0f;
+        }
+        uint32_t* any = reinterpret_cast<uint32_t*>(&stage);   // nothing else is there yet
+        if (lane == 0) any[wave] = 0;
+        if (mine) any[wave] = 1;
+        __syncthreads();
+        factors = __builtin_amdgcn_readfirstlane(any[0] | any[1] | any[2] | any[3]) != 0;
+        __syncthreads();
+    }
+    floatx4 acc[S][NB];
+#pragma unroll
+    for (int s = 0; s < S; s++)
+#pragma unroll
+        for (int n = 0; n < NB; n++) acc[s][n] = floatx4{0, 0, 0, 0};
+    if (factors) gemm_tiles<PARTS, GROUP, NB, true>(a, stage, s0, b0, acc);
+    else gemm_tiles<PARTS, GROUP, NB, false>(a, stage, s0, b0, acc);
+#pragma unroll
+    for (int n = 0; n < NB; n++) {
+        const int r = (b0 + (wave & 1) * NB + n) * 16 + c;
+        if (r >= u.rows) continue;
+        const float rs = a.row_scale ? a.row_scale[r] : 1.0f;
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            const int strip = s0 + (wave >> 1) * S + s;
+            if (strip < strips) put_four(u, r, strip * kStrip + 4 * g, acc[s][n] * rs);
+        }
+    }
+}
+
 // ------------------------------------------------------------------ host ---
 template <int PARTS, int GROUP, int S, int NB>
 static int batch_launch(Ctx* c, RowsArgs a)
@@ -262,9 +426,21 @@ static int batch_launch(Ctx* c, RowsArgs a)
     return launch(c, "q4_mul.batch", k_q4_batch<PARTS, GROUP, S, NB>, grid, dim3((unsigned)a.waves * 64), (size_t)a.waves * S * NB * 1024, a);
 }
 
+template <int PARTS, int GROUP, int NB>
+static int gemm_launch(Ctx* c, const RowsArgs& a)
+{
+    const size_t along = (size_t)(a.blocks + 2 * NB - 1) / (2 * NB), across = (size_t)(q4_strips(a.u.m.out) + 2 * kGemmStrips - 1) / (2 * kGemmStrips);
+    return launch(c, "q4_mul.gemm", k_q4_gemm<PARTS, GROUP, NB>, dim3((unsigned)(along * across)), dim3(256), 0, a);
+}
+
 template <int PARTS, int GROUP>
 static int batch_sized(Ctx* c, const RowsArgs& a)
 {
+    if (a.blocks > 4) {
+        if constexpr (PARTS == 1)
+            if (a.blocks > 16) return gemm_launch<PARTS, GROUP, 4>(c, a);
+        return gemm_launch<PARTS, GROUP, 2>(c, a);
+    }
     if (a.blocks == 1) return batch_launch<PARTS, GROUP, 2, 1>(c, a);
     if (a.blocks == 2 || PARTS == 2) return batch_launch<PARTS, GROUP, 1, 2>(c, a);
     return batch_launch<PARTS, GROUP, 2, PARTS == 2 ? 2 : 4>(c, a);
@@ -298,6 +474,7 @@ int q4_mul_rows(Ctx* c, const MulArgs& all)
         a.parts = reinterpret_cast<_Float16*>(c->q4_part);
         a.part_stride = values;
         a.blocks = (u.rows + 15) / 16;
+        a.factors = u.x_type == IAM_F32 || u.x_type == IAM_BF16 || u.x_groups > 1;
         float* factor = reinterpret_cast<float*>(c->q4_part + values * 2 * parts);
         a.factor = factor;
         // a scale for each tile goes with the tiles; one of the whole row at the end
