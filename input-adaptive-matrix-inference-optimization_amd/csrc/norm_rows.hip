@@ -10,7 +10,8 @@
 
 namespace iam {
 
-constexpr int kNormThreads = 256, kNormWaves = 4;
+constexpr int kNormMaxThreads = 1024, kNormMaxWaves = 16;
+constexpr int kNormMaxKept = 8;          // runs of 8 values that a thread keeps, at most
 
 struct NormArgs {
     const void* x;
@@ -25,91 +26,286 @@ struct NormArgs {
     float eps;
 };
 
-// the sum / largest value of the workgroup's, in every thread
+template <typename T>
+struct Eight {
+    T v[8];
+};
+// values i .. i + 7 of a row of n (zeros past it)
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T* p, int i, int n)
+{
+    if (i + 8 <= n) return __builtin_bit_cast(Eight<T>, *reinterpret_cast<const Pack<T, 8, (int)sizeof(T)>*>(p + i));
+    Eight<T> r;
+#pragma unroll
+    for (int e = 0; e < 8; e++) r.v[e] = i + e < n ? p[i + e] : (T)0.0f;
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_eight(T* p, int i, int n, const Eight<T>& x)
+{
+    if (i + 8 <= n) {
+        *reinterpret_cast<Pack<T, 8, (int)sizeof(T)>*>(p + i) = __builtin_bit_cast(Pack<T, 8, (int)sizeof(T)>, x);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        if (i + e < n) p[i + e] = x.v[e];
+}
+
+// the workgroup's sum / largest value, in every thread (red: LDS, a place a wave)
 __device__ __forceinline__ double block_sum(double v, double* red)
 {
     v = wave_sum(v);
-    __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0.0;
-    for (int w = 0; w < kNormWaves; w++) v += red[w];
+    const int waves = blockDim.x >> 6;
+    for (int w = 0; w < waves; w++) v += red[w];
     return v;
 }
-
-template <typename X, typename R>
-__device__ __forceinline__ float norm_h(const NormArgs& a, size_t row, int i)
+__device__ __forceinline__ double block_max(double v, double* red)
 {
-    const float x = to_f32(reinterpret_cast<const X*>(a.x)[row * a.x_stride + i]);
-    if (!a.r) return x;
-    return to_f32(from_f32<R>(x + to_f32(reinterpret_cast<const R*>(a.r)[row * a.r_stride + i])));
+    v = wave_max_t(v);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+    const int waves = blockDim.x >> 6;
+    for (int w = 1; w < waves; w++) v = fmax(v, red[w]);
+    return v;
+}
+// the largest of 16 neighbouring lanes', in each of them
+__device__ __forceinline__ double max16(double v)
+{
+    v = fmax(v, dpp_t<0x128>(v, v));
+    v = fmax(v, dpp_t<0x124>(v, v));
+    v = fmax(v, dpp_t<0x122>(v, v));
+    return fmax(v, dpp_t<0x121>(v, v));
 }
 
+// the magnitude of y, infinite where y is NaN
+__device__ __forceinline__ double size_of(double y) { return y != y ? (double)INFINITY : fabs(y); }
 // the scale of values whose largest magnitude is m: m / 127 or 448, NaN where one is not finite
 __device__ __forceinline__ float scale_of(double m, int type)
 {
     return m < (double)INFINITY ? (float)(m / (type == IAM_I8 ? 127.0 : 448.0)) : NAN;
 }
-__device__ __forceinline__ uint8_t number8(double y, float scale, int type)
+
+// y / s for r = 1 / s: the product's error taken out
+__device__ __forceinline__ double quotient(double y, double s, double r)
 {
-    if (!(scale > 0.0f)) return 0;
-    const double q = y / (double)scale;
-    if (type == IAM_I8) return (uint8_t)(int8_t)(int)fmin(fmax(rint(q), -127.0), 127.0);
-    // e4m3: three bits behind the leading one, steps of 2^-9 at least
-    const double m = fabs(q);
-    int e = -6;
-    if (m > 0.0) (void)frexp(m, &e);
-    e = max(e - 1, -6);
-    const int n = (int)rint(ldexp(m, 3 - e));   // 0 .. 16 steps of 2^(e - 3)
-    int bits = e == -6 && n < 8 ? n : (e + 7) * 8 + (n - 8);   // 16 steps are the next exponent's first
-    bits = min(bits, 0x7e);
-    return (uint8_t)(bits | (q < 0.0 ? 0x80 : 0));
+    const double q = y * r;
+    return __builtin_fma(__builtin_fma(-q, s, y), r, q);
+}
+// q rounded to fp32 to odd: one more rounding to fewer bits is then right
+__device__ __forceinline__ float to_odd(double q)
+{
+    const float f = (float)q;
+    const double e = q - (double)f;
+    int b = __float_as_int(f);
+    if (e != 0.0 && !(b & 1)) b += (e > 0.0) == (q > 0.0) ? 1 : -1;
+    return __int_as_float(b);
+}
+__device__ __forceinline__ uint32_t e4m3_of(double q) { return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(to_odd(q), 0.0f, 0, false) & 0xffu; }
+__device__ __forceinline__ uint32_t int8_of(double q) { return (uint32_t)(int)rint(fmin(fmax(q, -127.0), 127.0)) & 0xffu; }
+
+// the numbers of eight values, at p + i of a row of n
+__device__ __forceinline__ void put_numbers(uint8_t* p, int i, int n, const double* y, float scale, int type)
+{
+    Eight<uint8_t> o;
+    const double s = (double)scale, r = 1.0 / s;
+    const bool live = scale > 0.0f;
+    if (type == IAM_I8) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) o.v[e] = live ? (uint8_t)int8_of(quotient(y[e], s, r)) : (uint8_t)0;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) o.v[e] = live ? (uint8_t)e4m3_of(quotient(y[e], s, r)) : (uint8_t)0;
+    }
+    store_eight(p, i, n, o);
+}
+__device__ __forceinline__ void put_floats(void* p, size_t row, int i, int n, const double* y, int type)
+{
+    if (type == IAM_F32) {
+        Eight<float> o;
+#pragma unroll
+        for (int e = 0; e < 8; e++) o.v[e] = (float)y[e];
+        store_eight(reinterpret_cast<float*>(p) + row, i, n, o);
+    } else if (type == IAM_F16) {
+        Eight<_Float16> o;
+#pragma unroll
+        for (int e = 0; e < 8; e++) o.v[e] = (_Float16)to_odd(y[e]);
+        store_eight(reinterpret_cast<_Float16*>(p) + row, i, n, o);
+    } else {
+        Eight<__bf16> o;
+#pragma unroll
+        for (int e = 0; e < 8; e++) o.v[e] = (__bf16)to_odd(y[e]);
+        store_eight(reinterpret_cast<__bf16*>(p) + row, i, n, o);
+    }
 }
 
-// A workgroup takes a row, in three passes over it.
+// h of eight values: x + r, rounded to R
 template <typename X, typename R>
-__global__ __launch_bounds__(kNormThreads) void k_rmsnorm_rows(NormArgs a)
+__device__ __forceinline__ void sum_eight(const NormArgs& a, size_t row, int i, float* h)
 {
-    __shared__ double red[kNormWaves];
+    const Eight<X> x = load_eight(reinterpret_cast<const X*>(a.x) + row * a.x_stride, i, a.dim);
+    if (!a.r) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) h[e] = to_f32(x.v[e]);
+        return;
+    }
+    const Eight<R> r = load_eight(reinterpret_cast<const R*>(a.r) + row * a.r_stride, i, a.dim);
+#pragma unroll
+    for (int e = 0; e < 8; e++) h[e] = to_f32(from_f32<R>(to_f32(x.v[e]) + to_f32(r.v[e])));
+}
+template <typename R>
+__device__ __forceinline__ void keep_eight(const NormArgs& a, size_t row, int i, const float* h)
+{
+    Eight<R> o;
+#pragma unroll
+    for (int e = 0; e < 8; e++) o.v[e] = from_f32<R>(h[e]);
+    store_eight(reinterpret_cast<R*>(a.sum) + row * a.r_stride, i, a.dim, o);
+}
+__device__ __forceinline__ void gain_eight(const NormArgs& a, int i, const float* h, double inv, double* y)
+{
+    Eight<_Float16> g;
+    if (a.gain) g = load_eight(reinterpret_cast<const _Float16*>(a.gain), i, a.dim);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        y[e] = (double)h[e] * inv;
+        if (a.gain) y[e] *= (double)(float)g.v[e];
+    }
+}
+
+// A workgroup takes a row, which stays in its registers: J runs of 8 values a
+// thread.  Bound by memory where there are many rows; one row by the two
+// reductions.
+template <typename X, typename R, int J>
+__global__ __launch_bounds__(kNormMaxThreads) void k_rmsnorm_rows(NormArgs a)
+{
+    __shared__ double red[2][kNormMaxWaves];
     const size_t row = blockIdx.x;
-    const int tid = threadIdx.x;
+    const int step = blockDim.x * 8, i0 = threadIdx.x * 8;
+    float h[J][8];
     double ss = 0.0;
-    for (int i = tid; i < a.dim; i += kNormThreads) {
-        const double h = norm_h<X, R>(a, row, i);
-        ss += h * h;
-    }
-    const double inv = 1.0 / sqrt(block_sum(ss, red) / a.dim + (double)a.eps);
-    auto y_of = [&](int i) {
-        const double g = a.gain ? (double)(float)__builtin_bit_cast(_Float16, a.gain[i]) : 1.0;
-        return (double)norm_h<X, R>(a, row, i) * inv * g;
-    };
-    const bool eight = is_8bit_type(a.out_type);
-    if (eight) {
-        for (int g = tid >> 6; g < a.groups; g += kNormWaves) {
-            const int k0 = g * a.group, k1 = a.group ? min(a.dim, k0 + a.group) : a.dim;
-            double m = 0.0;
-            for (int i = k0 + (tid & 63); i < k1; i += 64) {
-                const double v = fabs(y_of(i));
-                m = v > m || v != v ? v : m;
-            }
-            for (int d = 1; d < 64; d *= 2) {
-                const double v = __shfl_xor(m, d);
-                m = v > m || v != v ? v : m;
-            }
-            if ((tid & 63) == 0) a.scale[row * a.groups + g] = scale_of(m, a.out_type);
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        if (J > 1 && i0 + j * step >= a.dim) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) h[j][e] = 0.0f;
+            continue;
         }
-        __syncthreads();
+        sum_eight<X, R>(a, row, i0 + j * step, h[j]);
     }
-    for (int i = tid; i < a.dim; i += kNormThreads) {
-        const double y = y_of(i);
-        const float h = norm_h<X, R>(a, row, i);
-        if (a.sum) reinterpret_cast<R*>(a.sum)[row * a.r_stride + i] = from_f32<R>(h);
-        const size_t at = row * a.out_stride + i;
-        if (eight)
-            reinterpret_cast<uint8_t*>(a.out)[at] = number8(y, a.scale[row * a.groups + (a.group ? i / a.group : 0)], a.out_type);
-        else if (a.out_type == IAM_F32) reinterpret_cast<float*>(a.out)[at] = (float)y;
-        else if (a.out_type == IAM_F16) reinterpret_cast<_Float16*>(a.out)[at] = (_Float16)y;
-        else reinterpret_cast<__bf16*>(a.out)[at] = (__bf16)y;
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) ss = __builtin_fma((double)h[j][e], (double)h[j][e], ss);
+        if (a.sum) keep_eight<R>(a, row, i0 + j * step, h[j]);
+    }
+    const double inv = 1.0 / sqrt(block_sum(ss, red[0]) / a.dim + (double)a.eps);
+    if (!is_8bit_type(a.out_type)) {
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            if (i0 + j * step >= a.dim) continue;
+            double y[8];
+            gain_eight(a, i0 + j * step, h[j], inv, y);
+            put_floats(a.out, row * a.out_stride, i0 + j * step, a.dim, y, a.out_type);
+        }
+        return;
+    }
+    uint8_t* out = reinterpret_cast<uint8_t*>(a.out) + row * a.out_stride;
+    if (a.group) {
+        // 16 threads' runs are a group
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const int i = i0 + j * step;
+            double y[8], m = 0.0;
+            if (i < a.dim) {
+                gain_eight(a, i, h[j], inv, y);
+#pragma unroll
+                for (int e = 0; e < 8; e++) m = i + e < a.dim ? fmax(m, size_of(y[e])) : m;
+            }
+            const float scale = scale_of(max16(m), a.out_type);
+            if (i >= a.dim) continue;
+            if ((threadIdx.x & 15) == 0) a.scale[row * a.groups + i / 128] = scale;
+            put_numbers(out, i, a.dim, y, scale, a.out_type);
+        }
+        return;
+    }
+    double m = 0.0;
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        const int i = i0 + j * step;
+        if (i >= a.dim) continue;
+        double y[8];
+        gain_eight(a, i, h[j], inv, y);
+#pragma unroll
+        for (int e = 0; e < 8; e++) m = i + e < a.dim ? fmax(m, size_of(y[e])) : m;
+    }
+    const float scale = scale_of(block_max(m, red[1]), a.out_type);
+    if (threadIdx.x == 0) a.scale[row] = scale;
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+        const int i = i0 + j * step;
+        if (i >= a.dim) continue;
+        double y[8];
+        gain_eight(a, i, h[j], inv, y);
+        put_numbers(out, i, a.dim, y, scale, a.out_type);
+    }
+}
+
+// The same for rows that a workgroup's registers do not hold (over 65536
+// values): three passes over the row, h from where it is kept, if it is.
+template <typename X, typename R>
+__global__ __launch_bounds__(kNormMaxThreads) void k_rmsnorm_long(NormArgs a)
+{
+    __shared__ double red[2][kNormMaxWaves];
+    const size_t row = blockIdx.x;
+    const int step = kNormMaxThreads * 8, i0 = threadIdx.x * 8;
+    double ss = 0.0;
+    for (int i = i0; i < a.dim; i += step) {
+        float h[8];
+        sum_eight<X, R>(a, row, i, h);
+#pragma unroll
+        for (int e = 0; e < 8; e++) ss = __builtin_fma((double)h[e], (double)h[e], ss);
+    }
+    const double inv = 1.0 / sqrt(block_sum(ss, red[0]) / a.dim + (double)a.eps);
+    const bool eight = is_8bit_type(a.out_type);
+    float scale = 0.0f;
+    if (eight && !a.group) {
+        double m = 0.0;
+        for (int i = i0; i < a.dim; i += step) {
+            float h[8];
+            double y[8];
+            sum_eight<X, R>(a, row, i, h);
+            gain_eight(a, i, h, inv, y);
+#pragma unroll
+            for (int e = 0; e < 8; e++) m = i + e < a.dim ? fmax(m, size_of(y[e])) : m;
+        }
+        scale = scale_of(block_max(m, red[1]), a.out_type);
+        if (threadIdx.x == 0) a.scale[row] = scale;
+    }
+    uint8_t* out = reinterpret_cast<uint8_t*>(a.out) + row * a.out_stride;
+    const int rounds = (a.dim + step - 1) / step;
+    for (int k = 0; k < rounds; k++) {
+        const int i = i0 + k * step;
+        float h[8];
+        double y[8], m = 0.0;
+        if (i < a.dim) {
+            sum_eight<X, R>(a, row, i, h);
+            gain_eight(a, i, h, inv, y);
+            if (a.sum) keep_eight<R>(a, row, i, h);
+#pragma unroll
+            for (int e = 0; e < 8; e++) m = i + e < a.dim ? fmax(m, size_of(y[e])) : m;
+        }
+        if (eight && a.group) scale = scale_of(max16(m), a.out_type);
+        if (i >= a.dim) continue;
+        if (!eight) {
+            put_floats(a.out, row * a.out_stride, i, a.dim, y, a.out_type);
+            continue;
+        }
+        if (a.group && (threadIdx.x & 15) == 0) a.scale[row * a.groups + i / 128] = scale;
+        put_numbers(out, i, a.dim, y, scale, a.out_type);
     }
 }
 
@@ -118,27 +314,55 @@ struct Read8Args {
     const float* scale;
     float* out;
     size_t stride;
-    int rows, dim, group, groups, type;
+    int dim, group, groups, type;
+    int parts;               // workgroups of a row
 };
 
-__global__ __launch_bounds__(256) void k_rows8_read(Read8Args a)
+constexpr int kReadThreads = 256;
+
+__global__ __launch_bounds__(kReadThreads) void k_rows8_read(Read8Args a)
 {
-    const size_t all = (size_t)a.rows * a.dim;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
-        const size_t row = i / a.dim;
-        const int k = (int)(i - row * a.dim);
-        const uint8_t b = a.x[row * a.stride + k];
-        const float v = a.type == IAM_I8 ? (float)(int8_t)b : e4m3_value(b);
-        a.out[i] = v * a.scale[row * a.groups + (a.group ? k / a.group : 0)];
+    const size_t row = blockIdx.x / a.parts;
+    const int i = ((int)(blockIdx.x - row * a.parts) * kReadThreads + (int)threadIdx.x) * 8;
+    if (i >= a.dim) return;
+    const Eight<uint8_t> b = [&] {
+        const uint8_t* p = a.x + row * a.stride;
+        if (i + 8 <= a.dim) return __builtin_bit_cast(Eight<uint8_t>, *reinterpret_cast<const Pack<uint8_t, 8, 1>*>(p + i));
+        Eight<uint8_t> r;
+#pragma unroll
+        for (int e = 0; e < 8; e++) r.v[e] = i + e < a.dim ? p[i + e] : (uint8_t)0;
+        return r;
+    }();
+    const float s = a.scale[row * a.groups + (a.group ? i / 128 : 0)];
+    Eight<float> o;
+#pragma unroll
+    for (int e = 0; e < 8; e++) o.v[e] = (a.type == IAM_I8 ? (float)(int8_t)b.v[e] : e4m3_value(b.v[e])) * s;
+    store_eight(a.out + row * a.dim, i, a.dim, o);
+}
+
+// ------------------------------------------------------------------ host ---
+template <typename X, typename R>
+static int norm_launch(Ctx* c, const NormArgs& a, int rows)
+{
+    const dim3 grid((unsigned)rows);
+    const int runs = (a.dim + 7) / 8;
+    if (runs > kNormMaxThreads * kNormMaxKept) return launch(c, "rmsnorm_rows", k_rmsnorm_long<X, R>, grid, dim3(kNormMaxThreads), 0, a);
+    // one run a thread, more where rows are long
+    int j = 1;
+    while (j < kNormMaxKept && runs > j * kNormMaxThreads) j *= 2;
+    const dim3 block((unsigned)(((runs + j - 1) / j + 63) / 64 * 64));
+    switch (j) {
+    case 1: return launch(c, "rmsnorm_rows", k_rmsnorm_rows<X, R, 1>, grid, block, 0, a);
+    case 2: return launch(c, "rmsnorm_rows", k_rmsnorm_rows<X, R, 2>, grid, block, 0, a);
+    case 4: return launch(c, "rmsnorm_rows", k_rmsnorm_rows<X, R, 4>, grid, block, 0, a);
+    default: return launch(c, "rmsnorm_rows", k_rmsnorm_rows<X, R, 8>, grid, block, 0, a);
     }
 }
 
 template <typename X>
 static int norm_typed(Ctx* c, const NormArgs& a, int r_type, int rows)
 {
-    const dim3 grid((unsigned)rows);
-    if (r_type == IAM_F32) return launch(c, "rmsnorm_rows", k_rmsnorm_rows<X, float>, grid, dim3(kNormThreads), 0, a);
-    return launch(c, "rmsnorm_rows", k_rmsnorm_rows<X, X>, grid, dim3(kNormThreads), 0, a);
+    return r_type == IAM_F32 ? norm_launch<X, float>(c, a, rows) : norm_launch<X, X>(c, a, rows);
 }
 
 }  // namespace iam
@@ -219,9 +443,15 @@ int iam_rows8_read(iam_ctx* c, const void* x, int type, size_t stride, const flo
     IAM_TRY(check_dev_range(c, out, yb, "rows8_read out"));
     IAM_REQUIRE(!overlaps(out, yb, x, xb) && !overlaps(out, yb, scale, sb), "rows8_read: out overlaps an input");
     DeviceGuard on(c);
-    const Read8Args a{reinterpret_cast<const uint8_t*>(x), scale, out, stride, rows, dim, group, groups, type};
-    const size_t blocks = std::min<size_t>((n * d + 255) / 256, 16384);
-    return launch(c, "rows8_read", k_rows8_read, dim3((unsigned)blocks), dim3(256), 0, a);
+    const int parts = (dim + kReadThreads * 8 - 1) / (kReadThreads * 8);
+    // at most 2^24 workgroups a launch
+    const int most = (1 << 24) / parts;
+    for (int r0 = 0; r0 < rows; r0 += most) {
+        const Read8Args a{reinterpret_cast<const uint8_t*>(x) + (size_t)r0 * stride, scale + (size_t)r0 * groups, out + (size_t)r0 * d, stride, dim, group,
+                          groups, type, parts};
+        IAM_TRY(launch(c, "rows8_read", k_rows8_read, dim3((unsigned)(std::min(most, rows - r0) * parts)), dim3(kReadThreads), 0, a));
+    }
+    return IAM_OK;
 }
 
 }  // extern "C"
