@@ -28,13 +28,14 @@ struct VerifyArgs {
     Rows target, draft;      // draft.x may be null
     int seqs, n, vocab;
     int segs, per;           // segments of a row, and their values (a multiple of a chunk)
+    int draw_segs, draw_per; // the same of the row that the last token is drawn from
     const int* tokens;
     const int* count;        // may be null
     const float* uniform;
     int* out;
     int* accepted;
     double* stat;            // [seqs (n + 1) + seqs n][segs][2]: largest logit, sum of exponentials; the best key (greedy)
-    double* part;            // [seqs][segs]: weights of the segment the last token is drawn from
+    double* part;            // [seqs][draw_segs]: weights of the segment the last token is drawn from
     uint32_t* ctr;           // [seqs], zero on entry (left zero)
 };
 
@@ -42,25 +43,51 @@ struct VerifyArgs {
 // 2^(t / 64) in fp64 for t <= 0: the table's 2^(j / 64) times a polynomial of the
 // rest f, |f| <= 1/2 (the series of e^(f ln 2 / 64) up to the fifth power: 4e-17).
 constexpr double kUnit = 64.0 * 1.44269504088896340736;   // t of e^1
+// 2^(j / 64)
+__constant__ const double kRoots[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
+};
+// The table is held 32 times, side by side: each lane reads its own banks, so
+// that 64 lanes' places do not meet.
+constexpr int kCopies = 32;
 struct ExpTable {
-    double t[64];
+    double t[64 * kCopies];
 };
 __device__ __forceinline__ void fill_table(ExpTable* e)
 {
-    if (threadIdx.x < 64) e->t[threadIdx.x] = exp2((double)threadIdx.x * 0.015625);
+    constexpr int each = kCopies / kVerWaves;
+    const double v = kRoots[threadIdx.x & 63];
+#pragma unroll
+    for (int i = 0; i < each; i++) e->t[(threadIdx.x & 63) * kCopies + (threadIdx.x >> 6) * each + (threadIdx.x + i) % each] = v;
 }
 __device__ __forceinline__ double exp_of(const ExpTable* e, double t)
 {
     constexpr double u = 1.0 / kUnit;
-    const double n = rint(t), f = t - n;
+    constexpr double whole = 6755399441055744.0;   // 1.5 2^52: what is added to it is rounded to whole numbers
+    const double tn = t + whole, f = t - (tn - whole);
     double p = u * u * u * u * u / 120.0;
     p = __builtin_fma(p, f, u * u * u * u / 24.0);
     p = __builtin_fma(p, f, u * u * u / 6.0);
     p = __builtin_fma(p, f, u * u / 2.0);
     p = __builtin_fma(p, f, u);
     p = __builtin_fma(p, f, 1.0);
-    const int i = (int)n;
-    return ldexp(p * e->t[i & 63], i >> 6);
+    const int i = (int)(uint32_t)__double_as_longlong(tn);
+    return ldexp(p * e->t[(i & 63) * kCopies + (threadIdx.x & (kCopies - 1))], i >> 6);
 }
 
 // What a row's exponentials are taken relative to: its largest logit.
@@ -74,43 +101,53 @@ struct Base {
 };
 
 // ---- reading a row
-// E values a thread of a chunk of 256 E, from place c0 on, runs of 16 bytes:
-// value e of the thread is at place_of(c0, e).  Outside [v0, v1), -inf.
-template <typename T, int E>
-__device__ __forceinline__ void load_chunk(const T* x, int c0, int v0, int v1, float* v)
+// E values a thread of a chunk of 256 E, from place c0 on, in runs of 8 that lie
+// 2048 values apart, or (ROW) all together: value e of the thread is at
+// place_of<E, ROW>(c0, e).  Outside [v0, v1), -inf.
+template <int E, bool ROW>
+__device__ __forceinline__ int place_of(int c0, int e)
 {
-    // the runs of 8 values (of fp32 two loads)
+    return ROW ? c0 + (int)threadIdx.x * E + e : c0 + (e / 8 * kVerThreads + (int)threadIdx.x) * 8 + e % 8;
+}
+template <typename T, int E, bool ROW = false>
+struct Runs {
     typedef Pack<T, 8, (int)sizeof(T)> Run;
     Run r[E / 8];
-    if (c0 >= v0 && c0 + kVerThreads * E <= v1) {
+
+    __device__ __forceinline__ void load(const T* x, int c0, int v0, int v1)
+    {
+        if (c0 >= v0 && c0 + kVerThreads * E <= v1) {
 #pragma unroll
-        for (int j = 0; j < E / 8; j++) r[j] = *reinterpret_cast<const Run*>(x + c0 + (j * kVerThreads + (int)threadIdx.x) * 8);
+            for (int j = 0; j < E / 8; j++) r[j] = *reinterpret_cast<const Run*>(x + place_of<E, ROW>(c0, j * 8));
+            return;
+        }
 #pragma unroll
-        for (int e = 0; e < E; e++) v[e] = to_f32(r[e / 8].v[e % 8]);
-        return;
-    }
+        for (int j = 0; j < E / 8; j++) {
+            const int i = place_of<E, ROW>(c0, j * 8);
+            if (i >= v0 && i + 8 <= v1) {
+                r[j] = *reinterpret_cast<const Run*>(x + i);
+            } else {
 #pragma unroll
-    for (int j = 0; j < E / 8; j++) {
-        const int i = c0 + (j * kVerThreads + (int)threadIdx.x) * 8;
-        if (i >= v0 && i + 8 <= v1) {
-            const Run q = *reinterpret_cast<const Run*>(x + i);
-#pragma unroll
-            for (int e = 0; e < 8; e++) v[j * 8 + e] = to_f32(q.v[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) v[j * 8 + e] = i + e >= v0 && i + e < v1 ? to_f32(x[i + e]) : -INFINITY;
+                for (int e = 0; e < 8; e++) r[j].v[e] = i + e >= v0 && i + e < v1 ? x[i + e] : (T)-INFINITY;
+            }
         }
     }
-}
-__device__ __forceinline__ int place_of(int c0, int e) { return c0 + (e / 8 * kVerThreads + (int)threadIdx.x) * 8 + e % 8; }
+    __device__ __forceinline__ float operator[](int e) const { return to_f32(r[e / 8].v[e % 8]); }
+};
 
 __device__ __forceinline__ size_t value_bytes(int type) { return type == IAM_F32 ? 4 : 2; }
-template <int E>
+template <int E, bool ROW = false>
 __device__ __forceinline__ void load_chunk(const Rows& r, size_t row, int c0, int v0, int v1, float* v)
 {
-    if (r.type == IAM_F32) load_chunk<float, E>(reinterpret_cast<const float*>(r.x) + row * r.stride, c0, v0, v1, v);
-    else if (r.type == IAM_F16) load_chunk<_Float16, E>(reinterpret_cast<const _Float16*>(r.x) + row * r.stride, c0, v0, v1, v);
-    else load_chunk<__bf16, E>(reinterpret_cast<const __bf16*>(r.x) + row * r.stride, c0, v0, v1, v);
+    auto take = [&](auto* x) __attribute__((always_inline)) {
+        Runs<std::remove_const_t<std::remove_pointer_t<decltype(x)>>, E, ROW> q;
+        q.load(x + row * r.stride, c0, v0, v1);
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = q[e];
+    };
+    if (r.type == IAM_F32) take(reinterpret_cast<const float*>(r.x));
+    else if (r.type == IAM_F16) take(reinterpret_cast<const _Float16*>(r.x));
+    else take(reinterpret_cast<const __bf16*>(r.x));
 }
 __device__ __forceinline__ float logit_of(const Rows& r, size_t row, int t)
 {
@@ -125,14 +162,14 @@ __device__ __forceinline__ float logit_of(const Rows& r, size_t row, int t)
 struct Segment {
     int o, v0, v1;
 };
-__device__ __forceinline__ Segment segment_of(const VerifyArgs& a, const Rows& r, size_t row, int seg)
+__device__ __forceinline__ Segment segment_of(const VerifyArgs& a, const Rows& r, size_t row, int seg, int per)
 {
     const size_t bytes = value_bytes(r.type);
     const int off = (int)(((uintptr_t)r.x + row * r.stride * bytes) / bytes % (16 / bytes));
     Segment s;
-    s.o = seg * a.per - off;
+    s.o = seg * per - off;
     s.v0 = max(s.o, 0);
-    s.v1 = a.vocab - s.o > a.per ? s.o + a.per : a.vocab;
+    s.v1 = a.vocab - s.o > per ? s.o + per : a.vocab;
     return s;
 }
 
@@ -160,7 +197,7 @@ __device__ __forceinline__ bool which_of(const VerifyArgs& a, int first, Which& 
 // The largest logit m of a segment and the sum of e^((x - m) / temperature); NaN
 // where there is a NaN or +inf, 0 where there is nothing but -inf.  Each wave
 // has its own m.  Bound by the fp64 arithmetic (17 instructions a value).
-template <int E>
+template <typename T, int E>
 __global__ __launch_bounds__(kVerThreads) void k_verify_rows(VerifyArgs a, int first)
 {
     __shared__ ExpTable table;
@@ -168,16 +205,19 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_rows(VerifyArgs a, int f
     __shared__ double wave_z[kVerWaves];
     Which w;
     if (!which_of(a, first, w)) return;
+    const Rows& r = w.draft ? a.draft : a.target;
+    const T* x = reinterpret_cast<const T*>(r.x) + w.row * r.stride;
+    const Segment g = segment_of(a, r, w.row, w.seg, a.per);
+    Runs<T, E> next;
+    if (g.o < g.v1) next.load(x, g.o, g.v0, g.v1);
     fill_table(&table);
     __syncthreads();
-    const Rows& r = w.draft ? a.draft : a.target;
-    const Segment g = segment_of(a, r, w.row, w.seg);
     float m = -INFINITY;
     double z = 0.0;
     bool bad = false;
     for (int c0 = g.o; c0 < g.v1; c0 += kVerThreads * E) {
-        float v[E];
-        load_chunk<E>(r, w.row, c0, g.v0, g.v1, v);
+        const Runs<T, E> v = next;
+        if (c0 + kVerThreads * E < g.v1) next.load(x, c0 + kVerThreads * E, g.v0, g.v1);
         float top = v[0];
 #pragma unroll
         for (int e = 1; e < E; e++) top = __builtin_elementwise_maximum(top, v[e]);
@@ -211,26 +251,11 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_rows(VerifyArgs a, int f
     }
 }
 
-// A row's largest logit and sum from its segments', in every lane; z is NaN where
-// the row has no distribution
+// A row's largest logit and sum; the sum is NaN where the row has no distribution
 struct Joined {
     float m;
     double z;
 };
-__device__ __forceinline__ Joined join_row(const VerifyArgs& a, size_t r, double unit)
-{
-    const int lane = threadIdx.x & 63;
-    float m = -INFINITY;
-    double z = 0.0;
-    if (lane < a.segs) {
-        m = (float)a.stat[(r * a.segs + lane) * 2];
-        z = a.stat[(r * a.segs + lane) * 2 + 1];
-    }
-    const float top = wave_max(m);
-    const double f = m == -INFINITY ? 0.0 : m == top ? 1.0 : exp(((double)m - (double)top) * (unit / kUnit));
-    const double sum = wave_sum(z != z ? z : z * f);
-    return {top, top == -INFINITY ? NAN : sum};
-}
 
 __device__ __forceinline__ double wave_scan(double v)
 {
@@ -256,65 +281,114 @@ struct Draw {
 template <int E>
 __device__ __forceinline__ void weights_of(const VerifyArgs& a, const Draw& d, const ExpTable* table, const Segment& g, int c0, double* w)
 {
-    float v[E];
-    load_chunk<E>(a.target, d.row, c0, g.v0, g.v1, v);
+    const bool two = d.less && a.draft.x;
+    float v[E], u[E];
+    load_chunk<E, true>(a.target, d.row, c0, g.v0, g.v1, v);
+    if (two) load_chunk<E, true>(a.draft, d.qrow, c0, g.v0, g.v1, u);
     const Base b{a.target.unit, (double)d.pm};
 #pragma unroll
     for (int e = 0; e < E; e++) w[e] = b.weight(table, v[e]) * d.pz;
-    if (!d.less) return;
-    if (!a.draft.x) {
+    if (two) {
+        const Base q{a.draft.unit, (double)d.qm};
 #pragma unroll
-        for (int e = 0; e < E; e++) w[e] = place_of(c0, e) == d.gone ? 0.0 : w[e];
-        return;
+        for (int e = 0; e < E; e++) w[e] = fmax(__builtin_fma(q.weight(table, u[e]), -d.qz, w[e]), 0.0);
+    } else if (d.less) {
+#pragma unroll
+        for (int e = 0; e < E; e++) w[e] = place_of<E, true>(c0, e) == d.gone ? 0.0 : w[e];
     }
-    load_chunk<E>(a.draft, d.qrow, c0, g.v0, g.v1, v);
-    const Base q{a.draft.unit, (double)d.qm};
-#pragma unroll
-    for (int e = 0; e < E; e++) w[e] = fmax(__builtin_fma(q.weight(table, v[e]), -d.qz, w[e]), 0.0);
 }
 
-// Workgroup (sequence, segment): which drafted tokens are kept (every workgroup
-// of the sequence finds out by itself), the weights of its segment of the row
-// that the next token is drawn from; the sequence's last workgroup finds the
-// segment in which their sum passes the random share, and the token in it.
-template <int E>
-__global__ __launch_bounds__(kVerThreads) void k_verify_pick(VerifyArgs a)
+constexpr int kDraw = 16;   // values of a thread's chunk in the row that a token is drawn from
+
+// Which drafted tokens of a sequence are kept, by every workgroup of it: the rows'
+// segments joined by `width` lanes a row, all rows at once where they
+// are few, then lane i judges token i.  p, q: LDS
+__device__ __forceinline__ int judge(const VerifyArgs& a, int s, int n, Joined* p, Joined* q)
 {
-    constexpr int J = E / 8;
-    __shared__ ExpTable table;
-    __shared__ Joined p[IAM_VERIFY_MAX_DRAFT + 1], q[IAM_VERIFY_MAX_DRAFT];
-    __shared__ int ok[IAM_VERIFY_MAX_DRAFT];
-    __shared__ double sums[J][kVerWaves], part[kVerMaxSegs];
-    __shared__ int last, picked;
-    const int s = blockIdx.x / a.segs, seg = blockIdx.x - s * a.segs, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int n = drafts_of(a, s);
+    const int tid = threadIdx.x, lane = tid & 63;
     const int* tokens = a.tokens + (size_t)s * a.n;
-    const float* uniform = a.uniform + (size_t)s * (a.n + 1);
-    fill_table(&table);
-    for (int i = wave; i <= n; i += kVerWaves) {
-        const size_t row = (size_t)s * (a.n + 1) + i, qrow = (size_t)s * a.n + i;
-        const Joined x = join_row(a, row, a.target.unit);
-        Joined y{0.0f, 1.0};
-        if (i < n && a.draft.x) y = join_row(a, (size_t)a.seqs * (a.n + 1) + qrow, a.draft.unit);
-        if (lane == 0) {
-            p[i] = x;
-            if (i < n) {
-                q[i] = y;
-                const int t = tokens[i];
-                bool keep = false;
-                if (t >= 0 && t < a.vocab) {
-                    const double pt = exp(((double)logit_of(a.target, row, t) - (double)x.m) * (a.target.unit / kUnit)) / x.z;
-                    const double qt = a.draft.x ? exp(((double)logit_of(a.draft, qrow, t) - (double)y.m) * (a.draft.unit / kUnit)) / y.z : 1.0;
-                    keep = (double)uniform[i] * qt < pt;
-                }
-                ok[i] = keep;
-            }
+    // what lane i needs of token i, on its way while the rows are joined
+    const int t = lane < n ? tokens[lane] : -1;
+    const bool there = t >= 0 && t < a.vocab;
+    const size_t row = (size_t)s * (a.n + 1) + lane, qrow = (size_t)s * a.n + lane;
+    float u = 0.0f, x = 0.0f, y = 0.0f;
+    if (there) {
+        u = a.uniform[(size_t)s * (a.n + 1) + lane];
+        x = logit_of(a.target, row, t);
+        if (a.draft.x) y = logit_of(a.draft, qrow, t);
+    }
+    int width = 1;
+    while (width < a.segs) width *= 2;
+    const int rows = n + 1 + (a.draft.x ? n : 0), g = tid & (width - 1);
+    for (int r0 = 0; r0 < rows; r0 += kVerThreads / width) {
+        const int r = r0 + tid / width, i = r <= n ? r : r - n - 1;
+        const size_t at = ((r <= n ? (size_t)s * (a.n + 1) : (size_t)a.seqs * (a.n + 1) + (size_t)s * a.n) + i) * a.segs + g;
+        const double unit = r <= n ? a.target.unit : a.draft.unit;
+        float m = -INFINITY;
+        double z = 0.0;
+        if (r < rows && g < a.segs) {
+            m = (float)a.stat[at * 2];
+            z = a.stat[at * 2 + 1];
         }
+        float top = m;
+        for (int d = 1; d < width; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        const double f = m == top ? 1.0 : m == -INFINITY ? 0.0 : exp(((double)m - (double)top) * (unit / kUnit));
+        z = z != z ? z : z * f;
+        for (int d = 1; d < width; d *= 2) z += __shfl_xor(z, d);
+        if (r < rows && g == 0) (r <= n ? p : q)[i] = {top, top == -INFINITY ? NAN : z};
     }
     __syncthreads();
-    int kept = 0;
-    while (kept < n && ok[kept]) kept++;
+    bool keep = false;
+    if (there) {
+        const Joined pi = p[lane];
+        const double pt = exp(((double)x - (double)pi.m) * (a.target.unit / kUnit)) / pi.z;
+        double qt = 1.0;
+        if (a.draft.x) {
+            const Joined qi = q[lane];
+            qt = exp(((double)y - (double)qi.m) * (a.draft.unit / kUnit)) / qi.z;
+        }
+        keep = (double)u * qt < pt;
+    }
+    const uint64_t wrong = __ballot(!keep);
+    return wrong ? __ffsll((unsigned long long)wrong) - 1 : 64;   // lanes from n on keep nothing
+}
+
+// the workgroup's sum of the weights of segment seg, in every thread
+__device__ __forceinline__ double segment_sum(const VerifyArgs& a, const Draw& d, const ExpTable* table, int seg, double* sums)
+{
+    const Segment g = segment_of(a, a.target, d.row, seg, a.draw_per);
+    double sum = 0.0;
+    for (int c0 = g.o; c0 < g.v1; c0 += kVerThreads * kDraw) {
+        double w[kDraw];
+        weights_of<kDraw>(a, d, table, g, c0, w);
+#pragma unroll
+        for (int e = 0; e < kDraw; e++) sum += w[e];
+    }
+    sum = wave_sum(sum);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int i = 0; i < kVerWaves; i++) sum += sums[i];
+    return sum;
+}
+
+// Workgroup (sequence, segment): which drafted tokens are kept, the weights of
+// its segment of the row that the next token is drawn from; the sequence's last
+// workgroup finds the segment in which their sum passes the random share, and
+// the token in it.
+__global__ __launch_bounds__(kVerThreads) void k_verify_pick(VerifyArgs a)
+{
+    __shared__ ExpTable table;
+    __shared__ Joined p[IAM_VERIFY_MAX_DRAFT + 1], q[IAM_VERIFY_MAX_DRAFT];
+    __shared__ double sums[kVerWaves], part[kVerMaxSegs];
+    __shared__ int last, picked;
+    const int s = blockIdx.x / a.draw_segs, seg = blockIdx.x - s * a.draw_segs, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int n = drafts_of(a, s);
+    fill_table(&table);
+    const int kept = judge(a, s, n, p, q);
     const Joined pk = p[kept];
+    const int* tokens = a.tokens + (size_t)s * a.n;
     int follow = -1;
     if (pk.z == pk.z) {
         Draw d;
@@ -331,115 +405,79 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_pick(VerifyArgs a)
             d.qz = 1.0 / q[kept].z;
             d.less = d.qz == d.qz;
         }
-        Segment g = segment_of(a, a.target, d.row, seg);
-        double sum = 0.0;
-        for (int c0 = g.o; c0 < g.v1; c0 += kVerThreads * E) {
-            double w[E];
-            weights_of<E>(a, d, &table, g, c0, w);
-#pragma unroll
-            for (int e = 0; e < E; e++) sum += w[e];
-        }
-        sum = wave_sum(sum);
-        if (lane == 0) sums[0][wave] = sum;
-        __syncthreads();
-        sum = 0.0;
-        for (int i = 0; i < kVerWaves; i++) sum += sums[0][i];
-        if (a.segs > 1) {
-            if (tid == 0) acc_put(a.part + (size_t)s * a.segs + seg, sum);
-            if (!acc_arrive(a.ctr + s, (uint32_t)a.segs, &last)) return;
-            if (tid < a.segs) part[tid] = acc_peek(a.part + (size_t)s * a.segs + tid);
+        const double sum = segment_sum(a, d, &table, seg, sums);
+        if (a.draw_segs > 1) {
+            if (tid == 0) acc_put(a.part + (size_t)s * a.draw_segs + seg, sum);
+            if (!acc_arrive(a.ctr + s, (uint32_t)a.draw_segs, &last)) return;
+            if (tid < a.draw_segs) part[tid] = acc_peek(a.part + (size_t)s * a.draw_segs + tid);
             if (tid == 0) a.ctr[s] = 0u;
         } else if (tid == 0) {
             part[0] = sum;
         }
-        __syncthreads();
-        double all = 0.0;
-        for (int i = 0; i < a.segs; i++) all += part[i];
-        if (d.less && !(all > 0.0)) {
-            // nowhere positive: p alone, whose segments' sums are at hand
-            d.less = false;
-            __syncthreads();
-            if (tid < a.segs) {
-                const double* st = a.stat + (d.row * a.segs + tid) * 2;
-                part[tid] = (float)st[0] == -INFINITY ? 0.0 : st[1] * exp((st[0] - (double)pk.m) * (a.target.unit / kUnit)) * d.pz;
-            }
-            __syncthreads();
-            all = 0.0;
-            for (int i = 0; i < a.segs; i++) all += part[i];
-        }
-        const double want = (double)uniform[a.n] * all;
-        // the segment in which the sum passes it (by rounding none: the last of any weight)
-        double before = 0.0;
-        int at = -1;
-        for (int i = 0; i < a.segs; i++) {
-            if (before + part[i] > want) {
-                at = i;
-                break;
-            }
-            before += part[i];
-        }
-        if (at < 0)
-            for (at = a.segs - 1; at > 0 && !(part[at] > 0.0); at--) before -= part[at];
         if (tid == 0) picked = -1;
-        g = segment_of(a, a.target, d.row, at);
-        int mine = -1;           // the last place of any weight
-        for (int c0 = g.o; c0 < g.v1; c0 += kVerThreads * E) {
-            double w[E], run[J];
-            weights_of<E>(a, d, &table, g, c0, w);
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < J; j++) {
-                run[j] = 0.0;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    run[j] += w[j * 8 + e];
-                    if (w[j * 8 + e] > 0.0) mine = place_of(c0, j * 8 + e);
-                }
-                const double t = wave_sum(run[j]);
-                if (lane == 0) sums[j][wave] = t;
+        __syncthreads();
+        double own = lane < a.draw_segs ? part[lane] : 0.0, upto = wave_scan(own);
+        if (d.less && !(__shfl(upto, 63) > 0.0)) {
+            // nowhere positive: p alone (seldom, if ever)
+            d.less = false;
+            for (int i = 0; i < a.draw_segs; i++) {
+                const double t = segment_sum(a, d, &table, i, sums);
+                if (lane == i) own = t;
             }
-            __syncthreads();
-            // the places are in the order of (run, wave, lane, value)
-            int hit = -1;
-            for (int i = 0; i < J * kVerWaves && hit < 0; i++) {
-                const double t = sums[i / kVerWaves][i % kVerWaves];
-                if (before + t > want) hit = i;
-                else before += t;
+            upto = wave_scan(own);
+        }
+        const double want = (double)a.uniform[(size_t)s * (a.n + 1) + a.n] * __shfl(upto, 63);
+        // the segment in which the sum passes it (by rounding none: the last of any weight)
+        const uint64_t past = __ballot(upto > want), some = __ballot(own > 0.0);
+        const int at = past ? __ffsll((unsigned long long)past) - 1 : some ? 63 - __clzll((long long)some) : 0;
+        const double left = __shfl(upto, max(at - 1, 0));
+        double before = at ? left : 0.0;
+        const Segment g = segment_of(a, a.target, d.row, at, a.draw_per);
+        int mine = -1;           // the thread's last place of any weight
+        for (int c0 = g.o; c0 < g.v1; c0 += kVerThreads * kDraw) {
+            double w[kDraw], run = 0.0;
+            weights_of<kDraw>(a, d, &table, g, c0, w);
+#pragma unroll
+            for (int e = 0; e < kDraw; e++) {
+                run += w[e];
+                if (w[e] > 0.0) mine = place_of<kDraw, true>(c0, e);
             }
-            if (hit < 0) continue;
-            if (wave == hit % kVerWaves) {
+            const double incl = wave_scan(run);
+            __syncthreads();
+            if (lane == 63) sums[wave] = incl;
+            __syncthreads();
+            int hit = 0;
+            for (; hit < kVerWaves; hit++) {
+                if (before + sums[hit] > want) break;
+                before += sums[hit];
+            }
+            if (hit == kVerWaves) continue;
+            if (wave == hit) {
+                // the first lane whose sum passes it: lane 63's does
+                const uint64_t over = __ballot(before + incl > want);
+                const double left = __shfl_up(incl, 1);
+                if (lane == __ffsll((unsigned long long)over) - 1) {
+                    double c = before + (lane ? left : 0.0);
+                    int place = -1;
 #pragma unroll
-                for (int j = 0; j < J; j++) {
-                    if (j != hit / kVerWaves) continue;
-                    const double incl = wave_scan(run[j]);
-                    const uint64_t over = __ballot(before + incl > want), some = __ballot(run[j] > 0.0);
-                    const int who = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
-                    if (lane == who) {
-                        double c = before + (incl - run[j]);
-                        int place = -1;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const bool open = place < 0 || !(c > want);
-                            c += w[j * 8 + e];
-                            if (open && w[j * 8 + e] > 0.0) place = place_of(c0, j * 8 + e);
-                        }
-                        picked = place;
+                    for (int e = 0; e < kDraw; e++) {
+                        if (w[e] > 0.0 && (place < 0 || !(c > want))) place = place_of<kDraw, true>(c0, e);
+                        c += w[e];
                     }
+                    picked = place;
                 }
             }
             break;
         }
         __syncthreads();
-        if (picked < 0) {
+        follow = picked;
+        if (follow < 0) {
             const uint32_t most = wave_max_u32((uint32_t)(mine + 1));
-            __syncthreads();
-            if (lane == 0) sums[0][wave] = (double)most;
+            if (lane == 0) sums[wave] = (double)most;
             __syncthreads();
             double best = 0.0;
-            for (int i = 0; i < kVerWaves; i++) best = fmax(best, sums[0][i]);
+            for (int i = 0; i < kVerWaves; i++) best = fmax(best, sums[i]);
             follow = (int)best - 1;
-        } else {
-            follow = picked;
         }
     } else if (seg != 0) {
         return;
@@ -464,7 +502,7 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_best(VerifyArgs a, int f
     __shared__ unsigned long long best[kVerWaves];
     Which w;
     if (!which_of(a, first, w)) return;
-    const Segment g = segment_of(a, a.target, w.row, w.seg);
+    const Segment g = segment_of(a, a.target, w.row, w.seg, a.per);
     float m = -INFINITY;
     int at = -1;
     bool bad = false;
@@ -474,7 +512,7 @@ __global__ __launch_bounds__(kVerThreads) void k_verify_best(VerifyArgs a, int f
 #pragma unroll
         for (int e = 0; e < E; e++) {
             bad |= !(v[e] < INFINITY);
-            at = v[e] > m ? place_of(c0, e) : at;
+            at = v[e] > m ? place_of<E, false>(c0, e) : at;
             m = fmaxf(m, v[e]);
         }
     }
@@ -519,32 +557,45 @@ __global__ __launch_bounds__(64) void k_verify_greedy(VerifyArgs a)
 
 // ------------------------------------------------------------------ host ---
 // workgroups that rows are cut into segments for
-constexpr int kVerTarget = 2048;
+constexpr int kVerTarget = 4096;
+
+// segments of a row for about `want` of them, in whole chunks
+static void cut_row(int vocab, int chunk, int want, int* segs, int* per)
+{
+    const int chunks = (int)(((int64_t)vocab + 7 + chunk - 1) / chunk);   // 7: values before the first that its chunk may hold
+    const int n = std::max(1, std::min({chunks, kVerMaxSegs, want})), each = (chunks + n - 1) / n;
+    *segs = (chunks + each - 1) / each;
+    *per = (int)std::min<int64_t>((int64_t)each * chunk, 0x7fffffff);
+}
 
 template <int E>
 static int verify_launch(Ctx* c, VerifyArgs a, bool greedy)
 {
-    constexpr int chunk = kVerThreads * E;
     const int targets = a.seqs * (a.n + 1), rows = targets + (a.draft.x ? a.seqs * a.n : 0);
-    const int chunks = (int)(((int64_t)a.vocab + 7 + chunk - 1) / chunk);   // 7: values before the first that its chunk may hold
-    const int want = std::max(1, std::min({chunks, kVerMaxSegs, (kVerTarget + rows - 1) / rows}));
-    const int each = (chunks + want - 1) / want;
-    a.segs = (chunks + each - 1) / each;
-    a.per = (int)std::min<int64_t>((int64_t)each * chunk, 0x7fffffff);
+    cut_row(a.vocab, kVerThreads * E, (kVerTarget + rows - 1) / rows, &a.segs, &a.per);
+    cut_row(a.vocab, kVerThreads * kDraw, (kVerTarget + a.seqs - 1) / a.seqs, &a.draw_segs, &a.draw_per);
     const size_t stats = (size_t)rows * a.segs * 2;
-    IAM_TRY(ensure_verify_scratch(c, stats + (size_t)a.seqs * a.segs, (size_t)a.seqs));
+    IAM_TRY(ensure_verify_scratch(c, stats + (size_t)a.seqs * a.draw_segs, (size_t)a.seqs));
     a.stat = c->ver_part;
     a.part = c->ver_part + stats;
     a.ctr = c->ver_ctr;
-    // at most 2^22 workgroups a launch
-    const int most = (1 << 22) / a.segs;
-    for (int r0 = 0; r0 < rows; r0 += most) {
-        const dim3 grid((unsigned)(std::min(most, rows - r0) * a.segs));
-        IAM_TRY(greedy ? launch(c, "verify_best", k_verify_best<E>, grid, dim3(kVerThreads), 0, a, r0)
-                       : launch(c, "verify_rows", k_verify_rows<E>, grid, dim3(kVerThreads), 0, a, r0));
-    }
+    // rows [r0, r1), at most 2^22 workgroups a launch
+    auto pass = [&](int r0, int r1, int type) {
+        const int most = (1 << 22) / a.segs;
+        for (; r0 < r1; r0 += most) {
+            const dim3 grid((unsigned)(std::min(most, r1 - r0) * a.segs)), block(kVerThreads);
+            if (greedy) IAM_TRY(launch(c, "verify_best", k_verify_best<E>, grid, block, 0, a, r0));
+            else if (type == IAM_F32) IAM_TRY(launch(c, "verify_rows", k_verify_rows<float, E>, grid, block, 0, a, r0));
+            else if (type == IAM_F16) IAM_TRY(launch(c, "verify_rows", k_verify_rows<_Float16, E>, grid, block, 0, a, r0));
+            else IAM_TRY(launch(c, "verify_rows", k_verify_rows<__bf16, E>, grid, block, 0, a, r0));
+        }
+        return IAM_OK;
+    };
+    const bool one = rows == targets || a.draft.type == a.target.type;
+    IAM_TRY(pass(0, one ? rows : targets, a.target.type));
+    if (!one) IAM_TRY(pass(targets, rows, a.draft.type));
     if (greedy) return launch(c, "verify_greedy", k_verify_greedy, dim3((unsigned)a.seqs), dim3(64), 0, a);
-    return launch(c, "verify_pick", k_verify_pick<E>, dim3((unsigned)(a.seqs * a.segs)), dim3(kVerThreads), 0, a);
+    return launch(c, "verify_pick", k_verify_pick, dim3((unsigned)(a.seqs * a.draw_segs)), dim3(kVerThreads), 0, a);
 }
 
 }  // namespace iam
