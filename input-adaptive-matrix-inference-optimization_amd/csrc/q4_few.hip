@@ -78,28 +78,30 @@ __device__ __forceinline__ void wave_sync()
     __builtin_amdgcn_wave_barrier();
 }
 
-// A workgroup takes a strip of 16 rows of the matrix; its waves deal the chunks
+// A workgroup takes S strips of 16 rows of the matrix; its waves deal the chunks
 // of 512 inputs among themselves.  A wave brings the rows' 512 values into its
 // own part of LDS as digits in the operands' order (16 lanes a tile, 8 values
-// each) while the weights are on their way, and needs no other wave until the
-// sums are joined.
-template <int D, int GROUP, bool ZEROS>
+// each) while the first strip's weights are on their way (a strip's come while
+// the one before is computed), and needs no other wave until the sums are joined.
+template <int D, int GROUP, bool ZEROS, int S>
 __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
 {
     extern __shared__ uint4 lds[];
     const MulArgs& u = a.u;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c = lane & 15;
-    const int strip = xcd_remap(blockIdx.x, gridDim.x), cols = u.rows * D;
+    const int strip0 = xcd_remap(blockIdx.x, gridDim.x) * S, last = q4_strips(u.m.out) - 1, cols = u.rows * D;
     uint4* digits = lds + wave * (32 * cols);                                       // [tile][step][g][col] 16 bytes
     float* factor = reinterpret_cast<float*>(lds + a.waves * (32 * cols)) + wave * 4 * kFewCols;   // [tile][row]
     const int col = min(c, cols - 1), mine = col / D;
-    floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    FewWeights<GROUP, ZEROS> now;
+    floatx4 acc[S];
+#pragma unroll
+    for (int s = 0; s < S; s++) acc[s] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    FewWeights<GROUP, ZEROS> buf[S > 1 ? 2 : 1];
     for (int chunk = wave; chunk < u.m.chunks; chunk += a.waves) {
         const int t16 = lane >> 4, k8 = lane & 15, k = chunk * kChunk + t16 * kTile + k8 * 8;
         Raw8 raw = load_raw8(u.x, u.x_type, 0, k, u.m.in);
         float xs = D == 1 || u.x_scale ? u.x_scale[u.x_groups > 1 ? min(chunk * 4 + t16, u.x_groups - 1) : 0] : 1.0f;
-        now.load(u.m, strip, chunk, lane);
+        buf[0].load(u.m, strip0, chunk, lane);
         uint2* to = reinterpret_cast<uint2*>(digits + ((t16 * 2 + (k8 >> 3)) * 4 + (k8 & 3)) * cols) + (k8 >> 2 & 1);
         for (int r = 0; r < u.rows; r++) {
             const Raw8 mine8 = raw;
@@ -143,61 +145,69 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
             }
         }
         wave_sync();
+        if constexpr (S > 1) buf[1].load(u.m, min(strip0 + 1, last), chunk, lane);
         const int tiles = min(4, u.m.tiles - chunk * 4);
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            if (t >= tiles) break;
-            const float f = factor[t * kFewCols + mine] * (ZEROS ? 1.0f : 0.0625f);
-            const uint32_t wd[4] = {now.w[t].x, now.w[t].y, now.w[t].z, now.w[t].w};
-            intx4 sum = {0, 0, 0, 0};
+        for (int sn = 0; sn < S; sn++) {
+            FewWeights<GROUP, ZEROS>& now = buf[sn & 1];
 #pragma unroll
-            for (int step = 0; step < 2; step++) {
-                const uint4 b = digits[((t * 2 + step) * 4 + g) * cols + col];
-                uint32_t lo[2], hi[2];
+            for (int t = 0; t < 4; t++) {
+                if (t >= tiles) break;
+                const float f = factor[t * kFewCols + mine] * (ZEROS ? 1.0f : 0.0625f);
+                const uint32_t wd[4] = {now.w[t].x, now.w[t].y, now.w[t].z, now.w[t].w};
+                intx4 sum = {0, 0, 0, 0};
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const int grp = (t * kTile + (step * 2 + j) * 32) / GROUP;
-                    uint32_t z4 = 0;
-                    if constexpr (ZEROS) z4 = __builtin_amdgcn_perm(0u, now.z[grp / 4], 0x01010101u * (grp % 4));
-                    widen8<ZEROS>(wd[step * 2 + j], z4, lo[j], hi[j]);
-                }
-                auto join = [&](int grp) {
-                    const uint32_t s0 = grp % 2 ? now.s[grp / 2].z : now.s[grp / 2].x, s1 = grp % 2 ? now.s[grp / 2].w : now.s[grp / 2].y;
-                    const half4 s = __builtin_bit_cast(half4, (uint64_t)s1 << 32 | s0);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[i] = __builtin_fmaf((float)sum[i], (float)s[i] * f, acc[i]);
-                    sum = intx4{0, 0, 0, 0};
-                };
-                if constexpr (GROUP == 32) {
+                for (int step = 0; step < 2; step++) {
+                    const uint4 b = digits[((t * 2 + step) * 4 + g) * cols + col];
+                    uint32_t lo[2], hi[2];
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        const long x8 = (long)((uint64_t)(j ? b.w : b.y) << 32 | (j ? b.z : b.x));
-                        sum = __builtin_amdgcn_mfma_i32_16x16x32_i8((long)((uint64_t)hi[j] << 32 | lo[j]), x8, sum, 0, 0, 0);
-                        join(t * 4 + step * 2 + j);
+                        const int grp = (t * kTile + (step * 2 + j) * 32) / GROUP;
+                        uint32_t z4 = 0;
+                        if constexpr (ZEROS) z4 = __builtin_amdgcn_perm(0u, now.z[grp / 4], 0x01010101u * (grp % 4));
+                        widen8<ZEROS>(wd[step * 2 + j], z4, lo[j], hi[j]);
                     }
-                } else {
-                    const intx4 w8 = {(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
-                    sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(w8, __builtin_bit_cast(intx4, b), sum, 0, 0, 0);
-                    if constexpr (GROUP == 64) join(t * 2 + step);
-                    else if (step == 1) join(t);
+                    auto join = [&](int grp) {
+                        const uint32_t s0 = grp % 2 ? now.s[grp / 2].z : now.s[grp / 2].x, s1 = grp % 2 ? now.s[grp / 2].w : now.s[grp / 2].y;
+                        const half4 s = __builtin_bit_cast(half4, (uint64_t)s1 << 32 | s0);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[sn][i] = __builtin_fmaf((float)sum[i], (float)s[i] * f, acc[sn][i]);
+                        sum = intx4{0, 0, 0, 0};
+                    };
+                    if constexpr (GROUP == 32) {
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            const long x8 = (long)((uint64_t)(j ? b.w : b.y) << 32 | (j ? b.z : b.x));
+                            sum = __builtin_amdgcn_mfma_i32_16x16x32_i8((long)((uint64_t)hi[j] << 32 | lo[j]), x8, sum, 0, 0, 0);
+                            join(t * 4 + step * 2 + j);
+                        }
+                    } else {
+                        const intx4 w8 = {(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
+                        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(w8, __builtin_bit_cast(intx4, b), sum, 0, 0, 0);
+                        if constexpr (GROUP == 64) join(t * 2 + step);
+                        else if (step == 1) join(t);
+                    }
                 }
             }
+            if (sn + 2 < S) now.load(u.m, min(strip0 + sn + 2, last), chunk, lane);
         }
         wave_sync();
     }
-    // the waves' sums: [wave][col][16]
+    // the waves' sums: [wave][strip][col][16]
     float* part = reinterpret_cast<float*>(lds);
     __syncthreads();
-    if (c < cols) *reinterpret_cast<floatx4*>(part + (wave * cols + c) * 16 + 4 * g) = acc;
+    if (c < cols)
+#pragma unroll
+        for (int s = 0; s < S; s++) *reinterpret_cast<floatx4*>(part + ((wave * S + s) * cols + c) * 16 + 4 * g) = acc[s];
     __syncthreads();
-    for (int i = tid; i < u.rows * 16; i += a.waves * 64) {
-        const int r = i >> 4, o = strip * kStrip + (i & 15);
+    for (int i = tid; i < S * u.rows * 16; i += a.waves * 64) {
+        const int r = i / (S * 16), s = i / 16 % S, o = (strip0 + s) * kStrip + (i & 15);
         float y = 0.0f;
 #pragma unroll
         for (int d = D - 1; d >= 0; d--) {
-            float s = 0.0f;
-            for (int w = 0; w < a.waves; w++) s += part[(w * cols + r * D + d) * 16 + (i & 15)];
-            y = __builtin_fmaf(y, 256.0f, s);
+            float sum = 0.0f;
+            for (int w = 0; w < a.waves; w++) sum += part[((w * S + s) * cols + r * D + d) * 16 + (i & 15)];
+            y = __builtin_fmaf(y, 256.0f, sum);
         }
         if (o < u.m.out) put_value(u.y, u.y_type, (size_t)r * u.y_stride + o, y);
     }
@@ -206,22 +216,41 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
 // ------------------------------------------------------------------ host ---
 int q4_few_most(int x_type) { return x_type == IAM_I8 ? kFewCols : kFewCols / 3; }
 
-template <int D, int GROUP>
+template <int D, int GROUP, int S>
 static int few_launch(Ctx* c, const FewArgs& a)
 {
     const int cols = a.u.rows * D;
-    const size_t stage = (size_t)a.waves * (32 * cols * 16 + 4 * kFewCols * 4), join = (size_t)a.waves * cols * 64;
-    const dim3 grid((unsigned)q4_strips(a.u.m.out)), block((unsigned)a.waves * 64);
-    return a.u.m.zeros ? launch(c, "q4_mul.few", k_q4_few<D, GROUP, true>, grid, block, std::max(stage, join), a)
-                       : launch(c, "q4_mul.few", k_q4_few<D, GROUP, false>, grid, block, std::max(stage, join), a);
+    const size_t stage = (size_t)a.waves * (32 * cols * 16 + 4 * kFewCols * 4), join = (size_t)a.waves * S * cols * 64;
+    const dim3 grid((unsigned)((q4_strips(a.u.m.out) + S - 1) / S)), block((unsigned)a.waves * 64);
+    return a.u.m.zeros ? launch(c, "q4_mul.few", k_q4_few<D, GROUP, true, S>, grid, block, std::max(stage, join), a)
+                       : launch(c, "q4_mul.few", k_q4_few<D, GROUP, false, S>, grid, block, std::max(stage, join), a);
+}
+
+template <int D, int GROUP>
+static int few_sized(Ctx* c, const FewArgs& a)
+{
+    // Several strips share the rows' digits where there are enough of them for
+    // the card all the same (one fp32 row, 32000 x 4096: 17.6 us by single strips,
+    // 14.0 by two, 12.9 by four; five bf16 rows 27.4, 18.7 and 15.2; 14336 x 4096 10.8,
+    // 8.7 and 8.7; 6144 x 4096 with groups of 64 7.9, 8.4 and 11.4).  Groups of 64
+    // fill the registers with two strips' scales, which pays for several rows
+    // only (28672 x 4096: one row 17.8, 18.5 and 19.0, five 26.7, 23.1 and 20.6); those of 32 do
+    // not fit at all.
+    const int strips = q4_strips(a.u.m.out), cols = a.u.rows * D;
+    if constexpr (GROUP > 32) {
+        if (strips >= (GROUP == 128 ? 768 : 1024) && (GROUP == 128 || cols > 4)) return few_launch<D, GROUP, 4>(c, a);
+        if constexpr (GROUP == 64)
+            if (strips >= 768 && cols > 4) return few_launch<D, GROUP, 2>(c, a);
+    }
+    return few_launch<D, GROUP, 1>(c, a);
 }
 
 template <int D>
 static int few_grouped(Ctx* c, const FewArgs& a)
 {
-    if (a.u.m.group == 32) return few_launch<D, 32>(c, a);
-    if (a.u.m.group == 64) return few_launch<D, 64>(c, a);
-    return few_launch<D, 128>(c, a);
+    if (a.u.m.group == 32) return few_sized<D, 32>(c, a);
+    if (a.u.m.group == 64) return few_sized<D, 64>(c, a);
+    return few_sized<D, 128>(c, a);
 }
 
 int q4_mul_few(Ctx* c, const MulArgs& u)
