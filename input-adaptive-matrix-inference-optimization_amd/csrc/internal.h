@@ -140,6 +140,11 @@ struct Ctx {
     // products with 4-bit weights: the rows of x in the operands' order
     uint8_t* q4_part = nullptr;
     size_t q4_part_cap = 0;
+    // and the sums of parts of the inputs, their arrival counters (zero between calls)
+    float* q4_sums = nullptr;
+    size_t q4_sums_cap = 0;
+    uint32_t* q4_ctr = nullptr;
+    size_t q4_ctr_cap = 0;
     // bumped whenever a context-owned scratch buffer is reallocated:
     // captured graphs hold those addresses and must be re-captured
     uint64_t scratch_gen = 0;
@@ -338,6 +343,8 @@ int ensure_kv8_scratch(Ctx* c, size_t floats, size_t counters);
 int ensure_lp_scratch(Ctx* c, size_t doubles, size_t counters);
 // products with 4-bit weights: bytes of operands
 int ensure_q4_scratch(Ctx* c, size_t bytes);
+// and floats of parts' sums, arrival counters
+int ensure_q4_sums(Ctx* c, size_t floats, size_t counters);
 // verification of drafted tokens: the same
 int ensure_verify_scratch(Ctx* c, size_t doubles, size_t counters);
 

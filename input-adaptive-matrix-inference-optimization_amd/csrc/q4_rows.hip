@@ -7,12 +7,14 @@
 // and low, of fp32 (22 bits).  4-bit weights become fp16 under the exponents of
 // 1024 and 64, n - zero exactly.  Products are then exact; a group's are added
 // in fp32 by the instructions and go to the row's sum with the group's scale.
+#include "accum.h"
 #include "q4_mul.h"
 
 namespace iam {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef unsigned long long ull2 __attribute__((ext_vector_type(2)));
 
 // ---- x in the operands' order
 // parts  fp16 [part][block of 16 rows][tile][j][lane 16 g + row][8]: inputs
@@ -88,6 +90,10 @@ struct RowsArgs {
     bool factors;             // whether factor may hold anything but 1
     int blocks;               // of 16 rows
     int waves;
+    // the inputs cut into parts for more workgroups, whose sums the last one to arrive joins
+    int splits;
+    float* sums;
+    uint32_t* ctr;            // zero on entry (left zero)
 };
 
 // Eight weights as fp16, n - zero: under the exponent of 1024 a number's step is
@@ -136,14 +142,15 @@ __device__ __forceinline__ void put_four(const MulArgs& u, int r, int o, floatx4
 // A workgroup takes S strips of the matrix and NB blocks of 16 rows; its waves
 // deal the tiles of 128 inputs among themselves and join their sums in LDS.
 // Every operand comes straight from memory in the order in which it is used.
-template <int PARTS, int GROUP, int S, int NB>
-__global__ __launch_bounds__(1024) void k_q4_batch(RowsArgs a)
+template <int PARTS, int GROUP, int S, int NB, int MOST>
+__global__ __launch_bounds__(64 * MOST) void k_q4_batch(RowsArgs a)
 {
     extern __shared__ floatx4 join[];
     constexpr int GT = kTile / GROUP;      // groups of a tile
     const MulArgs& u = a.u;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-    const int strips = q4_strips(u.m.out), s0 = xcd_remap(blockIdx.x, gridDim.x) * S, b0 = blockIdx.y * NB;
+    const int strips = q4_strips(u.m.out), groups = (strips + S - 1) / S, id = xcd_remap(blockIdx.x, gridDim.x);
+    const int split = id / groups, group = id - split * groups, s0 = group * S, b0 = blockIdx.y * NB;
     floatx4 acc[S][NB];
 #pragma unroll
     for (int s = 0; s < S; s++)
@@ -156,52 +163,48 @@ __global__ __launch_bounds__(1024) void k_q4_batch(RowsArgs a)
         strip[s] = min(s0 + s, strips - 1);
         words[s] = reinterpret_cast<const uint4*>(u.m.numbers) + (size_t)strip[s] * u.m.tiles * 64 + lane;
     }
-    uint4 next[S];
-    if (wave < u.m.tiles) {
-#pragma unroll
-        for (int s = 0; s < S; s++) next[s] = words[s][(size_t)wave * 64];
-    }
-    for (int t = wave; t < u.m.tiles; t += a.waves) {
+    // a tile's operands, scales and zero points
+    struct Tile {
         half8 x[PARTS][NB][4];
         float f[NB];
+        uint4 w[S];
+        half4 sc[S][GT];
+        uint32_t zero[S];
+    };
+    auto load = [&](Tile& o, int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            o.w[s] = words[s][(size_t)t * 64];
+            const size_t cell = (size_t)strip[s] * u.m.chunks + (t >> 2);
+            const half4* q = reinterpret_cast<const half4*>(u.m.scales) + (cell * 4 + g) * (4 * GT) + (t & 3) * GT;
+#pragma unroll
+            for (int i = 0; i < GT; i++) o.sc[s][i] = q[i];
+            o.zero[s] = 0x08080808u;
+            if (u.m.zeros) {
+                const uint8_t* z = u.m.zeros + (cell * kStrip + c) * (4 * GT) + (t & 3) * GT;
+                if constexpr (GT == 1) o.zero[s] = *z;
+                else if constexpr (GT == 2) o.zero[s] = *reinterpret_cast<const uint16_t*>(z);
+                else o.zero[s] = *reinterpret_cast<const uint32_t*>(z);
+            }
+        }
 #pragma unroll
         for (int n = 0; n < NB; n++) {
             const size_t cell = (size_t)min(b0 + n, a.blocks - 1) * u.m.tiles + t;
 #pragma unroll
             for (int p = 0; p < PARTS; p++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[p][n][j] = *reinterpret_cast<const half8*>(a.parts + p * a.part_stride + (cell * 4 + j) * 512 + lane * 8);
-            f[n] = a.factor[cell * 16 + c];
+                for (int j = 0; j < 4; j++) o.x[p][n][j] = *reinterpret_cast<const half8*>(a.parts + p * a.part_stride + (cell * 4 + j) * 512 + lane * 8);
+            o.f[n] = a.factor[cell * 16 + c];
         }
-        uint4 w[S];
-        half4 sc[S][GT];
-        uint32_t zero[S];
+    };
+    auto compute = [&](const Tile& o) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < S; s++) {
-            w[s] = next[s];
-            const size_t cell = (size_t)strip[s] * u.m.chunks + (t >> 2);
-            const half4* q = reinterpret_cast<const half4*>(u.m.scales) + (cell * 4 + g) * (4 * GT) + (t & 3) * GT;
-#pragma unroll
-            for (int i = 0; i < GT; i++) sc[s][i] = q[i];
-            zero[s] = 0x08080808u;
-            if (u.m.zeros) {
-                const uint8_t* z = u.m.zeros + (cell * kStrip + c) * (4 * GT) + (t & 3) * GT;
-                if constexpr (GT == 1) zero[s] = *z;
-                else if constexpr (GT == 2) zero[s] = *reinterpret_cast<const uint16_t*>(z);
-                else zero[s] = *reinterpret_cast<const uint32_t*>(z);
-            }
-        }
-        if (t + a.waves < u.m.tiles) {
-#pragma unroll
-            for (int s = 0; s < S; s++) next[s] = words[s][(size_t)(t + a.waves) * 64];
-        }
-#pragma unroll
-        for (int s = 0; s < S; s++) {
-            const uint32_t wd[4] = {w[s].x, w[s].y, w[s].z, w[s].w};
+            const uint32_t wd[4] = {o.w[s].x, o.w[s].y, o.w[s].z, o.w[s].w};
             half8 wide[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const Minus m = minus_of(zero[s] >> (8 * (j * 32 / GROUP)) & 255u);
+                const Minus m = minus_of(o.zero[s] >> (8 * (j * 32 / GROUP)) & 255u);
                 wide[j] = widen_half(wd[j], m.k1024, m.k64);
             }
 #pragma unroll
@@ -212,12 +215,20 @@ __global__ __launch_bounds__(1024) void k_q4_batch(RowsArgs a)
 #pragma unroll
                     for (int j = i * 4 / GT; j < (i + 1) * 4 / GT; j++)
 #pragma unroll
-                        for (int p = 0; p < PARTS; p++) d = mfma_f16(wide[j], x[p][n][j], d);
+                        for (int p = 0; p < PARTS; p++) d = mfma_f16(wide[j], o.x[p][n][j], d);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[s][n][e] = __builtin_fmaf(d[e] * f[n], (float)sc[s][i][e], acc[s][n][e]);
+                    for (int e = 0; e < 4; e++) acc[s][n][e] = __builtin_fmaf(d[e] * o.f[n], (float)o.sc[s][i][e], acc[s][n][e]);
                 }
             }
         }
+    };
+    for (int t = split * a.waves + wave; t < u.m.tiles; t += a.splits * a.waves) {
+        Tile o;
+        load(o, t);
+        // all loads before any use: left to itself the compiler saved registers and
+        // waited for a few at a time (32 fp32 rows, 4096 x 14336: 27 us against 17)
+        __builtin_amdgcn_sched_barrier(0);
+        compute(o);
     }
     if (a.waves > 1) {
 #pragma unroll
@@ -226,22 +237,48 @@ __global__ __launch_bounds__(1024) void k_q4_batch(RowsArgs a)
             for (int n = 0; n < NB; n++) join[(wave * S * NB + s * NB + n) * 64 + lane] = acc[s][n];
         __syncthreads();
     }
+    // value e of a lane is row 4 g + e of strip s, row c of block n
+    auto put = [&](int s, int n, floatx4 v) __attribute__((always_inline)) {
+        const int r = (b0 + n) * 16 + c;
+        if (s0 + s >= strips || r >= u.rows) return;
+        if (a.row_scale) v *= a.row_scale[r];
+        put_four(u, r, (s0 + s) * kStrip + 4 * g, v);
+    };
+    // the splits' sums: [group of strips][group of blocks][split][S * NB][lane] four floats
+    const size_t cell = (size_t)blockIdx.y * groups + group;
+    float* sums = a.sums + cell * a.splits * (S * NB * 256);
 #pragma unroll
-    for (int s = 0; s < S; s++)
-#pragma unroll
-        for (int n = 0; n < NB; n++) {
-            const int i = s * NB + n;
-            if (i % a.waves != wave) continue;
-            floatx4 v = acc[s][n];
-            if (a.waves > 1) {
-                v = join[i * 64 + lane];
-                for (int q = 1; q < a.waves; q++) v += join[(q * S * NB + i) * 64 + lane];
-            }
-            const int r = (b0 + n) * 16 + c;
-            if (s0 + s >= strips || r >= u.rows) continue;
-            if (a.row_scale) v *= a.row_scale[r];
-            put_four(u, r, (s0 + s) * kStrip + 4 * g, v);
+    for (int i = 0; i < S * NB; i++) {
+        if (i % a.waves != wave) continue;
+        floatx4 v = acc[i / NB][i % NB];
+        if (a.waves > 1) {
+            v = join[i * 64 + lane];
+            for (int q = 1; q < a.waves; q++) v += join[(q * S * NB + i) * 64 + lane];
         }
+        if (a.splits == 1) {
+            put(i / NB, i % NB, v);
+        } else {
+            const ull2 two = __builtin_bit_cast(ull2, v);
+            unsigned long long* to = reinterpret_cast<unsigned long long*>(sums + ((size_t)split * (S * NB) + i) * 256 + lane * 4);
+            acc_put(to, two[0]);
+            acc_put(to + 1, two[1]);
+        }
+    }
+    if (a.splits == 1) return;
+    __shared__ int last;
+    if (!acc_arrive(a.ctr + cell, (uint32_t)a.splits, &last)) return;
+    if (threadIdx.x == 0) a.ctr[cell] = 0u;
+    for (int i = wave; i < S * NB; i += a.waves) {
+        floatx4 v = {0, 0, 0, 0};
+        for (int q = 0; q < a.splits; q++) {
+            unsigned long long* from = reinterpret_cast<unsigned long long*>(sums + ((size_t)q * (S * NB) + i) * 256 + lane * 4);
+            ull2 two;
+            two[0] = acc_peek(from);
+            two[1] = acc_peek(from + 1);
+            v += __builtin_bit_cast(floatx4, two);
+        }
+        put(i / NB, i % NB, v);
+    }
 }
 
 // Many rows: a workgroup takes 64 WO rows of the matrix and 32 NB of x, its
@@ -264,51 +301,55 @@ struct Gemm {
 };
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 // LDS reads in one piece of assembly with their wait: the compiler, which
 // cannot tell the stages apart, would wait for all loads in flight to LDS
 // before any of them.
-__device__ __forceinline__ void read_runs8(uint32_t at, u32x4* r)
+// x's operands of 32 rows (two blocks): (j, p) at 1024 j + 512 p
+__device__ __forceinline__ void read_rows32(uint32_t at, u32x4* r)
 {
     asm volatile(
-        "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:1024\n\tds_read_b128 %2, %8 offset:2048\n\tds_read_b128 %3, %8 offset:3072\n\t"
-        "ds_read_b128 %4, %8 offset:4096\n\tds_read_b128 %5, %8 offset:5120\n\tds_read_b128 %6, %8 offset:6144\n\tds_read_b128 %7, %8 offset:7168\n\t"
+        "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:512\n\tds_read_b128 %2, %8 offset:1024\n\tds_read_b128 %3, %8 offset:1536\n\t"
+        "ds_read_b128 %4, %8 offset:2048\n\tds_read_b128 %5, %8 offset:2560\n\tds_read_b128 %6, %8 offset:3072\n\tds_read_b128 %7, %8 offset:3584\n\t"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
         : "v"(at)
         : "memory");
 }
-__device__ __forceinline__ void read_runs16(uint32_t at, u32x4* r)
+// and of 64 rows
+__device__ __forceinline__ void read_rows64(uint32_t at, u32x4* r)
 {
     asm volatile(
-        "ds_read_b128 %0, %16\n\tds_read_b128 %1, %16 offset:1024\n\tds_read_b128 %2, %16 offset:2048\n\tds_read_b128 %3, %16 offset:3072\n\t"
-        "ds_read_b128 %4, %16 offset:4096\n\tds_read_b128 %5, %16 offset:5120\n\tds_read_b128 %6, %16 offset:6144\n\tds_read_b128 %7, %16 offset:7168\n\t"
-        "ds_read_b128 %8, %16 offset:8192\n\tds_read_b128 %9, %16 offset:9216\n\tds_read_b128 %10, %16 offset:10240\n\tds_read_b128 %11, %16 offset:11264\n\t"
-        "ds_read_b128 %12, %16 offset:12288\n\tds_read_b128 %13, %16 offset:13312\n\tds_read_b128 %14, %16 offset:14336\n\tds_read_b128 %15, %16 offset:15360\n\t"
+        "ds_read_b128 %0, %16\n\tds_read_b128 %1, %16 offset:512\n\tds_read_b128 %2, %16 offset:1024\n\tds_read_b128 %3, %16 offset:1536\n\t"
+        "ds_read_b128 %4, %16 offset:2048\n\tds_read_b128 %5, %16 offset:2560\n\tds_read_b128 %6, %16 offset:3072\n\tds_read_b128 %7, %16 offset:3584\n\t"
+        "ds_read_b128 %8, %16 offset:8192\n\tds_read_b128 %9, %16 offset:8704\n\tds_read_b128 %10, %16 offset:9216\n\tds_read_b128 %11, %16 offset:9728\n\t"
+        "ds_read_b128 %12, %16 offset:10240\n\tds_read_b128 %13, %16 offset:10752\n\tds_read_b128 %14, %16 offset:11264\n\tds_read_b128 %15, %16 offset:11776\n\t"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]), "=&v"(r[8]), "=&v"(r[9]), "=&v"(r[10]),
           "=&v"(r[11]), "=&v"(r[12]), "=&v"(r[13]), "=&v"(r[14]), "=&v"(r[15])
         : "v"(at)
         : "memory");
 }
-// four strips' words, zero points and scales of the first group
-__device__ __forceinline__ void read_words(uint32_t words, uint32_t zeros, uint32_t scales, u32x4* w, uint32_t* z, u32x2* s)
+// two pairs of strips: words (pair, p) at 2048 pair + 512 p, zero points, scales of the first group
+__device__ __forceinline__ void read_words(uint32_t words, uint32_t zeros, uint32_t scales, u32x4* w, uint32_t* z, u32x4* s)
 {
     asm volatile(
-        "ds_read_b128 %0, %12\n\tds_read_b128 %1, %12 offset:1024\n\tds_read_b128 %2, %12 offset:2048\n\tds_read_b128 %3, %12 offset:3072\n\t"
-        "ds_read_b32 %4, %13\n\tds_read_b32 %5, %13 offset:64\n\tds_read_b32 %6, %13 offset:128\n\tds_read_b32 %7, %13 offset:192\n\t"
-        "ds_read_b64 %8, %14\n\tds_read_b64 %9, %14 offset:32\n\tds_read_b64 %10, %14 offset:64\n\tds_read_b64 %11, %14 offset:96\n\t"
+        "ds_read_b128 %0, %10\n\tds_read_b128 %1, %10 offset:512\n\tds_read_b128 %2, %10 offset:2048\n\tds_read_b128 %3, %10 offset:2560\n\t"
+        "ds_read_b32 %4, %11\n\tds_read_b32 %5, %11 offset:128\n\t"
+        "ds_read2_b64 %6, %12 offset0:0 offset1:2\n\tds_read2_b64 %7, %12 offset0:4 offset1:6\n\t"
+        "ds_read2_b64 %8, %12 offset0:8 offset1:10\n\tds_read2_b64 %9, %12 offset0:12 offset1:14\n\t"
         "s_waitcnt lgkmcnt(0)"
-        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(z[0]), "=&v"(z[1]), "=&v"(z[2]), "=&v"(z[3]), "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
+        : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3]), "=&v"(z[0]), "=&v"(z[1]), "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
         : "v"(words), "v"(zeros), "v"(scales)
         : "memory");
 }
-// four strips' scales of a group
-__device__ __forceinline__ void read_scales(uint32_t at, u32x2* s)
+// their scales of a group: rows 8 i .. 8 i + 7 of a pair are in half i % 2 of s[2 pair + i / 2]
+__device__ __forceinline__ void read_scales(uint32_t at, u32x4* s)
 {
     asm volatile(
-        "ds_read_b64 %0, %4\n\tds_read_b64 %1, %4 offset:32\n\tds_read_b64 %2, %4 offset:64\n\tds_read_b64 %3, %4 offset:96\n\t"
+        "ds_read2_b64 %0, %4 offset0:0 offset1:2\n\tds_read2_b64 %1, %4 offset0:4 offset1:6\n\t"
+        "ds_read2_b64 %2, %4 offset0:8 offset1:10\n\tds_read2_b64 %3, %4 offset0:12 offset1:14\n\t"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
         : "v"(at)
@@ -321,12 +362,13 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_
 // instruction and its results' first use, where the compiler leaves out the
 // wait states of the edge that jumps.
 template <int PARTS, int GROUP, int NB, int WO, int STAGES, bool FACTORS, bool SECOND>
-__device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP, NB, WO, STAGES>& stage, int s0, int b0, floatx4 (&acc)[kGemmStrips][NB])
+__device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP, NB, WO, STAGES>& stage, int s0, int b0, floatx16 (&acc)[2][NB / 2])
 {
     typedef Gemm<PARTS, GROUP, NB, WO, STAGES> G;
-    constexpr int GT = G::GT, S = G::S;
+    constexpr int GT = G::GT, S = G::S, N = NB / 2;
     const MulArgs& u = a.u;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int c = lane & 15, side = lane >> 4 & 1, half = lane >> 5;   // row (of x or the matrix) 16 side + c, inputs 8 half and on of 16
     const int wo = wave >> 1, wx = wave & 1, last = q4_strips(u.m.out) - 1;
     typedef const __attribute__((address_space(1))) void* From;
     typedef __attribute__((address_space(3))) void* To;
@@ -378,10 +420,10 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
             }
         }
     };
-    float f[NB];
+    float f[N];
     auto load_factors = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < NB; n++) f[n] = a.factor[((size_t)min(b0 + wx * NB + n, a.blocks - 1) * u.m.tiles + t) * 16 + c];
+        for (int n = 0; n < N; n++) f[n] = a.factor[((size_t)min(b0 + wx * NB + 2 * n + side, a.blocks - 1) * u.m.tiles + t) * 16 + c];
     };
     if constexpr (FACTORS) load_factors(0);
 #pragma unroll
@@ -400,7 +442,7 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
     };
     // Two groups of four waves, one of each on a SIMD, take turns: one reads its
     // operands while the other computes.  (All in step read together, with the
-    // matrix instructions idle: .)
+    // matrix instructions idle, 4096 rows of 14336 x 4096 took 534 us against 479.)
     constexpr bool TURNS = G::WAVES == 8;
     arrived();
     meet();
@@ -409,71 +451,77 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
     for (int t = 0; t < u.m.tiles; t++) {
         // Every wave's loads of this tile have arrived, and every wave has read
         // the tile before, whose place the newest tile takes.
-        float fn[NB];
+        float fn[N];
         if constexpr (FACTORS) {
 #pragma unroll
-            for (int n = 0; n < NB; n++) fn[n] = f[n];
+            for (int n = 0; n < N; n++) fn[n] = f[n];
             load_factors(min(t + 1, u.m.tiles - 1));
         }
         fetch(min(t + STAGES - 1, u.m.tiles - 1), free_buf);   // behind the last tile, the last one again
         const uint32_t at = base + buf * G::BYTES;
         free_buf = buf;
         buf = buf + 1 == STAGES ? 0 : buf + 1;
-        u32x4 x[PARTS][NB * 4], w[S];
-        u32x2 sc[GT][S];
-        uint32_t zero[S];
-        read_words(at + (G::X + wo * S) * 1024 + lane16, at + G::ZEROS + wo * S * 64 + c * 4, at + G::SCALES + wo * S * 32 + g * 8, w, zero, sc[0]);
+        u32x4 x[PARTS][N * 8], w[4], sc[GT][4];
+        uint32_t zero[2];
+        const uint32_t mine = (uint32_t)(half * 16 + c) * 16u;
+        read_words(at + (G::X + wo * S + side) * 1024 + mine, at + G::ZEROS + (wo * S + side) * 64 + c * 4, at + G::SCALES + wo * S * 32 + half * 8, w, zero, sc[0]);
 #pragma unroll
-        for (int i = 1; i < GT; i++) read_scales(at + G::SCALES + i * G::STRIPS * 32 + wo * S * 32 + g * 8, sc[i]);
+        for (int i = 1; i < GT; i++) read_scales(at + G::SCALES + i * G::STRIPS * 32 + wo * S * 32 + half * 8, sc[i]);
 #pragma unroll
         for (int p = 0; p < PARTS; p++) {
-            const uint32_t from = at + (p * 2 + wx) * NB * 4096 + lane16;
-            if constexpr (NB == 4) read_runs16(from, x[p]);
-            else read_runs8(from, x[p]);
+            const uint32_t from = at + ((p * 2 + wx) * NB + side) * 4096 + mine;
+            if constexpr (N == 2) read_rows64(from, x[p]);
+            else read_rows32(from, x[p]);
         }
         // the next tile's loads, as late as the other group's turn allows
         if constexpr (SECOND) arrived();
         if constexpr (TURNS) meet();
 #pragma unroll
-        for (int s = 0; s < S; s++) {
-            half8 wide[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t z = !u.m.zeros ? 8u
-                                   : GT == 1  ? zero[s] >> (8 * (t & 3))
-                                   : GT == 2  ? zero[s] >> (16 * (t & 1) + 8 * (j >> 1))
-                                              : zero[s] >> (8 * j);
-                const Minus m = minus_of(z & 255u);
-                wide[j] = widen_half(w[s][j], m.k1024, m.k64);
-            }
+        for (int s = 0; s < 2; s++) {       // pairs of strips
 #pragma unroll
             for (int i = 0; i < GT; i++) {
-                floatx4 d[NB];
-                const half4 scale = __builtin_bit_cast(half4, sc[i][s]);
+                const uint32_t z = !u.m.zeros ? 8u
+                                   : GT == 1  ? zero[s] >> (8 * (t & 3))
+                                   : GT == 2  ? zero[s] >> (16 * (t & 1) + 8 * i)
+                                              : zero[s] >> (8 * i);
+                const Minus m = minus_of(z & 255u);
+                floatx16 d[PARTS][N];
 #pragma unroll
-                for (int n = 0; n < NB; n++) d[n] = floatx4{0, 0, 0, 0};
+                for (int p = 0; p < PARTS; p++)
 #pragma unroll
-                for (int j = i * 4 / GT; j < (i + 1) * 4 / GT; j++)
+                    for (int n = 0; n < N; n++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) d[p][n][e] = 0.0f;
+#pragma unroll
+                for (int k = i * 8 / GT; k < (i + 1) * 8 / GT; k++) {      // 16 inputs: word k / 2, g = 2 (k % 2) + half
+                    const half8 wide = widen_half(w[s * 2 + k % 2][k / 2], m.k1024, m.k64);
 #pragma unroll
                     for (int p = 0; p < PARTS; p++)
 #pragma unroll
-                        for (int n = 0; n < NB; n++) d[n] = mfma_f16(wide[j], __builtin_bit_cast(half8, x[p][n * 4 + j]), d[n]);
+                        for (int n = 0; n < N; n++)
+                            d[p][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wide, __builtin_bit_cast(half8, x[p][n * 8 + k]), d[p][n], 0, 0, 0);
+                }
 #pragma unroll
-                for (int n = 0; n < NB; n++)
+                for (int n = 0; n < N; n++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[s][n][e] = __builtin_fmaf(FACTORS ? d[n][e] * fn[n] : d[n][e], (float)scale[e], acc[s][n][e]);
+                    for (int e = 0; e < 16; e++) {
+                        const half8 scale = __builtin_bit_cast(half8, sc[i][s * 2 + e / 8]);
+                        float v = d[0][n][e];
+                        if constexpr (PARTS == 2) v += d[1][n][e];
+                        if constexpr (FACTORS) v *= fn[n];
+                        acc[s][n][e] = __builtin_fmaf(v, (float)scale[e % 8], acc[s][n][e]);
+                    }
             }
             if constexpr (GT > 1) __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (GT == 1) {
-            // the widening of the next strip and the sums of the last between
-            // the matrix instructions (by strips, as below: ); smaller groups
-            // would spill
-            __builtin_amdgcn_sched_group_barrier(0x2, 40, 0);
+            // the widening of the next inputs and the sums of the last pair between
+            // the matrix instructions (smaller groups would spill)
+            __builtin_amdgcn_sched_group_barrier(0x2, 20, 0);
 #pragma unroll
-            for (int i = 0; i < S * NB * 4 * PARTS; i++) {
+            for (int i = 0; i < 16 * N * PARTS; i++) {
                 __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, 8, 0);
             }
         }
         if constexpr (!SECOND) arrived();
@@ -491,7 +539,7 @@ __global__ __launch_bounds__(128 * WO, 2) void k_q4_gemm(RowsArgs a)
     constexpr int S = kGemmStrips, STRIPS = S * WO;
     __shared__ Gemm<PARTS, GROUP, NB, WO, STAGES> stage;
     const MulArgs& u = a.u;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int strips = q4_strips(u.m.out);
     // panels of kGemmPanel along x's rows, the matrix's rows outermost in a panel
     const int along = (a.blocks + 2 * NB - 1) / (2 * NB), across = (strips + STRIPS - 1) / STRIPS;
@@ -518,11 +566,13 @@ __global__ __launch_bounds__(128 * WO, 2) void k_q4_gemm(RowsArgs a)
         factors = __builtin_amdgcn_readfirstlane(all) != 0;
         __syncthreads();
     }
-    floatx4 acc[S][NB];
+    floatx16 acc[2][NB / 2];
 #pragma unroll
-    for (int s = 0; s < S; s++)
+    for (int s = 0; s < 2; s++)
 #pragma unroll
-        for (int n = 0; n < NB; n++) acc[s][n] = floatx4{0, 0, 0, 0};
+        for (int n = 0; n < NB / 2; n++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[s][n][e] = 0.0f;
     auto tiles = [&](auto with_factors) __attribute__((always_inline)) {
         constexpr bool F = decltype(with_factors)::value;
         if (WO == 4 && wave >= 4) gemm_tiles<PARTS, GROUP, NB, WO, STAGES, F, WO == 4>(a, stage, s0, b0, acc);
@@ -530,29 +580,51 @@ __global__ __launch_bounds__(128 * WO, 2) void k_q4_gemm(RowsArgs a)
     };
     if (factors) tiles(std::true_type{});
     else tiles(std::false_type{});
+    // value 4 i + e of a lane is row 8 i + 4 (lane / 32) + e of the pair of strips
 #pragma unroll
-    for (int n = 0; n < NB; n++) {
-        const int r = (b0 + (wave & 1) * NB + n) * 16 + c;
+    for (int n = 0; n < NB / 2; n++) {
+        const int r = (b0 + (wave & 1) * NB + 2 * n) * 16 + (lane & 31);
         if (r >= u.rows) continue;
         const float rs = a.row_scale ? a.row_scale[r] : 1.0f;
 #pragma unroll
-        for (int s = 0; s < S; s++) {
-            const int strip = s0 + (wave >> 1) * S + s;
-            if (strip < strips) put_four(u, r, strip * kStrip + 4 * g, acc[s][n] * rs);
-        }
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int o = (s0 + (wave >> 1) * S) * kStrip + 32 * s + 8 * i + 4 * (lane >> 5);
+                if (o < u.m.out) put_four(u, r, o, floatx4{acc[s][n][4 * i], acc[s][n][4 * i + 1], acc[s][n][4 * i + 2], acc[s][n][4 * i + 3]} * rs);
+            }
     }
 }
 
 // ------------------------------------------------------------------ host ---
-template <int PARTS, int GROUP, int S, int NB>
+constexpr int kMaxSplits = 8;
+constexpr int kMinTiles = 16;      // of a split (64 bf16 rows, 1024 x 14336: 13.0 us at 32, 10.6 at 16, 13.4 at 10)
+
+template <int PARTS, int GROUP, int S, int NB, int MOST>
 static int batch_launch(Ctx* c, RowsArgs a)
 {
-    // as many waves as there are tiles, up to 16 and what LDS holds of their sums
-    const int most = std::min(16, 160 / (S * NB));
-    const int rounds = (a.u.m.tiles + most - 1) / most;
-    a.waves = (a.u.m.tiles + rounds - 1) / rounds;
-    const dim3 grid((unsigned)((q4_strips(a.u.m.out) + S - 1) / S), (unsigned)((a.blocks + NB - 1) / NB));
-    return launch(c, "q4_mul.batch", k_q4_batch<PARTS, GROUP, S, NB>, grid, dim3((unsigned)a.waves * 64), (size_t)a.waves * S * NB * 1024, a);
+    const int groups = (q4_strips(a.u.m.out) + S - 1) / S, across = (a.blocks + NB - 1) / NB;
+    // inputs cut for about a workgroup a CU
+    a.splits = S == 1 ? 1 : std::max(1, std::min({256 / (groups * across), kMaxSplits, a.u.m.tiles / kMinTiles}));
+    // waves share a workgroup's tiles evenly
+    const int each = (a.u.m.tiles + a.splits - 1) / a.splits, rounds = (each + MOST - 1) / MOST;
+    a.waves = (each + rounds - 1) / rounds;
+    if (a.splits > 1) {
+        IAM_TRY(ensure_q4_sums(c, (size_t)groups * across * a.splits * (S * NB * 256), (size_t)groups * across));
+        a.sums = c->q4_sums;
+        a.ctr = c->q4_ctr;
+    }
+    return launch(c, "q4_mul.batch", k_q4_batch<PARTS, GROUP, S, NB, MOST>, dim3((unsigned)(groups * a.splits), (unsigned)across),
+                  dim3((unsigned)a.waves * 64), (size_t)a.waves * S * NB * 1024, a);
+}
+
+template <int PARTS, int GROUP, int S, int MOST>
+static int batch_blocks(Ctx* c, const RowsArgs& a)
+{
+    // (two parts of four blocks would not fit the registers)
+    if (a.blocks == 1) return batch_launch<PARTS, GROUP, S, 1, MOST>(c, a);
+    if (a.blocks == 2 || PARTS == 2) return batch_launch<PARTS, GROUP, S, 2, MOST>(c, a);
+    return batch_launch<PARTS, GROUP, S, PARTS == 2 ? 2 : 4, MOST>(c, a);
 }
 
 template <int PARTS, int GROUP, int NB, int WO, int STAGES>
@@ -569,13 +641,31 @@ static int batch_sized(Ctx* c, const RowsArgs& a)
         if constexpr (PARTS == 2) {
             return gemm_launch<PARTS, GROUP, 2, 4, 3>(c, a);
         } else {
-            if (a.blocks > 32) return gemm_launch<PARTS, GROUP, 4, 4, 3>(c, a);
-            return gemm_launch<PARTS, GROUP, 2, 2, 3>(c, a);
+            // The shape whose workgroups, dealt to 256 CUs, take the least: a
+            // tile of 128 inputs takes 0.86 us in one of 128 x 64 products alone
+            // on a CU and 0.67 each of several, 1.07 in one of 256 x 64, 1.6 in one of
+            // 256 x 128 (389 rows, 6144 x 4096: 46, 42 and 57 us; 4096 rows, 14336 x
+            // 4096: 645, 614 and 497; 256 rows, 6144 x 4096: 32, 38 and 55).
+            auto rounds = [&](int strips, int blocks) {
+                const size_t n = (size_t)((q4_strips(a.u.m.out) + strips - 1) / strips) * ((a.blocks + blocks - 1) / blocks);
+                return (double)((n + 255) / 256);
+            };
+            const double one = rounds(8, 4), t0 = one == 1.0 ? 0.86 : 0.67 * one, t1 = 1.07 * rounds(16, 4), t2 = 1.6 * rounds(16, 8);
+            // (groups of 32 have too many scales for the widest one's registers)
+            if constexpr (GROUP > 32)
+                if (t2 <= t0 && t2 <= t1) return gemm_launch<PARTS, GROUP, 4, 4, 3>(c, a);
+            return t1 < t0 ? gemm_launch<PARTS, GROUP, 2, 4, 3>(c, a) : gemm_launch<PARTS, GROUP, 2, 2, 3>(c, a);
         }
     }
-    if (a.blocks == 1) return batch_launch<PARTS, GROUP, 2, 1>(c, a);
-    if (a.blocks == 2 || PARTS == 2) return batch_launch<PARTS, GROUP, 1, 2>(c, a);
-    return batch_launch<PARTS, GROUP, 2, PARTS == 2 ? 2 : 4>(c, a);
+    // A strip a workgroup fills the card where there are few and the row is
+    // short (32 bf16 rows, 1024 x 4096: 5.4 us against 6.5 of two; 4096 x 4096:
+    // 6.3 and 6.8).  Two of them read x's parts half as often and cut long rows
+    // instead (4096 x 14336: 13.9 and 12.5; 64 rows of 2048 x 8192: 14.0 and 11.4); four
+    // where there are still enough (14336 x 4096: 11.3 of two, 10.7 of four;
+    // 64 rows 19.2 and 15.0; 8192 x 8192: 11.3 and 12.5).
+    const int strips = q4_strips(a.u.m.out);
+    if (strips <= 256 && a.u.m.tiles < 64) return batch_blocks<PARTS, GROUP, 1, 16>(c, a);
+    return strips < 800 ? batch_blocks<PARTS, GROUP, 2, 8>(c, a) : batch_blocks<PARTS, GROUP, 4, 8>(c, a);
 }
 
 template <int PARTS>

@@ -165,6 +165,12 @@ int ensure_q4_scratch(Ctx* c, size_t bytes)
     return grow_zeroed(c, (void**)&c->q4_part, &c->q4_part_cap, bytes, 1, "q4 operands");
 }
 
+int ensure_q4_sums(Ctx* c, size_t floats, size_t counters)
+{
+    IAM_TRY(grow_zeroed(c, (void**)&c->q4_sums, &c->q4_sums_cap, floats, sizeof(float), "q4 partial sums"));
+    return grow_zeroed(c, (void**)&c->q4_ctr, &c->q4_ctr_cap, counters, sizeof(uint32_t), "q4 counter");
+}
+
 int ensure_verify_scratch(Ctx* c, size_t doubles, size_t counters)
 {
     IAM_TRY(grow_zeroed(c, (void**)&c->ver_part, &c->ver_part_cap, doubles, sizeof(double), "verification partials"));
