@@ -6,7 +6,8 @@
 // a power of two where its largest value lies outside [2^-2, 2^15)), two, high
 // and low, of fp32 (22 bits).  4-bit weights become fp16 under the exponents of
 // 1024 and 64, n - zero exactly.  Products are then exact; a group's are added
-// in fp32 by the instructions and go to the row's sum with the group's scale.
+// in fp32 by the instructions and go to the row's sum with the group's scale
+// times that power (together first: a sum of large x alone may pass fp32).
 #include "accum.h"
 #include "q4_mul.h"
 
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(64 * MOST) void k_q4_batch(RowsArgs a)
 #pragma unroll
                         for (int p = 0; p < PARTS; p++) d = mfma_f16(wide[j], o.x[p][n][j], d);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[s][n][e] = __builtin_fmaf(d[e] * o.f[n], (float)o.sc[s][i][e], acc[s][n][e]);
+                    for (int e = 0; e < 4; e++) acc[s][n][e] = __builtin_fmaf(d[e], o.f[n] * (float)o.sc[s][i][e], acc[s][n][e]);
                 }
             }
         }
@@ -508,8 +509,9 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
                         const half8 scale = __builtin_bit_cast(half8, sc[i][s * 2 + e / 8]);
                         float v = d[0][n][e];
                         if constexpr (PARTS == 2) v += d[1][n][e];
-                        if constexpr (FACTORS) v *= fn[n];
-                        acc[s][n][e] = __builtin_fmaf(v, (float)scale[e % 8], acc[s][n][e]);
+                        float by = (float)scale[e % 8];
+                        if constexpr (FACTORS) by *= fn[n];
+                        acc[s][n][e] = __builtin_fmaf(v, by, acc[s][n][e]);
                     }
             }
             if constexpr (GT > 1) __builtin_amdgcn_sched_barrier(0);
@@ -623,8 +625,8 @@ static int batch_blocks(Ctx* c, const RowsArgs& a)
 {
     // (two parts of four blocks would not fit the registers)
     if (a.blocks == 1) return batch_launch<PARTS, GROUP, S, 1, MOST>(c, a);
-    if (a.blocks == 2 || PARTS == 2) return batch_launch<PARTS, GROUP, S, 2, MOST>(c, a);
-    return batch_launch<PARTS, GROUP, S, PARTS == 2 ? 2 : 4, MOST>(c, a);
+    if (a.blocks == 2) return batch_launch<PARTS, GROUP, S, 2, MOST>(c, a);
+    return batch_launch<PARTS, GROUP, S, PARTS == 2 || S == 1 ? 2 : 4, MOST>(c, a);
 }
 
 template <int PARTS, int GROUP, int NB, int WO, int STAGES>
@@ -657,14 +659,14 @@ static int batch_sized(Ctx* c, const RowsArgs& a)
             return t1 < t0 ? gemm_launch<PARTS, GROUP, 2, 4, 3>(c, a) : gemm_launch<PARTS, GROUP, 2, 2, 3>(c, a);
         }
     }
-    // A strip a workgroup fills the card where there are few and the row is
-    // short (32 bf16 rows, 1024 x 4096: 5.4 us against 6.5 of two; 4096 x 4096:
-    // 6.3 and 6.8).  Two of them read x's parts half as often and cut long rows
-    // instead (4096 x 14336: 13.9 and 12.5; 64 rows of 2048 x 8192: 14.0 and 11.4); four
-    // where there are still enough (14336 x 4096: 11.3 of two, 10.7 of four;
-    // 64 rows 19.2 and 15.0; 8192 x 8192: 11.3 and 12.5).
+    // Up to 32 rows a strip a workgroup fills the card where there are few and the
+    // matrix's rows are short (32 bf16 rows, 1024 x 4096: 5.4 us against 6.5 of two;
+    // 4096 x 4096: 6.3 and 6.8).  Two of them read x's parts half as often and cut
+    // long rows instead (4096 x 14336: 13.9 and 12.5; 64 rows of 2048 x 8192: 14.0 and
+    // 10.2); four where there are still enough (14336 x 4096: 11.3 of two, 10.7 of
+    // four; 64 rows 19.2 and 15.0; 8192 x 8192: 11.3 and 12.5).
     const int strips = q4_strips(a.u.m.out);
-    if (strips <= 256 && a.u.m.tiles < 64) return batch_blocks<PARTS, GROUP, 1, 16>(c, a);
+    if (a.blocks <= 2 && strips <= 256 && a.u.m.tiles < 64) return batch_blocks<PARTS, GROUP, 1, 16>(c, a);
     return strips < 800 ? batch_blocks<PARTS, GROUP, 2, 8>(c, a) : batch_blocks<PARTS, GROUP, 4, 8>(c, a);
 }
 
@@ -676,13 +678,14 @@ static int batch_grouped(Ctx* c, const RowsArgs& a)
     return batch_sized<PARTS, 128>(c, a);
 }
 
-// rows of a pass: what x takes as parts stays small beside the card's memory
+// rows of a pass: what x takes as parts stays small beside the card's memory,
+// and a launch has at most 2^30 threads (one for 32 products)
 constexpr int kRowsSlice = 1 << 14;
 
 int q4_mul_rows(Ctx* c, const MulArgs& all)
 {
     const int parts = all.x_type == IAM_F32 ? 2 : 1;
-    const int slice = std::min(all.rows, kRowsSlice);
+    const int slice = (int)std::min<int64_t>(std::min(all.rows, kRowsSlice), ((int64_t)1 << 35) / (q4_strips(all.m.out) * kStrip));
     const size_t blocks = (size_t)(slice + 15) / 16, values = blocks * all.m.tiles * 2048;
     IAM_TRY(ensure_q4_scratch(c, values * 2 * parts + blocks * all.m.tiles * 64));
     for (int r0 = 0; r0 < all.rows; r0 += slice) {

@@ -123,6 +123,32 @@ def test_values_far_apart(iam, ctx, rows, type):
     P.close(got, v @ w.values().T, R.product_bound(v, w.values()), "f32")
 
 
+@pytest.mark.parametrize("rows", [1, 20, 140])
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_values_near_the_largest(iam, ctx, rows, type):
+    """Sums that only the scales bring back into fp32's range: of 640 weights up
+    to 15 * 2^-10 and x up to 2^126 they stay below 2^126 * 640 * 15 / 1024, and
+    random signs keep them below 2^127."""
+    rng = np.random.default_rng(8)
+    w = R.random_weights(rng, 40, 640, 128, False)
+    w.scale[:] = 2.0 ** -10
+    x = rng.uniform(-1, 1, (rows, 640)) * 2.0 ** 126
+    words, v = P.to_type(x, type)
+    want = v @ w.values().T
+    assert np.abs(want).max() < 2.0 ** 127
+    m = packed(iam, ctx, w)
+    got = product(ctx, m, words, None, type, "f32")
+    m.free()
+    P.close(got, want, R.product_bound(v, w.values()), "f32")
+
+
+def test_many_rows_and_outputs(iam, ctx):
+    """More rows than a pass takes, more strips than a launch packs."""
+    rng = np.random.default_rng(9)
+    check(iam, ctx, rng, (1 << 14) + 37, 40, 20, 32, True, "bf16", "f32")
+    check(iam, ctx, rng, 1, 1, (1 << 19) + 17, 32, False, "f32", "f32")
+
+
 @pytest.mark.parametrize("rows", [1, 9, 130])
 @pytest.mark.parametrize("type", P.TYPES)
 def test_not_finite_rows(iam, ctx, rows, type):
