@@ -419,10 +419,22 @@ int iam_rmsnorm_rows(iam_ctx* c, const void* x, int type, size_t x_stride, const
         }
     }
     DeviceGuard on(c);
-    const NormArgs a{x, r, sum, gain, out, scale, x_stride, r_stride, out_stride, dim, group, groups, out_type, eps};
-    if (type == IAM_F32) return norm_typed<float>(c, a, r_type, rows);
-    if (type == IAM_F16) return norm_typed<_Float16>(c, a, r_type, rows);
-    return norm_typed<__bf16>(c, a, r_type, rows);
+    NormArgs a{x, r, sum, gain, out, scale, x_stride, r_stride, out_stride, dim, group, groups, out_type, eps};
+    auto move = [](auto* p, size_t bytes) { return p ? decltype(p)(const_cast<uint8_t*>(reinterpret_cast<const uint8_t*>(p)) + bytes) : p; };
+    // at most 2^20 rows (2^30 threads) a launch
+    constexpr int kSlice = 1 << 20;
+    for (int r0 = 0; r0 < rows; r0 += kSlice) {
+        const int some = std::min(kSlice, rows - r0);
+        if (type == IAM_F32) IAM_TRY(norm_typed<float>(c, a, r_type, some));
+        else if (type == IAM_F16) IAM_TRY(norm_typed<_Float16>(c, a, r_type, some));
+        else IAM_TRY(norm_typed<__bf16>(c, a, r_type, some));
+        a.x = move(a.x, kSlice * x_stride * xb);
+        a.r = move(a.r, kSlice * r_stride * rb);
+        a.sum = move(a.sum, kSlice * r_stride * rb);
+        a.out = move(a.out, kSlice * out_stride * ob);
+        a.scale = move(a.scale, (size_t)kSlice * groups * 4);
+    }
+    return IAM_OK;
 }
 
 int iam_rows8_read(iam_ctx* c, const void* x, int type, size_t stride, const float* scale, int group, int rows, int dim, float* out)
@@ -444,8 +456,8 @@ int iam_rows8_read(iam_ctx* c, const void* x, int type, size_t stride, const flo
     IAM_REQUIRE(!overlaps(out, yb, x, xb) && !overlaps(out, yb, scale, sb), "rows8_read: out overlaps an input");
     DeviceGuard on(c);
     const int parts = (dim + kReadThreads * 8 - 1) / (kReadThreads * 8);
-    // at most 2^24 workgroups a launch
-    const int most = (1 << 24) / parts;
+    // at most 2^22 workgroups (2^30 threads) a launch
+    const int most = (1 << 22) / parts;
     for (int r0 = 0; r0 < rows; r0 += most) {
         const Read8Args a{reinterpret_cast<const uint8_t*>(x) + (size_t)r0 * stride, scale + (size_t)r0 * groups, out + (size_t)r0 * d, stride, dim, group,
                           groups, type, parts};

@@ -186,10 +186,9 @@ int iam_q4_pack(iam_ctx* c, const iam_q4_matrix* m, const uint8_t* n, const uint
     }
     DeviceGuard on(c);
     PackArgs a{q4_of(m), reinterpret_cast<uint32_t*>(m->numbers), m->scales, m->zeros, n, scale, zero};
-    // at most 2^15 strips (of a grid's second dimension) a launch
-    constexpr int kSlice = 1 << 15;
-    const int strips = q4_strips(m->out_dim);
-    for (int s0 = 0; s0 < strips; s0 += kSlice) {
+    // at most 2^22 workgroups (2^30 threads) a launch, 2^15 strips (of a grid's second dimension)
+    const int strips = q4_strips(m->out_dim), most = std::min(1 << 15, (1 << 22) / a.m.chunks);
+    for (int s0 = 0; s0 < strips; s0 += most) {
         PackArgs b = a;
         const size_t row0 = (size_t)s0 * kStrip;
         b.m.out -= (int)row0;
@@ -199,7 +198,7 @@ int iam_q4_pack(iam_ctx* c, const iam_q4_matrix* m, const uint8_t* n, const uint
         b.n += row0 * (((size_t)m->in_dim + 1) / 2);
         b.scale += row0 * groups;
         if (b.zero) b.zero += row0 * groups;
-        IAM_TRY(launch(c, "q4_pack", k_q4_pack, dim3(a.m.chunks, std::min(kSlice, strips - s0)), dim3(kQ4Threads), 0, b));
+        IAM_TRY(launch(c, "q4_pack", k_q4_pack, dim3(a.m.chunks, std::min(most, strips - s0)), dim3(kQ4Threads), 0, b));
     }
     return IAM_OK;
 }

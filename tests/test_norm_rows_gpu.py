@@ -110,6 +110,13 @@ def test_rows(ctx, rows, dim, type, out_type):
     check(ctx, rows_of(rng, rows, dim), type, r, r_type, gain, out_type, 128 * (k // 2 % 2) if out_type in R.LARGEST else 0, keep=k % 5 != 0)
 
 
+@pytest.mark.parametrize("out_type,group", [("f32", 0), ("int8", 0)])
+def test_more_rows_than_a_launch(ctx, out_type, group):
+    rng = np.random.default_rng(8)
+    rows, dim = (1 << 20) + 5, 2
+    check(ctx, rows_of(rng, rows, dim), "f32", rows_of(rng, rows, dim), "f32", np.array([0.5, 2.0]), out_type, group, strides=(3, 2, 4))
+
+
 @pytest.mark.parametrize("type,r_type,out_type,strides", [("f32", "f32", "int8", (5001, 4999, 5003)), ("f16", "f16", "f16", (4998, 4997, 5005)), ("bf16", "f32", "e4m3", (5008, 5008, 5008)),
                                                           ("bf16", "bf16", "bf16", (4996, 5000, 5001)), ("f16", "f32", "int8", (5000, 5000, 5000))])
 def test_strides(ctx, type, r_type, out_type, strides):
