@@ -71,13 +71,6 @@ __device__ __forceinline__ uint32_t max16(uint32_t v)
     return max(v, dpp_t<0x121>(v, v));
 }
 
-// A wave's LDS operations take place in order: this keeps them in the order they are written in.
-__device__ __forceinline__ void wave_sync()
-{
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // A workgroup takes S strips of 16 rows of the matrix; its waves deal the chunks
 // of 512 inputs among themselves.  A wave brings the rows' 512 values into its
 // own part of LDS as digits in the operands' order (16 lanes a tile, 8 values

@@ -106,4 +106,11 @@ int q4_mul_few(Ctx* c, const MulArgs& a);
 // any number of them
 int q4_mul_rows(Ctx* c, const MulArgs& a);
 
+// A wave's LDS operations take place in order: this keeps them in the order they are written in.
+__device__ __forceinline__ void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 }  // namespace iam

@@ -21,6 +21,7 @@ typedef unsigned long long ull2 __attribute__((ext_vector_type(2)));
 // parts  fp16 [part][block of 16 rows][tile][j][lane 16 g + row][8]: inputs
 //        32 j + 8 g and on of the tile
 // factor fp32 [block][tile][16]: what the tile's values were divided by
+// scaled [block][tile]: whether any of these is not 1
 struct PrepArgs {
     const void* x;
     int type;
@@ -30,6 +31,7 @@ struct PrepArgs {
     _Float16* parts;
     size_t part_stride;      // values of a part
     float* factor;
+    uint8_t* scaled;
     int parts_n;
 };
 
@@ -78,7 +80,10 @@ __global__ __launch_bounds__(kPrepThreads) void k_q4_prep(PrepArgs a)
         *reinterpret_cast<half8*>(a.parts + at + (j * 64 + lane) * 8) = h;
         if (a.parts_n == 2) *reinterpret_cast<half8*>(a.parts + a.part_stride + at + (j * 64 + lane) * 8) = l;
     }
-    if (g == 0) a.factor[((size_t)block * a.tiles + tile) * 16 + c] = f;
+    const size_t cell = (size_t)block * a.tiles + tile;
+    if (g == 0) a.factor[cell * 16 + c] = f;
+    const bool scaled = __any(f != 1.0f);
+    if (lane == 0) a.scaled[cell] = scaled;
 }
 
 // ---- the products
@@ -87,8 +92,8 @@ struct RowsArgs {
     const _Float16* parts;
     size_t part_stride;
     const float* factor;
+    const uint8_t* scaled;    // null: no factor can be anything but 1
     const float* row_scale;   // of a whole row, or null
-    bool factors;             // whether factor may hold anything but 1
     int blocks;               // of 16 rows
     int waves;
     // the inputs cut into parts for more workgroups, whose sums the last one to arrive joins
@@ -138,6 +143,23 @@ __device__ __forceinline__ void put_four(const MulArgs& u, int r, int o, floatx4
 #pragma unroll
     for (int i = 0; i < 4; i++)
         if (o + i < u.m.out) put_value(u.y, u.y_type, at + i, v[i]);
+}
+
+// eight of them in 16 bits, from o on
+__device__ __forceinline__ void put_eight(const MulArgs& u, int r, int o, floatx4 v, floatx4 w)
+{
+    const size_t at = (size_t)r * u.y_stride + o;
+    if (o + 8 <= u.m.out) {
+        if (u.y_type == IAM_F16)
+            *reinterpret_cast<Pack<_Float16, 8, 2>*>(reinterpret_cast<_Float16*>(u.y) + at) = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3],
+                                                                                              (_Float16)w[0], (_Float16)w[1], (_Float16)w[2], (_Float16)w[3]};
+        else
+            *reinterpret_cast<Pack<__bf16, 8, 2>*>(reinterpret_cast<__bf16*>(u.y) + at) = {(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3],
+                                                                                          (__bf16)w[0], (__bf16)w[1], (__bf16)w[2], (__bf16)w[3]};
+        return;
+    }
+    put_four(u, r, o, v);
+    if (o + 4 < u.m.out) put_four(u, r, o + 4, w);
 }
 
 // A workgroup takes S strips of the matrix and NB blocks of 16 rows; its waves
@@ -363,7 +385,7 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_
 // instruction and its results' first use, where the compiler leaves out the
 // wait states of the edge that jumps.
 template <int PARTS, int GROUP, int NB, int WO, int STAGES, bool FACTORS, bool SECOND>
-__device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP, NB, WO, STAGES>& stage, int s0, int b0, floatx16 (&acc)[2][NB / 2])
+__device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP, NB, WO, STAGES>& stage, int s0, int b0, int t0, int t1, floatx16 (&acc)[2][NB / 2])
 {
     typedef Gemm<PARTS, GROUP, NB, WO, STAGES> G;
     constexpr int GT = G::GT, S = G::S, N = NB / 2;
@@ -426,9 +448,9 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
 #pragma unroll
         for (int n = 0; n < N; n++) f[n] = a.factor[((size_t)min(b0 + wx * NB + 2 * n + side, a.blocks - 1) * u.m.tiles + t) * 16 + c];
     };
-    if constexpr (FACTORS) load_factors(0);
+    if constexpr (FACTORS) load_factors(t0);
 #pragma unroll
-    for (int t = 0; t < STAGES - 1; t++) fetch(min(t, u.m.tiles - 1), t);
+    for (int t = 0; t < STAGES - 1; t++) fetch(min(t0 + t, t1 - 1), t);
     int buf = 0, free_buf = STAGES - 1;
     const uint32_t base = lds_address(stage.at);
     // A wave's loads of a tile are done when no more are in flight than the
@@ -449,16 +471,16 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
     meet();
     if constexpr (SECOND) meet();
 #pragma unroll 1
-    for (int t = 0; t < u.m.tiles; t++) {
+    for (int t = t0; t < t1; t++) {
         // Every wave's loads of this tile have arrived, and every wave has read
         // the tile before, whose place the newest tile takes.
         float fn[N];
         if constexpr (FACTORS) {
 #pragma unroll
             for (int n = 0; n < N; n++) fn[n] = f[n];
-            load_factors(min(t + 1, u.m.tiles - 1));
+            load_factors(min(t + 1, t1 - 1));
         }
-        fetch(min(t + STAGES - 1, u.m.tiles - 1), free_buf);   // behind the last tile, the last one again
+        fetch(min(t + STAGES - 1, t1 - 1), free_buf);   // behind the last tile, the last one again
         const uint32_t at = base + buf * G::BYTES;
         free_buf = buf;
         buf = buf + 1 == STAGES ? 0 : buf + 1;
@@ -545,25 +567,23 @@ __global__ __launch_bounds__(128 * WO, 2) void k_q4_gemm(RowsArgs a)
     const int strips = q4_strips(u.m.out);
     // panels of kGemmPanel along x's rows, the matrix's rows outermost in a panel
     const int along = (a.blocks + 2 * NB - 1) / (2 * NB), across = (strips + STRIPS - 1) / STRIPS;
-    const int id = xcd_remap(blockIdx.x, gridDim.x), panel = id / (kGemmPanel * across), p0 = panel * kGemmPanel;
+    const int all = xcd_remap(blockIdx.x, gridDim.x), split = all / (along * across), id = all - split * along * across;
+    const int panel = id / (kGemmPanel * across), p0 = panel * kGemmPanel;
     const int width = min(kGemmPanel, along - p0), in_panel = id - panel * kGemmPanel * across;
     const int xt = p0 + in_panel % width, ot = in_panel / width;
     const int s0 = ot * STRIPS, b0 = xt * 2 * NB;
+    const int each = (u.m.tiles + a.splits - 1) / a.splits, t0 = split * each, t1 = min(t0 + each, u.m.tiles);
     bool factors = false;
-    if (a.factors) {
-        // whether any is not 1
-        const int blocks = min(2 * NB, a.blocks - b0);
-        const float4* q = reinterpret_cast<const float4*>(a.factor + (size_t)b0 * u.m.tiles * 16);
+    if (a.scaled) {
         bool mine = false;
-        for (int i = threadIdx.x; i < blocks * u.m.tiles * 4; i += 128 * WO) {
-            const float4 v = q[i];
-            mine |= v.x != 1.0f || v.y != 1.0f || v.z != 1.0f || v.w != 1.0f;
-        }
+        for (int i = threadIdx.x; i < min(2 * NB, a.blocks - b0) * u.m.tiles; i += 128 * WO) mine |= a.scaled[(size_t)b0 * u.m.tiles + i] != 0;
         uint32_t* any = reinterpret_cast<uint32_t*>(&stage);   // nothing else is there yet
-        if (lane == 0) any[wave] = 0;
-        if (mine) any[wave] = 1;
+        if (threadIdx.x < 2 * WO) any[threadIdx.x] = 0u;
+        __syncthreads();
+        if (__any(mine) && lane == 0) any[wave] = 1u;
         __syncthreads();
         uint32_t all = 0;
+#pragma unroll
         for (int i = 0; i < 2 * WO; i++) all |= any[i];
         factors = __builtin_amdgcn_readfirstlane(all) != 0;
         __syncthreads();
@@ -577,24 +597,84 @@ __global__ __launch_bounds__(128 * WO, 2) void k_q4_gemm(RowsArgs a)
             for (int e = 0; e < 16; e++) acc[s][n][e] = 0.0f;
     auto tiles = [&](auto with_factors) __attribute__((always_inline)) {
         constexpr bool F = decltype(with_factors)::value;
-        if (WO == 4 && wave >= 4) gemm_tiles<PARTS, GROUP, NB, WO, STAGES, F, WO == 4>(a, stage, s0, b0, acc);
-        else gemm_tiles<PARTS, GROUP, NB, WO, STAGES, F, false>(a, stage, s0, b0, acc);
+        if (WO == 4 && wave >= 4) gemm_tiles<PARTS, GROUP, NB, WO, STAGES, F, WO == 4>(a, stage, s0, b0, t0, t1, acc);
+        else gemm_tiles<PARTS, GROUP, NB, WO, STAGES, F, false>(a, stage, s0, b0, t0, t1, acc);
     };
     if (factors) tiles(std::true_type{});
     else tiles(std::false_type{});
-    // value 4 i + e of a lane is row 8 i + 4 (lane / 32) + e of the pair of strips
+    if (a.splits > 1) {
+        // the splits' sums: [workgroup's place][split][four values][thread], past the
+        // XCD's L2, joined in the splits' order by the last one to arrive
+        constexpr int FOURS = 2 * (NB / 2) * 4, THREADS = 128 * WO, SOME = 8, ROUND = 4;
+        constexpr int SC1 = 16;   // cache policy: at the point of coherence of the card
+        const auto place = __builtin_amdgcn_make_buffer_rsrc(a.sums + (size_t)id * a.splits * (FOURS * THREADS * 4), 0, a.splits * (FOURS * THREADS * 16), 0x00020000);
+        const int mine = (int)threadIdx.x * 16;
+#pragma unroll
+        for (int i = 0; i < FOURS; i++) {
+            floatx16& v = acc[i / (NB * 2)][i / 4 % (NB / 2)];
+            const floatx4 four = {v[i % 4 * 4], v[i % 4 * 4 + 1], v[i % 4 * 4 + 2], v[i % 4 * 4 + 3]};
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, four), place, mine, (split * FOURS + i) * (THREADS * 16), SC1);
+            v[i % 4 * 4] = v[i % 4 * 4 + 1] = v[i % 4 * 4 + 2] = v[i % 4 * 4 + 3] = 0.0f;
+        }
+        if (!acc_arrive(a.ctr + id, (uint32_t)a.splits, reinterpret_cast<int*>(&stage))) return;
+        __syncthreads();   // every wave has read the answer, whose place is another's
+        if (threadIdx.x == 0) a.ctr[id] = 0u;
+#pragma unroll
+        for (int i0 = 0; i0 < FOURS; i0 += SOME)
+            for (int q = 0; q < a.splits; q += ROUND) {
+                u32x4 v[ROUND][SOME];
+#pragma unroll
+                for (int j = 0; j < ROUND; j++)
+#pragma unroll
+                    for (int i = 0; i < SOME; i++)
+                        v[j][i] = __builtin_amdgcn_raw_buffer_load_b128(place, mine, (min(q + j, a.splits - 1) * FOURS + i0 + i) * (THREADS * 16), SC1);
+#pragma unroll
+                for (int j = 0; j < ROUND; j++)
+#pragma unroll
+                    for (int i = 0; i < SOME; i++) {
+                        const floatx4 four = __builtin_bit_cast(floatx4, v[j][i]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[(i0 + i) / (NB * 2)][(i0 + i) / 4 % (NB / 2)][(i0 + i) % 4 * 4 + e] += q + j < a.splits ? four[e] : 0.0f;
+                    }
+            }
+    }
+    // Value 4 i + e of a lane is row 8 i + 4 (lane / 32) + e of the pair of strips.
+    // 32 rows of x at a time turn in the wave's own part of LDS, for whole lines of
+    // y (64 results of a row): pieces of 16 bytes, as the registers hold them, took 2
+    // us more (389 rows, 6144 x 4096).
+    constexpr int ROW = S * kStrip + 4;    // floats of a row in LDS
+    float* turn = reinterpret_cast<float*>(&stage) + wave * (32 * ROW);
+    static_assert(sizeof(stage) >= 2 * WO * 32 * ROW * 4, "32 rows of every wave");
+    const int o0 = (s0 + (wave >> 1) * S) * kStrip, there = min(u.m.out - o0, S * kStrip);
 #pragma unroll
     for (int n = 0; n < NB / 2; n++) {
-        const int r = (b0 + (wave & 1) * NB + 2 * n) * 16 + (lane & 31);
-        if (r >= u.rows) continue;
-        const float rs = a.row_scale ? a.row_scale[r] : 1.0f;
+        const int r0 = (b0 + (wave & 1) * NB + 2 * n) * 16;
+        const float rs = a.row_scale ? a.row_scale[min(r0 + (lane & 31), u.rows - 1)] : 1.0f;
 #pragma unroll
         for (int s = 0; s < 2; s++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int o = (s0 + (wave >> 1) * S) * kStrip + 32 * s + 8 * i + 4 * (lane >> 5);
-                if (o < u.m.out) put_four(u, r, o, floatx4{acc[s][n][4 * i], acc[s][n][4 * i + 1], acc[s][n][4 * i + 2], acc[s][n][4 * i + 3]} * rs);
+            for (int i = 0; i < 4; i++)
+                *reinterpret_cast<floatx4*>(turn + (lane & 31) * ROW + 32 * s + 8 * i + 4 * (lane >> 5)) =
+                    floatx4{acc[s][n][4 * i], acc[s][n][4 * i + 1], acc[s][n][4 * i + 2], acc[s][n][4 * i + 3]} * rs;
+        wave_sync();
+        // four or eight results a lane
+        auto at = [&](int r, int o) { return *reinterpret_cast<const floatx4*>(turn + r * ROW + o); };
+        if (u.y_type == IAM_F32) {
+            const int o = (lane & 15) * 4;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int r = i * 4 + (lane >> 4);
+                if (r0 + r < u.rows && o < there) put_four(u, r0 + r, o0 + o, at(r, o));
             }
+        } else {
+            const int o = (lane & 7) * 8;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int r = i * 8 + (lane >> 3);
+                if (r0 + r < u.rows && o < there) put_eight(u, r0 + r, o0 + o, at(r, o), at(r, o + 4));
+            }
+        }
+        wave_sync();
     }
 }
 
@@ -630,10 +710,42 @@ static int batch_blocks(Ctx* c, const RowsArgs& a)
 }
 
 template <int PARTS, int GROUP, int NB, int WO, int STAGES>
-static int gemm_launch(Ctx* c, const RowsArgs& a)
+static int gemm_launch(Ctx* c, RowsArgs a, int splits)
 {
     const size_t along = (size_t)(a.blocks + 2 * NB - 1) / (2 * NB), across = (size_t)(q4_strips(a.u.m.out) + kGemmStrips * WO - 1) / (kGemmStrips * WO);
-    return launch(c, "q4_mul.gemm", k_q4_gemm<PARTS, GROUP, NB, WO, STAGES>, dim3((unsigned)(along * across)), dim3(128 * WO), 0, a);
+    a.splits = splits;
+    if (splits > 1) {
+        IAM_TRY(ensure_q4_sums(c, along * across * splits * (NB * WO * 2048), along * across));
+        a.sums = c->q4_sums;
+        a.ctr = c->q4_ctr;
+    }
+    return launch(c, "q4_mul.gemm", k_q4_gemm<PARTS, GROUP, NB, WO, STAGES>, dim3((unsigned)(along * across * splits)), dim3(128 * WO), 0, a);
+}
+
+// How long workgroups of 64 wo x 32 nb products take for all of them, with the
+// inputs cut into the number of parts that is best: 5 us, what `round` says n
+// workgroups' tiles of 128 inputs take on 256 CUs, and for several parts the
+// join.  Fitted to measured times: of 64 x 128 (128 rows, 6144 x 4096) 29.3 us in one
+// part and 21.9 in two, 256 x 64 35.2 and 26.1, 256 x 128 51.7 and 37.5; 389 rows 44.5 and
+// 45.9, 39.7 and 53.5, 54.6 and 42.8; 4096 rows, 14336 x 4096 650, 608 and 494 in one;
+// 128 rows, 1024 x 14336 90.7 in one, 22.1 in eight.
+struct GemmCost {
+    double us;
+    int splits;
+};
+template <typename F>
+static GemmCost gemm_cost(const RowsArgs& a, int nb, int wo, F round)
+{
+    const int64_t cells = (int64_t)((a.blocks + 2 * nb - 1) / (2 * nb)) * ((q4_strips(a.u.m.out) + kGemmStrips * wo - 1) / (kGemmStrips * wo));
+    GemmCost best{INFINITY, 1};
+    // (more parts than give every CU four workgroups are not looked at)
+    for (int s = 1; s <= kMaxSplits && (s == 1 || (s * cells <= 1024 && a.u.m.tiles >= 4 * s)); s++) {
+        const int each = (a.u.m.tiles + s - 1) / s, splits = (a.u.m.tiles + each - 1) / each;
+        const double mb = wo * nb * 8192e-6 * splits;   // of a place's sums
+        const double us = 5.0 + each * round((int)(cells * splits)) + (s > 1 ? 2.0 + 10.0 * mb + 0.25 * mb * (double)cells : 0.0);
+        if (us < best.us) best = {us, splits};
+    }
+    return best;
 }
 
 template <int PARTS, int GROUP>
@@ -641,22 +753,15 @@ static int batch_sized(Ctx* c, const RowsArgs& a)
 {
     if (a.blocks > 4) {
         if constexpr (PARTS == 2) {
-            return gemm_launch<PARTS, GROUP, 2, 4, 3>(c, a);
+            return gemm_launch<PARTS, GROUP, 2, 4, 3>(c, a, gemm_cost(a, 2, 4, [](int n) { return 1.5 * ((n + 255) / 256); }).splits);
         } else {
-            // The shape whose workgroups, dealt to 256 CUs, take the least: a
-            // tile of 128 inputs takes 0.86 us in one of 128 x 64 products alone
-            // on a CU and 0.67 each of several, 1.07 in one of 256 x 64, 1.6 in one of
-            // 256 x 128 (389 rows, 6144 x 4096: 46, 42 and 57 us; 4096 rows, 14336 x
-            // 4096: 645, 614 and 497; 256 rows, 6144 x 4096: 32, 38 and 55).
-            auto rounds = [&](int strips, int blocks) {
-                const size_t n = (size_t)((q4_strips(a.u.m.out) + strips - 1) / strips) * ((a.blocks + blocks - 1) / blocks);
-                return (double)((n + 255) / 256);
-            };
-            const double one = rounds(8, 4), t0 = one == 1.0 ? 0.86 : 0.67 * one, t1 = 1.07 * rounds(16, 4), t2 = 1.6 * rounds(16, 8);
+            const GemmCost small = gemm_cost(a, 2, 2, [](int n) { return n <= 256 ? 0.76 : n <= 512 ? 1.24 : 0.72 * ((n + 255) / 256); });
+            const GemmCost tall = gemm_cost(a, 2, 4, [](int n) { return 1.05 * ((n + 255) / 256); });
+            const GemmCost wide = gemm_cost(a, 4, 4, [](int n) { return 2.0 * ((n - 1) / 256) + 1.45 + 0.55 * ((n - 1) % 256 + 1) / 256; });
             // (groups of 32 have too many scales for the widest one's registers)
             if constexpr (GROUP > 32)
-                if (t2 <= t0 && t2 <= t1) return gemm_launch<PARTS, GROUP, 4, 4, 3>(c, a);
-            return t1 < t0 ? gemm_launch<PARTS, GROUP, 2, 4, 3>(c, a) : gemm_launch<PARTS, GROUP, 2, 2, 3>(c, a);
+                if (wide.us <= small.us && wide.us <= tall.us) return gemm_launch<PARTS, GROUP, 4, 4, 3>(c, a, wide.splits);
+            return tall.us < small.us ? gemm_launch<PARTS, GROUP, 2, 4, 3>(c, a, tall.splits) : gemm_launch<PARTS, GROUP, 2, 2, 3>(c, a, small.splits);
         }
     }
     // Up to 32 rows a strip a workgroup fills the card where there are few and the
@@ -687,7 +792,7 @@ int q4_mul_rows(Ctx* c, const MulArgs& all)
     const int parts = all.x_type == IAM_F32 ? 2 : 1;
     const int slice = (int)std::min<int64_t>(std::min(all.rows, kRowsSlice), ((int64_t)1 << 35) / (q4_strips(all.m.out) * kStrip));
     const size_t blocks = (size_t)(slice + 15) / 16, values = blocks * all.m.tiles * 2048;
-    IAM_TRY(ensure_q4_scratch(c, values * 2 * parts + blocks * all.m.tiles * 64));
+    IAM_TRY(ensure_q4_scratch(c, values * 2 * parts + blocks * all.m.tiles * (64 + 1)));
     for (int r0 = 0; r0 < all.rows; r0 += slice) {
         MulArgs u = all;
         u.rows = std::min(slice, all.rows - r0);
@@ -699,14 +804,15 @@ int q4_mul_rows(Ctx* c, const MulArgs& all)
         a.parts = reinterpret_cast<_Float16*>(c->q4_part);
         a.part_stride = values;
         a.blocks = (u.rows + 15) / 16;
-        a.factors = u.x_type == IAM_F32 || u.x_type == IAM_BF16 || u.x_groups > 1;
         float* factor = reinterpret_cast<float*>(c->q4_part + values * 2 * parts);
+        uint8_t* scaled = reinterpret_cast<uint8_t*>(factor + blocks * all.m.tiles * 16);
         a.factor = factor;
+        a.scaled = u.x_type == IAM_F32 || u.x_type == IAM_BF16 || u.x_groups > 1 ? scaled : nullptr;
         // a scale for each tile goes with the tiles; one of the whole row at the end
         const bool by_tile = u.x_groups > 1;
         a.row_scale = by_tile ? nullptr : u.x_scale;
         const PrepArgs p{u.x, u.x_type, u.x_stride, by_tile ? u.x_scale : nullptr, u.rows, u.m.in, u.m.tiles,
-                         reinterpret_cast<_Float16*>(c->q4_part), values, factor, parts};
+                         reinterpret_cast<_Float16*>(c->q4_part), values, factor, scaled, parts};
         const dim3 grid((unsigned)((u.m.tiles + 3) / 4), (unsigned)a.blocks);
         IAM_TRY(launch(c, "q4_mul.prepare", k_q4_prep, grid, dim3(kPrepThreads), 0, p));
         IAM_TRY(parts == 2 ? batch_grouped<2>(c, a) : batch_grouped<1>(c, a));
