@@ -26,36 +26,39 @@ struct FewWeights {
     static constexpr int PER = kChunk / GROUP;
     uint4 w[4];
     uint4 s[PER / 2];                 // [PER][4] halves
-    uint32_t z[ZEROS ? PER / 4 : 1];  // [PER] bytes of the lane's row
+    uint32_t z[ZEROS ? PER / 4 : 1];  // [PER] bytes of the lane's row, 16 - zero
 
-    __device__ __forceinline__ void load(const Q4& m, int strip, int chunk, int lane)
+    // tile t's words, and the scales and zero points whose last one is the tile's:
+    // what an earlier strip had there has been used
+    __device__ __forceinline__ void load(const Q4& m, int strip, int chunk, int lane, int t)
     {
-        const int tiles = m.tiles - chunk * 4;
-        const uint4* p = reinterpret_cast<const uint4*>(m.numbers) + ((size_t)strip * m.tiles + chunk * 4) * 64 + lane;
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-            if (t < tiles) w[t] = p[t * 64];
+        constexpr int S_TILES = PER > 8 ? 1 : 8 / PER, Z_TILES = 16 / PER;   // tiles of an s (two for 32), of a z
+        if (chunk * 4 + t < m.tiles) w[t] = reinterpret_cast<const uint4*>(m.numbers)[((size_t)strip * m.tiles + chunk * 4 + t) * 64 + lane];
         const size_t cell = (size_t)strip * m.chunks + chunk;
-        const uint4* q = reinterpret_cast<const uint4*>(m.scales) + (cell * 4 + (lane >> 4)) * (PER / 2);
+        if ((t + 1) % S_TILES == 0) {
+            const uint4* q = reinterpret_cast<const uint4*>(m.scales) + (cell * 4 + (lane >> 4)) * (PER / 2);
+            constexpr int N = PER > 8 ? 2 : 1;
 #pragma unroll
-        for (int i = 0; i < PER / 2; i++) s[i] = q[i];
-        if constexpr (ZEROS) {
-            const uint32_t* r = reinterpret_cast<const uint32_t*>(m.zeros) + (cell * kStrip + (lane & 15)) * (PER / 4);
-#pragma unroll
-            for (int i = 0; i < PER / 4; i++) z[i] = r[i];
+            for (int i = 0; i < N; i++) s[t / S_TILES * N + i] = q[t / S_TILES * N + i];
         }
+        if constexpr (ZEROS)
+            if ((t + 1) % Z_TILES == 0) {
+                const uint32_t* r = reinterpret_cast<const uint32_t*>(m.zeros) + (cell * kStrip + (lane & 15)) * (PER / 4);
+                z[t / Z_TILES] = 0x10101010u - r[t / Z_TILES];
+            }
     }
 };
 
 // Eight weights as signed bytes: without zero points 16 (n - 8) (the stored four
 // bits are n - 8 in two's complement, at the top of a byte 16 times that),
-// with them n - zero.
+// with them n - zero + 16 (16 times the sum of x's digits is taken off by an
+// instruction of its own, on the matrix units that have the time).
 template <bool ZEROS>
 __device__ __forceinline__ void widen8(uint32_t w, uint32_t zero4, uint32_t& lo, uint32_t& hi)
 {
     if constexpr (ZEROS) {
-        lo = (((w & 0x0f0f0f0fu) ^ 0x88888888u) - zero4) ^ 0x80808080u;          // 128 + n - zero, no borrows
-        hi = (((w >> 4 & 0x0f0f0f0fu) ^ 0x88888888u) - zero4) ^ 0x80808080u;
+        lo = ((w & 0x0f0f0f0fu) ^ 0x08080808u) + zero4;
+        hi = ((w >> 4 & 0x0f0f0f0fu) ^ 0x08080808u) + zero4;
     } else {
         lo = w << 4 & 0xf0f0f0f0u;
         hi = w & 0xf0f0f0f0u;
@@ -74,8 +77,9 @@ __device__ __forceinline__ uint32_t max16(uint32_t v)
 // A workgroup takes S strips of 16 rows of the matrix; its waves deal the chunks
 // of 512 inputs among themselves.  A wave brings the rows' 512 values into its
 // own part of LDS as digits in the operands' order (16 lanes a tile, 8 values
-// each) while the first strip's weights are on their way (a strip's come while
-// the one before is computed), and needs no other wave until the sums are joined.
+// each) while the first strip's weights are on their way (a strip's tile comes as
+// soon as the one before has been computed), and needs no other wave until the
+// sums are joined.
 template <int D, int GROUP, bool ZEROS, int S>
 __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
 {
@@ -89,12 +93,13 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
     floatx4 acc[S];
 #pragma unroll
     for (int s = 0; s < S; s++) acc[s] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    FewWeights<GROUP, ZEROS> buf[S > 1 ? 2 : 1];
+    FewWeights<GROUP, ZEROS> now;
     for (int chunk = wave; chunk < u.m.chunks; chunk += a.waves) {
         const int t16 = lane >> 4, k8 = lane & 15, k = chunk * kChunk + t16 * kTile + k8 * 8;
         Raw8 raw = load_raw8(u.x, u.x_type, 0, k, u.m.in);
         float xs = D == 1 || u.x_scale ? u.x_scale[u.x_groups > 1 ? min(chunk * 4 + t16, u.x_groups - 1) : 0] : 1.0f;
-        buf[0].load(u.m, strip0, chunk, lane);
+#pragma unroll
+        for (int t = 0; t < 4; t++) now.load(u.m, strip0, chunk, lane, t);
         uint2* to = reinterpret_cast<uint2*>(digits + ((t16 * 2 + (k8 >> 3)) * 4 + (k8 & 3)) * cols) + (k8 >> 2 & 1);
         for (int r = 0; r < u.rows; r++) {
             const Raw8 mine8 = raw;
@@ -138,51 +143,56 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
             }
         }
         wave_sync();
-        if constexpr (S > 1) buf[1].load(u.m, min(strip0 + 1, last), chunk, lane);
         const int tiles = min(4, u.m.tiles - chunk * 4);
 #pragma unroll
         for (int sn = 0; sn < S; sn++) {
-            FewWeights<GROUP, ZEROS>& now = buf[sn & 1];
 #pragma unroll
             for (int t = 0; t < 4; t++) {
-                if (t >= tiles) break;
-                const float f = factor[t * kFewCols + mine] * (ZEROS ? 1.0f : 0.0625f);
-                const uint32_t wd[4] = {now.w[t].x, now.w[t].y, now.w[t].z, now.w[t].w};
-                intx4 sum = {0, 0, 0, 0};
+                if (t < tiles) {
+                    const float f = factor[t * kFewCols + mine] * (ZEROS ? 1.0f : 0.0625f);
+                    const uint32_t wd[4] = {now.w[t].x, now.w[t].y, now.w[t].z, now.w[t].w};
+                    intx4 sum = {0, 0, 0, 0};
+                    floatx4 part = {0.0f, 0.0f, 0.0f, 0.0f};   // of the tile, without f
 #pragma unroll
-                for (int step = 0; step < 2; step++) {
-                    const uint4 b = digits[((t * 2 + step) * 4 + g) * cols + col];
-                    uint32_t lo[2], hi[2];
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const int grp = (t * kTile + (step * 2 + j) * 32) / GROUP;
-                        uint32_t z4 = 0;
-                        if constexpr (ZEROS) z4 = __builtin_amdgcn_perm(0u, now.z[grp / 4], 0x01010101u * (grp % 4));
-                        widen8<ZEROS>(wd[step * 2 + j], z4, lo[j], hi[j]);
-                    }
-                    auto join = [&](int grp) {
-                        const uint32_t s0 = grp % 2 ? now.s[grp / 2].z : now.s[grp / 2].x, s1 = grp % 2 ? now.s[grp / 2].w : now.s[grp / 2].y;
-                        const half4 s = __builtin_bit_cast(half4, (uint64_t)s1 << 32 | s0);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) acc[sn][i] = __builtin_fmaf((float)sum[i], (float)s[i] * f, acc[sn][i]);
-                        sum = intx4{0, 0, 0, 0};
-                    };
-                    if constexpr (GROUP == 32) {
+                    for (int step = 0; step < 2; step++) {
+                        const uint4 b = digits[((t * 2 + step) * 4 + g) * cols + col];
+                        uint32_t lo[2], hi[2];
 #pragma unroll
                         for (int j = 0; j < 2; j++) {
-                            const long x8 = (long)((uint64_t)(j ? b.w : b.y) << 32 | (j ? b.z : b.x));
-                            sum = __builtin_amdgcn_mfma_i32_16x16x32_i8((long)((uint64_t)hi[j] << 32 | lo[j]), x8, sum, 0, 0, 0);
-                            join(t * 4 + step * 2 + j);
+                            const int grp = (t * kTile + (step * 2 + j) * 32) / GROUP;
+                            uint32_t z4 = 0;
+                            if constexpr (ZEROS) z4 = __builtin_amdgcn_perm(0u, now.z[grp / 4], 0x01010101u * (grp % 4));
+                            widen8<ZEROS>(wd[step * 2 + j], z4, lo[j], hi[j]);
                         }
-                    } else {
-                        const intx4 w8 = {(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
-                        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(w8, __builtin_bit_cast(intx4, b), sum, 0, 0, 0);
-                        if constexpr (GROUP == 64) join(t * 2 + step);
-                        else if (step == 1) join(t);
+                        auto join = [&](int grp) {
+                            const uint32_t s0 = grp % 2 ? now.s[grp / 2].z : now.s[grp / 2].x, s1 = grp % 2 ? now.s[grp / 2].w : now.s[grp / 2].y;
+                            const half4 s = __builtin_bit_cast(half4, (uint64_t)s1 << 32 | s0);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) part[i] = __builtin_fmaf((float)sum[i], (float)s[i], part[i]);
+                            sum = intx4{0, 0, 0, 0};
+                        };
+                        if constexpr (GROUP == 32) {
+#pragma unroll
+                            for (int j = 0; j < 2; j++) {
+                                const long x8 = (long)((uint64_t)(j ? b.w : b.y) << 32 | (j ? b.z : b.x));
+                                if constexpr (ZEROS) sum = __builtin_amdgcn_mfma_i32_16x16x32_i8((long)0xf0f0f0f0f0f0f0f0ull, x8, sum, 0, 0, 0);
+                                sum = __builtin_amdgcn_mfma_i32_16x16x32_i8((long)((uint64_t)hi[j] << 32 | lo[j]), x8, sum, 0, 0, 0);
+                                join(t * 4 + step * 2 + j);
+                            }
+                        } else {
+                            constexpr int less = (int)0xf0f0f0f0u;   // -16, four times
+                            const intx4 w8 = {(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
+                            if constexpr (ZEROS) sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(intx4{less, less, less, less}, __builtin_bit_cast(intx4, b), sum, 0, 0, 0);
+                            sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(w8, __builtin_bit_cast(intx4, b), sum, 0, 0, 0);
+                            if constexpr (GROUP == 64) join(t * 2 + step);
+                            else if (step == 1) join(t);
+                        }
                     }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[sn][i] = __builtin_fmaf(part[i], f, acc[sn][i]);
                 }
+                if (sn + 1 < S) now.load(u.m, min(strip0 + sn + 1, last), chunk, lane, t);
             }
-            if (sn + 2 < S) now.load(u.m, min(strip0 + sn + 2, last), chunk, lane);
         }
         wave_sync();
     }
@@ -222,19 +232,14 @@ static int few_launch(Ctx* c, const FewArgs& a)
 template <int D, int GROUP>
 static int few_sized(Ctx* c, const FewArgs& a)
 {
-    // Several strips share the rows' digits where there are enough of them for
-    // the card all the same (one fp32 row, 32000 x 4096: 17.6 us by single strips,
-    // 14.0 by two, 12.9 by four; five bf16 rows 27.4, 18.7 and 15.2; 14336 x 4096 10.8,
-    // 8.7 and 8.7; 6144 x 4096 with groups of 64 7.9, 8.4 and 11.4).  Groups of 64
-    // fill the registers with two strips' scales, which pays for several rows
-    // only (28672 x 4096: one row 17.8, 18.5 and 19.0, five 26.7, 23.1 and 20.6); those of 32 do
-    // not fit at all.
-    const int strips = q4_strips(a.u.m.out), cols = a.u.rows * D;
-    if constexpr (GROUP > 32) {
-        if (strips >= (GROUP == 128 ? 768 : 1024) && (GROUP == 128 || cols > 4)) return few_launch<D, GROUP, 4>(c, a);
-        if constexpr (GROUP == 64)
-            if (strips >= 768 && cols > 4) return few_launch<D, GROUP, 2>(c, a);
-    }
+    // Several strips share the rows' digits, and a strip's weights come while the
+    // one before is computed, where there are enough for the card all the same
+    // (one bf16 row, 28672 x 4096 with groups of 64 and zero points: 17.3 us by single
+    // strips, 15.1 by two, 13.1 by four, 23.8 by eight; five rows 26.1, 20.0 and 15.6;
+    // 8192 x 8192 with groups of 128 11.0, 9.4 and 9.1, 6144 x 4096 5.7, 6.2 and 7.1).
+    // Groups of 32 with zero points and four strips do not fit the registers (28672 x
+    // 4096: 20.1, 17.4 and 23.0).
+    if (q4_strips(a.u.m.out) >= 512) return few_launch<D, GROUP, GROUP == 32 ? 2 : 4>(c, a);
     return few_launch<D, GROUP, 1>(c, a);
 }
 
