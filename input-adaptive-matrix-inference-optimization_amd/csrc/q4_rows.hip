@@ -1,5 +1,5 @@
 // Products of many rows (batches, prompts) with 4-bit weights, on the fp16 matrix
-// instructions.
+// instructions, and those of more than 64 rows in int8 on the 8-bit ones.
 //
 // A launch of its own brings x into the instructions' order as fp16: one part
 // of values that fp16 holds (fp16 and 8-bit numbers; bf16 of a tile of 128 after
@@ -19,7 +19,8 @@ typedef unsigned long long ull2 __attribute__((ext_vector_type(2)));
 
 // ---- x in the operands' order
 // parts  fp16 [part][block of 16 rows][tile][j][lane 16 g + row][8]: inputs
-//        32 j + 8 g and on of the tile
+//        32 j + 8 g and on of the tile.  Or int8 [block of 16 rows][tile][j][lane
+//        16 half + row][16]: eight inputs from 32 j + 8 half on, eight from 16 further on
 // factor fp32 [block][tile][16]: what the tile's values were divided by
 // scaled [block][tile]: whether any of these is not 1
 struct PrepArgs {
@@ -32,7 +33,7 @@ struct PrepArgs {
     size_t part_stride;      // values of a part
     float* factor;
     uint8_t* scaled;
-    int parts_n;
+    int parts_n;             // 0: 8-bit rows as they are
 };
 
 constexpr int kPrepThreads = 256;
@@ -46,11 +47,13 @@ __global__ __launch_bounds__(kPrepThreads) void k_q4_prep(PrepArgs a)
     const int row = block * 16 + c;
     const bool there = row < a.rows;
     float v[4][8];
+    uint2 bytes[4];
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const Raw8 r = load_raw8(a.x, a.type, (size_t)(there ? row : 0) * a.stride, tile * kTile + 32 * j + 8 * g, there ? a.in : 0);
         values8(r, a.type, v[j]);
+        bytes[j] = {r.a.x, r.a.y};
 #pragma unroll
         for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(v[j][e]) & 0x7fffffffu);
     }
@@ -70,6 +73,13 @@ __global__ __launch_bounds__(kPrepThreads) void k_q4_prep(PrepArgs a)
     const size_t at = ((size_t)block * a.tiles + tile) * 4 * 64 * 8;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
+        if (a.parts_n == 0) {
+            // as the bytes of widened weights lie
+            const uint32_t p = bytes[j].x, q = bytes[j].y;
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.parts) + at + ((j * 32 + (g & 1) * 16 + c) * 16 + (g >> 1) * 8)) =
+                uint2{__builtin_amdgcn_perm(q, p, 0x05010400u), __builtin_amdgcn_perm(q, p, 0x07030602u)};
+            continue;
+        }
         half8 h, l;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
@@ -94,6 +104,7 @@ struct RowsArgs {
     const float* factor;
     const uint8_t* scaled;    // null: no factor can be anything but 1
     const float* row_scale;   // of a whole row, or null
+    bool bytes;               // parts in 8 bits
     int blocks;               // of 16 rows
     int waves;
     // the inputs cut into parts for more workgroups, whose sums the last one to arrive joins
@@ -112,6 +123,19 @@ __device__ __forceinline__ half8 widen_half(uint32_t w, uint32_t minus1024, uint
     const half2v c = __builtin_bit_cast(half2v, (v & 0x000f000fu) ^ 0x64086408u) + __builtin_bit_cast(half2v, minus1024);
     const half2v d = __builtin_bit_cast(half2v, (v & 0x00f000f0u) ^ 0x54805480u) + __builtin_bit_cast(half2v, minus64);
     return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Four weights as signed bytes (of the word's low or high halves of bytes): without
+// zero points 16 (n - 8), with them n - zero.
+template <bool ZEROS>
+__device__ __forceinline__ uint32_t widen_low(uint32_t w, uint32_t zero4)
+{
+    return ZEROS ? (((w & 0x0f0f0f0fu) ^ 0x88888888u) - zero4) ^ 0x80808080u : w << 4 & 0xf0f0f0f0u;   // 128 + n - zero: no borrows
+}
+template <bool ZEROS>
+__device__ __forceinline__ uint32_t widen_high(uint32_t w, uint32_t zero4)
+{
+    return ZEROS ? widen_low<true>(w >> 4, zero4) : w & 0xf0f0f0f0u;
 }
 
 // what is subtracted for a zero point: -(1024 + zero) and -(64 + zero), twice
@@ -311,10 +335,13 @@ __global__ __launch_bounds__(64 * MOST) void k_q4_batch(RowsArgs a)
 constexpr int kGemmStrips = 4;     // of a wave
 constexpr int kGemmPanel = 8;      // workgroups side by side along x's rows that run together
 
+// PARTS: of x in fp16; 0 and -1: x in 8 bits, with weights that have zero points (-1) or none.
 template <int PARTS, int GROUP, int NB, int WO, int STAGES>
 struct Gemm {
+    static constexpr bool BYTE = PARTS <= 0;
+    static constexpr int BLOCK = BYTE ? 2 : 4;     // KB of a tile of 16 rows
     static constexpr int GT = kTile / GROUP, S = kGemmStrips, WAVES = 2 * WO, STRIPS = S * WO;
-    static constexpr int X = PARTS * 2 * NB * 4, RUNS = X + STRIPS, SHARE = RUNS / WAVES;
+    static constexpr int X = (BYTE ? 1 : PARTS) * 2 * NB * BLOCK, RUNS = X + STRIPS, SHARE = RUNS / WAVES;
     static constexpr int SCALES = RUNS * 1024;                      // [group][strip][g] four halves
     static constexpr int ZEROS = SCALES + GT * STRIPS * 32;         // [strip][row] words
     static constexpr int BYTES = ZEROS + STRIPS * 64;
@@ -325,6 +352,7 @@ struct Gemm {
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef int intx16 __attribute__((ext_vector_type(16)));
 
 // LDS reads in one piece of assembly with their wait: the compiler, which
 // cannot tell the stages apart, would wait for all loads in flight to LDS
@@ -351,6 +379,27 @@ __device__ __forceinline__ void read_rows64(uint32_t at, u32x4* r)
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]), "=&v"(r[8]), "=&v"(r[9]), "=&v"(r[10]),
           "=&v"(r[11]), "=&v"(r[12]), "=&v"(r[13]), "=&v"(r[14]), "=&v"(r[15])
+        : "v"(at)
+        : "memory");
+}
+// 32 rows in 8 bits: j at 512 j
+__device__ __forceinline__ void read_bytes32(uint32_t at, u32x4* r)
+{
+    asm volatile(
+        "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:512\n\tds_read_b128 %2, %4 offset:1024\n\tds_read_b128 %3, %4 offset:1536\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+        : "v"(at)
+        : "memory");
+}
+// and 64
+__device__ __forceinline__ void read_bytes64(uint32_t at, u32x4* r)
+{
+    asm volatile(
+        "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:512\n\tds_read_b128 %2, %8 offset:1024\n\tds_read_b128 %3, %8 offset:1536\n\t"
+        "ds_read_b128 %4, %8 offset:4096\n\tds_read_b128 %5, %8 offset:4608\n\tds_read_b128 %6, %8 offset:5120\n\tds_read_b128 %7, %8 offset:5632\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
         : "v"(at)
         : "memory");
 }
@@ -389,6 +438,7 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
 {
     typedef Gemm<PARTS, GROUP, NB, WO, STAGES> G;
     constexpr int GT = G::GT, S = G::S, N = NB / 2;
+    constexpr int P = G::BYTE ? 1 : PARTS, OPS = G::BYTE ? 4 : 8;    // parts, matrix instructions of 32 rows and a pair of strips
     const MulArgs& u = a.u;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int c = lane & 15, side = lane >> 4 & 1, half = lane >> 5;   // row (of x or the matrix) 16 side + c, inputs 8 half and on of 16
@@ -407,8 +457,8 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
     for (int q = 0; q < G::SHARE; q++) {
         const int i = wave + G::WAVES * q;
         if ((q + 1) * G::WAVES <= G::X) {
-            const int b = min(b0 + (i >> 2) % (2 * NB), a.blocks - 1), p = (i >> 2) / (2 * NB);
-            run[q] = reinterpret_cast<const uint8_t*>(a.parts + p * a.part_stride + ((size_t)b * u.m.tiles * 4 + (i & 3)) * 512);
+            const int b = min(b0 + i / G::BLOCK % (2 * NB), a.blocks - 1), p = i / G::BLOCK / (2 * NB);
+            run[q] = reinterpret_cast<const uint8_t*>(a.parts + p * a.part_stride) + ((size_t)b * u.m.tiles * G::BLOCK + i % G::BLOCK) * 1024;
         } else {
             run[q] = u.m.numbers + (size_t)min(s0 + i - G::X, last) * u.m.tiles * 1024;
         }
@@ -429,7 +479,7 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
         char* to = reinterpret_cast<char*>(stage.at[buf]);
 #pragma unroll
         for (int q = 0; q < G::SHARE; q++) {
-            const uint8_t* src = run[q] + (uint32_t)t * ((q + 1) * G::WAVES <= G::X ? 4096u : 1024u);
+            const uint8_t* src = run[q] + (uint32_t)t * ((q + 1) * G::WAVES <= G::X ? G::BLOCK * 1024u : 1024u);
             __builtin_amdgcn_global_load_lds((From)(src + lane16), (To)(to + (wave + G::WAVES * q) * 1024), 16, 0, 0);
         }
 #pragma unroll
@@ -484,16 +534,18 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
         const uint32_t at = base + buf * G::BYTES;
         free_buf = buf;
         buf = buf + 1 == STAGES ? 0 : buf + 1;
-        u32x4 x[PARTS][N * 8], w[4], sc[GT][4];
+        u32x4 x[P][N * OPS], w[4], sc[GT][4];
         uint32_t zero[2];
         const uint32_t mine = (uint32_t)(half * 16 + c) * 16u;
         read_words(at + (G::X + wo * S + side) * 1024 + mine, at + G::ZEROS + (wo * S + side) * 64 + c * 4, at + G::SCALES + wo * S * 32 + half * 8, w, zero, sc[0]);
 #pragma unroll
         for (int i = 1; i < GT; i++) read_scales(at + G::SCALES + i * G::STRIPS * 32 + wo * S * 32 + half * 8, sc[i]);
 #pragma unroll
-        for (int p = 0; p < PARTS; p++) {
-            const uint32_t from = at + ((p * 2 + wx) * NB + side) * 4096 + mine;
-            if constexpr (N == 2) read_rows64(from, x[p]);
+        for (int p = 0; p < P; p++) {
+            const uint32_t from = at + ((p * 2 + wx) * NB + side) * (G::BLOCK * 1024) + mine;
+            if constexpr (G::BYTE && N == 2) read_bytes64(from, x[p]);
+            else if constexpr (G::BYTE) read_bytes32(from, x[p]);
+            else if constexpr (N == 2) read_rows64(from, x[p]);
             else read_rows32(from, x[p]);
         }
         // the next tile's loads, as late as the other group's turn allows
@@ -507,30 +559,45 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
                                    : GT == 1  ? zero[s] >> (8 * (t & 3))
                                    : GT == 2  ? zero[s] >> (16 * (t & 1) + 8 * i)
                                               : zero[s] >> (8 * i);
-                const Minus m = minus_of(z & 255u);
-                floatx16 d[PARTS][N];
+                std::conditional_t<G::BYTE, intx16, floatx16> d[P][N];
 #pragma unroll
-                for (int p = 0; p < PARTS; p++)
+                for (int p = 0; p < P; p++)
 #pragma unroll
                     for (int n = 0; n < N; n++)
 #pragma unroll
-                        for (int e = 0; e < 16; e++) d[p][n][e] = 0.0f;
+                        for (int e = 0; e < 16; e++) d[p][n][e] = 0;
+                if constexpr (G::BYTE) {
+                    const uint32_t z4 = (z & 255u) * 0x01010101u;
 #pragma unroll
-                for (int k = i * 8 / GT; k < (i + 1) * 8 / GT; k++) {      // 16 inputs: word k / 2, g = 2 (k % 2) + half
-                    const half8 wide = widen_half(w[s * 2 + k % 2][k / 2], m.k1024, m.k64);
-#pragma unroll
-                    for (int p = 0; p < PARTS; p++)
+                    for (int j = i * 4 / GT; j < (i + 1) * 4 / GT; j++) {      // 32 inputs: word j of g = half and 2 + half
+                        intx4 wide;
+                        wide[0] = (int)widen_low<(PARTS < 0)>(w[s * 2][j], z4);
+                        wide[1] = (int)widen_high<(PARTS < 0)>(w[s * 2][j], z4);
+                        wide[2] = (int)widen_low<(PARTS < 0)>(w[s * 2 + 1][j], z4);
+                        wide[3] = (int)widen_high<(PARTS < 0)>(w[s * 2 + 1][j], z4);
 #pragma unroll
                         for (int n = 0; n < N; n++)
-                            d[p][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wide, __builtin_bit_cast(half8, x[p][n * 8 + k]), d[p][n], 0, 0, 0);
+                            d[0][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wide, __builtin_bit_cast(intx4, x[0][n * 4 + j]), d[0][n], 0, 0, 0);
+                    }
+                } else {
+                    const Minus m = minus_of(z & 255u);
+#pragma unroll
+                    for (int k = i * 8 / GT; k < (i + 1) * 8 / GT; k++) {      // 16 inputs: word k / 2, g = 2 (k % 2) + half
+                        const half8 wide = widen_half(w[s * 2 + k % 2][k / 2], m.k1024, m.k64);
+#pragma unroll
+                        for (int p = 0; p < P; p++)
+#pragma unroll
+                            for (int n = 0; n < N; n++)
+                                d[p][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wide, __builtin_bit_cast(half8, x[p][n * 8 + k]), d[p][n], 0, 0, 0);
+                    }
                 }
 #pragma unroll
                 for (int n = 0; n < N; n++)
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
                         const half8 scale = __builtin_bit_cast(half8, sc[i][s * 2 + e / 8]);
-                        float v = d[0][n][e];
-                        if constexpr (PARTS == 2) v += d[1][n][e];
+                        float v = (float)d[0][n][e];
+                        if constexpr (P == 2) v += d[1][n][e];
                         float by = (float)scale[e % 8];
                         if constexpr (FACTORS) by *= fn[n];
                         acc[s][n][e] = __builtin_fmaf(v, by, acc[s][n][e]);
@@ -543,9 +610,9 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
             // the matrix instructions (smaller groups would spill)
             __builtin_amdgcn_sched_group_barrier(0x2, 20, 0);
 #pragma unroll
-            for (int i = 0; i < 16 * N * PARTS; i++) {
+            for (int i = 0; i < 2 * OPS * N * P; i++) {
                 __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x2, 8, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, G::BYTE ? 14 : 8, 0);
             }
         }
         if constexpr (!SECOND) arrived();
@@ -649,7 +716,7 @@ __global__ __launch_bounds__(128 * WO, 2) void k_q4_gemm(RowsArgs a)
 #pragma unroll
     for (int n = 0; n < NB / 2; n++) {
         const int r0 = (b0 + (wave & 1) * NB + 2 * n) * 16;
-        const float rs = a.row_scale ? a.row_scale[min(r0 + (lane & 31), u.rows - 1)] : 1.0f;
+        const float rs = (a.row_scale ? a.row_scale[min(r0 + (lane & 31), u.rows - 1)] : 1.0f) * (PARTS == 0 ? 0.0625f : 1.0f);
 #pragma unroll
         for (int s = 0; s < 2; s++)
 #pragma unroll
@@ -728,7 +795,8 @@ static int gemm_launch(Ctx* c, RowsArgs a, int splits)
 // join.  Fitted to measured times: of 64 x 128 (128 rows, 6144 x 4096) 29.3 us in one
 // part and 21.9 in two, 256 x 64 35.2 and 26.1, 256 x 128 51.7 and 37.5; 389 rows 44.5 and
 // 45.9, 39.7 and 53.5, 54.6 and 42.8; 4096 rows, 14336 x 4096 650, 608 and 494 in one;
-// 128 rows, 1024 x 14336 90.7 in one, 22.1 in eight.
+// 128 rows, 1024 x 14336 90.7 in one, 22.1 in eight.  Rows in 8 bits: 389 of them 30.3
+// and 29.8 by 64 x 128, 30.8 and 42.9, 41.2 and 37.5; 4096, 14336 x 4096 387, 453 and 350.
 struct GemmCost {
     double us;
     int splits;
@@ -749,20 +817,34 @@ static GemmCost gemm_cost(const RowsArgs& a, int nb, int wo, F round)
 }
 
 template <int PARTS, int GROUP>
+static int gemm_sized(Ctx* c, const RowsArgs& a)
+{
+    // (groups of 32 have too many scales for the widest shape's registers; rows in
+    // 8 bits were never best by 256 x 64)
+    if constexpr (PARTS == 2) {
+        return gemm_launch<PARTS, GROUP, 2, 4, 3>(c, a, gemm_cost(a, 2, 4, [](int n) { return 1.5 * ((n + 255) / 256); }).splits);
+    } else if constexpr (PARTS <= 0) {
+        const GemmCost small = gemm_cost(a, 2, 2, [](int n) { return n <= 256 ? 0.55 : n <= 512 ? 0.8 : 0.41 * ((n + 255) / 256); });
+        const GemmCost wide = gemm_cost(a, 4, 4, [](int n) { return 1.45 * ((n - 1) / 256) + 1.0 + 0.4 * ((n - 1) % 256 + 1) / 256; });
+        if constexpr (GROUP > 32)
+            if (wide.us <= small.us) return gemm_launch<PARTS, GROUP, 4, 4, 3>(c, a, wide.splits);
+        return gemm_launch<PARTS, GROUP, 2, 2, 3>(c, a, small.splits);
+    } else {
+        const GemmCost small = gemm_cost(a, 2, 2, [](int n) { return n <= 256 ? 0.76 : n <= 512 ? 1.24 : 0.72 * ((n + 255) / 256); });
+        const GemmCost tall = gemm_cost(a, 2, 4, [](int n) { return 1.05 * ((n + 255) / 256); });
+        const GemmCost wide = gemm_cost(a, 4, 4, [](int n) { return 2.0 * ((n - 1) / 256) + 1.45 + 0.55 * ((n - 1) % 256 + 1) / 256; });
+        if constexpr (GROUP > 32)
+            if (wide.us <= small.us && wide.us <= tall.us) return gemm_launch<PARTS, GROUP, 4, 4, 3>(c, a, wide.splits);
+        return tall.us < small.us ? gemm_launch<PARTS, GROUP, 2, 4, 3>(c, a, tall.splits) : gemm_launch<PARTS, GROUP, 2, 2, 3>(c, a, small.splits);
+    }
+}
+
+template <int PARTS, int GROUP>
 static int batch_sized(Ctx* c, const RowsArgs& a)
 {
     if (a.blocks > 4) {
-        if constexpr (PARTS == 2) {
-            return gemm_launch<PARTS, GROUP, 2, 4, 3>(c, a, gemm_cost(a, 2, 4, [](int n) { return 1.5 * ((n + 255) / 256); }).splits);
-        } else {
-            const GemmCost small = gemm_cost(a, 2, 2, [](int n) { return n <= 256 ? 0.76 : n <= 512 ? 1.24 : 0.72 * ((n + 255) / 256); });
-            const GemmCost tall = gemm_cost(a, 2, 4, [](int n) { return 1.05 * ((n + 255) / 256); });
-            const GemmCost wide = gemm_cost(a, 4, 4, [](int n) { return 2.0 * ((n - 1) / 256) + 1.45 + 0.55 * ((n - 1) % 256 + 1) / 256; });
-            // (groups of 32 have too many scales for the widest one's registers)
-            if constexpr (GROUP > 32)
-                if (wide.us <= small.us && wide.us <= tall.us) return gemm_launch<PARTS, GROUP, 4, 4, 3>(c, a, wide.splits);
-            return tall.us < small.us ? gemm_launch<PARTS, GROUP, 2, 4, 3>(c, a, tall.splits) : gemm_launch<PARTS, GROUP, 2, 2, 3>(c, a, small.splits);
-        }
+        if (a.bytes) return a.u.m.zeros ? gemm_sized<-1, GROUP>(c, a) : gemm_sized<0, GROUP>(c, a);
+        return gemm_sized<PARTS, GROUP>(c, a);
     }
     // Up to 32 rows a strip a workgroup fills the card where there are few and the
     // matrix's rows are short (32 bf16 rows, 1024 x 4096: 5.4 us against 6.5 of two;
@@ -804,6 +886,7 @@ int q4_mul_rows(Ctx* c, const MulArgs& all)
         a.parts = reinterpret_cast<_Float16*>(c->q4_part);
         a.part_stride = values;
         a.blocks = (u.rows + 15) / 16;
+        a.bytes = u.x_type == IAM_I8 && a.blocks > 4;
         float* factor = reinterpret_cast<float*>(c->q4_part + values * 2 * parts);
         uint8_t* scaled = reinterpret_cast<uint8_t*>(factor + blocks * all.m.tiles * 16);
         a.factor = factor;
@@ -812,7 +895,7 @@ int q4_mul_rows(Ctx* c, const MulArgs& all)
         const bool by_tile = u.x_groups > 1;
         a.row_scale = by_tile ? nullptr : u.x_scale;
         const PrepArgs p{u.x, u.x_type, u.x_stride, by_tile ? u.x_scale : nullptr, u.rows, u.m.in, u.m.tiles,
-                         reinterpret_cast<_Float16*>(c->q4_part), values, factor, scaled, parts};
+                         reinterpret_cast<_Float16*>(c->q4_part), values, factor, scaled, a.bytes ? 0 : parts};
         const dim3 grid((unsigned)((u.m.tiles + 3) / 4), (unsigned)a.blocks);
         IAM_TRY(launch(c, "q4_mul.prepare", k_q4_prep, grid, dim3(kPrepThreads), 0, p));
         IAM_TRY(parts == 2 ? batch_grouped<2>(c, a) : batch_grouped<1>(c, a));
