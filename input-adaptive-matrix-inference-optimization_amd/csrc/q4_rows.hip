@@ -1,10 +1,10 @@
 // Products of many rows (batches, prompts) with 4-bit weights, on the fp16 matrix
 // instructions, and those of more than 64 rows in int8 on the 8-bit ones.
 //
-// A launch of its own brings x into the instructions' order as fp16: one part
-// of values that fp16 holds (fp16 and 8-bit numbers; bf16 of a tile of 128 after
-// a power of two where its largest value lies outside [2^-2, 2^15)), two, high
-// and low, of fp32 (22 bits).  4-bit weights become fp16 under the exponents of
+// A launch of its own brings x into the instructions' order, bytes as they are,
+// the rest as fp16: one part of values that fp16 holds (fp16 and 8-bit numbers;
+// bf16 of a tile of 128 after a power of two where its largest value lies outside
+// [2^-2, 2^15)), two, high and low, of fp32 (22 bits).  4-bit weights become fp16 under the exponents of
 // 1024 and 64, n - zero exactly.  Products are then exact; a group's are added
 // in fp32 by the instructions and go to the row's sum with the group's scale
 // times that power (together first: a sum of large x alone may pass fp32).
@@ -865,14 +865,15 @@ static int batch_grouped(Ctx* c, const RowsArgs& a)
     return batch_sized<PARTS, 128>(c, a);
 }
 
-// rows of a pass: what x takes as parts stays small beside the card's memory,
-// and a launch has at most 2^30 threads (one for 32 products)
+// rows of a pass: what x takes as parts stays small beside the card's memory
+// (2^29 values), and a launch has at most 2^30 threads (one for 32 products)
 constexpr int kRowsSlice = 1 << 14;
 
 int q4_mul_rows(Ctx* c, const MulArgs& all)
 {
     const int parts = all.x_type == IAM_F32 ? 2 : 1;
-    const int slice = (int)std::min<int64_t>(std::min(all.rows, kRowsSlice), ((int64_t)1 << 35) / (q4_strips(all.m.out) * kStrip));
+    const int slice = (int)std::min({(int64_t)all.rows, (int64_t)kRowsSlice, ((int64_t)1 << 29) / (all.m.tiles * kTile),
+                                     ((int64_t)1 << 35) / (q4_strips(all.m.out) * kStrip)});
     const size_t blocks = (size_t)(slice + 15) / 16, values = blocks * all.m.tiles * 2048;
     IAM_TRY(ensure_q4_scratch(c, values * 2 * parts + blocks * all.m.tiles * (64 + 1)));
     for (int r0 = 0; r0 < all.rows; r0 += slice) {

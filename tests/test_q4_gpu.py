@@ -142,6 +142,14 @@ def test_values_near_the_largest(iam, ctx, rows, type):
     P.close(got, want, R.product_bound(v, w.values()), "f32")
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("type,x_group", [("f32", 0), ("bf16", 0), ("int8", 0), ("int8", 128)])
+def test_workgroups_for_every_unit(iam, ctx, type, x_group, group, zeros):
+    """As many products as the widest workgroups take."""
+    check(iam, ctx, np.random.default_rng(group), 2040, 300, 4090, group, zeros, type, "f32" if zeros else "bf16", x_group, y_stride=4095)
+
+
 def test_many_rows_and_outputs(iam, ctx):
     """More rows than a pass takes, more strips than a launch packs."""
     rng = np.random.default_rng(9)
