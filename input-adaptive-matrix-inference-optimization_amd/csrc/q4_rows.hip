@@ -113,6 +113,8 @@ struct RowsArgs {
     uint32_t* ctr;            // zero on entry (left zero)
 };
 
+constexpr int kMaxSplits = 8;
+
 // Eight weights as fp16, n - zero: under the exponent of 1024 a number's step is
 // 1, under that of 64 it is 1/16.
 __device__ __forceinline__ half8 widen_half(uint32_t w, uint32_t minus1024, uint32_t minus64)
@@ -316,14 +318,18 @@ __global__ __launch_bounds__(64 * MOST) void k_q4_batch(RowsArgs a)
     if (!acc_arrive(a.ctr + cell, (uint32_t)a.splits, &last)) return;
     if (threadIdx.x == 0) a.ctr[cell] = 0u;
     for (int i = wave; i < S * NB; i += a.waves) {
-        floatx4 v = {0, 0, 0, 0};
-        for (int q = 0; q < a.splits; q++) {
-            unsigned long long* from = reinterpret_cast<unsigned long long*>(sums + ((size_t)q * (S * NB) + i) * 256 + lane * 4);
-            ull2 two;
-            two[0] = acc_peek(from);
-            two[1] = acc_peek(from + 1);
-            v += __builtin_bit_cast(floatx4, two);
+        // all of them on the way at once
+        ull2 two[kMaxSplits];
+#pragma unroll
+        for (int q = 0; q < kMaxSplits; q++) {
+            unsigned long long* from = reinterpret_cast<unsigned long long*>(sums + ((size_t)min(q, a.splits - 1) * (S * NB) + i) * 256 + lane * 4);
+            two[q][0] = acc_peek(from);
+            two[q][1] = acc_peek(from + 1);
         }
+        floatx4 v = {0, 0, 0, 0};
+#pragma unroll
+        for (int q = 0; q < kMaxSplits; q++)
+            if (q < a.splits) v += __builtin_bit_cast(floatx4, two[q]);
         put(i / NB, i % NB, v);
     }
 }
@@ -746,7 +752,6 @@ __global__ __launch_bounds__(128 * WO, 2) void k_q4_gemm(RowsArgs a)
 }
 
 // ------------------------------------------------------------------ host ---
-constexpr int kMaxSplits = 8;
 constexpr int kMinTiles = 16;      // of a split (64 bf16 rows, 1024 x 14336: 13.0 us at 32, 10.6 at 16, 13.4 at 10)
 
 template <int PARTS, int GROUP, int S, int NB, int MOST>
