@@ -752,14 +752,17 @@ __global__ __launch_bounds__(128 * WO, 2) void k_q4_gemm(RowsArgs a)
 }
 
 // ------------------------------------------------------------------ host ---
-constexpr int kMinTiles = 16;      // of a split (64 bf16 rows, 1024 x 14336: 13.0 us at 32, 10.6 at 16, 13.4 at 10)
-
 template <int PARTS, int GROUP, int S, int NB, int MOST>
 static int batch_launch(Ctx* c, RowsArgs a)
 {
     const int groups = (q4_strips(a.u.m.out) + S - 1) / S, across = (a.blocks + NB - 1) / NB;
-    // inputs cut for about a workgroup a CU
-    a.splits = S == 1 ? 1 : std::max(1, std::min({256 / (groups * across), kMaxSplits, a.u.m.tiles / kMinTiles}));
+    // The inputs are cut for about a workgroup a CU: by 16 tiles and more (64 bf16
+    // rows, 1024 x 14336: 10.6 us, 13.0 by 32), from four operands of x a tile on by 8
+    // (64 bf16 rows, 1024 x 4096: 7.6 us, 9.0 by 16; 32 fp32 rows 6.3 and 8.4, but 64 of
+    // 1024 x 2048 7.6 and 6.7), single strips of fewer not at all (8 rows: 4.4 whole, 5.1 by 16).
+    constexpr bool MANY = PARTS * NB >= 4;
+    const int parts = MANY ? a.u.m.tiles >= 32 ? a.u.m.tiles / 8 : 1 : S == 1 ? 1 : a.u.m.tiles / 16;
+    a.splits = std::max(1, std::min({256 / (groups * across), kMaxSplits, parts}));
     // waves share a workgroup's tiles evenly
     const int each = (a.u.m.tiles + a.splits - 1) / a.splits, rounds = (each + MOST - 1) / MOST;
     a.waves = (each + rounds - 1) / rounds;
