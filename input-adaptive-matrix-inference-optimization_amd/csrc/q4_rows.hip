@@ -839,7 +839,7 @@ static int gemm_sized(Ctx* c, const RowsArgs& a)
         return gemm_launch<PARTS, GROUP, 2, 2, 3>(c, a, small.splits);
     } else {
         const GemmCost small = gemm_cost(a, 2, 2, [](int n) { return n <= 256 ? 0.76 : n <= 512 ? 1.24 : 0.72 * ((n + 255) / 256); });
-        const GemmCost tall = gemm_cost(a, 2, 4, [](int n) { return 1.05 * ((n + 255) / 256); });
+        const GemmCost tall = gemm_cost(a, 2, 4, [](int n) { return 1.36 * ((n - 1) / 256) + 0.85 + 0.35 * ((n - 1) % 256 + 1) / 256; });
         const GemmCost wide = gemm_cost(a, 4, 4, [](int n) { return 2.0 * ((n - 1) / 256) + 1.45 + 0.55 * ((n - 1) % 256 + 1) / 256; });
         if constexpr (GROUP > 32)
             if (wide.us <= small.us && wide.us <= tall.us) return gemm_launch<PARTS, GROUP, 4, 4, 3>(c, a, wide.splits);
