@@ -368,7 +368,7 @@ __device__ __forceinline__ void read_rows32(uint32_t at, u32x4* r)
 {
     asm volatile(
         "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:512\n\tds_read_b128 %2, %8 offset:1024\n\tds_read_b128 %3, %8 offset:1536\n\t"
-        "ds_read_b128 %4, %8 offset:2048\n\tds_read_b128 %5, %8 offset:2560\n\tds_read_b128 %6, %8 offset:3072\n\tds_read_b128 %7, %8 offset:3584\n\t"
+        "ds_read_b128 %4, %8 offset:2048\n\tds_read_b128 %5, %8 offset:2560\n\tds_read_b128 %6, %8 offset:0xc00\n\tds_read_b128 %7, %8 offset:3584\n\t"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
         : "v"(at)
@@ -379,7 +379,7 @@ __device__ __forceinline__ void read_rows64(uint32_t at, u32x4* r)
 {
     asm volatile(
         "ds_read_b128 %0, %16\n\tds_read_b128 %1, %16 offset:512\n\tds_read_b128 %2, %16 offset:1024\n\tds_read_b128 %3, %16 offset:1536\n\t"
-        "ds_read_b128 %4, %16 offset:2048\n\tds_read_b128 %5, %16 offset:2560\n\tds_read_b128 %6, %16 offset:3072\n\tds_read_b128 %7, %16 offset:3584\n\t"
+        "ds_read_b128 %4, %16 offset:2048\n\tds_read_b128 %5, %16 offset:2560\n\tds_read_b128 %6, %16 offset:0xc00\n\tds_read_b128 %7, %16 offset:3584\n\t"
         "ds_read_b128 %8, %16 offset:8192\n\tds_read_b128 %9, %16 offset:8704\n\tds_read_b128 %10, %16 offset:9216\n\tds_read_b128 %11, %16 offset:9728\n\t"
         "ds_read_b128 %12, %16 offset:10240\n\tds_read_b128 %13, %16 offset:10752\n\tds_read_b128 %14, %16 offset:11264\n\tds_read_b128 %15, %16 offset:11776\n\t"
         "s_waitcnt lgkmcnt(0)"

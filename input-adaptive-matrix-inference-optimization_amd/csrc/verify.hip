@@ -333,7 +333,7 @@ __device__ __forceinline__ void weights_of(const VerifyArgs& a, const Draw& d, c
 // Which drafted tokens of a sequence are kept, by every workgroup of it: the rows'
 // segments joined by `width` lanes a row, all rows at once where they
 // are few, then lane i judges token i.  p, q: LDS
-__device__ __forceinline__ int judge(const VerifyArgs& a, int s, int n, Joined* p, Joined* q)
+__device__ __forceinline__ int kept_of(const VerifyArgs& a, int s, int n, Joined* p, Joined* q)
 {
     const int tid = threadIdx.x, lane = tid & 63;
     const int* tokens = a.tokens + (size_t)s * a.n;
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(kVerThreads, 4) void k_verify_pick(VerifyArgs a)
     const int n = drafts_of(a, s), parts = a.draw_segs * kVerWaves;
     const double share = (double)a.uniform[(size_t)s * (a.n + 1) + a.n];
     fill_table(&table);
-    const int kept = judge(a, s, n, p, q);
+    const int kept = kept_of(a, s, n, p, q);
     const Joined pk = p[kept];
     const int* tokens = a.tokens + (size_t)s * a.n;
     int follow = -1;
