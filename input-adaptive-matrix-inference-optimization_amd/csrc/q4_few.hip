@@ -8,6 +8,7 @@
 // columns are the rows' digits: three of a float row (22 bits of the tile's
 // largest value and its sign), one of an int8 row.  4-bit weights become bytes
 // with three instructions for eight of them, and what one row costs, five cost too.
+#include "accum.h"
 #include "q4_mul.h"
 
 namespace iam {
@@ -15,10 +16,15 @@ namespace iam {
 struct FewArgs {
     MulArgs u;
     int waves;      // of a workgroup
+    // the inputs cut into parts for more workgroups, whose sums the last one to arrive joins
+    int splits;
+    float* sums;
+    uint32_t* ctr;  // zero on entry (left zero)
 };
 
 constexpr int kFewMaxWaves = 16;
 constexpr int kFewCols = 16;
+constexpr int kFewSplits = 8;
 
 // A strip's words of a chunk, its scales and zero points, in a lane's registers.
 template <int GROUP, bool ZEROS>
@@ -86,7 +92,8 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
     extern __shared__ uint4 lds[];
     const MulArgs& u = a.u;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c = lane & 15;
-    const int strip0 = xcd_remap(blockIdx.x, gridDim.x) * S, last = q4_strips(u.m.out) - 1, cols = u.rows * D;
+    const int last = q4_strips(u.m.out) - 1, groups = (last + S) / S, id = xcd_remap(blockIdx.x, gridDim.x);
+    const int split = id / groups, group = id - split * groups, strip0 = group * S, cols = u.rows * D;
     uint4* digits = lds + wave * (32 * cols);                                       // [tile][step][g][col] 16 bytes
     float* factor = reinterpret_cast<float*>(lds + a.waves * (32 * cols)) + wave * 4 * kFewCols;   // [tile][row]
     const int col = min(c, cols - 1), mine = col / D;
@@ -94,7 +101,7 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
 #pragma unroll
     for (int s = 0; s < S; s++) acc[s] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     FewWeights<GROUP, ZEROS> now;
-    for (int chunk = wave; chunk < u.m.chunks; chunk += a.waves) {
+    for (int chunk = split * a.waves + wave; chunk < u.m.chunks; chunk += a.splits * a.waves) {
         const int t16 = lane >> 4, k8 = lane & 15, k = chunk * kChunk + t16 * kTile + k8 * 8;
         Raw8 raw = load_raw8(u.x, u.x_type, 0, k, u.m.in);
         float xs = D == 1 || u.x_scale ? u.x_scale[u.x_groups > 1 ? min(chunk * 4 + t16, u.x_groups - 1) : 0] : 1.0f;
@@ -203,8 +210,14 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
 #pragma unroll
         for (int s = 0; s < S; s++) *reinterpret_cast<floatx4*>(part + ((wave * S + s) * cols + c) * 16 + 4 * g) = acc[s];
     __syncthreads();
-    for (int i = tid; i < S * u.rows * 16; i += a.waves * 64) {
-        const int r = i / (S * 16), s = i / 16 % S, o = (strip0 + s) * kStrip + (i & 15);
+    const int values = S * u.rows * 16;
+    auto put = [&](int i, float y) {
+        const int r = i / (S * 16), o = (strip0 + i / 16 % S) * kStrip + (i & 15);
+        if (o < u.m.out) put_value(u.y, u.y_type, (size_t)r * u.y_stride + o, y);
+    };
+    float* sums = a.sums + (size_t)group * a.splits * values;
+    for (int i = tid; i < values; i += a.waves * 64) {
+        const int r = i / (S * 16), s = i / 16 % S;
         float y = 0.0f;
 #pragma unroll
         for (int d = D - 1; d >= 0; d--) {
@@ -212,7 +225,20 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
             for (int w = 0; w < a.waves; w++) sum += part[((w * S + s) * cols + r * D + d) * 16 + (i & 15)];
             y = __builtin_fmaf(y, 256.0f, sum);
         }
-        if (o < u.m.out) put_value(u.y, u.y_type, (size_t)r * u.y_stride + o, y);
+        if (a.splits == 1) put(i, y);
+        else acc_put(sums + split * values + i, y);
+    }
+    if (a.splits == 1) return;
+    __shared__ int arrived;
+    if (!acc_arrive(a.ctr + group, (uint32_t)a.splits, &arrived)) return;
+    if (tid == 0) a.ctr[group] = 0u;
+    for (int i = tid; i < values; i += a.waves * 64) {
+        float each[kFewSplits], y = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kFewSplits; q++) each[q] = acc_peek(sums + min(q, a.splits - 1) * values + i);
+#pragma unroll
+        for (int q = 0; q < kFewSplits; q++) y += q < a.splits ? each[q] : 0.0f;
+        put(i, y);
     }
 }
 
@@ -224,7 +250,7 @@ static int few_launch(Ctx* c, const FewArgs& a)
 {
     const int cols = a.u.rows * D;
     const size_t stage = (size_t)a.waves * (32 * cols * 16 + 4 * kFewCols * 4), join = (size_t)a.waves * S * cols * 64;
-    const dim3 grid((unsigned)((q4_strips(a.u.m.out) + S - 1) / S)), block((unsigned)a.waves * 64);
+    const dim3 grid((unsigned)((q4_strips(a.u.m.out) + S - 1) / S * a.splits)), block((unsigned)a.waves * 64);
     return a.u.m.zeros ? launch(c, "q4_mul.few", k_q4_few<D, GROUP, true, S>, grid, block, std::max(stage, join), a)
                        : launch(c, "q4_mul.few", k_q4_few<D, GROUP, false, S>, grid, block, std::max(stage, join), a);
 }
@@ -257,8 +283,21 @@ int q4_mul_few(Ctx* c, const MulArgs& u)
     // A wave for each chunk, as many as 160 KB of LDS hold digits of (512 bytes
     // a column and 256 of factors each).
     const int most = std::min(kFewMaxWaves, (160 * 1024) / (512 * cols + 256));
-    const int rounds = (u.m.chunks + most - 1) / most;
-    const FewArgs a{u, (u.m.chunks + rounds - 1) / rounds};
+    FewArgs a{};
+    a.u = u;
+    // Where a workgroup's waves would take several turns the inputs are cut, for
+    // about a workgroup a CU (four fp32 rows, 1024 x 14336: 11.0 us whole, 8.6 cut;
+    // 1024 x 8192 in one turn 7.2 and 7.2; one row of 1024 x 14336 7.3 and 6.6, but 7.7
+    // and 8.1 of 2048 x 14336 in two).
+    const int strips = q4_strips(u.m.out), fit = 256 / strips;
+    a.splits = u.m.chunks > most && fit > (u.rows > 1 ? 1 : 2) ? std::min({fit, kFewSplits, u.m.chunks / 4}) : 1;
+    if (a.splits > 1) {
+        IAM_TRY(ensure_q4_sums(c, (size_t)strips * a.splits * u.rows * kStrip, (size_t)strips));
+        a.sums = c->q4_sums;
+        a.ctr = c->q4_ctr;
+    }
+    const int each = (u.m.chunks + a.splits - 1) / a.splits, rounds = (each + most - 1) / most;
+    a.waves = (each + rounds - 1) / rounds;
     return u.x_type == IAM_I8 ? few_grouped<1>(c, a) : few_grouped<3>(c, a);
 }
 

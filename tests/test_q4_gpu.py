@@ -150,6 +150,14 @@ def test_workgroups_for_every_unit(iam, ctx, type, x_group, group, zeros):
     check(iam, ctx, np.random.default_rng(group), 2040, 300, 4090, group, zeros, type, "f32" if zeros else "bf16", x_group, y_stride=4095)
 
 
+@pytest.mark.parametrize("type", ["f32", "f16", "int8", "e4m3"])
+@pytest.mark.parametrize("rows,inp,out", [(1, 14336, 200), (5, 9000, 130), (3, 20000, 1500), (2, 8193, 17), (4, 70001, 16)])
+def test_few_rows_of_long_inputs(iam, ctx, rows, inp, out, type):
+    rng = np.random.default_rng(rows + inp)
+    for k in range(2):     # the counters are left as they were
+        check(iam, ctx, rng, rows, inp, out, (32, 64, 128)[(rows + k) % 3], k == 1, type, "f32", 128 * k if type not in P.TYPES else 0)
+
+
 def test_many_rows_and_outputs(iam, ctx):
     """More rows than a pass takes, more strips than a launch packs."""
     rng = np.random.default_rng(9)
