@@ -177,8 +177,9 @@ __device__ __forceinline__ void gain_eight(const NormArgs& a, int i, const float
 }
 
 // A workgroup takes a row, which stays in its registers: J runs of 8 values a
-// thread.  Bound by memory where there are many rows; one row by the two
-// reductions.
+// thread.  Bound by memory where there are many rows (4096 of 4096, bf16 on an fp32
+// residual that is kept, to e4m3: 43 us, 4.3 TB/s); one row by the launch and the
+// two reductions (4.5 us).
 template <typename X, typename R, int J>
 __global__ __launch_bounds__(kNormMaxThreads) void k_rmsnorm_rows(NormArgs a)
 {

