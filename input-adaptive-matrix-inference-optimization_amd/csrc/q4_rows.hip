@@ -621,12 +621,15 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
         }
         if constexpr (GT == 1) {
             // the widening of the next inputs and the sums of the last pair between
-            // the matrix instructions (smaller groups would spill)
+            // the matrix instructions (smaller groups would spill); with 8 for 7 4096 rows
+            // of 14336 x 4096 took 481 us for 478, with 14 for 11 389 int8 rows 28.5 for 27.5,
+            // with 11 for 14 4096 of them 328 for 309
+            constexpr int BETWEEN = !G::BYTE ? 7 : NB == 2 ? 11 : 14;
             __builtin_amdgcn_sched_group_barrier(0x2, 20, 0);
 #pragma unroll
             for (int i = 0; i < 2 * OPS * N * P; i++) {
                 __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x2, G::BYTE ? 14 : 8, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, BETWEEN, 0);
             }
         }
         if constexpr (!SECOND) arrived();
