@@ -596,8 +596,9 @@ int iam_rows8_read(iam_ctx* ctx, const void* x_dev, int type, size_t stride, con
  * A row of the target with a NaN, a +inf or nothing but -inf has no
  * distribution: its token is rejected, and the one that follows is -1.  Where
  * the draft's row has none the token is rejected and the next is drawn from p,
- * as it is where p - q is nowhere positive.  temperatures are 2^-64 to 2^64
- * (or 0, as above); n_draft 0 .. 64; random numbers lie in [0, 1). */
+ * as it is where p - q is nowhere positive (where its positive parts add up to
+ * less than 1e-12: fp64's rounding).  temperatures are 2^-64 to 2^64 (or 0, as
+ * above); n_draft 0 .. 64; random numbers lie in [0, 1). */
 #define IAM_VERIFY_MAX_DRAFT 64
 int iam_verify_drafts(iam_ctx* ctx, const void* target_dev, int target_type, size_t target_stride,
                       const void* draft_dev, int draft_type, size_t draft_stride, int n_seq, int n_draft, int vocab,

@@ -15,6 +15,10 @@ namespace iam {
 
 constexpr int kVerThreads = 256, kVerWaves = 4;
 constexpr int kVerMaxSegs = 64;
+// p - q counts as nowhere positive where its positive parts add up to less: each
+// of p and q is off by 2e-13 of itself at most (the exponentials' 4e-14, and
+// fp64 sums in an order that depends on where a row lies)
+constexpr double kNowhere = 1e-12;
 
 // One kind of rows of logits (the target's, or the draft's)
 struct Rows {
@@ -321,8 +325,9 @@ __device__ __forceinline__ void weights_of(const VerifyArgs& a, const Draw& d, c
         const Base q(a.draft.unit, d.qm);
 #pragma unroll
         for (int e = 0; e < E; e++) {
+            // rounded like p (no fma): equal rows leave 0, not p's rounding error
             const ExpParts t = q.weight(table, u[e]);
-            w[e] = fmax(__builtin_fma(t.p * t.e, -d.qz, w[e]), 0.0);
+            w[e] = fmax(w[e] - t.p * t.e * d.qz, 0.0);
         }
     } else if (d.less) {
 #pragma unroll
@@ -456,8 +461,8 @@ __global__ __launch_bounds__(kVerThreads, 4) void k_verify_pick(VerifyArgs a)
             return sum;
         };
         double whole = take(), upto = wave_scan(whole);
-        if (d.less && !(__shfl(upto, 63) > 0.0)) {
-            // nowhere positive: p alone (seldom, if ever)
+        if (d.less && !(__shfl(upto, 63) > kNowhere)) {
+            // nowhere positive: p alone (a token that neither row gives any probability)
             d.less = false;
             __syncthreads();
             for (int i = 0; i < a.draw_segs; i++) {

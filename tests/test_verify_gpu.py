@@ -200,6 +200,28 @@ def test_calls_repeat(ctx):
         assert all(np.array_equal(a, b) for a, b in zip(first, again))
 
 
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("stride,draft_stride", [(0, 0), (1, 3)])
+@pytest.mark.parametrize("vocab", [9, 1000, 4000, 40000])
+def test_rejected_where_the_distributions_are_equal(ctx, vocab, stride, draft_stride, type):
+    """A token that both rows give no probability: p - q is 0 everywhere, however
+    the two rows lie in memory, and the next token is drawn from p."""
+    rng = np.random.default_rng(vocab)
+    S, n = 24, 2
+    x = rng.normal(0, 1.5, (S, n + 1, vocab))
+    x[::2, :, rng.integers(0, vocab, 8)] += 6
+    x[S // 2:] = np.round(x[S // 2:])                          # many equal ones
+    t = np.stack([rng.permutation(vocab)[:n] for _ in range(S)])
+    x[np.arange(S)[:, None], np.arange(n)[None], t] = -np.inf
+    u = rng.random((S, n + 1)).astype(np.float32)
+    _, acc = check(ctx, x, x[:, :n].copy(), t, None, u, 1.0, type=type, draft_type=type, stride=vocab + stride if stride else 0,
+                   draft_stride=vocab + draft_stride if draft_stride else 0)
+    assert (acc == 0).all()
+    if type == "f32":
+        # the same distributions at other temperatures
+        check(ctx, x, 4 * P.to_type(x[:, :n], "f32")[1], t, None, u, 0.7, draft_temperature=2.8, stride=vocab + stride if stride else 0)
+
+
 def test_refusals(iam, ctx):
     x, y = ctx.empty(2 * 4 * 100, np.float32), ctx.empty(2 * 3 * 100, np.float32)
     t, u, c, o, a = ctx.upload(np.zeros(6, np.int32)), ctx.upload(np.zeros(8, np.float32)), ctx.upload(np.zeros(2, np.int32)), ctx.empty(8, np.int32), ctx.empty(2, np.int32)
