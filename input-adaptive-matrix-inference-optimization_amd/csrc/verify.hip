@@ -416,7 +416,7 @@ __global__ __launch_bounds__(kVerThreads, 4) void k_verify_pick(VerifyArgs a)
     __shared__ ExpTable table;
     __shared__ Joined p[IAM_VERIFY_MAX_DRAFT + 1], q[IAM_VERIFY_MAX_DRAFT];
     __shared__ double sums[kVerWaves], part[kVerMaxSegs * kVerWaves];
-    __shared__ int last, picked;
+    __shared__ int last, found[kVerWaves];
     const int s = blockIdx.x / a.draw_segs, seg = blockIdx.x - s * a.draw_segs, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int n = drafts_of(a, s), parts = a.draw_segs * kVerWaves;
     const double share = (double)a.uniform[(size_t)s * (a.n + 1) + a.n];
@@ -450,7 +450,6 @@ __global__ __launch_bounds__(kVerThreads, 4) void k_verify_pick(VerifyArgs a)
         } else if (lane == 0) {
             part[wave] = sum;
         }
-        if (tid == 0) picked = -1;
         __syncthreads();
         // lane i: segment i
         double own[kVerWaves];
@@ -475,8 +474,10 @@ __global__ __launch_bounds__(kVerThreads, 4) void k_verify_pick(VerifyArgs a)
         }
         const double want = share * __shfl(upto, 63);
         // the segment, then the part, in which the sum passes it (by rounding none:
-        // the last of any weight)
-        const uint64_t past = __ballot(upto > want), some = __ballot(whole > 0.0);
+        // the last of any weight).  Of those with any weight: the scan adds in a tree,
+        // and behind the border a weightless one's sum may differ from the one before
+        // by rounding.
+        const uint64_t past = __ballot(whole > 0.0 && upto > want), some = __ballot(whole > 0.0);
         const int at = past ? __ffsll((unsigned long long)past) - 1 : some ? 63 - __clzll((long long)some) : 0;
         const double left = __shfl(upto, max(at - 1, 0));
         double before = at ? left : 0.0, sofar = before;
@@ -505,33 +506,31 @@ __global__ __launch_bounds__(kVerThreads, 4) void k_verify_pick(VerifyArgs a)
             __syncthreads();
             if (lane == 63) sums[wave] = incl;
             __syncthreads();
-            int hit = 0;
-            for (; hit < kVerWaves; hit++) {
-                if (before + sums[hit] > want) break;
-                before += sums[hit];
-            }
-            if (hit == kVerWaves) continue;
-            if (wave == hit) {
-                // the first lane whose sum passes it: lane 63's does
-                const uint64_t over = __ballot(before + incl > want);
-                const double left = __shfl_up(incl, 1);
-                if (lane == __ffsll((unsigned long long)over) - 1) {
-                    double c = before + (lane ? left : 0.0);
-                    int place = -1;
+            // each wave's first lane of any weight whose sum passes it, then the first wave's
+            double start = before;
+            for (int i = 0; i < wave; i++) start += sums[i];
+            const uint64_t over = __ballot(run > 0.0 && start + incl > want);
+            const double left = __shfl_up(incl, 1);
+            if (lane == (over ? __ffsll((unsigned long long)over) - 1 : 0)) {
+                double c = start + (lane ? left : 0.0);
+                int place = -1;
 #pragma unroll
-                    for (int e = 0; e < kLast; e++) {
-                        if (w[e] > 0.0 && (place < 0 || !(c > want))) place = i0 + e;
-                        c += w[e];
-                    }
-                    picked = place;
+                for (int e = 0; e < kLast; e++) {
+                    if (w[e] > 0.0 && (place < 0 || !(c > want))) place = i0 + e;
+                    c += w[e];
                 }
+                found[wave] = over ? place : -1;
             }
-            break;
+            __syncthreads();
+            for (int i = 0; i < kVerWaves; i++) {
+                if (follow < 0) follow = found[i];
+                before += sums[i];
+            }
+            if (follow >= 0) break;
         }
-        __syncthreads();
-        follow = picked;
         if (follow < 0) {
             const uint32_t most = wave_max_u32((uint32_t)(mine + 1));
+            __syncthreads();
             if (lane == 0) sums[wave] = (double)most;
             __syncthreads();
             double best = 0.0;

@@ -222,6 +222,27 @@ def test_rejected_where_the_distributions_are_equal(ctx, vocab, stride, draft_st
         check(ctx, x, 4 * P.to_type(x[:, :n], "f32")[1], t, None, u, 0.7, draft_temperature=2.8, stride=vocab + stride if stride else 0)
 
 
+@pytest.mark.parametrize("vocab,span", [(600, 512), (2041, 300), (9000, 9000)])
+def test_borders_behind_masked_tokens(ctx, vocab, span):
+    """Equal logits among masked ones and random numbers on their borders: by
+    rounding the token on one side of the border or the other, and no third."""
+    rng = np.random.default_rng(1)
+    x, u, sides = [], [], []
+    for count in (3, 6, 12, 20, 24, 28, 40, 48, 56, 80, 88, 96, 100, 200):
+        for _ in range(8):
+            at = np.sort(rng.choice(span, count, replace=False))
+            row = np.full(vocab, -np.inf)
+            row[at] = 1.5
+            for j in range(1, count):
+                if float(np.float32(j / count)) * count == j:
+                    x.append(row)
+                    u.append(j / count)
+                    sides.append((at[j - 1], at[j]))
+    x, S = np.array(x)[:, None], len(x)
+    out = run(ctx, x, None, np.zeros((S, 0)), None, np.array(u, np.float32)[:, None], 1.0)[2][:, 0]
+    assert ((out[:, None] == np.array(sides)).any(1)).all()
+
+
 def test_refusals(iam, ctx):
     x, y = ctx.empty(2 * 4 * 100, np.float32), ctx.empty(2 * 3 * 100, np.float32)
     t, u, c, o, a = ctx.upload(np.zeros(6, np.int32)), ctx.upload(np.zeros(8, np.float32)), ctx.upload(np.zeros(2, np.int32)), ctx.empty(8, np.int32), ctx.empty(2, np.int32)
