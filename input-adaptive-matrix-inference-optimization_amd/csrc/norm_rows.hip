@@ -105,7 +105,14 @@ __device__ __forceinline__ float to_odd(double q)
     if (e != 0.0 && !(b & 1)) b += (e > 0.0) == (q > 0.0) ? 1 : -1;
     return __int_as_float(b);
 }
-__device__ __forceinline__ uint32_t e4m3_of(double q) { return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(to_odd(q), 0.0f, 0, false) & 0xffu; }
+// (a scale of a few of the smallest fp32 numbers may be rounded to two thirds of what
+// it should be: quotients then lie past the largest number, which the
+// conversion would answer with NaN)
+__device__ __forceinline__ uint32_t e4m3_of(double q)
+{
+    const float f = __builtin_amdgcn_fmed3f(to_odd(q), -448.0f, 448.0f);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f, 0.0f, 0, false) & 0xffu;
+}
 __device__ __forceinline__ uint32_t int8_of(double q) { return (uint32_t)(int)rint(fmin(fmax(q, -127.0), 127.0)) & 0xffu; }
 
 // the numbers of eight values, at p + i of a row of n

@@ -175,6 +175,20 @@ def test_ties_of_the_numbers(ctx):
         assert np.array_equal(R.values8(b, out_type)[0], P.numbers(steps, out_type))
 
 
+@pytest.mark.parametrize("out_type", ["int8", "e4m3"])
+@pytest.mark.parametrize("group", [0, 128])
+def test_subnormal_scales(ctx, out_type, group):
+    """Groups whose scale is a few of the smallest fp32 numbers: quotients up to
+    1.5 times the largest number."""
+    rng = np.random.default_rng(4)
+    x = np.zeros((12, 260))
+    for r, top in enumerate((60, 64, 100, 190, 200, 300, 600, 671, 672, 1000, 1500, 5000)):
+        x[r] = rng.integers(-top, top + 1, 260)
+        x[r, 5], x[r, 130] = top, -top
+    # eps 1 is all of the root: y = x
+    check(ctx, x * 2.0 ** -149, "f32", out_type=out_type, group=group, eps=1.0)
+
+
 def test_refusals(iam, ctx):
     x, r, s, out = (ctx.empty(4 * 100, np.float32) for _ in range(4))
     g, sc = ctx.empty(100, np.uint16), ctx.empty(4, np.float32)
