@@ -97,12 +97,13 @@ __device__ __forceinline__ double quotient(double y, double s, double r)
     return __builtin_fma(__builtin_fma(-q, s, y), r, q);
 }
 // q rounded to fp32 to odd: one more rounding to fewer bits is then right
+// (infinities and NaN, whose e is NaN, as they are)
 __device__ __forceinline__ float to_odd(double q)
 {
     const float f = (float)q;
     const double e = q - (double)f;
     int b = __float_as_int(f);
-    if (e != 0.0 && !(b & 1)) b += (e > 0.0) == (q > 0.0) ? 1 : -1;
+    if (fabs(e) > 0.0 && !(b & 1)) b += (e > 0.0) == (q > 0.0) ? 1 : -1;
     return __int_as_float(b);
 }
 // (a scale of a few of the smallest fp32 numbers may be rounded to two thirds of what

@@ -189,6 +189,18 @@ def test_subnormal_scales(ctx, out_type, group):
     check(ctx, x * 2.0 ** -149, "f32", out_type=out_type, group=group, eps=1.0)
 
 
+@pytest.mark.parametrize("out_type", P.TYPES)
+@pytest.mark.parametrize("dim", [60, 70001])
+def test_infinite_gains(ctx, out_type, dim):
+    rng = np.random.default_rng(5)
+    x = rng.normal(0, 1, (3, dim))
+    gain = np.ones(dim)
+    gain[3:40:2], gain[4:40:4] = np.inf, -np.inf
+    y = run(ctx, x, "f32", gain=gain, out_type=out_type)[3]
+    at = np.isinf(gain)
+    assert np.array_equal(y[:, at], np.sign(x[:, at]) * gain[at]) and np.isfinite(y[:, ~at]).all()
+
+
 def test_refusals(iam, ctx):
     x, r, s, out = (ctx.empty(4 * 100, np.float32) for _ in range(4))
     g, sc = ctx.empty(100, np.uint16), ctx.empty(4, np.float32)
