@@ -421,8 +421,8 @@ int iam_rmsnorm_rows(iam_ctx* c, const void* x, int type, size_t x_stride, const
         IAM_TRY(check_dev_range(c, part[i].p, part[i].bytes, part[i].what));
         for (int j = 0; j < i; j++) {
             if (!part[j].p || !part[j].written) continue;
-            const bool in_place = (part[i].p == r && part[j].p == sum && sum == r) ||
-                                  (part[i].p == x && part[j].p == out && out == x && out_type == type && out_stride == x_stride);
+            // the residual's sum where the residual was, y where x was
+            const bool in_place = (i == 4 && j == 1 && sum == r) || (i == 3 && j == 0 && out == x && out_type == type && out_stride == x_stride);
             IAM_REQUIRE(in_place || !overlaps(part[i].p, part[i].bytes, part[j].p, part[j].bytes),
                         "rmsnorm_rows: an output overlaps another array");
         }

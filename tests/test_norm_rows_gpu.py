@@ -201,6 +201,20 @@ def test_infinite_gains(ctx, out_type, dim):
     assert np.array_equal(y[:, at], np.sign(x[:, at]) * gain[at]) and np.isfinite(y[:, ~at]).all()
 
 
+def test_refused_overlaps_of_inputs(iam, ctx):
+    """x and the residual may be one array, but then neither is written over."""
+    x, s, out = (ctx.empty(4 * 100, np.float32) for _ in range(3))
+    g = ctx.empty(100, np.uint16)
+    ok = dict(x=x, type="f32", n_rows=2, dim=100, gain=g, eps=EPS, out=out, out_type="f32", residual=x, residual_type="f32", sum=s)
+    ctx.rmsnorm_rows(**ok)
+    for bad in (dict(sum=x), dict(sum=x, x_stride=200), dict(out=x), dict(out=x, residual_stride=200), dict(sum=x, type="f16", x_stride=200), dict(out=x, out_type="f16", type="f16")):
+        with pytest.raises(iam.IamError) as e:
+            ctx.rmsnorm_rows(**dict(ok, **bad))
+        assert e.value.code == iam.IAM_E_INVALID, bad
+    for b in (x, s, out, g):
+        b.free()
+
+
 def test_refusals(iam, ctx):
     x, r, s, out = (ctx.empty(4 * 100, np.float32) for _ in range(4))
     g, sc = ctx.empty(100, np.uint16), ctx.empty(4, np.float32)
