@@ -6,8 +6,9 @@
 // bf16 of a tile of 128 after a power of two where its largest value lies outside
 // [2^-2, 2^15)), two, high and low, of fp32 (22 bits).  4-bit weights become fp16 under the exponents of
 // 1024 and 64, n - zero exactly.  Products are then exact; a group's are added
-// in fp32 by the instructions and go to the row's sum with the group's scale
-// times that power (together first: a sum of large x alone may pass fp32).
+// in fp32 by the instructions and go to the row's sum with the group's scale and
+// that power: times the scale first, as a sum of large x times the power alone
+// may pass fp32's range, and so may the two together at either end.
 #include "accum.h"
 #include "q4_mul.h"
 
@@ -22,7 +23,12 @@ typedef unsigned long long ull2 __attribute__((ext_vector_type(2)));
 //        32 j + 8 g and on of the tile.  Or int8 [block of 16 rows][tile][j][lane
 //        16 half + row][16]: eight inputs from 32 j + 8 half on, eight from 16 further on
 // factor fp32 [block][tile][16]: what the tile's values were divided by
-// scaled [block][tile]: whether any of these is not 1
+// scaled [block][tile]: kScaled if any of these is not 1, kFar too if one is far from it
+constexpr uint8_t kScaled = 1, kFar = 2;
+// A factor up to 2^64 times a weights' scale (below 2^16) and a sum (up to 2^22 a
+// tile, 2^13 tiles) stays in fp32's range, and one from 2^-100 on times a scale
+// (from 2^-24 on) keeps its bits.
+__device__ __forceinline__ bool is_far(float f) { return f != 0.0f && !(fabsf(f) >= 0x1p-100f && fabsf(f) <= 0x1p64f); }
 struct PrepArgs {
     const void* x;
     int type;
@@ -92,8 +98,8 @@ __global__ __launch_bounds__(kPrepThreads) void k_q4_prep(PrepArgs a)
     }
     const size_t cell = (size_t)block * a.tiles + tile;
     if (g == 0) a.factor[cell * 16 + c] = f;
-    const bool scaled = __any(f != 1.0f);
-    if (lane == 0) a.scaled[cell] = scaled;
+    const bool scaled = __any(f != 1.0f), far = __any(is_far(f));
+    if (lane == 0) a.scaled[cell] = (scaled ? kScaled : 0) | (far ? kFar : 0);
 }
 
 // ---- the products
@@ -269,7 +275,7 @@ __global__ __launch_bounds__(64 * MOST) void k_q4_batch(RowsArgs a)
 #pragma unroll
                         for (int p = 0; p < PARTS; p++) d = mfma_f16(wide[j], o.x[p][n][j], d);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[s][n][e] = __builtin_fmaf(d[e], o.f[n] * (float)o.sc[s][i][e], acc[s][n][e]);
+                    for (int e = 0; e < 4; e++) acc[s][n][e] = __builtin_fmaf(d[e] * (float)o.sc[s][i][e], o.f[n], acc[s][n][e]);
                 }
             }
         }
@@ -443,11 +449,15 @@ __device__ __forceinline__ void read_scales(uint32_t at, u32x4* s)
 }
 __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
 
-// Tiles of a workgroup's products, with x's factors or (they are all 1) without.
-// The two are loops of their own: no branch may lie between a matrix
+// Tiles of a workgroup's products, without x's factors (they are all 1), with
+// their products with the weights' scales, or with the two apart (some are far
+// from 1; 4096 int8 rows of 14336 x 4096 in tiles of their own scale: 383 us, 361 with
+// the products, which need not wait for the matrix instructions).
+// Each is a loop of its own: no branch may lie between a matrix
 // instruction and its results' first use, where the compiler leaves out the
 // wait states of the edge that jumps.
-template <int PARTS, int GROUP, int NB, int WO, int STAGES, bool FACTORS, bool SECOND>
+enum class Factors { none, with_scales, apart };
+template <int PARTS, int GROUP, int NB, int WO, int STAGES, Factors FACTORS, bool SECOND>
 __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP, NB, WO, STAGES>& stage, int s0, int b0, int t0, int t1, floatx16 (&acc)[2][NB / 2])
 {
     typedef Gemm<PARTS, GROUP, NB, WO, STAGES> G;
@@ -512,7 +522,7 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
 #pragma unroll
         for (int n = 0; n < N; n++) f[n] = a.factor[((size_t)min(b0 + wx * NB + 2 * n + side, a.blocks - 1) * u.m.tiles + t) * 16 + c];
     };
-    if constexpr (FACTORS) load_factors(t0);
+    if constexpr (FACTORS != Factors::none) load_factors(t0);
 #pragma unroll
     for (int t = 0; t < STAGES - 1; t++) fetch(min(t0 + t, t1 - 1), t);
     int buf = 0, free_buf = STAGES - 1;
@@ -539,7 +549,7 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
         // Every wave's loads of this tile have arrived, and every wave has read
         // the tile before, whose place the newest tile takes.
         float fn[N];
-        if constexpr (FACTORS) {
+        if constexpr (FACTORS != Factors::none) {
 #pragma unroll
             for (int n = 0; n < N; n++) fn[n] = f[n];
             load_factors(min(t + 1, t1 - 1));
@@ -613,7 +623,11 @@ __device__ __forceinline__ void gemm_tiles(const RowsArgs& a, Gemm<PARTS, GROUP,
                         float v = (float)d[0][n][e];
                         if constexpr (P == 2) v += d[1][n][e];
                         float by = (float)scale[e % 8];
-                        if constexpr (FACTORS) by *= fn[n];
+                        if constexpr (FACTORS == Factors::with_scales) by *= fn[n];
+                        if constexpr (FACTORS == Factors::apart) {
+                            v *= PARTS == 0 ? by * 0.0625f : by;
+                            by = fn[n];
+                        }
                         acc[s][n][e] = __builtin_fmaf(v, by, acc[s][n][e]);
                     }
             }
@@ -646,6 +660,7 @@ __global__ __launch_bounds__(128 * WO, 2) void k_q4_gemm(RowsArgs a)
 {
     constexpr int S = kGemmStrips, STRIPS = S * WO;
     __shared__ Gemm<PARTS, GROUP, NB, WO, STAGES> stage;
+    __shared__ float rest;    // what the weights' 16 times leave to the end (in a register it cost 389 int8 rows 0.9 us)
     const MulArgs& u = a.u;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int strips = q4_strips(u.m.out);
@@ -657,21 +672,21 @@ __global__ __launch_bounds__(128 * WO, 2) void k_q4_gemm(RowsArgs a)
     const int xt = p0 + in_panel % width, ot = in_panel / width;
     const int s0 = ot * STRIPS, b0 = xt * 2 * NB;
     const int each = (u.m.tiles + a.splits - 1) / a.splits, t0 = split * each, t1 = min(t0 + each, u.m.tiles);
-    bool factors = false;
+    uint32_t factors = 0;
     if (a.scaled) {
-        bool mine = false;
-        for (int i = threadIdx.x; i < min(2 * NB, a.blocks - b0) * u.m.tiles; i += 128 * WO) mine |= a.scaled[(size_t)b0 * u.m.tiles + i] != 0;
+        uint32_t mine = 0;
+        for (int i = threadIdx.x; i < min(2 * NB, a.blocks - b0) * u.m.tiles; i += 128 * WO) mine |= a.scaled[(size_t)b0 * u.m.tiles + i];
         uint32_t* any = reinterpret_cast<uint32_t*>(&stage);   // nothing else is there yet
-        if (threadIdx.x < 2 * WO) any[threadIdx.x] = 0u;
-        __syncthreads();
-        if (__any(mine) && lane == 0) any[wave] = 1u;
+        mine = (__any(mine & kScaled) ? kScaled : 0u) | (__any(mine & kFar) ? kFar : 0u);
+        if (lane == 0) any[wave] = mine;
         __syncthreads();
         uint32_t all = 0;
 #pragma unroll
         for (int i = 0; i < 2 * WO; i++) all |= any[i];
-        factors = __builtin_amdgcn_readfirstlane(all) != 0;
+        factors = __builtin_amdgcn_readfirstlane(all);
         __syncthreads();
     }
+    if (PARTS == 0 && threadIdx.x == 0) rest = factors & kFar ? 1.0f : 0.0625f;
     floatx16 acc[2][NB / 2];
 #pragma unroll
     for (int s = 0; s < 2; s++)
@@ -680,12 +695,13 @@ __global__ __launch_bounds__(128 * WO, 2) void k_q4_gemm(RowsArgs a)
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[s][n][e] = 0.0f;
     auto tiles = [&](auto with_factors) __attribute__((always_inline)) {
-        constexpr bool F = decltype(with_factors)::value;
+        constexpr Factors F = decltype(with_factors)::value;
         if (WO == 4 && wave >= 4) gemm_tiles<PARTS, GROUP, NB, WO, STAGES, F, WO == 4>(a, stage, s0, b0, t0, t1, acc);
         else gemm_tiles<PARTS, GROUP, NB, WO, STAGES, F, false>(a, stage, s0, b0, t0, t1, acc);
     };
-    if (factors) tiles(std::true_type{});
-    else tiles(std::false_type{});
+    if (factors & kFar) tiles(std::integral_constant<Factors, Factors::apart>{});
+    else if (factors) tiles(std::integral_constant<Factors, Factors::with_scales>{});
+    else tiles(std::integral_constant<Factors, Factors::none>{});
     if (a.splits > 1) {
         // the splits' sums: [workgroup's place][split][four values][thread], past the
         // XCD's L2, joined in the splits' order by the last one to arrive
@@ -733,7 +749,7 @@ __global__ __launch_bounds__(128 * WO, 2) void k_q4_gemm(RowsArgs a)
 #pragma unroll
     for (int n = 0; n < NB / 2; n++) {
         const int r0 = (b0 + (wave & 1) * NB + 2 * n) * 16;
-        const float rs = (a.row_scale ? a.row_scale[min(r0 + (lane & 31), u.rows - 1)] : 1.0f) * (PARTS == 0 ? 0.0625f : 1.0f);
+        const float rs = (a.row_scale ? a.row_scale[min(r0 + (lane & 31), u.rows - 1)] : 1.0f) * (PARTS == 0 ? rest : 1.0f);
 #pragma unroll
         for (int s = 0; s < 2; s++)
 #pragma unroll

@@ -269,6 +269,33 @@ def test_quantize_not_finite(iam, ctx):
         b.free()
 
 
+@pytest.mark.parametrize("rows", [1, 5, 20, 140])
+@pytest.mark.parametrize("type", ["f32", "bf16", "int8", "e4m3"])
+def test_large_values_and_large_scales(iam, ctx, rows, type):
+    """Values near the largest under zero weights, beside others whose products
+    with scales of 2^15 stay small: a tile's power of two (or its scale) and
+    the weights' scale together pass fp32's range."""
+    rng = np.random.default_rng(9)
+    w = R.random_weights(rng, 40, 640, 64, False)
+    w.scale[:] = 2.0 ** 15
+    w.n[:] = 8
+    w.n[:, 3::64] = rng.integers(0, 16, (40, 10))
+    m = packed(iam, ctx, w)
+    own = np.arange(640) % 64 == 3
+    if type in P.TYPES:
+        words, v = P.to_type(rng.choice([-1, 1], (rows, 640)) * np.where(own, 2.0 ** 106, 2.0 ** 127), type)
+        scale = None
+    else:
+        q = np.where(own, rng.choice([-1, 1], (rows, 640)), 100 if type == "int8" else 96.0)
+        scale = np.full((rows, 5), 2.0 ** 106, np.float32)
+        scale[:, 1], q[:, 128 + 3:256:64] = 2.0 ** 127, 0
+        words, v = R.bytes_of(q, type), q * R.spread(scale, 128, 640)
+    got = product(ctx, m, words, scale, type, "f32", 0 if scale is None else 128)
+    m.free()
+    # whole multiples of 2^121, at most 80 of them in any sum of an output's
+    assert np.array_equal(got, v @ w.values().T)
+
+
 def test_refusals(iam, ctx):
     m = iam.Q4Matrix(ctx, 40, 300, 64)
     z = iam.Q4Matrix(ctx, 40, 300, 64, zeros=True)
