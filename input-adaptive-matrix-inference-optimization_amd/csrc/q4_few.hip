@@ -89,10 +89,11 @@ __device__ __forceinline__ uint32_t max16(uint32_t v)
 // each) while the first strip's weights are on their way (a strip's tile comes as
 // soon as the one before has been computed), and needs no other wave until the
 // sums are joined.
-template <int D, int GROUP, bool ZEROS, int S>
+template <int D, bool E4M3, int GROUP, bool ZEROS, int S>
 __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
 {
     extern __shared__ uint4 lds[];
+    constexpr bool SCALED = D == 1 || E4M3;
     const MulArgs& u = a.u;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int last = q4_strips(u.m.out) - 1, groups = (last + S) / S, id = xcd_remap(blockIdx.x, gridDim.x);
@@ -100,6 +101,11 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
     uint4* digits = lds + wave * (32 * cols);                                       // [tile][step][g][col] 16 bytes
     float* factor = reinterpret_cast<float*>(lds + a.waves * (32 * cols)) + wave * 4 * kFewCols;   // [tile][row]
     const int col = min(c, cols - 1), mine = col / D;
+    // What a tile's sums are times: the digit's place, less the weights' 16 and
+    // e4m3 numbers' 2^13.  (At the end alone, the sums of digits of the smallest
+    // results would be subnormal and those of the largest infinite.)  A power of
+    // two takes it exactly, a scale might not: 8-bit rows' sums are times it first.
+    const float place = ldexpf(1.0f, 8 * (col - mine * D) - (ZEROS ? 0 : 4) - (E4M3 ? 13 : 0));
     floatx4 acc[S];
 #pragma unroll
     for (int s = 0; s < S; s++) acc[s] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -107,7 +113,7 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
     for (int chunk = split * a.waves + wave; chunk < u.m.chunks; chunk += a.splits * a.waves) {
         const int t16 = lane >> 4, k8 = lane & 15, k = chunk * kChunk + t16 * kTile + k8 * 8;
         Raw8 raw = load_raw8(u.x, u.x_type, 0, k, u.m.in);
-        float xs = D == 1 || u.x_scale ? u.x_scale[u.x_groups > 1 ? min(chunk * 4 + t16, u.x_groups - 1) : 0] : 1.0f;
+        float xs = SCALED ? u.x_scale[u.x_groups > 1 ? min(chunk * 4 + t16, u.x_groups - 1) : 0] : 1.0f;
 #pragma unroll
         for (int t = 0; t < 4; t++) now.load(u.m, strip0, chunk, lane, t);
         uint2* to = reinterpret_cast<uint2*>(digits + ((t16 * 2 + (k8 >> 3)) * 4 + (k8 & 3)) * cols) + (k8 >> 2 & 1);
@@ -116,7 +122,7 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
             const float scale = xs;
             if (r + 1 < u.rows) {
                 raw = load_raw8(u.x, u.x_type, (size_t)(r + 1) * u.x_stride, k, u.m.in);
-                if (D == 1 || u.x_scale)
+                if constexpr (SCALED)
                     xs = u.x_scale[(size_t)(r + 1) * u.x_groups + (u.x_groups > 1 ? min(chunk * 4 + t16, u.x_groups - 1) : 0)];
             }
             if constexpr (D == 1) {
@@ -125,15 +131,17 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
                 if (k8 == 0) factor[t16 * kFewCols + r] = scale;
             } else {
                 float v[8];
-                values8(mine8, u.x_type, v);
+                values8(mine8, E4M3 ? IAM_E4M3 : u.x_type, v);
                 uint32_t top = 0;
 #pragma unroll
                 for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
                 top = max16(top);
                 // n = round(v 2^(148 - e)), below 2^22; 2^(e - 148) back (NaN
                 // where a value is not finite).  Tiles below 2^-102 count as if
-                // they were that large.
-                const uint32_t e8 = max(top >> 23, 24u);
+                // they were that large; e4m3 numbers, at most 448 and whole multiples
+                // of 2^-9, have one power, which goes to `place` so that the smallest
+                // scales keep their bits.
+                const uint32_t e8 = E4M3 ? 135u : max(top >> 23, 24u);
                 const float up = __uint_as_float((275u - e8) << 23);
                 uint32_t n[8];
 #pragma unroll
@@ -149,7 +157,7 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
                     at[2] = {__builtin_amdgcn_perm(a1, a0, 0x07060302u) ^ 0x80808080u, __builtin_amdgcn_perm(b1, b0, 0x07060302u) ^ 0x80808080u};
                     at[4] = {__builtin_amdgcn_perm(a3, a2, 0x05040100u) ^ 0x80808080u, __builtin_amdgcn_perm(b3, b2, 0x05040100u) ^ 0x80808080u};
                 }
-                if (k8 == 0) factor[t16 * kFewCols + r] = top >= 0x7f800000u ? NAN : __uint_as_float((e8 - 21u) << 23) * scale;
+                if (k8 == 0) factor[t16 * kFewCols + r] = top >= 0x7f800000u ? NAN : E4M3 ? scale : __uint_as_float((e8 - 21u) << 23);
             }
         }
         wave_sync();
@@ -159,7 +167,7 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 if (t < tiles) {
-                    const float f = factor[t * kFewCols + mine] * (ZEROS ? 1.0f : 0.0625f);
+                    const float f = SCALED ? factor[t * kFewCols + mine] : factor[t * kFewCols + mine] * place;
                     const uint32_t wd[4] = {now.w[t].x, now.w[t].y, now.w[t].z, now.w[t].w};
                     intx4 sum = {0, 0, 0, 0};
                     floatx4 part = {0.0f, 0.0f, 0.0f, 0.0f};   // of the tile, without f
@@ -199,7 +207,7 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[sn][i] = __builtin_fmaf(part[i], f, acc[sn][i]);
+                    for (int i = 0; i < 4; i++) acc[sn][i] = __builtin_fmaf(SCALED && !(D == 1 && ZEROS) ? part[i] * place : part[i], f, acc[sn][i]);
                 }
                 if (sn + 1 < S) now.load(u.m, min(strip0 + sn + 1, last), chunk, lane, t);
             }
@@ -226,7 +234,7 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
         for (int d = D - 1; d >= 0; d--) {
             float sum = 0.0f;
             for (int w = 0; w < a.waves; w++) sum += part[((w * S + s) * cols + r * D + d) * 16 + (i & 15)];
-            y = __builtin_fmaf(y, 256.0f, sum);
+            y += sum;
         }
         if (a.splits == 1) put(i, y);
         else acc_put(sums + split * values + i, y);
@@ -248,17 +256,17 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
 // ------------------------------------------------------------------ host ---
 int q4_few_most(int x_type) { return x_type == IAM_I8 ? kFewCols : kFewCols / 3; }
 
-template <int D, int GROUP, int S>
+template <int D, bool E4M3, int GROUP, int S>
 static int few_launch(Ctx* c, const FewArgs& a)
 {
     const int cols = a.u.rows * D;
     const size_t stage = (size_t)a.waves * (32 * cols * 16 + 4 * kFewCols * 4), join = (size_t)a.waves * S * cols * 64;
     const dim3 grid((unsigned)((q4_strips(a.u.m.out) + S - 1) / S * a.splits)), block((unsigned)a.waves * 64);
-    return a.u.m.zeros ? launch(c, "q4_mul.few", k_q4_few<D, GROUP, true, S>, grid, block, std::max(stage, join), a)
-                       : launch(c, "q4_mul.few", k_q4_few<D, GROUP, false, S>, grid, block, std::max(stage, join), a);
+    return a.u.m.zeros ? launch(c, "q4_mul.few", k_q4_few<D, E4M3, GROUP, true, S>, grid, block, std::max(stage, join), a)
+                       : launch(c, "q4_mul.few", k_q4_few<D, E4M3, GROUP, false, S>, grid, block, std::max(stage, join), a);
 }
 
-template <int D, int GROUP>
+template <int D, bool E4M3, int GROUP>
 static int few_sized(Ctx* c, const FewArgs& a)
 {
     // Several strips share the rows' digits, and a strip's weights come while the
@@ -268,16 +276,16 @@ static int few_sized(Ctx* c, const FewArgs& a)
     // 8192 x 8192 with groups of 128 11.0, 9.4 and 9.1, 6144 x 4096 5.7, 6.2 and 7.1).
     // Groups of 32 with zero points and four strips do not fit the registers (28672 x
     // 4096: 20.1, 17.4 and 23.0).
-    if (q4_strips(a.u.m.out) >= 512) return few_launch<D, GROUP, GROUP == 32 ? 2 : 4>(c, a);
-    return few_launch<D, GROUP, 1>(c, a);
+    if (q4_strips(a.u.m.out) >= 512) return few_launch<D, E4M3, GROUP, GROUP == 32 ? 2 : 4>(c, a);
+    return few_launch<D, E4M3, GROUP, 1>(c, a);
 }
 
-template <int D>
+template <int D, bool E4M3>
 static int few_grouped(Ctx* c, const FewArgs& a)
 {
-    if (a.u.m.group == 32) return few_sized<D, 32>(c, a);
-    if (a.u.m.group == 64) return few_sized<D, 64>(c, a);
-    return few_sized<D, 128>(c, a);
+    if (a.u.m.group == 32) return few_sized<D, E4M3, 32>(c, a);
+    if (a.u.m.group == 64) return few_sized<D, E4M3, 64>(c, a);
+    return few_sized<D, E4M3, 128>(c, a);
 }
 
 int q4_mul_few(Ctx* c, const MulArgs& u)
@@ -301,7 +309,8 @@ int q4_mul_few(Ctx* c, const MulArgs& u)
     }
     const int each = (u.m.chunks + a.splits - 1) / a.splits, rounds = (each + most - 1) / most;
     a.waves = (each + rounds - 1) / rounds;
-    return u.x_type == IAM_I8 ? few_grouped<1>(c, a) : few_grouped<3>(c, a);
+    if (u.x_type == IAM_I8) return few_grouped<1, false>(c, a);
+    return u.x_type == IAM_E4M3 ? few_grouped<3, true>(c, a) : few_grouped<3, false>(c, a);
 }
 
 }  // namespace iam

@@ -296,6 +296,23 @@ def test_large_values_and_large_scales(iam, ctx, rows, type):
     assert np.array_equal(got, v @ w.values().T)
 
 
+@pytest.mark.parametrize("size", [3e-37, 1e34])
+@pytest.mark.parametrize("x_group", [0, 128])
+@pytest.mark.parametrize("type", ["int8", "e4m3"])
+@pytest.mark.parametrize("rows", [1, 4, 20, 140])
+def test_scales_of_rows_near_the_limits(iam, ctx, rows, type, x_group, size):
+    rng = np.random.default_rng(rows)
+    w = R.random_weights(rng, 70, 1000, 64, True)
+    w.scale[:] = w.scale.astype(np.float64) / 10000 if size < 1 else w.scale
+    words, scale, v = rows_of(rng, rows, 1000, type, x_group)
+    scale = (scale * np.float64(size)).astype(np.float32)
+    v = R.values8(words, type) * R.spread(scale, x_group, 1000)
+    m = packed(iam, ctx, w)
+    got = product(ctx, m, words, scale, type, "f32", x_group)
+    m.free()
+    P.close(got, v @ w.values().T, R.product_bound(v, w.values()), "f32")
+
+
 def test_refusals(iam, ctx):
     m = iam.Q4Matrix(ctx, 40, 300, 64)
     z = iam.Q4Matrix(ctx, 40, 300, 64, zeros=True)
