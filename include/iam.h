@@ -548,7 +548,8 @@ int iam_q4_read(iam_ctx* ctx, const iam_q4_matrix* matrix, int first_row, int n_
  * x_scale_dev [n_rows][1] (x_group 0) or [n_rows][ceil(in_dim / 128)] (x_group
  * 128).  y is of a float type, rounded once.  Products of whole numbers are
  * exact and sums fp32; a float row enters to 22 bits of the largest value of
- * its 128 inputs (or of 2^-102, if that is larger) or better.  Matrices that share their input are one matrix of
+ * its 128 inputs (or of 2^-102, if that is larger) or better, up to four fp32
+ * rows to 30 (of 2^-96).  Matrices that share their input are one matrix of
  * their rows.  A row of x that holds an infinity or a NaN (or a scale that is
  * one) gives infinities and NaN in its own row of y only.  y may not overlap
  * the inputs. */

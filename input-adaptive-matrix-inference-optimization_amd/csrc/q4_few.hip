@@ -5,12 +5,14 @@
 //   y[r][o] = sum over d of 256^d  sum over tiles, groups of
 //             (2^e[r][tile] scale[o][group]) * (sum over the group of n_d[r][k] (w[o][k] - zero))
 // The innermost sums are exact, on the 8-bit matrix instructions, whose 16
-// columns are the rows' digits: three of a float row (22 bits of the tile's
-// largest value and its sign), one of an int8 row.  4-bit weights become bytes
-// with three instructions for eight of them, and five rows take no more matrix
-// instructions than one.  One row of 28672 x 4096 (groups of 64, zero points) takes
-// 13.0 us, 4.9 TB/s; bound by reads, and where there are few of them by the chain
-// of x's loads, its digits, the weights' use and the waves' joining (4.3 us).
+// columns are the rows' digits: three of a row in 16 bits or e4m3 (22 bits of the
+// tile's largest value and its sign), four of an fp32 row (30 bits: values from
+// 2^-6 of the largest on enter whole), one of an int8 row.  4-bit weights become
+// bytes with three instructions for eight of them, and four or five rows take no
+// more matrix instructions than one.  One row of 28672 x 4096 (groups of 64, zero
+// points) takes 13.0 us, 4.9 TB/s; bound by reads, and where there are few of them
+// by the chain of x's loads, its digits, the weights' use and the waves' joining
+// (4.3 us).  Four fp32 rows of 6144 x 4096 take 7.7 us.
 #include "accum.h"
 #include "q4_mul.h"
 
@@ -19,6 +21,7 @@ namespace iam {
 struct FewArgs {
     MulArgs u;
     int waves;      // of a workgroup
+    int rows;       // of a workgroup
     // the inputs cut into parts for more workgroups, whose sums the last one to arrive joins
     int splits;
     float* sums;
@@ -28,6 +31,7 @@ struct FewArgs {
 constexpr int kFewMaxWaves = 16;
 constexpr int kFewCols = 16;
 constexpr int kFewSplits = 8;
+constexpr int kFewLds = 160 * 1024;
 
 // A strip's words of a chunk, its scales and zero points, in a lane's registers.
 template <int GROUP, bool ZEROS>
@@ -74,6 +78,10 @@ __device__ __forceinline__ void widen8(uint32_t w, uint32_t zero4, uint32_t& lo,
     }
 }
 
+// Columns are an odd number of 16 bytes apart in LDS: lanes that write a column's
+// next inputs meet other banks.
+__host__ __device__ constexpr int few_pitch(int cols) { return cols | 1; }
+
 // the largest of 16 neighbouring lanes', in each of them
 __device__ __forceinline__ uint32_t max16(uint32_t v)
 {
@@ -94,12 +102,20 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
 {
     extern __shared__ uint4 lds[];
     constexpr bool SCALED = D == 1 || E4M3;
-    const MulArgs& u = a.u;
+    const int x_type = D == 1 ? IAM_I8 : D == 4 ? IAM_F32 : E4M3 ? IAM_E4M3 : a.u.x_type;
+    MulArgs u = a.u;
+    if (D == 4 && gridDim.y > 1) {       // (else there is one part)
+        const int r0 = blockIdx.y * a.rows;
+        u.rows = min(a.rows, u.rows - r0);
+        u.x = reinterpret_cast<const float*>(u.x) + (size_t)r0 * u.x_stride;
+        u.y = reinterpret_cast<uint8_t*>(u.y) + (size_t)r0 * u.y_stride * (u.y_type == IAM_F32 ? 4 : 2);
+    }
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int last = q4_strips(u.m.out) - 1, groups = (last + S) / S, id = xcd_remap(blockIdx.x, gridDim.x);
     const int split = id / groups, group = id - split * groups, strip0 = group * S, cols = u.rows * D;
-    uint4* digits = lds + wave * (32 * cols);                                       // [tile][step][g][col] 16 bytes
-    float* factor = reinterpret_cast<float*>(lds + a.waves * (32 * cols)) + wave * 4 * kFewCols;   // [tile][row]
+    const int pitch = few_pitch(cols);
+    uint4* digits = lds + wave * (32 * pitch);                                      // [tile][step][g][col] 16 bytes
+    float* factor = reinterpret_cast<float*>(lds + a.waves * (32 * pitch)) + wave * 4 * kFewCols;   // [tile][row]
     const int col = min(c, cols - 1), mine = col / D;
     // What a tile's sums are times: the digit's place, less the weights' 16 and
     // e4m3 numbers' 2^13.  (At the end alone, the sums of digits of the smallest
@@ -112,16 +128,16 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
     FewWeights<GROUP, ZEROS> now;
     for (int chunk = split * a.waves + wave; chunk < u.m.chunks; chunk += a.splits * a.waves) {
         const int t16 = lane >> 4, k8 = lane & 15, k = chunk * kChunk + t16 * kTile + k8 * 8;
-        Raw8 raw = load_raw8(u.x, u.x_type, 0, k, u.m.in);
+        Raw8 raw = load_raw8(u.x, x_type, 0, k, u.m.in);
         float xs = SCALED ? u.x_scale[u.x_groups > 1 ? min(chunk * 4 + t16, u.x_groups - 1) : 0] : 1.0f;
 #pragma unroll
         for (int t = 0; t < 4; t++) now.load(u.m, strip0, chunk, lane, t);
-        uint2* to = reinterpret_cast<uint2*>(digits + ((t16 * 2 + (k8 >> 3)) * 4 + (k8 & 3)) * cols) + (k8 >> 2 & 1);
+        uint2* to = reinterpret_cast<uint2*>(digits + ((t16 * 2 + (k8 >> 3)) * 4 + (k8 & 3)) * pitch) + (k8 >> 2 & 1);
         for (int r = 0; r < u.rows; r++) {
             const Raw8 mine8 = raw;
             const float scale = xs;
             if (r + 1 < u.rows) {
-                raw = load_raw8(u.x, u.x_type, (size_t)(r + 1) * u.x_stride, k, u.m.in);
+                raw = load_raw8(u.x, x_type, (size_t)(r + 1) * u.x_stride, k, u.m.in);
                 if constexpr (SCALED)
                     xs = u.x_scale[(size_t)(r + 1) * u.x_groups + (u.x_groups > 1 ? min(chunk * 4 + t16, u.x_groups - 1) : 0)];
             }
@@ -131,7 +147,7 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
                 if (k8 == 0) factor[t16 * kFewCols + r] = scale;
             } else {
                 float v[8];
-                values8(mine8, E4M3 ? IAM_E4M3 : u.x_type, v);
+                values8(mine8, x_type, v);
                 uint32_t top = 0;
 #pragma unroll
                 for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
@@ -140,24 +156,26 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
                 // where a value is not finite).  Tiles below 2^-102 count as if
                 // they were that large; e4m3 numbers, at most 448 and whole multiples
                 // of 2^-9, have one power, which goes to `place` so that the smallest
-                // scales keep their bits.
-                const uint32_t e8 = E4M3 ? 135u : max(top >> 23, 24u);
-                const float up = __uint_as_float((275u - e8) << 23);
-                uint32_t n[8];
+                // scales keep their bits.  fp32: 2^(156 - e), below 2^30, from 2^-96 on.
+                const uint32_t e8 = E4M3 ? 135u : max(top >> 23, D == 4 ? 30u : 24u);
+                const float up = __uint_as_float(((D == 4 ? 283u : 275u) - e8) << 23);
+                uint32_t n[8];               // 128 more in each digit makes them whole bytes
 #pragma unroll
-                for (int e = 0; e < 8; e++)   // 1.5 2^23 + n has n in its low bits; 128 more in each digit makes them whole bytes
-                    n[e] = __float_as_uint(__builtin_fmaf(v[e], up, 12582912.0f)) + (0x00808080u - 0x4b400000u);
-                {
-                    const uint32_t a0 = __builtin_amdgcn_perm(n[4], n[0], 0x05010400u), a1 = __builtin_amdgcn_perm(n[5], n[1], 0x05010400u);
-                    const uint32_t b0 = __builtin_amdgcn_perm(n[6], n[2], 0x05010400u), b1 = __builtin_amdgcn_perm(n[7], n[3], 0x05010400u);
-                    const uint32_t a2 = __builtin_amdgcn_perm(n[4], n[0], 0x0c0c0602u), a3 = __builtin_amdgcn_perm(n[5], n[1], 0x0c0c0602u);
-                    const uint32_t b2 = __builtin_amdgcn_perm(n[6], n[2], 0x0c0c0602u), b3 = __builtin_amdgcn_perm(n[7], n[3], 0x0c0c0602u);
-                    uint2* at = to + r * 2 * D;
-                    at[0] = {__builtin_amdgcn_perm(a1, a0, 0x05040100u) ^ 0x80808080u, __builtin_amdgcn_perm(b1, b0, 0x05040100u) ^ 0x80808080u};
-                    at[2] = {__builtin_amdgcn_perm(a1, a0, 0x07060302u) ^ 0x80808080u, __builtin_amdgcn_perm(b1, b0, 0x07060302u) ^ 0x80808080u};
-                    at[4] = {__builtin_amdgcn_perm(a3, a2, 0x05040100u) ^ 0x80808080u, __builtin_amdgcn_perm(b3, b2, 0x05040100u) ^ 0x80808080u};
+                for (int e = 0; e < 8; e++) {
+                    if constexpr (D == 4) n[e] = (uint32_t)(int)(v[e] * up) + 0x80808080u;
+                    else n[e] = __float_as_uint(__builtin_fmaf(v[e], up, 12582912.0f)) + (0x00808080u - 0x4b400000u);   // 1.5 2^23 + n has n in its low bits
                 }
-                if (k8 == 0) factor[t16 * kFewCols + r] = top >= 0x7f800000u ? NAN : E4M3 ? scale : __uint_as_float((e8 - 21u) << 23);
+                // digits d and d + 1 of two values, then each of four
+                auto two = [&](int lo, int hi, uint32_t sel) { return __builtin_amdgcn_perm(n[hi], n[lo], sel); };
+                uint2* at = to + r * 2 * D;
+#pragma unroll
+                for (int d = 0; d < D; d += 2) {
+                    const uint32_t sel = d == 0 ? 0x05010400u : D == 4 ? 0x07030602u : 0x0c0c0602u;
+                    const uint32_t a0 = two(0, 4, sel), a1 = two(1, 5, sel), b0 = two(2, 6, sel), b1 = two(3, 7, sel);
+                    at[2 * d] = {__builtin_amdgcn_perm(a1, a0, 0x05040100u) ^ 0x80808080u, __builtin_amdgcn_perm(b1, b0, 0x05040100u) ^ 0x80808080u};
+                    if (d + 1 < D) at[2 * d + 2] = {__builtin_amdgcn_perm(a1, a0, 0x07060302u) ^ 0x80808080u, __builtin_amdgcn_perm(b1, b0, 0x07060302u) ^ 0x80808080u};
+                }
+                if (k8 == 0) factor[t16 * kFewCols + r] = top >= 0x7f800000u ? NAN : E4M3 ? scale : __uint_as_float((e8 - (D == 4 ? 29u : 21u)) << 23);
             }
         }
         wave_sync();
@@ -173,7 +191,7 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
                     floatx4 part = {0.0f, 0.0f, 0.0f, 0.0f};   // of the tile, without f
 #pragma unroll
                     for (int step = 0; step < 2; step++) {
-                        const uint4 b = digits[((t * 2 + step) * 4 + g) * cols + col];
+                        const uint4 b = digits[((t * 2 + step) * 4 + g) * pitch + col];
                         uint32_t lo[2], hi[2];
 #pragma unroll
                         for (int j = 0; j < 2; j++) {
@@ -226,7 +244,8 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
         const int r = i / (S * 16), o = (strip0 + i / 16 % S) * kStrip + (i & 15);
         if (o < u.m.out) put_value(u.y, u.y_type, (size_t)r * u.y_stride + o, y);
     };
-    float* sums = a.sums + (size_t)group * a.splits * values;
+    const size_t cell = (size_t)blockIdx.y * groups + group;
+    float* sums = a.sums + cell * a.splits * (S * a.rows * 16);
     for (int i = tid; i < values; i += a.waves * 64) {
         const int r = i / (S * 16), s = i / 16 % S;
         float y = 0.0f;
@@ -241,8 +260,8 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
     }
     if (a.splits == 1) return;
     __shared__ int arrived;
-    if (!acc_arrive(a.ctr + group, (uint32_t)a.splits, &arrived)) return;
-    if (tid == 0) a.ctr[group] = 0u;
+    if (!acc_arrive(a.ctr + cell, (uint32_t)a.splits, &arrived)) return;
+    if (tid == 0) a.ctr[cell] = 0u;
     for (int i = tid; i < values; i += a.waves * 64) {
         float each[kFewSplits], y = 0.0f;
 #pragma unroll
@@ -254,21 +273,21 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void k_q4_few(FewArgs a)
 }
 
 // ------------------------------------------------------------------ host ---
-int q4_few_most(int x_type) { return x_type == IAM_I8 ? kFewCols : kFewCols / 3; }
+static int digits_of(int x_type) { return x_type == IAM_I8 ? 1 : x_type == IAM_F32 ? 4 : 3; }
 
-template <int D, bool E4M3, int GROUP, int S>
-static int few_launch(Ctx* c, const FewArgs& a)
+// How a call's rows, strips and chunks are dealt.
+struct FewPlan {
+    int digits, rows, row_parts;   // rows of a workgroup, and in how many of these the rows are
+    int together;                  // strips of a workgroup
+    int splits, waves;
+    size_t lds;
+};
+static FewPlan few_plan(const MulArgs& u)
 {
-    const int cols = a.u.rows * D;
-    const size_t stage = (size_t)a.waves * (32 * cols * 16 + 4 * kFewCols * 4), join = (size_t)a.waves * S * cols * 64;
-    const dim3 grid((unsigned)((q4_strips(a.u.m.out) + S - 1) / S * a.splits)), block((unsigned)a.waves * 64);
-    return a.u.m.zeros ? launch(c, "q4_mul.few", k_q4_few<D, E4M3, GROUP, true, S>, grid, block, std::max(stage, join), a)
-                       : launch(c, "q4_mul.few", k_q4_few<D, E4M3, GROUP, false, S>, grid, block, std::max(stage, join), a);
-}
-
-template <int D, bool E4M3, int GROUP>
-static int few_sized(Ctx* c, const FewArgs& a)
-{
+    FewPlan p{};
+    p.digits = digits_of(u.x_type);
+    p.row_parts = (u.rows * p.digits + kFewCols - 1) / kFewCols;
+    p.rows = (u.rows + p.row_parts - 1) / p.row_parts;
     // Several strips share the rows' digits, and a strip's weights come while the
     // one before is computed, where there are enough for the card all the same
     // (one bf16 row, 28672 x 4096 with groups of 64 and zero points: 17.3 us by single
@@ -276,41 +295,75 @@ static int few_sized(Ctx* c, const FewArgs& a)
     // 8192 x 8192 with groups of 128 11.0, 9.4 and 9.1, 6144 x 4096 5.7, 6.2 and 7.1).
     // Groups of 32 with zero points and four strips do not fit the registers (28672 x
     // 4096: 20.1, 17.4 and 23.0).
-    if (q4_strips(a.u.m.out) >= 512) return few_launch<D, E4M3, GROUP, GROUP == 32 ? 2 : 4>(c, a);
-    return few_launch<D, E4M3, GROUP, 1>(c, a);
-}
-
-template <int D, bool E4M3>
-static int few_grouped(Ctx* c, const FewArgs& a)
-{
-    if (a.u.m.group == 32) return few_sized<D, E4M3, 32>(c, a);
-    if (a.u.m.group == 64) return few_sized<D, E4M3, 64>(c, a);
-    return few_sized<D, E4M3, 128>(c, a);
-}
-
-int q4_mul_few(Ctx* c, const MulArgs& u)
-{
-    const int cols = u.x_type == IAM_I8 ? u.rows : u.rows * 3;
+    const int strips = q4_strips(u.m.out);
+    p.together = strips < 512 ? 1 : u.m.group == 32 ? 2 : 4;
     // A wave for each chunk, as many as 160 KB of LDS hold digits of (512 bytes
     // a column and 256 of factors each).
-    const int most = std::min(kFewMaxWaves, (160 * 1024) / (512 * cols + 256));
-    FewArgs a{};
-    a.u = u;
+    const int cols = p.rows * p.digits, most = std::min(kFewMaxWaves, kFewLds / (512 * few_pitch(cols) + 256));
     // Where a workgroup's waves would take several turns the inputs are cut, for
     // about a workgroup a CU (four fp32 rows, 1024 x 14336: 11.0 us whole, 8.6 cut;
     // 1024 x 8192 in one turn 7.2 and 7.2; one row of 1024 x 14336 7.3 and 6.6, but 7.7
     // and 8.1 of 2048 x 14336 in two).
-    const int strips = q4_strips(u.m.out), fit = 256 / strips;
-    a.splits = u.m.chunks > most && fit > (u.rows > 1 ? 1 : 2) ? std::min({fit, kFewSplits, u.m.chunks / 4}) : 1;
-    if (a.splits > 1) {
-        IAM_TRY(ensure_q4_sums(c, (size_t)strips * a.splits * u.rows * kStrip, (size_t)strips));
+    const int fit = 256 / strips;
+    p.splits = u.m.chunks > most && fit > (u.rows > 1 ? 1 : 2) ? std::min({fit, kFewSplits, u.m.chunks / 4}) : 1;
+    const int each = (u.m.chunks + p.splits - 1) / p.splits, rounds = (each + most - 1) / most;
+    p.waves = (each + rounds - 1) / rounds;
+    const size_t stage = (size_t)p.waves * (512 * few_pitch(cols) + 256), join = (size_t)p.waves * p.together * cols * 64;
+    p.lds = std::max(stage, join);
+    return p;
+}
+
+bool q4_takes_few(const MulArgs& u)
+{
+    if ((int64_t)u.rows * digits_of(u.x_type) <= kFewCols) return true;
+    if (u.x_type != IAM_F32 || u.rows > 5) return false;
+    // Five fp32 rows, as three and two: where the workgroups of both run in one round
+    // and a half at most (6144 x 4096 9.3 us, 12.3 with fp16 parts; 14336 x 4096 10.2
+    // and 15.2; 4096 x 14336 and 32000 x 4096, in two rounds, 19.1 and 24.3, but 17.3 and 21.6).
+    const FewPlan p = few_plan(u);
+    const int64_t all = (int64_t)((q4_strips(u.m.out) + p.together - 1) / p.together) * p.splits * p.row_parts;
+    return 2 * all <= 3 * 256 * (int64_t)std::min<size_t>(kFewLds / p.lds, 32 / p.waves);
+}
+
+template <int D, bool E4M3, int GROUP, int S>
+static int few_launch(Ctx* c, const FewArgs& a, const FewPlan& p)
+{
+    const dim3 grid((unsigned)((q4_strips(a.u.m.out) + S - 1) / S * a.splits), (unsigned)p.row_parts), block((unsigned)a.waves * 64);
+    return a.u.m.zeros ? launch(c, "q4_mul.few", k_q4_few<D, E4M3, GROUP, true, S>, grid, block, p.lds, a)
+                       : launch(c, "q4_mul.few", k_q4_few<D, E4M3, GROUP, false, S>, grid, block, p.lds, a);
+}
+
+template <int D, bool E4M3, int GROUP>
+static int few_sized(Ctx* c, const FewArgs& a, const FewPlan& p)
+{
+    return p.together == 1 ? few_launch<D, E4M3, GROUP, 1>(c, a, p) : few_launch<D, E4M3, GROUP, GROUP == 32 ? 2 : 4>(c, a, p);
+}
+
+template <int D, bool E4M3>
+static int few_grouped(Ctx* c, const FewArgs& a, const FewPlan& p)
+{
+    if (a.u.m.group == 32) return few_sized<D, E4M3, 32>(c, a, p);
+    if (a.u.m.group == 64) return few_sized<D, E4M3, 64>(c, a, p);
+    return few_sized<D, E4M3, 128>(c, a, p);
+}
+
+int q4_mul_few(Ctx* c, const MulArgs& u)
+{
+    const FewPlan p = few_plan(u);
+    FewArgs a{};
+    a.u = u;
+    a.rows = p.rows;
+    a.waves = p.waves;
+    a.splits = p.splits;
+    if (p.splits > 1) {
+        const size_t cells = (size_t)q4_strips(u.m.out) * p.row_parts;    // (single strips)
+        IAM_TRY(ensure_q4_sums(c, cells * p.splits * p.rows * kStrip, cells));
         a.sums = c->q4_sums;
         a.ctr = c->q4_ctr;
     }
-    const int each = (u.m.chunks + a.splits - 1) / a.splits, rounds = (each + most - 1) / most;
-    a.waves = (each + rounds - 1) / rounds;
-    if (u.x_type == IAM_I8) return few_grouped<1, false>(c, a);
-    return u.x_type == IAM_E4M3 ? few_grouped<3, true>(c, a) : few_grouped<3, false>(c, a);
+    if (p.digits == 1) return few_grouped<1, false>(c, a, p);
+    if (p.digits == 4) return few_grouped<4, false>(c, a, p);
+    return u.x_type == IAM_E4M3 ? few_grouped<3, true>(c, a, p) : few_grouped<3, false>(c, a, p);
 }
 
 }  // namespace iam

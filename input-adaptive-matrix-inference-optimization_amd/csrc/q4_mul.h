@@ -100,8 +100,8 @@ __device__ __forceinline__ void values8(const Raw8& r, int type, float* v)
     }
 }
 
-// rows that fit the one-launch kernel for few of them
-int q4_few_most(int x_type);
+// one launch for few rows: whether it takes these
+bool q4_takes_few(const MulArgs& a);
 int q4_mul_few(Ctx* c, const MulArgs& a);
 // any number of them
 int q4_mul_rows(Ctx* c, const MulArgs& a);

@@ -40,5 +40,5 @@ extern "C" int iam_q4_mul(iam_ctx* c, const iam_q4_matrix* m, const void* x, int
     a.y = y;
     a.y_type = y_type;
     a.y_stride = y_stride;
-    return rows <= q4_few_most(x_type) ? q4_mul_few(c, a) : q4_mul_rows(c, a);
+    return q4_takes_few(a) ? q4_mul_few(c, a) : q4_mul_rows(c, a);
 }

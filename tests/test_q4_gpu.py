@@ -313,6 +313,51 @@ def test_scales_of_rows_near_the_limits(iam, ctx, rows, type, x_group, size):
     P.close(got, v @ w.values().T, R.product_bound(v, w.values()), "f32")
 
 
+EXACT = [(1, 4096, 1024), (1, 14336, 40), (1, 14336, 200), (2, 8193, 17), (3, 20000, 1500), (4, 9000, 130), (4, 70001, 16), (4, 1100, 8209), (5, 2048, 100), (5, 9000, 130),
+         (6, 14336, 64), (11, 900, 12817), (33, 14336, 40), (48, 4096, 64), (64, 900, 12817), (100, 5000, 31), (150, 4096, 100), (300, 14336, 300)]
+
+
+@pytest.mark.parametrize("type", P.TYPES)
+@pytest.mark.parametrize("rows,inp,out", EXACT)
+def test_every_bit_of_x(iam, ctx, rows, inp, out, type):
+    """Each output takes one input alone, times a power of two, so the result is
+    equal if all bits of it enter: 24 of fp32 (20 where two fp16 parts take it),
+    of values within 2^-6 of their tile's largest."""
+    rng = np.random.default_rng(rows + inp + out)
+    group, zeros = (32, 64, 128)[(rows + out) % 3], rows % 2 == 0
+    bits = 24 if rows <= 4 else 20
+    x = rng.integers(2 ** (bits - 6), 2 ** bits, (rows, inp)) | 1
+    x = x * rng.choice([-1.0, 1.0], x.shape) * np.repeat(np.exp2(rng.integers(-5, 6, -(-inp // 128)) * (1 if type == "f16" else 6) - bits), 128)[:inp]
+    words, v = P.to_type(x, type)
+    w = R.random_weights(rng, out, inp, group, zeros)
+    w.scale[:] = np.exp2(rng.integers(-3, 4, w.scale.shape))
+    w.n[:] = 8 if not zeros else np.repeat(np.clip(w.zero, 1, 14), group, 1)[:, :inp]
+    if zeros:
+        w.zero[:] = np.clip(w.zero, 1, 14)
+    at, sign = rng.integers(0, inp, out), rng.choice([-1, 1], out)
+    w.n[np.arange(out), at] += sign
+    m = packed(iam, ctx, w)
+    got = product(ctx, m, words, None, type, "f32")
+    m.free()
+    assert np.array_equal(got, v[:, at] * sign * w.scale.astype(np.float64)[np.arange(out), at // group])
+
+
+@pytest.mark.parametrize("size", [1e-28, 2e-30])
+@pytest.mark.parametrize("rows", [1, 4, 5, 20, 140])
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_tiny_values(iam, ctx, rows, type, size):
+    """Around the size from which on values have a power of their own."""
+    rng = np.random.default_rng(10)
+    w = R.random_weights(rng, 40, 640, 64, rows % 2 == 0)
+    words, v = P.to_type(rng.normal(0, 1, (rows, 640)) * size * np.repeat([1, 0.3, 2, 0.1, 5], 128), type)
+    m = packed(iam, ctx, w)
+    got = product(ctx, m, words, None, type, "f32")
+    m.free()
+    # below 2^-102 to 22 bits of that: 2^-124 a value
+    room = R.product_bound(v, w.values()) + 2.0 ** -124 * np.abs(w.values()).sum(1)
+    P.close(got, v @ w.values().T, room, "f32")
+
+
 def test_refusals(iam, ctx):
     m = iam.Q4Matrix(ctx, 40, 300, 64)
     z = iam.Q4Matrix(ctx, 40, 300, 64, zeros=True)
