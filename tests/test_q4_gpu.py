@@ -358,6 +358,16 @@ def test_tiny_values(iam, ctx, rows, type, size):
     P.close(got, v @ w.values().T, room, "f32")
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows,inp,out,type", [(1, 1100, 8209, "f32"), (4, 700, 8209, "f32"), (5, 1100, 8209, "f32"), (5, 700, 8225, "bf16"), (3, 1540, 8240, "e4m3"), (16, 1100, 8209, "int8"),
+                                               (7, 700, 12817, "f16"), (20, 900, 12833, "f32"), (33, 700, 12817, "f32"), (64, 700, 12801, "bf16"), (40, 1100, 12817, "e4m3")])
+def test_strips_that_share_a_workgroup(iam, ctx, rows, inp, out, type, group, zeros):
+    """Matrices of so many rows that a workgroup takes several strips: inputs that
+    end inside a chunk, the last workgroup short of strips."""
+    check(iam, ctx, np.random.default_rng(group + rows), rows, inp, out, group, zeros, type, "f32")
+
+
 def test_refusals(iam, ctx):
     m = iam.Q4Matrix(ctx, 40, 300, 64)
     z = iam.Q4Matrix(ctx, 40, 300, 64, zeros=True)
