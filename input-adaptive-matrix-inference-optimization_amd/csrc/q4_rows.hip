@@ -749,13 +749,14 @@ __global__ __launch_bounds__(128 * WO, 2) void k_q4_gemm(RowsArgs a)
 #pragma unroll
     for (int n = 0; n < NB / 2; n++) {
         const int r0 = (b0 + (wave & 1) * NB + 2 * n) * 16;
-        const float rs = (a.row_scale ? a.row_scale[min(r0 + (lane & 31), u.rows - 1)] : 1.0f) * (PARTS == 0 ? rest : 1.0f);
+        const float rs = a.row_scale ? a.row_scale[min(r0 + (lane & 31), u.rows - 1)] : 1.0f;
+        const float first = PARTS == 0 ? rest : 1.0f;    // before the row's scale, which may be among the smallest numbers
 #pragma unroll
         for (int s = 0; s < 2; s++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 *reinterpret_cast<floatx4*>(turn + (lane & 31) * ROW + 32 * s + 8 * i + 4 * (lane >> 5)) =
-                    floatx4{acc[s][n][4 * i], acc[s][n][4 * i + 1], acc[s][n][4 * i + 2], acc[s][n][4 * i + 3]} * rs;
+                    floatx4{acc[s][n][4 * i], acc[s][n][4 * i + 1], acc[s][n][4 * i + 2], acc[s][n][4 * i + 3]} * first * rs;
         wave_sync();
         // four or eight results a lane
         auto at = [&](int r, int o) { return *reinterpret_cast<const floatx4*>(turn + r * ROW + o); };

@@ -368,6 +368,25 @@ def test_strips_that_share_a_workgroup(iam, ctx, rows, inp, out, type, group, ze
     check(iam, ctx, np.random.default_rng(group + rows), rows, inp, out, group, zeros, type, "f32")
 
 
+@pytest.mark.parametrize("unit", [2.0 ** -149, 2.0 ** -126])
+@pytest.mark.parametrize("x_group", [0, 128])
+@pytest.mark.parametrize("type", ["int8", "e4m3"])
+@pytest.mark.parametrize("rows", [1, 4, 20, 140])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_smallest_scales_of_rows(iam, ctx, rows, type, x_group, unit, zeros):
+    """Scales of a few of the smallest numbers: whole multiples of 2^10 units, below
+    640 * 15 * 15 * 7 < 2^21 of them, which fp32 holds."""
+    rng = np.random.default_rng(rows)
+    w = R.random_weights(rng, 70, 640, 64, zeros)
+    w.scale[:] = 2.0 ** 10
+    q = rng.integers(-15, 16, (rows, 640)).astype(np.float64)
+    scale = (rng.integers(1, 8, (rows, 5 if x_group else 1)) * unit).astype(np.float32)
+    m = packed(iam, ctx, w)
+    got = product(ctx, m, R.bytes_of(q, type), scale, type, "f32", x_group)
+    m.free()
+    assert np.array_equal(got, (q * R.spread(scale, x_group, 640)) @ w.values().T)
+
+
 def test_refusals(iam, ctx):
     m = iam.Q4Matrix(ctx, 40, 300, 64)
     z = iam.Q4Matrix(ctx, 40, 300, 64, zeros=True)
