@@ -25,7 +25,7 @@ typedef unsigned long long ull2 __attribute__((ext_vector_type(2)));
 // factor fp32 [block][tile][16]: what the tile's values were divided by
 // scaled [block][tile]: kScaled if any of these is not 1, kFar too if one is far from it
 constexpr uint8_t kScaled = 1, kFar = 2;
-// A factor up to 2^64 times a weights' scale (below 2^16) and a sum (up to 2^22 a
+// A factor up to 2^64 times a weights' scale (below 2^16) and a sum (below 2^27 a
 // tile, 2^13 tiles) stays in fp32's range, and one from 2^-100 on times a scale
 // (from 2^-24 on) keeps its bits.
 __device__ __forceinline__ bool is_far(float f) { return f != 0.0f && !(fabsf(f) >= 0x1p-100f && fabsf(f) <= 0x1p64f); }

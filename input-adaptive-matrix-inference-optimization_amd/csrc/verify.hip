@@ -16,8 +16,8 @@ namespace iam {
 constexpr int kVerThreads = 256, kVerWaves = 4;
 constexpr int kVerMaxSegs = 64;
 // p - q counts as nowhere positive where its positive parts add up to less: each
-// of p and q is off by 2e-13 of itself at most (the exponentials' 4e-14, and
-// fp64 sums in an order that depends on where a row lies)
+// of p and q is off by about 1e-13 of itself (the exponentials' 4e-14, and fp64
+// sums in an order that depends on where a row lies)
 constexpr double kNowhere = 1e-12;
 
 // One kind of rows of logits (the target's, or the draft's)
